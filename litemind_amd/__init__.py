@@ -79,6 +79,35 @@ class MlaConfig(C.Structure):
     ]
 
 
+class PagedStep(C.Structure):
+    """lm_paged_step: the requests of one serving step; the arrays are device addresses (include/litemind_serving.h)."""
+
+    _fields_ = [
+        ("requests", C.c_int64),
+        ("tokens", C.c_int64),
+        ("pages", C.c_int64),
+        ("page_size", C.c_int32),
+        ("table_width", C.c_int32),
+        ("max_added", C.c_int32),
+        ("reserved", C.c_int32),
+        ("cached", C.c_void_p),
+        ("added", C.c_void_p),
+        ("table", C.c_void_p),
+        ("ring", C.c_void_p),
+        ("queue_in", C.c_void_p),
+        ("queue_out", C.c_void_p),
+        ("lengths", C.c_void_p),
+        ("starts", C.c_void_p),
+        ("positions", C.c_void_p),
+        ("slots", C.c_void_p),
+        ("info", C.c_void_p),
+    ]
+
+
+STEP_OK, STEP_LENGTH, STEP_TOKENS, STEP_PAGES = range(4)  # LM_STEP_*: PagedStep.info[0] after a plan
+# lm_sampling: one row's settings, as a numpy structured type
+SAMPLING = np.dtype([("temperature", np.float32), ("top_k", np.int32), ("top_p", np.float32), ("min_p", np.float32)])
+
 _P = C.c_void_p
 _I32 = C.c_int32
 _I64 = C.c_int64
@@ -162,6 +191,9 @@ PROTOTYPES = {
     "lm_kv_cache_write": [_P, _I32, _I64, _I64, _P, _P, _P],
     "lm_kv_cache_truncate": [_P, _I32, _I64],
     "lm_decoder_forward": [_P, _I32, _I32, _P, _I64, _I64, _I32],
+    "lm_page_plan": [_P, _P],
+    "lm_paged_attention": [_P, _P, _P, _P, _I32, _I32, _I32, _I32, _F, _P],
+    "lm_sample": [_P, _P, _I64, _I64, _I64, _P, _P, _P, _P],
 }
 _RESTYPE = {"lm_last_error": C.c_char_p}
 
@@ -506,6 +538,23 @@ class Context:
 
     def decoder_forward(self, first, last, hidden, tokens, position0, path=PATH_AUTO) -> None:
         self._check(self.lib.lm_decoder_forward(self.handle, first, last, _ptr(hidden), tokens, position0, path))
+
+    # ---- many requests at once (include/litemind_serving.h) ----
+    def page_plan(self, step: PagedStep) -> None:
+        """Pages, starts, positions and slots of a step's new tokens from the requests' lengths (lm_page_plan)."""
+        self._check(self.lib.lm_page_plan(self.handle, C.byref(step)))
+
+    def paged_attention(self, step: PagedStep, q, pool, heads: int, scale: float, out, dtype: int = DT_F16,
+                        rank: int = 512, rope: int = 64) -> None:
+        """Latent attention of the step's tokens over their requests' pages (lm_paged_attention)."""
+        self._check(self.lib.lm_paged_attention(self.handle, C.byref(step), _ptr(q), _ptr(pool), dtype, heads, rank,
+                                                rope, scale, _ptr(out)))
+
+    def sample(self, logits, rows: int, vocab: int, settings, uniform, token, probability=None,
+               row_stride: int = 0) -> None:
+        """The next token of each row of logits from its settings (SAMPLING) and a random number (lm_sample)."""
+        self._check(self.lib.lm_sample(self.handle, _ptr(logits), rows, vocab, row_stride or vocab, _ptr(settings),
+                                       _ptr(uniform), _ptr(token), _ptr(probability)))
 
     def moe_forward_noalloc(self, layer, x, tokens, y, bias=None, idx=None, w=None, logits=None) -> None:
         """lm_moe_forward_noalloc: the single-token kernel per token, scratch in a fixed device array."""

@@ -9,6 +9,7 @@
 #include "litemind_moe.h"
 #include "lm_error.h"
 #include "lm_internal.h"
+#include "serve_internal.h"
 
 #include <algorithm>
 #include <cstdio>
@@ -206,6 +207,7 @@ struct lm_context {
     float* head_x = nullptr;
     lm::HeadBest* head_partial = nullptr;  // per-block candidates of the greedy choice
     lm::AttnState* attention = nullptr;  // lm_attention_configure: MLA weights, rotary tables, KV caches
+    lm::ServeState* serve = nullptr;     // the operators of litemind_serving.h, at their first call
     int32_t graphs = 0;  // live lm_stack_graph captures (they hold the workspace's pointers)
     // lm_clock_probe_*: its own stream (default priority) and sample buffer
     hipStream_t probe_stream = nullptr;
@@ -990,6 +992,8 @@ lm::ContextInfo lm::context_info(const lm_context* ctx) {
 
 lm::AttnState*& lm::context_attention(lm_context* ctx) { return ctx->attention; }
 
+lm::ServeState*& lm::context_serve(lm_context* ctx) { return ctx->serve; }
+
 namespace {
 
 // h += FFN(rms_norm(h)) (src/DeepSeekRunner.cpp:265-290) for one layer.  The
@@ -1157,6 +1161,7 @@ int lm_context_destroy(lm_context* ctx) {
     (void)hipFree(w.spec_sync);
     lm::attention_release(ctx->attention);
     ctx->attention = nullptr;
+    lm::serve_release(ctx->serve);
     if (ctx->staging != nullptr) {
         (void)hipHostFree(ctx->staging);
     }
@@ -1183,7 +1188,8 @@ int lm_synchronize(lm_context* ctx) {
         return fail(LM_EINVAL, "null context");
     }
     LM_HIP(hipStreamSynchronize(ctx->stream));
-    return check_decode_error(ctx);
+    const int rc = check_decode_error(ctx);
+    return rc != LM_OK ? rc : lm::serve_check_error(ctx);
 }
 
 int lm_alloc(lm_context* ctx, size_t bytes, void** out_dev) {
@@ -1221,8 +1227,9 @@ int lm_copy_d2h(lm_context* ctx, void* dst_host, const void* src_dev, size_t byt
     }
     LM_HIP(hipMemcpyAsync(dst_host, src_dev, bytes, hipMemcpyDeviceToHost, ctx->stream));
     LM_HIP(hipStreamSynchronize(ctx->stream));
-    // the copied data may come from a decode whose wait gave up
-    return check_decode_error(ctx);
+    // the copied data may come from a decode whose wait gave up, or from pages outside a pool
+    const int rc = check_decode_error(ctx);
+    return rc != LM_OK ? rc : lm::serve_check_error(ctx);
 }
 
 int lm_memset(lm_context* ctx, void* dst_dev, int32_t value, size_t bytes) {

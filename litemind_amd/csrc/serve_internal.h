@@ -1,0 +1,79 @@
+// serve_internal.h -- what the kernels of the paged cache and of sampling
+// (k_pages.hip, k_paged.hip, k_sample.hip) share with the ABI over them
+// (lm_serve.hip, lm_attn.hip).
+#pragma once
+
+#include "litemind_serving.h"
+#include "lm_internal.h"
+
+namespace lm {
+
+// A planned step as the attention reads it: lm_paged_step's device arrays, with
+// the sizes that every kernel checks what it reads against.
+struct PagedView {
+    const int32_t* table;
+    const int32_t* lengths;
+    const int32_t* starts;
+    int64_t pages;
+    int32_t requests, tokens, page_size, table_width;
+    uint32_t* error;  // set to 1 (host memory) where a page id lies outside the pool
+};
+
+// Tokens that request r has in its pages and adds, within the arrays' bounds:
+// rows first .. first + added - 1 of the step, which see keys 0 .. cached + i.
+struct PagedRequest {
+    int32_t first, added, cached;
+};
+__device__ inline PagedRequest paged_request(const PagedView& v, int32_t r) {
+    PagedRequest q;
+    const int64_t room = static_cast<int64_t>(v.table_width) * v.page_size;
+    const int32_t length = static_cast<int32_t>(min(static_cast<int64_t>(v.lengths[r]), room));
+    q.first = min(max(v.starts[r], 0), v.tokens);
+    q.added = max(0, min(min(v.starts[r + 1], v.tokens) - q.first, length));
+    q.cached = length - q.added;
+    return q;
+}
+
+// A page id of the table: ids outside the pool read page 0 and set the error word.
+__device__ inline int64_t checked_page(const PagedView& v, int32_t page) {
+    if (static_cast<uint32_t>(page) >= static_cast<uint64_t>(v.pages)) {
+        __hip_atomic_store(v.error, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+        return 0;
+    }
+    return page;
+}
+
+hipError_t launch_page_plan(const lm_paged_step& step, hipStream_t s);
+
+// Attention of the step's tokens: q [tokens][heads][rank + rope], pool
+// [pages][page_size][rank + rope], out [tokens][heads][rank], BF16 or fp16.
+struct PagedAttention {
+    PagedView view;
+    const void* q;
+    const void* pool;
+    void* out;
+    int32_t bf16;
+    int32_t heads, rank, rope;
+    int32_t max_added;
+    float scale;
+};
+hipError_t launch_paged_attention(const PagedAttention& a, hipStream_t s);
+
+struct SampleArgs {
+    const float* logits;
+    int64_t rows, vocab, stride;
+    const lm_sampling* settings;
+    const float* uniform;
+    int32_t* token;
+    float* probability;  // or null
+};
+hipError_t launch_sample(const SampleArgs& a, hipStream_t s);
+
+// ---- services of lm_serve.hip ----
+struct ServeState;
+ServeState*& context_serve(lm_context* ctx);
+void serve_release(ServeState* st);
+// LM_EKERNEL, once, where a kernel met a page id outside the pool.
+int serve_check_error(lm_context* ctx);
+
+}  // namespace lm
