@@ -20,6 +20,9 @@ struct ServeState {
     // Host memory that the kernels write when a table names a page outside the
     // pool: read without a copy once the stream has drained.
     uint32_t* error = nullptr;
+    // Sums of blocks whose keys are shared by several workgroups: a fixed size,
+    // so captured graphs keep their pointer. Steps on the stream take turns.
+    void* parts = nullptr;
 };
 
 void serve_release(ServeState* st) {
@@ -27,6 +30,7 @@ void serve_release(ServeState* st) {
         return;
     }
     (void)hipHostFree(st->error);
+    (void)hipFree(st->parts);
     delete st;
 }
 
@@ -65,10 +69,12 @@ int serve_state(lm_context* ctx, lm::ServeState** out) {
             return fail(LM_EINVAL, "the context's first paged attention cannot be captured: call it once before");
         }
         auto* made = new lm::ServeState();
-        const hipError_t err = hipHostMalloc(reinterpret_cast<void**>(&made->error), sizeof(uint32_t),
-                                             hipHostMallocMapped | hipHostMallocCoherent);
+        hipError_t err = hipHostMalloc(reinterpret_cast<void**>(&made->error), sizeof(uint32_t),
+                                       hipHostMallocMapped | hipHostMallocCoherent);
+        if (err == hipSuccess) {
+            err = hipMalloc(&made->parts, static_cast<size_t>(lm::paged_workspace_bytes()));
+        }
         if (err != hipSuccess) {
-            made->error = nullptr;
             lm::serve_release(made);
             (void)hipGetLastError();
             return fail(LM_ENOMEM, std::string("serving state: ") + hipGetErrorString(err));
@@ -195,7 +201,7 @@ int lm_paged_attention(lm_context* ctx, const lm_paged_step* step, const void* q
         a.rope = rope;
         a.max_added = s.max_added;
         a.scale = scale;
-        LM_SERVE_HIP(lm::launch_paged_attention(a, info.stream));
+        LM_SERVE_HIP(lm::launch_paged_attention(a, st->parts, info.stream));
         return LM_OK;
     } catch (const std::bad_alloc&) {
         return fail(LM_ENOMEM, "host allocation failed");

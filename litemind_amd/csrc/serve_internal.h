@@ -57,7 +57,11 @@ struct PagedAttention {
     int32_t max_added;
     float scale;
 };
-hipError_t launch_paged_attention(const PagedAttention& a, hipStream_t s);
+// Whether rows of this width go to the matrix cores; they need a workspace of
+// paged_workspace_bytes(), whatever the step.
+bool paged_tiled(int32_t rank, int32_t rope);
+int64_t paged_workspace_bytes();
+hipError_t launch_paged_attention(const PagedAttention& a, void* workspace, hipStream_t s);
 
 struct SampleArgs {
     const float* logits;
