@@ -14,7 +14,7 @@
 // Rows of 576 values (rank 512, rope 64: DeepSeek-V2's) go to the matrix cores,
 // in blocks of query rows of one request:
 //   few rows (paged_rows16_kernel): 16 rows, each wave on key tiles of its own
-//   many (paged_rows128_kernel): 128 rows, 32 per wave, tiles shared by the waves
+//   many (paged_rows64_kernel): 64 rows, tiles and products shared by the waves
 // Any other widths take paged_any_kernel.
 //
 // The blocks' key tiles are shared out evenly: the grid's workgroups cut the
@@ -25,6 +25,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace lm {
 namespace {
@@ -75,25 +76,24 @@ struct Half<bf16> {
 
 // ---- sharing out the tiles ----
 // Block b of a request (rows b M .. of its added heads rows) costs the keys that
-// its last token sees, as a line in b: cached + kExtra + (b + 1) M / heads, in
-// whole numbers below. kExtra stands for what a block costs besides its tiles.
+// its last token sees, as a line in b and times heads, which keeps it whole:
+// (cached + kExtra) heads + (b + 1) M. kExtra stands for what a block costs
+// besides its tiles.
 constexpr int kExtra = 64;
-// Cost per workgroup below which fewer take part.
+// Keys per workgroup below which fewer take part.
 constexpr int kLeast = 128;
 
 struct Shares {
     int32_t heads, rows;  // rows: M
-    __device__ int32_t blocks(const PagedRequest& r) const {
-        return static_cast<int32_t>((static_cast<int64_t>(r.added) * heads + rows - 1) / rows);
-    }
+    __device__ int32_t blocks(const PagedRequest& r) const { return (r.added * heads + rows - 1) / rows; }
     // Cost of the request's first b blocks.
     __device__ int64_t cost(const PagedRequest& r, int32_t b) const {
-        return static_cast<int64_t>(b) * (r.cached + kExtra) + static_cast<int64_t>(b) * (b + 1) / 2 * rows / heads;
+        return static_cast<int64_t>(b) * (r.cached + kExtra) * heads + static_cast<int64_t>(b) * (b + 1) / 2 * rows;
     }
     // Tiles of block b.
     __device__ int32_t tiles(const PagedRequest& r, int32_t b) const {
-        const int64_t last = min(static_cast<int64_t>(b + 1) * rows, static_cast<int64_t>(r.added) * heads) - 1;
-        return (r.cached + static_cast<int32_t>(last / heads) + kTile) / kTile;
+        const int32_t last = min((b + 1) * rows, r.added * heads) - 1;
+        return (r.cached + last / heads + kTile) / kTile;
     }
 };
 
@@ -136,7 +136,7 @@ __device__ inline Piece find_piece(const PagedView& v, const Shares& sh, int32_t
     }
     Piece p;
     p.total = total;
-    p.parts = static_cast<int32_t>(max(int64_t{1}, min(static_cast<int64_t>(kGrid), total / kLeast)));
+    p.parts = static_cast<int32_t>(max(int64_t{1}, min(static_cast<int64_t>(kGrid), total / (int64_t{kLeast} * sh.heads))));
     p.begin = g < p.parts ? border(total, p.parts, g) : total;
     p.end = g < p.parts ? border(total, p.parts, g + 1) : total;
     if (p.begin >= before && p.begin < before + own) {
@@ -289,6 +289,13 @@ struct PageWalk {
     }
 };
 
+// The same value, made anew where it stands: kept from becoming a register that
+// lives through a loop for every constant that is added to it.
+__device__ inline int here(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
 // ---- few rows ----
 // 16 query rows, four waves. A wave takes every fourth tile of the segment into
 // a buffer of its own, without a barrier: S^T of 2 x 18 and out^T of 32 products
@@ -333,13 +340,12 @@ __global__ __launch_bounds__(256) void paged_rows16_kernel(const TileArgs a) {
     Segment s;
     while (walk.next(a.view, s)) {
         const int64_t row0 = static_cast<int64_t>(s.req.first) * a.heads + static_cast<int64_t>(s.block) * kRows16;
-        const int rows = static_cast<int>(min(static_cast<int64_t>(kRows16),
-                                              static_cast<int64_t>(s.req.added) * a.heads - s.block * int64_t{kRows16}));
+        const int rows = min(kRows16, s.req.added * a.heads - s.block * kRows16);
         const int32_t keys = s.req.cached + s.req.added;
         // this lane's query row; the last key that it sees, and that all rows see
         const int own = min(col, rows - 1);
-        const int32_t sees = s.req.cached + static_cast<int32_t>((s.block * int64_t{kRows16} + own) / a.heads);
-        const int32_t all_see = s.req.cached + static_cast<int32_t>(s.block * int64_t{kRows16} / a.heads);
+        const int32_t sees = s.req.cached + (s.block * kRows16 + own) / a.heads;
+        const int32_t all_see = s.req.cached + s.block * kRows16 / a.heads;
         vec8 q[18];
         {
             const E* const from_q = static_cast<const E*>(a.q) + (row0 + own) * kWidth + 8 * grp;
@@ -518,6 +524,422 @@ __global__ __launch_bounds__(256) void paged_rows16_kernel(const TileArgs a) {
     }
 }
 
+// ---- many rows ----
+// 64 query rows, four waves. The waves share tiles of 32 keys, which come straight
+// to LDS four deep, and split each product differently:
+//   S^T   wave (kh, rh): keys 16 kh .. + 15 for rows 32 rh .. + 31; its queries
+//         stay in 144 registers, 36 products of 16 x 16 x 32 a tile
+//   out^T channels 128 w .. + 127 of wave w for all rows; 128 registers of sums,
+//         16 products of 32 x 32 x 16 a tile
+// The weights pass through LDS. One barrier a tile: between two, the waves run
+// the scores of tile t + 1 and the context of tile t, which do not depend on each
+// other, so either's latencies are filled by the other's products. 32 rows with
+// all 512 channels per wave, without the exchange, would take 256 + 16 registers
+// of sums, and the matrix cores' results go to 256.
+//
+// The weights' reference m, one per row, has to be the same for all waves: it
+// follows the rows' maxima one barrier late, and only where a row passed it by
+// more than 2^kSlack, which keeps the weights in 16 bits' range; the tile's
+// weights are then made anew. (fp32 sums do not mind the factor.)
+constexpr int kRows64 = 64;
+constexpr float kSlack = 10.0f;
+
+// Non-finite values as 0: keys that some row must not see weigh 0 there, and 0
+// times NaN or infinity is not 0. (Rows that see such a key have a NaN weight.)
+template <class E>
+__device__ inline short8v finite_or_zero(short8v v) {
+    constexpr short kExponent = sizeof(E) == 2 && __is_same(E, bf16) ? 0x7f80 : 0x7c00;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        v[e] = (v[e] & kExponent) == kExponent ? short{0} : v[e];
+    }
+    return v;
+}
+
+template <class E>
+__global__ __launch_bounds__(256, 1) void paged_rows64_kernel(const TileArgs a) {
+    using H = Half<E>;
+    typedef typename H::vec8 vec8;
+    typedef typename H::vec4 vec4;
+    // one array per stage: the compiler tracks loads to LDS per array
+    __shared__ __align__(16) char s0[kTileBytes], s1[kTileBytes], s2[kTileBytes], s3[kTileBytes];
+    __shared__ __align__(16) char weights[2][kRows64 * kTile * 2];
+    __shared__ float tops[2][2][kRows64];
+    __shared__ int64_t scratch[8];
+    char* const ring[4] = {s0, s1, s2, s3};
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int kh = wave & 1, rh = wave >> 1;
+    const int col = lane & 15, grp = lane >> 4;     // of 16 x 16 products
+    const int col32 = lane & 31, half = lane >> 5;  // of 32 x 32 products
+    Walk walk;
+    walk.sh = Shares{a.heads, kRows64};
+    walk.p = find_piece(a.view, walk.sh, blockIdx.x, scratch);
+    if (tid == 0) {
+        a.parts.heads[blockIdx.x].rows = 0;
+    }
+    if (walk.p.begin >= walk.p.end) {
+        return;
+    }
+    walk.start(a.view);
+    // The wave loads rows 8 wave .. + 7 of a tile, 9 loads of 64 units.
+    auto place = [&](int j, int of, int& row, int& unit) {
+        const int at = 64 * j + of;
+        const int r = at / kUnits;
+        row = 8 * (wave & 1) + r;  // of 16
+        unit = (at - r * kUnits) ^ swizzle(row);
+    };
+    unsigned from[9];
+#pragma unroll
+    for (int j = 0; j < 9; ++j) {
+        int row, unit;
+        place(j, lane, row, unit);
+        from[j] = static_cast<unsigned>(row * kRowBytes + unit * 16);
+    }
+    // Where the lane's reads of a tile begin; the rest is constant offsets, since
+    // the swizzle changes the low three bits of a unit only.
+    int key_at[2], value_at[2][2], weight_from[2], weight_to[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        key_at[i] = unit_at(16 * kh + col, 4 * i + grp);
+        const int row = 32 * i + col32, to = 32 * rh + 16 * i + col;
+        weight_from[i] = row * 64 + ((half ^ (row >> 2 & 1)) * 16 | (row >> 3 & 1) * 32);
+        weight_to[i] = to * 64 + ((2 * kh + (grp >> 1)) ^ (to >> 2 & 3)) * 16 + (grp & 1) * 8;
+#pragma unroll
+        for (int odd = 0; odd < 2; ++odd) {
+            const int r = 8 * half + 4 * i + ((lane & 15) >> 2);
+            value_at[i][odd] = unit_at(r, 4 * odd + 2 * (lane >> 4 & 1) + ((lane & 3) >> 1)) + (lane & 1) * 8 +
+                               wave * 256;
+        }
+    }
+    Segment s;
+    while (walk.next(a.view, s)) {
+        const int in_request = s.block * kRows64;  // the block's first row
+        const int64_t row0 = static_cast<int64_t>(s.req.first) * a.heads + in_request;
+        const int rows = min(kRows64, s.req.added * a.heads - in_request);
+        const int32_t last = s.req.cached + s.req.added - 1;
+        const int32_t all_see = s.req.cached + in_request / a.heads;
+        int32_t sees[2];
+        vec8 q[2][18];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const int own = min(32 * rh + 16 * b + col, rows - 1);
+            sees[b] = s.req.cached + (in_request + own) / a.heads;
+            const E* const from_q = static_cast<const E*>(a.q) + (row0 + own) * kWidth + 8 * grp;
+#pragma unroll
+            for (int ks = 0; ks < 18; ++ks) {
+                q[b][ks] = *reinterpret_cast<const vec8*>(from_q + 32 * ks);
+            }
+        }
+        if (a.negative) {
+#pragma unroll
+            for (int ks = 0; ks < 18; ++ks) {
+                q[0][ks] = -q[0][ks];
+                q[1][ks] = -q[1][ks];
+            }
+        }
+        PageWalk pages;
+        pages.start(a.view, s.request);
+        auto issue = [&](int32_t t, char* to) {
+            const int32_t key = t * kTile + 16 * (wave >> 1);
+            const int32_t first = min(key, last & ~15);
+            const char* const base =
+                static_cast<const char*>(a.pool) + pages.at(a.view, a.page_mul, first) * kRowBytes;
+            const __amdgpu_buffer_rsrc_t res =
+                __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 16 * kRowBytes, kBufferWord3);
+            to += 8 * wave * kRowBytes;
+            if (key + 15 <= last) {
+#pragma unroll
+                for (int j = 0; j < 9; ++j) {
+                    buffer_lds16(res, to + j * 1024, from[j], 0);
+                }
+            } else {  // rows past the last key: the last key's once more
+                const int of = here(lane);
+#pragma unroll
+                for (int j = 0; j < 9; ++j) {
+                    int row, unit;
+                    place(j, of, row, unit);
+                    const int r = min(key + row, last) - first;
+                    buffer_lds16(res, to + j * 1024, static_cast<unsigned>(r * kRowBytes + unit * 16), 0);
+                }
+            }
+        };
+        f32x16 o[2][4] = {};
+        f32x4 sc[2];             // scores of the newest tile
+        float m = kNone;         // reference of row `lane`, the same in every wave
+        float ref[2];            // times c, of this lane's rows of the scores
+        float l[2] = {0.0f, 0.0f};
+        ref[0] = ref[1] = 0.0f;
+        // The products of an interval in eight steps, each step's operands read
+        // during the one before: k-steps 9 i / 4 .. of the scores of the tile in
+        // `next`, channel tile i % 4 of keys 16 (i / 4) .. of the context of the
+        // tile in `now`.
+        auto products = [&](auto with_scores, const char* next, auto with_context, const char* now, const char* wt,
+                            auto sanitize) {
+            constexpr bool S = decltype(with_scores)::value, C = decltype(with_context)::value;
+            vec8 kf[2][3], vf[2], pf[2][2];
+            const int k_at[2] = {here(key_at[0]), here(key_at[1])};
+            const int v_at[2][2] = {{here(value_at[0][0]), here(value_at[0][1])},
+                                    {here(value_at[1][0]), here(value_at[1][1])}};
+            auto read = [&](int i) {
+                if constexpr (S) {
+#pragma unroll
+                    for (int ks = 9 * i / 4; ks < 9 * (i + 1) / 4; ++ks) {
+                        kf[i & 1][ks - 9 * i / 4] =
+                            *reinterpret_cast<const vec8*>(next + k_at[ks & 1] + (ks >> 1) * 128);
+                    }
+                }
+                if constexpr (C) {
+                    const int st = i / 4, ct = i % 4;
+                    if (ct == 0) {
+#pragma unroll
+                        for (int rb = 0; rb < 2; ++rb) {
+                            pf[st][rb] = *reinterpret_cast<const vec8*>(wt + (weight_from[rb] ^ st * 32));
+                        }
+                    }
+                    short8v v;
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const short4v part = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (lds_short4*)(now + v_at[k][ct & 1] + st * 16 * kRowBytes + (ct >> 1) * 128));
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            v[4 * k + e] = part[e];
+                        }
+                    }
+                    vf[i & 1] = __builtin_bit_cast(vec8, v);
+                }
+            };
+            if constexpr (S) {
+                sc[0] = sc[1] = f32x4{};
+            }
+            read(0);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (i < 7) {
+                    read(i + 1);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (C) {
+                    vec8 f = vf[i & 1];
+                    if constexpr (decltype(sanitize)::value) {
+                        f = __builtin_bit_cast(vec8, finite_or_zero<E>(__builtin_bit_cast(short8v, f)));
+                    }
+                    o[0][i % 4] = H::mfma32(f, pf[i / 4][0], o[0][i % 4]);
+                    o[1][i % 4] = H::mfma32(f, pf[i / 4][1], o[1][i % 4]);
+                }
+                if constexpr (S) {
+#pragma unroll
+                    for (int ks = 9 * i / 4; ks < 9 * (i + 1) / 4; ++ks) {
+                        const vec8 k = kf[i & 1][ks - 9 * i / 4];
+                        sc[0] = H::mfma16(k, q[0][ks], sc[0]);
+                        sc[1] = H::mfma16(k, q[1][ks], sc[1]);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        auto mask = [&](int32_t t) {
+            if (t * kTile + kTile - 1 > all_see) {
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        sc[b][e] = t * kTile + 16 * kh + 4 * grp + e > sees[b] ? kNone : sc[b][e];
+                    }
+                }
+            }
+        };
+        // the rows' maxima of the newest tile
+        auto pass = [&](float (*top)[kRows64]) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                float high = fmaxf(fmaxf(sc[b][0], sc[b][1]), fmaxf(sc[b][2], sc[b][3]));
+                high = fmaxf(high, __shfl_xor(high, 16));
+                high = fmaxf(high, __shfl_xor(high, 32));
+                if (grp == 0) {
+                    top[kh][32 * rh + 16 * b + col] = high;
+                }
+            }
+        };
+        auto weigh = [&](char* wt, float (&sum)[2]) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                vec4 p;
+                sum[b] = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][e], a.c, -ref[b]));
+                    sum[b] += w;
+                    p[e] = static_cast<E>(w);
+                }
+                *reinterpret_cast<vec4*>(wt + weight_to[b]) = p;
+            }
+        };
+        auto meet = [] {
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_waitcnt(0xc07f);  // the weights are written
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        __syncthreads();  // the block before is done with the ring
+        if (s.tile0 < s.tile1) {
+            issue(s.tile0, ring[0]);
+        }
+        if (s.tile0 + 1 < s.tile1) {
+            issue(s.tile0 + 1, ring[1]);
+        }
+        float sum[2] = {0.0f, 0.0f};  // of the newest tile's weights
+        // Between two barriers: context of tile t (stage u), scores of t + 1.
+        const std::true_type yes;
+        const std::false_type no;
+        // tile t's weights and t + 1 are in; passes on the reference
+        auto begin = [&](int32_t t, int u) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (t + 2 < s.tile1) {
+                __builtin_amdgcn_s_waitcnt(0x0F70 | 9);
+            } else {
+                __builtin_amdgcn_s_waitcnt(0x0F70);
+            }
+            meet();
+            if (t + 3 < s.tile1) {
+                issue(t + 3, ring[(u + 3) & 3]);
+            }
+            const float(*const top)[kRows64] = tops[u & 1];
+            const float high = lane < rows ? fmaxf(top[0][lane], top[1][lane]) : kNone;
+            if (__any((high - m) * a.c > kSlack)) {
+                const float up = fmaxf(m, high);
+                const float alpha = up == kNone ? 1.0f : __builtin_amdgcn_exp2f((m - up) * a.c);
+                m = up;
+#pragma unroll
+                for (int rb = 0; rb < 2; ++rb) {
+                    const float f = __shfl(alpha, 32 * rb + col32);
+#pragma unroll
+                    for (int ct = 0; ct < 4; ++ct) {
+                        o[rb][ct] *= f;
+                    }
+                }
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const int row = 32 * rh + 16 * b + col;
+                    l[b] *= __shfl(alpha, row);
+                    const float mine = __shfl(up, row);
+                    ref[b] = mine == kNone ? 0.0f : mine * a.c;
+                }
+                weigh(weights[u & 1], sum);
+                meet();
+            }
+            l[0] += sum[0];
+            l[1] += sum[1];
+        };
+        if (s.tile0 < s.tile1) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (s.tile0 + 1 < s.tile1) {
+                __builtin_amdgcn_s_waitcnt(0x0F70 | 9);
+            } else {
+                __builtin_amdgcn_s_waitcnt(0x0F70);
+            }
+            meet();
+            if (s.tile0 + 2 < s.tile1) {
+                issue(s.tile0 + 2, ring[2]);
+            }
+            products(yes, ring[0], no, nullptr, nullptr, no);
+            mask(s.tile0);
+            pass(tops[0]);
+            weigh(weights[0], sum);
+            // tiles that all rows see, the next one too
+            const int32_t full = min(s.tile1 - 1, (all_see + 1) / kTile - 1);
+            int32_t t = s.tile0;
+            for (; t + 4 <= full; t += 4) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    begin(t + u, u);
+                    products(yes, ring[(u + 1) & 3], yes, ring[u], weights[u & 1], no);
+                    pass(tops[(u + 1) & 1]);
+                    weigh(weights[(u + 1) & 1], sum);
+                }
+            }
+            // the others
+            for (; t < s.tile1; t += 4) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    if (t + u < s.tile1) {
+                        begin(t + u, u);
+                        if (t + u + 1 < s.tile1) {
+                            products(yes, ring[(u + 1) & 3], no, nullptr, nullptr, no);
+                            mask(t + u + 1);
+                        }
+                        products(no, nullptr, yes, ring[u], weights[u & 1], yes);
+                        if (t + u + 1 < s.tile1) {
+                            pass(tops[(u + 1) & 1]);
+                            weigh(weights[(u + 1) & 1], sum);
+                        }
+                    }
+                }
+            }
+        }
+        // the totals: the rows' parts of both key halves meet in `tops`
+        __syncthreads();
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            l[b] += __shfl_xor(l[b], 16);
+            l[b] += __shfl_xor(l[b], 32);
+            if (grp == 0) {
+                tops[0][kh][32 * rh + 16 * b + col] = l[b];
+            }
+        }
+        __syncthreads();
+        const bool whole = s.begins && s.ends;
+        const int slot = 2 * static_cast<int>(blockIdx.x) + (s.begins ? 1 : 0);
+        // o[rb][ct] register e: channel 128 wave + 32 ct + 8 (e / 4) + 4 half + e % 4 of row 32 rb + col32
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb) {
+            const int row = 32 * rb + col32;
+            if (row < rows) {
+                if (whole) {
+                    const float inv = 1.0f / (tops[0][0][row] + tops[0][1][row]);
+                    E* const to = static_cast<E*>(a.out) + (row0 + row) * kRank + 128 * wave + 4 * half;
+#pragma unroll
+                    for (int ct = 0; ct < 4; ++ct) {
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            vec4 out;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                out[e] = static_cast<E>(o[rb][ct][4 * g + e] * inv);
+                            }
+                            *reinterpret_cast<vec4*>(to + 32 * ct + 8 * g) = out;
+                        }
+                    }
+                } else {
+                    float* const to = a.parts.sums + (static_cast<int64_t>(slot) * kRows64 + row) * kRank + 128 * wave +
+                                      4 * half;
+#pragma unroll
+                    for (int ct = 0; ct < 4; ++ct) {
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            f32x4 out;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                out[e] = o[rb][ct][4 * g + e];
+                            }
+                            *reinterpret_cast<f32x4*>(to + 32 * ct + 8 * g) = out;
+                        }
+                    }
+                }
+            }
+        }
+        if (!whole && tid < rows) {
+            float* const to = a.parts.stats + (static_cast<int64_t>(slot) * kRows64 + tid) * 2;
+            to[0] = m == kNone ? kNone : m * a.c;
+            to[1] = tops[0][0][tid] + tops[0][1][tid];
+        }
+        if (s.begins && !s.ends && tid == 0) {
+            a.parts.heads[blockIdx.x] = PartHead{row0, rows, s.parts_after};
+        }
+    }
+}
+
 // The parts of cut blocks added up: workgroup (g, y) takes rows y, y + gridDim.y, ..
 // of the block that piece g began and did not end. 64 lanes hold 512 channels,
 // the four waves alternate parts.
@@ -682,17 +1104,26 @@ hipError_t launch(const PagedAttention& a, void* workspace, hipStream_t s) {
     // a scale of 0 weighs all keys alike, as one this small does, and leaves -infinity what it is
     t.c = std::max(std::fabs(a.scale) * 1.4426950408889634f, 1e-30f);
     char* w = static_cast<char*>(workspace);
+    const int m = paged_block_rows(a.max_added, a.heads);
     t.parts.heads = reinterpret_cast<PartHead*>(w);
     w += round_up(sizeof(PartHead) * kGrid, 256);
     t.parts.stats = reinterpret_cast<float*>(w);
-    w += round_up(sizeof(float) * 2 * kGrid * kRows16 * 2, 256);
+    w += round_up(sizeof(float) * 2 * kGrid * m * 2, 256);
     t.parts.sums = reinterpret_cast<float*>(w);
-    hipLaunchKernelGGL(paged_rows16_kernel<E>, dim3(kGrid), dim3(256), 0, s, t);
+    if (m == kRows16) {
+        hipLaunchKernelGGL(paged_rows16_kernel<E>, dim3(kGrid), dim3(256), 0, s, t);
+    } else {
+        hipLaunchKernelGGL(paged_rows64_kernel<E>, dim3(kGrid), dim3(256), 0, s, t);
+    }
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) {
         return err;
     }
-    hipLaunchKernelGGL((paged_join_kernel<E, kRows16>), dim3(kGrid, kRows16), dim3(256), 0, s, t);
+    if (m == kRows16) {
+        hipLaunchKernelGGL((paged_join_kernel<E, kRows16>), dim3(kGrid, kRows16), dim3(256), 0, s, t);
+    } else {
+        hipLaunchKernelGGL((paged_join_kernel<E, kRows64>), dim3(kGrid, 16), dim3(256), 0, s, t);
+    }
     return hipGetLastError();
 }
 
@@ -700,9 +1131,13 @@ hipError_t launch(const PagedAttention& a, void* workspace, hipStream_t s) {
 
 bool paged_tiled(int32_t rank, int32_t rope) { return rank == kRank && rope == kRope; }
 
-int64_t paged_workspace_bytes() {
-    return round_up(sizeof(PartHead) * kGrid, 256) + round_up(sizeof(float) * 2 * kGrid * kRows16 * 2, 256) +
-           static_cast<int64_t>(sizeof(float)) * 2 * kGrid * kRows16 * kRank;
+int paged_block_rows(int32_t max_added, int32_t heads) {
+    return static_cast<int64_t>(max_added) * heads <= kRows16 ? kRows16 : kRows64;
+}
+
+int64_t paged_workspace_bytes(int rows) {
+    return round_up(sizeof(PartHead) * kGrid, 256) + round_up(sizeof(float) * 2 * kGrid * rows * 2, 256) +
+           static_cast<int64_t>(sizeof(float)) * 2 * kGrid * rows * kRank;
 }
 
 hipError_t launch_paged_attention(const PagedAttention& a, void* workspace, hipStream_t s) {

@@ -20,9 +20,11 @@ struct ServeState {
     // Host memory that the kernels write when a table names a page outside the
     // pool: read without a copy once the stream has drained.
     uint32_t* error = nullptr;
-    // Sums of blocks whose keys are shared by several workgroups: a fixed size,
-    // so captured graphs keep their pointer. Steps on the stream take turns.
-    void* parts = nullptr;
+    // Sums of blocks whose keys are shared by several workgroups, for blocks of
+    // 16 and of 64 query rows (17 and 67 MB): of a fixed size each, so captured
+    // graphs keep their pointers. Steps on the stream take turns.
+    void* parts16 = nullptr;
+    void* parts64 = nullptr;
 };
 
 void serve_release(ServeState* st) {
@@ -30,7 +32,8 @@ void serve_release(ServeState* st) {
         return;
     }
     (void)hipHostFree(st->error);
-    (void)hipFree(st->parts);
+    (void)hipFree(st->parts16);
+    (void)hipFree(st->parts64);
     delete st;
 }
 
@@ -57,30 +60,47 @@ bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
     return x < y + b_bytes && y < x + a_bytes;
 }
 
-// The context's serving state, made at the first call that needs it (not while
-// its stream is being captured: the allocation would end the capture).
-int serve_state(lm_context* ctx, lm::ServeState** out) {
+// The context's serving state, and with `rows` the workspace of blocks of that
+// many query rows, made at the first call that needs them (not while the stream
+// is being captured: an allocation would end the capture).
+int serve_state(lm_context* ctx, int rows, lm::ServeState** out, void** parts) {
     lm::ServeState*& st = lm::context_serve(ctx);
+    *parts = nullptr;
+    void** const at = st == nullptr || rows == 0 ? nullptr : rows == 16 ? &st->parts16 : &st->parts64;
+    if (st != nullptr && (at == nullptr || *at != nullptr)) {
+        *out = st;
+        *parts = at == nullptr ? nullptr : *at;
+        return LM_OK;
+    }
+    const lm::ContextInfo info = lm::context_info(ctx);
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    LM_SERVE_HIP(hipStreamIsCapturing(info.stream, &capture));
+    if (capture != hipStreamCaptureStatusNone) {
+        return fail(LM_EINVAL, "the context's first paged attention of a kind cannot be captured: call it once before");
+    }
+    hipError_t err = hipSuccess;
     if (st == nullptr) {
-        const lm::ContextInfo info = lm::context_info(ctx);
-        hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
-        LM_SERVE_HIP(hipStreamIsCapturing(info.stream, &capture));
-        if (capture != hipStreamCaptureStatusNone) {
-            return fail(LM_EINVAL, "the context's first paged attention cannot be captured: call it once before");
-        }
         auto* made = new lm::ServeState();
-        hipError_t err = hipHostMalloc(reinterpret_cast<void**>(&made->error), sizeof(uint32_t),
-                                       hipHostMallocMapped | hipHostMallocCoherent);
+        err = hipHostMalloc(reinterpret_cast<void**>(&made->error), sizeof(uint32_t),
+                            hipHostMallocMapped | hipHostMallocCoherent);
         if (err == hipSuccess) {
-            err = hipMalloc(&made->parts, static_cast<size_t>(lm::paged_workspace_bytes()));
+            *made->error = 0;
+            st = made;
+        } else {
+            delete made;
         }
+    }
+    if (err == hipSuccess && rows != 0) {
+        void** const to = rows == 16 ? &st->parts16 : &st->parts64;
+        err = hipMalloc(to, static_cast<size_t>(lm::paged_workspace_bytes(rows)));
         if (err != hipSuccess) {
-            lm::serve_release(made);
-            (void)hipGetLastError();
-            return fail(LM_ENOMEM, std::string("serving state: ") + hipGetErrorString(err));
+            *to = nullptr;
         }
-        *made->error = 0;
-        st = made;
+        *parts = *to;
+    }
+    if (err != hipSuccess) {
+        (void)hipGetLastError();  // or the next launch would report it
+        return fail(LM_ENOMEM, std::string("paged attention's workspace: ") + hipGetErrorString(err));
     }
     *out = st;
     return LM_OK;
@@ -185,7 +205,8 @@ int lm_paged_attention(lm_context* ctx, const lm_paged_step* step, const void* q
         const lm::ContextInfo info = lm::context_info(ctx);
         LM_SERVE_HIP(hipSetDevice(info.device));
         lm::ServeState* st = nullptr;
-        rc = serve_state(ctx, &st);
+        void* parts = nullptr;
+        rc = serve_state(ctx, lm::paged_tiled(rank, rope) ? lm::paged_block_rows(s.max_added, heads) : 0, &st, &parts);
         if (rc != LM_OK) {
             return rc;
         }
@@ -201,7 +222,7 @@ int lm_paged_attention(lm_context* ctx, const lm_paged_step* step, const void* q
         a.rope = rope;
         a.max_added = s.max_added;
         a.scale = scale;
-        LM_SERVE_HIP(lm::launch_paged_attention(a, st->parts, info.stream));
+        LM_SERVE_HIP(lm::launch_paged_attention(a, parts, info.stream));
         return LM_OK;
     } catch (const std::bad_alloc&) {
         return fail(LM_ENOMEM, "host allocation failed");

@@ -57,10 +57,12 @@ struct PagedAttention {
     int32_t max_added;
     float scale;
 };
-// Whether rows of this width go to the matrix cores; they need a workspace of
+// Whether rows of this width go to the matrix cores, in blocks of
+// paged_block_rows() query rows (16 or 64) that need a workspace of
 // paged_workspace_bytes(), whatever the step.
 bool paged_tiled(int32_t rank, int32_t rope);
-int64_t paged_workspace_bytes();
+int paged_block_rows(int32_t max_added, int32_t heads);
+int64_t paged_workspace_bytes(int rows);
 hipError_t launch_paged_attention(const PagedAttention& a, void* workspace, hipStream_t s);
 
 struct SampleArgs {
