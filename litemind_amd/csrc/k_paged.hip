@@ -793,8 +793,8 @@ __global__ __launch_bounds__(256, 1) void paged_rows64_kernel(const TileArgs a) 
         // Between two barriers: context of tile t (stage u), scores of t + 1.
         const std::true_type yes;
         const std::false_type no;
-        // tile t's weights and t + 1 are in; passes on the reference
-        auto begin = [&](int32_t t, int u) {
+        // tile t's weights and tile t + 1 are in
+        auto arrive = [&](int32_t t, int u) {
             __builtin_amdgcn_sched_barrier(0);
             if (t + 2 < s.tile1) {
                 __builtin_amdgcn_s_waitcnt(0x0F70 | 9);
@@ -805,66 +805,82 @@ __global__ __launch_bounds__(256, 1) void paged_rows64_kernel(const TileArgs a) 
             if (t + 3 < s.tile1) {
                 issue(t + 3, ring[(u + 3) & 3]);
             }
-            const float(*const top)[kRows64] = tops[u & 1];
-            const float high = lane < rows ? fmaxf(top[0][lane], top[1][lane]) : kNone;
-            if (__any((high - m) * a.c > kSlack)) {
-                const float up = fmaxf(m, high);
-                const float alpha = up == kNone ? 1.0f : __builtin_amdgcn_exp2f((m - up) * a.c);
-                m = up;
+        };
+        // the largest score of row `lane` in the tile whose maxima are in `top`
+        auto largest = [&](const float (*top)[kRows64]) {
+            return lane < rows ? fmaxf(top[0][lane], top[1][lane]) : kNone;
+        };
+        auto follow = [&](float high, float* alpha) {
+            const float up = fmaxf(m, high);
+            *alpha = up == kNone ? 1.0f : __builtin_amdgcn_exp2f((m - up) * a.c);
+            m = up;
 #pragma unroll
-                for (int rb = 0; rb < 2; ++rb) {
-                    const float f = __shfl(alpha, 32 * rb + col32);
-#pragma unroll
-                    for (int ct = 0; ct < 4; ++ct) {
-                        o[rb][ct] *= f;
-                    }
-                }
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const int row = 32 * rh + 16 * b + col;
-                    l[b] *= __shfl(alpha, row);
-                    const float mine = __shfl(up, row);
-                    ref[b] = mine == kNone ? 0.0f : mine * a.c;
-                }
-                weigh(weights[u & 1], sum);
-                meet();
+            for (int b = 0; b < 2; ++b) {
+                const float mine = __shfl(up, 32 * rh + 16 * b + col);
+                ref[b] = mine == kNone ? 0.0f : mine * a.c;
             }
-            l[0] += sum[0];
-            l[1] += sum[1];
         };
         if (s.tile0 < s.tile1) {
-            __builtin_amdgcn_sched_barrier(0);
-            if (s.tile0 + 1 < s.tile1) {
-                __builtin_amdgcn_s_waitcnt(0x0F70 | 9);
-            } else {
-                __builtin_amdgcn_s_waitcnt(0x0F70);
-            }
-            meet();
-            if (s.tile0 + 2 < s.tile1) {
-                issue(s.tile0 + 2, ring[2]);
-            }
+            arrive(s.tile0 - 1, 3);
             products(yes, ring[0], no, nullptr, nullptr, no);
             mask(s.tile0);
             pass(tops[0]);
+            meet();
+            float alpha;
+            follow(largest(tops[0]), &alpha);
             weigh(weights[0], sum);
-            // tiles that all rows see, the next one too
+            // tiles up to here are seen by all rows, and the next one too
             const int32_t full = min(s.tile1 - 1, (all_see + 1) / kTile - 1);
             int32_t t = s.tile0;
-            for (; t + 4 <= full; t += 4) {
+            while (t < s.tile1) {
+                // A reference left behind, or a tile that rows may not see, is
+                // for the loop after this one: the sums are touched by products
+                // alone here, and stay in the registers that products use.
+                int late = 0;
+                float high = kNone;
+                for (; t + 4 <= full; t += 4) {
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    begin(t + u, u);
-                    products(yes, ring[(u + 1) & 3], yes, ring[u], weights[u & 1], no);
-                    pass(tops[(u + 1) & 1]);
-                    weigh(weights[(u + 1) & 1], sum);
+                    for (int u = 0; u < 4; ++u) {
+                        arrive(t + u, u);
+                        high = largest(tops[u & 1]);
+                        if (__builtin_expect(__any((high - m) * a.c > kSlack), 0)) {
+                            late = u + 1;
+                            break;
+                        }
+                        l[0] += sum[0];
+                        l[1] += sum[1];
+                        products(yes, ring[(u + 1) & 3], yes, ring[u], weights[u & 1], no);
+                        pass(tops[(u + 1) & 1]);
+                        weigh(weights[(u + 1) & 1], sum);
+                    }
+                    if (late != 0) {
+                        break;
+                    }
                 }
-            }
-            // the others
-            for (; t < s.tile1; t += 4) {
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    if (t + u < s.tile1) {
-                        begin(t + u, u);
+                    if (u + 1 >= late && t + u < s.tile1) {
+                        if (u + 1 != late) {
+                            arrive(t + u, u);
+                            high = largest(tops[u & 1]);
+                        }
+                        if (__any((high - m) * a.c > kSlack)) {
+                            follow(high, &alpha);
+#pragma unroll
+                            for (int rb = 0; rb < 2; ++rb) {
+                                const float f = __shfl(alpha, 32 * rb + col32);
+#pragma unroll
+                                for (int ct = 0; ct < 4; ++ct) {
+                                    o[rb][ct] *= f;
+                                }
+                            }
+                            l[0] *= __shfl(alpha, 32 * rh + col);
+                            l[1] *= __shfl(alpha, 32 * rh + 16 + col);
+                            weigh(weights[u & 1], sum);
+                            meet();
+                        }
+                        l[0] += sum[0];
+                        l[1] += sum[1];
                         if (t + u + 1 < s.tile1) {
                             products(yes, ring[(u + 1) & 3], no, nullptr, nullptr, no);
                             mask(t + u + 1);
@@ -876,6 +892,7 @@ __global__ __launch_bounds__(256, 1) void paged_rows64_kernel(const TileArgs a) 
                         }
                     }
                 }
+                t += 4;
             }
         }
         // the totals: the rows' parts of both key halves meet in `tops`
