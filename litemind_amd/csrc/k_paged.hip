@@ -12,10 +12,8 @@
 // tile by transposing LDS reads. Scores never leave the registers.
 //
 // Rows of 576 values (rank 512, rope 64: DeepSeek-V2's) go to the matrix cores,
-// in blocks of query rows of one request:
-//   few rows (paged_rows16_kernel): 16 rows, each wave on key tiles of its own
-//   many (paged_rows64_kernel): 64 rows, tiles and products shared by the waves
-// Any other widths take paged_any_kernel.
+// in blocks of 64 query rows of one request, or of 16 where no request has more
+// (paged_rows_kernel). Any other widths take paged_any_kernel.
 //
 // The blocks' key tiles are shared out evenly: the grid's workgroups cut the
 // line of all blocks' costs into equal pieces, found from the lengths on the
@@ -249,16 +247,21 @@ struct TileArgs {
     Parts parts;
 };
 
-// Where 16-byte unit u of row r lies in a tile in LDS. A 16-lane group of a key
-// read takes one unit of 16 rows, a transposing read two or four neighbouring
-// units of eight or four rows: with the unit's low three bits XORed by the
-// reversed bits of r / 2, and rows 8 units apart modulo the 16 that the banks
-// hold, all are free of conflicts.
-__device__ inline int swizzle(int r) {
-    const int k = (r >> 1) & 7;
-    return (k & 1) << 2 | (k & 2) | k >> 2;
+// A tile in LDS: per eight rows their 64 units of latent (16 bytes each), a row
+// after the other, then their eight units of rotary key. A load fills 64 units,
+// so a row's latent is one load and eight rotary keys are one. Units are XORed by
+// row so that LDS reads are free of bank conflicts: a 16-lane group of a key read
+// takes one unit of 16 rows; 32 lanes of a transposing read four neighbouring
+// units of four rows, or two of eight. Bits 2 and 3 come from the row within
+// four, bits 0 and 1 from the fours; rotary rows are 8 units apart.
+constexpr int kEightBytes = 8 * kRowBytes;  // 9216
+__device__ inline int swizzle(int r) { return (r & 3) << 2 | (r >> 2 & 2) | (r >> 2 & 1); }
+__device__ inline int latent_at(int r, int u) {
+    return (r >> 3) * kEightBytes + (r & 7) * 1024 + ((u ^ swizzle(r)) << 4);
 }
-__device__ inline int unit_at(int r, int u) { return r * kRowBytes + ((u ^ swizzle(r)) << 4); }
+__device__ inline int rotary_at(int r, int u) {
+    return (r >> 3) * kEightBytes + 8192 + (r & 7) * 128 + ((u ^ (r >> 1 & 7)) << 4);
+}
 
 // The pages of one request's keys, 64 table entries at a time in the lanes.
 struct PageWalk {
@@ -296,259 +299,33 @@ __device__ inline int here(int v) {
     return v;
 }
 
-// ---- few rows ----
-// 16 query rows, four waves. A wave takes every fourth tile of the segment into
-// a buffer of its own, without a barrier: S^T of 2 x 18 and out^T of 32 products
-// of 16 x 16 x 32 a tile. The waves' sums meet in LDS at the segment's end.
-constexpr int kRows16 = 16;
-
-template <class E>
-__global__ __launch_bounds__(256) void paged_rows16_kernel(const TileArgs a) {
-    using H = Half<E>;
-    typedef typename H::vec8 vec8;
-    __shared__ __align__(16) char tiles[4][kTileBytes];
-    __shared__ float stats[4][kRows16][2];
-    __shared__ int64_t scratch[8];
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int col = lane & 15, grp = lane >> 4;
-    Walk walk;
-    walk.sh = Shares{a.heads, kRows16};
-    walk.p = find_piece(a.view, walk.sh, blockIdx.x, scratch);
-    if (tid == 0) {
-        a.parts.heads[blockIdx.x].rows = 0;
-    }
-    if (walk.p.begin >= walk.p.end) {
-        return;
-    }
-    walk.start(a.view);
-    char* const tile = tiles[wave];
-    // Loads: 16 rows are 18 loads of 64 units; load j's lane takes position
-    // 64 j + lane, row and unit as below.
-    auto place = [&](int j, int& row, int& unit) {
-        const int at = 64 * j + lane;
-        row = at / kUnits;
-        unit = (at - row * kUnits) ^ swizzle(row);
-    };
-    unsigned from[18];
-#pragma unroll
-    for (int j = 0; j < 18; ++j) {
-        int row, unit;
-        place(j, row, unit);
-        from[j] = static_cast<unsigned>(row * kRowBytes + unit * 16);
-    }
-    Segment s;
-    while (walk.next(a.view, s)) {
-        const int64_t row0 = static_cast<int64_t>(s.req.first) * a.heads + static_cast<int64_t>(s.block) * kRows16;
-        const int rows = min(kRows16, s.req.added * a.heads - s.block * kRows16);
-        const int32_t keys = s.req.cached + s.req.added;
-        // this lane's query row; the last key that it sees, and that all rows see
-        const int own = min(col, rows - 1);
-        const int32_t sees = s.req.cached + (s.block * kRows16 + own) / a.heads;
-        const int32_t all_see = s.req.cached + s.block * kRows16 / a.heads;
-        vec8 q[18];
-        {
-            const E* const from_q = static_cast<const E*>(a.q) + (row0 + own) * kWidth + 8 * grp;
-#pragma unroll
-            for (int ks = 0; ks < 18; ++ks) {
-                q[ks] = *reinterpret_cast<const vec8*>(from_q + 32 * ks);
-            }
-            if (a.negative) {
-#pragma unroll
-                for (int ks = 0; ks < 18; ++ks) {
-                    q[ks] = -q[ks];
-                }
-            }
-        }
-        PageWalk pages;
-        pages.start(a.view, s.request);
-        f32x4 o[32] = {};
-        float m = kNone, l = 0.0f;
-        for (int32_t t = s.tile0 + wave; t < s.tile1; t += 4) {
-            // the tile before has been read
-            __builtin_amdgcn_s_waitcnt(0xc07f);
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int32_t key = t * kTile + 16 * half, last = keys - 1;
-                const int32_t first = min(key, last & ~15);
-                const char* const base =
-                    static_cast<const char*>(a.pool) + pages.at(a.view, a.page_mul, first) * kRowBytes;
-                const __amdgpu_buffer_rsrc_t res =
-                    __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 16 * kRowBytes, kBufferWord3);
-                char* const to = tile + half * 16 * kRowBytes;
-                if (key + 15 <= last) {
-#pragma unroll
-                    for (int j = 0; j < 18; ++j) {
-                        buffer_lds16(res, to + j * 1024, from[j], 0);
-                    }
-                } else {  // rows past the last key: the last key's once more
-#pragma unroll
-                    for (int j = 0; j < 18; ++j) {
-                        int row, unit;
-                        place(j, row, unit);
-                        const int r = min(key + row, last) - first;
-                        buffer_lds16(res, to + j * 1024, static_cast<unsigned>(r * kRowBytes + unit * 16), 0);
-                    }
-                }
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            __builtin_amdgcn_s_waitcnt(0x0070 | 0x0F00);  // vmcnt(0)
-            __builtin_amdgcn_sched_barrier(0);
-            f32x4 sc[2] = {};
-#pragma unroll
-            for (int ks = 0; ks < 18; ++ks) {
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb) {
-                    const vec8 k = *reinterpret_cast<const vec8*>(tile + unit_at(16 * kb + col, 4 * ks + grp));
-                    sc[kb] = H::mfma16(k, q[ks], sc[kb]);
-                }
-            }
-            // register e of sc[kb]: key 32 t + 16 kb + 4 grp + e
-            bool guard = false;
-            uint32_t bad = 0;  // bit 4 kb + e: a key that some row must not see is not finite
-            if (t * kTile + kTile - 1 > all_see) {
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float v = sc[kb][e];
-                        const uint64_t odd = __ballot(!(v - v == 0.0f));
-                        bad |= (odd >> (16 * grp) & 0xffff) != 0 ? 1u << (4 * kb + e) : 0u;
-                        if (t * kTile + 16 * kb + 4 * grp + e > sees) {
-                            sc[kb][e] = kNone;
-                        }
-                    }
-                }
-                guard = __any(bad != 0);
-            }
-            float top = kNone;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                top = fmaxf(top, fmaxf(sc[0][e], sc[1][e]));
-            }
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            const float up = fmaxf(m, top);
-            if (__any(up > m)) {
-                const float alpha = up == kNone ? 1.0f : __builtin_amdgcn_exp2f((m - up) * a.c);
-                l *= alpha;
-#pragma unroll
-                for (int ct = 0; ct < 32; ++ct) {
-                    o[ct] *= alpha;
-                }
-                m = up;
-            }
-            const float mc = m == kNone ? 0.0f : m * a.c;
-            vec8 p;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i / 4][i % 4], a.c, -mc));
-                l += w;
-                p[i] = static_cast<E>(w);
-            }
-            const int vrow = 4 * grp + (col >> 2), vlow = (col & 3) >> 1, vbyte = (col & 1) * 8;
-#pragma unroll
-            for (int ct = 0; ct < 32; ++ct) {
-                short8v v;
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb) {
-                    const short4v part = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (lds_short4*)(tile + unit_at(16 * kb + vrow, 2 * ct + vlow) + vbyte));
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        v[4 * kb + e] = part[e];
-                    }
-                }
-                if (guard) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        v[i] = (bad >> i & 1) != 0 ? short{0} : v[i];
-                    }
-                }
-                o[ct] = H::mfma16(__builtin_bit_cast(vec8, v), p, o[ct]);
-            }
-        }
-        l += __shfl_xor(l, 16);
-        l += __shfl_xor(l, 32);
-        // join the waves: o[ct] register e is channel 16 ct + 4 grp + e of row `col`
-        __syncthreads();
-        float* const mine = reinterpret_cast<float*>(tile);
-#pragma unroll
-        for (int ct = 0; ct < 32; ++ct) {
-            *reinterpret_cast<f32x4*>(mine + col * kRank + ((16 * ct + 4 * grp) ^ (col << 2 & 28))) = o[ct];
-        }
-        if (grp == 0) {
-            stats[wave][col][0] = m == kNone ? kNone : m * a.c;
-            stats[wave][col][1] = l;
-        }
-        __syncthreads();
-        const bool whole = s.begins && s.ends;
-        const int slot = 2 * static_cast<int>(blockIdx.x) + (s.begins ? 1 : 0);
-        for (int i = tid; i < rows * (kRank / 4); i += 256) {
-            const int r = i / (kRank / 4), ch = i % (kRank / 4) * 4;
-            float high = kNone, total = 0.0f;
-            for (int w = 0; w < 4; ++w) {
-                high = fmaxf(high, stats[w][r][0]);
-            }
-            f32x4 sum = {};
-            for (int w = 0; w < 4; ++w) {
-                const float weight = stats[w][r][0] == kNone ? 0.0f : __builtin_amdgcn_exp2f(stats[w][r][0] - high);
-                total = __builtin_fmaf(weight, stats[w][r][1], total);
-                const f32x4 v = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(tiles[w]) + r * kRank +
-                                                                (ch ^ (r << 2 & 28)));
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    sum[e] = __builtin_fmaf(weight, v[e], sum[e]);
-                }
-            }
-            if (whole) {
-                typename H::vec4 out;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    out[e] = static_cast<E>(sum[e] / total);
-                }
-                *reinterpret_cast<typename H::vec4*>(static_cast<E*>(a.out) + (row0 + r) * kRank + ch) = out;
-            } else {
-                *reinterpret_cast<f32x4*>(a.parts.sums + (static_cast<int64_t>(slot) * kRows16 + r) * kRank + ch) = sum;
-                if (ch == 0) {
-                    float* const st = a.parts.stats + (static_cast<int64_t>(slot) * kRows16 + r) * 2;
-                    st[0] = high;
-                    st[1] = total;
-                }
-            }
-        }
-        if (s.begins && !s.ends && tid == 0) {
-            a.parts.heads[blockIdx.x] = PartHead{row0, rows, s.parts_after};
-        }
-        __syncthreads();
-    }
-}
-
-// ---- many rows ----
-// 64 query rows, four waves. The waves share tiles of 32 keys, which come straight
+// ---- blocks of query rows ----
+// M = 64 rows, four waves. The waves share tiles of 32 keys, which come straight
 // to LDS four deep, and split each product differently:
 //   S^T   wave (kh, rh): keys 16 kh .. + 15 for rows 32 rh .. + 31; its queries
 //         stay in 144 registers, 36 products of 16 x 16 x 32 a tile
 //   out^T channels 128 w .. + 127 of wave w for all rows; 128 registers of sums,
 //         16 products of 32 x 32 x 16 a tile
-// The weights pass through LDS. One barrier a tile: between two, the waves run
-// the scores of tile t + 1 and the context of tile t, which do not depend on each
-// other, so either's latencies are filled by the other's products. 32 rows with
-// all 512 channels per wave, without the exchange, would take 256 + 16 registers
-// of sums, and the matrix cores' results go to 256.
+// (M = 16: keys 16 kh .. for all rows, on both rh; 32 registers, 8 products of
+// 16 x 16 x 32.) The weights pass through LDS. One barrier a tile: between two,
+// the waves run the scores of tile t + 1 and the context of tile t, which do not
+// depend on each other, and the weights of t + 1 beside the last of the context.
+// A wave with 32 rows and all channels would need no exchange, but 256 + 16
+// registers of sums, where the matrix cores' results go to 256.
 //
-// The weights' reference m, one per row, has to be the same for all waves: it
-// follows the rows' maxima one barrier late, and only where a row passed it by
-// more than 2^kSlack, which keeps the weights in 16 bits' range; the tile's
-// weights are then made anew. (fp32 sums do not mind the factor.)
-constexpr int kRows64 = 64;
+// The weights' reference m, one per row, has to be the same for all waves: it is
+// moved only where a row's scores pass it by more than kSlack (in powers of
+// two), which a wave tells the others at the next barrier; the tile's weights
+// are then made anew. fp32 sums do not mind the factor, and 16-bit weights up to
+// 2^kSlack round as those up to 1 do.
 constexpr float kSlack = 10.0f;
+constexpr float kUnset = -1e30f;  // reference of a row without a score yet: any finite one passes it
 
 // Non-finite values as 0: keys that some row must not see weigh 0 there, and 0
 // times NaN or infinity is not 0. (Rows that see such a key have a NaN weight.)
 template <class E>
 __device__ inline short8v finite_or_zero(short8v v) {
-    constexpr short kExponent = sizeof(E) == 2 && __is_same(E, bf16) ? 0x7f80 : 0x7c00;
+    constexpr short kExponent = std::is_same_v<E, bf16> ? 0x7f80 : 0x7c00;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         v[e] = (v[e] & kExponent) == kExponent ? short{0} : v[e];
@@ -556,24 +333,30 @@ __device__ inline short8v finite_or_zero(short8v v) {
     return v;
 }
 
-template <class E>
-__global__ __launch_bounds__(256, 1) void paged_rows64_kernel(const TileArgs a) {
+template <class E, int M>
+__global__ __launch_bounds__(256, 1) void paged_rows_kernel(const TileArgs a) {
+    static_assert(M == 64 || M == 16);
     using H = Half<E>;
     typedef typename H::vec8 vec8;
     typedef typename H::vec4 vec4;
+    constexpr bool kWide = M == 64;
+    constexpr int NB = kWide ? 2 : 1;        // blocks of 16 rows in a wave's scores
+    constexpr int NO = 8;                    // sums: [2][4] of 32 x 32, or [8] of 16 x 16
+    using Sum = std::conditional_t<kWide, f32x16, f32x4>;
     // one array per stage: the compiler tracks loads to LDS per array
     __shared__ __align__(16) char s0[kTileBytes], s1[kTileBytes], s2[kTileBytes], s3[kTileBytes];
-    __shared__ __align__(16) char weights[2][kRows64 * kTile * 2];
-    __shared__ float tops[2][2][kRows64];
+    __shared__ __align__(16) char weights[2][M * kTile * 2];
+    __shared__ float tops[2][M];
+    __shared__ int late_flags[4];
     __shared__ int64_t scratch[8];
     char* const ring[4] = {s0, s1, s2, s3};
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int kh = wave & 1, rh = wave >> 1;
+    const int kh = wave & 1, rh = kWide ? wave >> 1 : 0;
     const int col = lane & 15, grp = lane >> 4;     // of 16 x 16 products
     const int col32 = lane & 31, half = lane >> 5;  // of 32 x 32 products
     Walk walk;
-    walk.sh = Shares{a.heads, kRows64};
+    walk.sh = Shares{a.heads, M};
     walk.p = find_piece(a.view, walk.sh, blockIdx.x, scratch);
     if (tid == 0) {
         a.parts.heads[blockIdx.x].rows = 0;
@@ -582,47 +365,87 @@ __global__ __launch_bounds__(256, 1) void paged_rows64_kernel(const TileArgs a) 
         return;
     }
     walk.start(a.view);
-    // The wave loads rows 8 wave .. + 7 of a tile, 9 loads of 64 units.
-    auto place = [&](int j, int of, int& row, int& unit) {
-        const int at = 64 * j + of;
-        const int r = at / kUnits;
-        row = 8 * (wave & 1) + r;  // of 16
-        unit = (at - r * kUnits) ^ swizzle(row);
-    };
-    unsigned from[9];
-#pragma unroll
-    for (int j = 0; j < 9; ++j) {
-        int row, unit;
-        place(j, lane, row, unit);
-        from[j] = static_cast<unsigned>(row * kRowBytes + unit * 16);
-    }
-    // Where the lane's reads of a tile begin; the rest is constant offsets, since
-    // the swizzle changes the low three bits of a unit only.
-    int key_at[2], value_at[2][2], weight_from[2], weight_to[2];
+    // The wave loads rows 8 wave .. + 7 of a tile: eight latents, and their rotary
+    // keys in one load, of which this lane takes
+    const int rotary_from = (lane >> 3) * kRowBytes + 1024 + (((lane & 7) ^ ((8 * wave + (lane >> 3)) >> 1 & 7)) << 4);
+    // Where the lane's reads of a tile begin. The scores' k-step ks reads latent
+    // unit 4 ks + grp, bits 2 and 3 of which the swizzle changes: ks & 3 is XORed
+    // in, the rest is a constant offset; so are channel tiles below. A row of
+    // weights is 64 bytes, its four units XORed by row / 4.
+    const int key_at = latent_at(16 * kh + col, grp);
+    const int rotary_key_at = rotary_at(16 * kh + col, grp);
+    int value_at[2], weight_from[NB], weight_to[NB];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        key_at[i] = unit_at(16 * kh + col, 4 * i + grp);
-        const int row = 32 * i + col32, to = 32 * rh + 16 * i + col;
-        weight_from[i] = row * 64 + ((half ^ (row >> 2 & 1)) * 16 | (row >> 3 & 1) * 32);
-        weight_to[i] = to * 64 + ((2 * kh + (grp >> 1)) ^ (to >> 2 & 3)) * 16 + (grp & 1) * 8;
+        // the first or second four of the lane's eight keys
+        const int r = 8 * (kWide ? half : grp) + 4 * i + ((lane & 15) >> 2);
+        const int u = kWide ? 2 * (lane >> 4 & 1) + ((lane & 3) >> 1) : (lane & 3) >> 1;
+        value_at[i] = latent_at(r, u) + (lane & 1) * 8 + wave * 256;
+    }
 #pragma unroll
-        for (int odd = 0; odd < 2; ++odd) {
-            const int r = 8 * half + 4 * i + ((lane & 15) >> 2);
-            value_at[i][odd] = unit_at(r, 4 * odd + 2 * (lane >> 4 & 1) + ((lane & 3) >> 1)) + (lane & 1) * 8 +
-                               wave * 256;
-        }
+    for (int b = 0; b < NB; ++b) {
+        const int row = kWide ? 32 * b + col32 : col, to = 32 * rh + 16 * b + col;
+        weight_from[b] = row * 64 + (((kWide ? half : grp) ^ (row >> 2 & 3)) << 4);
+        weight_to[b] = to * 64 + (((2 * kh + (grp >> 1)) ^ (to >> 2 & 3)) << 4) + (grp & 1) * 8;
     }
     Segment s;
     while (walk.next(a.view, s)) {
-        const int in_request = s.block * kRows64;  // the block's first row
+        const int in_request = s.block * M;  // the block's first row
         const int64_t row0 = static_cast<int64_t>(s.req.first) * a.heads + in_request;
-        const int rows = min(kRows64, s.req.added * a.heads - in_request);
+        const int rows = min(M, s.req.added * a.heads - in_request);
         const int32_t last = s.req.cached + s.req.added - 1;
         const int32_t all_see = s.req.cached + in_request / a.heads;
-        int32_t sees[2];
-        vec8 q[2][18];
+        PageWalk pages;
+        pages.start(a.view, s.request);
+        auto issue = [&](int32_t t, char* to) {
+            const int32_t key = t * kTile + 16 * (wave >> 1);
+            const int32_t first = min(key, last & ~15);
+            const char* const base =
+                static_cast<const char*>(a.pool) + pages.at(a.view, a.page_mul, first) * kRowBytes;
+            const __amdgpu_buffer_rsrc_t res =
+                __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 16 * kRowBytes, kBufferWord3);
+            to += wave * kEightBytes;
+            const int eight = 8 * (wave & 1), of = here(lane * 16);
+            if (key + 15 <= last) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
+                for (int r = 0; r < 8; ++r) {
+                    buffer_lds16(res, to + r * 1024, static_cast<unsigned>(of ^ (swizzle(r) | (wave & 1) << 1) << 4),
+                                 static_cast<unsigned>((eight + r) * kRowBytes));
+                }
+                buffer_lds16(res, to + 8192, static_cast<unsigned>(rotary_from),
+                             static_cast<unsigned>(eight * kRowBytes));
+            } else {  // rows past the last key: the last key's once more
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    buffer_lds16(res, to + r * 1024, static_cast<unsigned>(of ^ (swizzle(r) | (wave & 1) << 1) << 4),
+                                 static_cast<unsigned>((min(key + eight + r, last) - first) * kRowBytes));
+                }
+                const int r = of >> 7;  // lane / 8
+                buffer_lds16(res, to + 8192,
+                             static_cast<unsigned>(rotary_from + (min(key + eight + r, last) - first - r) * kRowBytes),
+                             0);
+            }
+        };
+        auto meet = [] {
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_waitcnt(0xc07f);  // this wave's LDS writes are done
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        __syncthreads();  // the block before is done with LDS
+        if (tid < 4) {
+            late_flags[tid] = 0;
+        }
+        if (s.tile0 < s.tile1) {
+            issue(s.tile0, ring[0]);
+        }
+        if (s.tile0 + 1 < s.tile1) {
+            issue(s.tile0 + 1, ring[1]);
+        }
+        int32_t sees[NB];
+        vec8 q[NB][18];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
             const int own = min(32 * rh + 16 * b + col, rows - 1);
             sees[b] = s.req.cached + (in_request + own) / a.heads;
             const E* const from_q = static_cast<const E*>(a.q) + (row0 + own) * kWidth + 8 * grp;
@@ -633,116 +456,154 @@ __global__ __launch_bounds__(256, 1) void paged_rows64_kernel(const TileArgs a) 
         }
         if (a.negative) {
 #pragma unroll
-            for (int ks = 0; ks < 18; ++ks) {
-                q[0][ks] = -q[0][ks];
-                q[1][ks] = -q[1][ks];
+            for (int b = 0; b < NB; ++b) {
+#pragma unroll
+                for (int ks = 0; ks < 18; ++ks) {
+                    q[b][ks] = -q[b][ks];
+                }
             }
         }
-        PageWalk pages;
-        pages.start(a.view, s.request);
-        auto issue = [&](int32_t t, char* to) {
-            const int32_t key = t * kTile + 16 * (wave >> 1);
-            const int32_t first = min(key, last & ~15);
-            const char* const base =
-                static_cast<const char*>(a.pool) + pages.at(a.view, a.page_mul, first) * kRowBytes;
-            const __amdgpu_buffer_rsrc_t res =
-                __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 16 * kRowBytes, kBufferWord3);
-            to += 8 * wave * kRowBytes;
-            if (key + 15 <= last) {
+        Sum o[NO] = {};
+        f32x4 sc[NB];             // scores of the newest tile
+        float m = kNone;          // reference of row `lane`, the same in every wave
+        float ref[NB], l[NB], sum[NB];  // of this lane's rows: reference times c, total, the newest tile's
 #pragma unroll
-                for (int j = 0; j < 9; ++j) {
-                    buffer_lds16(res, to + j * 1024, from[j], 0);
+        for (int b = 0; b < NB; ++b) {
+            ref[b] = kUnset;
+            l[b] = sum[b] = 0.0f;
+        }
+        // the newest tile's weights; tells whether a score passes the reference
+        auto weigh = [&](char* wt) {
+            float over = kNone;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                vec4 p;
+                float w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float x = __builtin_fmaf(sc[b][e], a.c, -ref[b]);
+                    over = fmaxf(over, x);
+                    w[e] = __builtin_amdgcn_exp2f(x);
+                    p[e] = static_cast<E>(w[e]);
                 }
-            } else {  // rows past the last key: the last key's once more
-                const int of = here(lane);
-#pragma unroll
-                for (int j = 0; j < 9; ++j) {
-                    int row, unit;
-                    place(j, of, row, unit);
-                    const int r = min(key + row, last) - first;
-                    buffer_lds16(res, to + j * 1024, static_cast<unsigned>(r * kRowBytes + unit * 16), 0);
+                sum[b] = (w[0] + w[1]) + (w[2] + w[3]);
+                *reinterpret_cast<vec4*>(wt + weight_to[b]) = p;
+            }
+            return over;
+        };
+        auto tell = [&](float over, int u) {
+            if (__builtin_expect(__any(over > kSlack), 0)) {
+                if (lane == 0) {
+                    late_flags[u] = 1;
                 }
             }
         };
-        f32x16 o[2][4] = {};
-        f32x4 sc[2];             // scores of the newest tile
-        float m = kNone;         // reference of row `lane`, the same in every wave
-        float ref[2];            // times c, of this lane's rows of the scores
-        float l[2] = {0.0f, 0.0f};
-        ref[0] = ref[1] = 0.0f;
-        // The products of an interval in eight steps, each step's operands read
-        // during the one before: k-steps 9 i / 4 .. of the scores of the tile in
-        // `next`, channel tile i % 4 of keys 16 (i / 4) .. of the context of the
-        // tile in `now`.
+        // The products of an interval: scores of the tile in `next` (S), context of
+        // the tile in `now` (C), each step's operands read during the one before.
+        // The scores take the first half, so that `weights_of` runs beside the
+        // second half of the context.
         auto products = [&](auto with_scores, const char* next, auto with_context, const char* now, const char* wt,
-                            auto sanitize) {
+                            bool sanitize, auto middle, auto weights_of) {
             constexpr bool S = decltype(with_scores)::value, C = decltype(with_context)::value;
-            vec8 kf[2][3], vf[2], pf[2][2];
-            const int k_at[2] = {here(key_at[0]), here(key_at[1])};
-            const int v_at[2][2] = {{here(value_at[0][0]), here(value_at[0][1])},
-                                    {here(value_at[1][0]), here(value_at[1][1])}};
+            // step i: k-steps 3 i .. + 2 of the scores (i < 6), part `unit(i)` of the context
+            auto unit = [](int i) { return i < 5 ? i : i == 5 ? -1 : i - 1; };
+            vec8 kf[2][3], vf[2], pf[NB];
+            const int k_at = here(key_at), r_at = here(rotary_key_at);
+            const int v_at[2] = {here(value_at[0]), here(value_at[1])};
             auto read = [&](int i) {
-                if constexpr (S) {
+                if (S && i < 6) {
 #pragma unroll
-                    for (int ks = 9 * i / 4; ks < 9 * (i + 1) / 4; ++ks) {
-                        kf[i & 1][ks - 9 * i / 4] =
-                            *reinterpret_cast<const vec8*>(next + k_at[ks & 1] + (ks >> 1) * 128);
+                    for (int k = 0; k < 3; ++k) {
+                        const int ks = 3 * i + k;
+                        kf[i & 1][k] = *reinterpret_cast<const vec8*>(
+                            next + (ks < 16 ? (k_at ^ (ks & 3) << 6) + (ks >> 2) * 256 : r_at ^ (ks & 1) << 6));
                     }
                 }
-                if constexpr (C) {
-                    const int st = i / 4, ct = i % 4;
-                    if (ct == 0) {
-#pragma unroll
-                        for (int rb = 0; rb < 2; ++rb) {
-                            pf[st][rb] = *reinterpret_cast<const vec8*>(wt + (weight_from[rb] ^ st * 32));
-                        }
-                    }
+                const int n = unit(i);
+                if (C && n >= 0) {
+                    // M = 64: keys 16 st .. + 15, channels 32 ct ..; M = 16: all keys, channels 16 ct ..
+                    const int st = kWide ? n / 4 : 0, ct = kWide ? n % 4 : n;
                     short8v v;
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        const short4v part = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (lds_short4*)(now + v_at[k][ct & 1] + st * 16 * kRowBytes + (ct >> 1) * 128));
+                        // a channel tile is four units (M = 16: two), a wave's channels 16
+                        const int from_here =
+                            kWide ? (v_at[k] ^ ct << 6) + st * 2 * kEightBytes : v_at[k] ^ ct << 5;
+                        const short4v part = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(now + from_here));
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             v[4 * k + e] = part[e];
                         }
                     }
-                    vf[i & 1] = __builtin_bit_cast(vec8, v);
+                    vf[n & 1] = __builtin_bit_cast(vec8, v);
+                }
+            };
+            auto read_weights = [&](int st) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    pf[b] = *reinterpret_cast<const vec8*>(wt + (weight_from[b] ^ st * 32));
                 }
             };
             if constexpr (S) {
-                sc[0] = sc[1] = f32x4{};
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    sc[b] = f32x4{};
+                }
+            }
+            if constexpr (C) {
+                read_weights(0);
             }
             read(0);
+            middle();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (i < 7) {
+            for (int i = 0; i < 9; ++i) {
+                if (i < 8) {
                     read(i + 1);
                 }
-                __builtin_amdgcn_sched_barrier(0);
-                if constexpr (C) {
-                    vec8 f = vf[i & 1];
-                    if constexpr (decltype(sanitize)::value) {
+                if (i <= 6) {
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                const int n = unit(i);
+                if (C && n >= 0) {
+                    vec8 f = vf[n & 1];
+                    if (sanitize) {
                         f = __builtin_bit_cast(vec8, finite_or_zero<E>(__builtin_bit_cast(short8v, f)));
                     }
-                    o[0][i % 4] = H::mfma32(f, pf[i / 4][0], o[0][i % 4]);
-                    o[1][i % 4] = H::mfma32(f, pf[i / 4][1], o[1][i % 4]);
-                }
-                if constexpr (S) {
-#pragma unroll
-                    for (int ks = 9 * i / 4; ks < 9 * (i + 1) / 4; ++ks) {
-                        const vec8 k = kf[i & 1][ks - 9 * i / 4];
-                        sc[0] = H::mfma16(k, q[0][ks], sc[0]);
-                        sc[1] = H::mfma16(k, q[1][ks], sc[1]);
+                    if constexpr (kWide) {
+                        o[n % 4] = H::mfma32(f, pf[0], o[n % 4]);
+                        o[4 + n % 4] = H::mfma32(f, pf[NB - 1], o[4 + n % 4]);
+                    } else {
+                        o[n] = H::mfma16(f, pf[0], o[n]);
+                    }
+                    if (kWide && n == 3) {
+                        read_weights(1);
                     }
                 }
-                __builtin_amdgcn_sched_barrier(0);
+                if (S && i < 6) {
+#pragma unroll
+                    for (int k = 0; k < 3; ++k) {
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) {
+                            sc[b] = H::mfma16(kf[i & 1][k], q[b][3 * i + k], sc[b]);
+                        }
+                    }
+                }
+                if (i < 6) {
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if (i == 6) {
+                    weights_of();
+                }
             }
+            __builtin_amdgcn_sched_barrier(0);
         };
+        const std::true_type yes;
+        const std::false_type no;
+        const auto nothing = [] {};
         auto mask = [&](int32_t t) {
             if (t * kTile + kTile - 1 > all_see) {
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
+                for (int b = 0; b < NB; ++b) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         sc[b][e] = t * kTile + 16 * kh + 4 * grp + e > sees[b] ? kNone : sc[b][e];
@@ -750,51 +611,32 @@ __global__ __launch_bounds__(256, 1) void paged_rows64_kernel(const TileArgs a) 
                 }
             }
         };
-        // the rows' maxima of the newest tile
-        auto pass = [&](float (*top)[kRows64]) {
+        // moves the reference to the rows' largest scores of the newest tile;
+        // returns the factor of row `lane`'s sums so far
+        auto follow = [&] {
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
+            for (int b = 0; b < NB; ++b) {
                 float high = fmaxf(fmaxf(sc[b][0], sc[b][1]), fmaxf(sc[b][2], sc[b][3]));
                 high = fmaxf(high, __shfl_xor(high, 16));
                 high = fmaxf(high, __shfl_xor(high, 32));
                 if (grp == 0) {
-                    top[kh][32 * rh + 16 * b + col] = high;
+                    tops[kh][32 * rh + 16 * b + col] = high;
                 }
             }
-        };
-        auto weigh = [&](char* wt, float (&sum)[2]) {
+            meet();
+            const int row = min(lane, rows - 1);  // (rows past the last are the last once more)
+            const float up = fmaxf(m, fmaxf(tops[0][row], tops[1][row]));
+            const float alpha = up == kNone ? 1.0f : __builtin_amdgcn_exp2f((m - up) * a.c);
+            m = up;
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                vec4 p;
-                sum[b] = 0.0f;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][e], a.c, -ref[b]));
-                    sum[b] += w;
-                    p[e] = static_cast<E>(w);
-                }
-                *reinterpret_cast<vec4*>(wt + weight_to[b]) = p;
+            for (int b = 0; b < NB; ++b) {
+                const float mine = __shfl(up, 32 * rh + 16 * b + col);
+                ref[b] = mine == kNone ? kUnset : mine * a.c;
             }
+            return alpha;
         };
-        auto meet = [] {
-            __builtin_amdgcn_sched_barrier(0);
-            __builtin_amdgcn_s_waitcnt(0xc07f);  // the weights are written
-            __builtin_amdgcn_s_barrier();
-            __builtin_amdgcn_sched_barrier(0);
-        };
-        __syncthreads();  // the block before is done with the ring
-        if (s.tile0 < s.tile1) {
-            issue(s.tile0, ring[0]);
-        }
-        if (s.tile0 + 1 < s.tile1) {
-            issue(s.tile0 + 1, ring[1]);
-        }
-        float sum[2] = {0.0f, 0.0f};  // of the newest tile's weights
-        // Between two barriers: context of tile t (stage u), scores of t + 1.
-        const std::true_type yes;
-        const std::false_type no;
         // tile t's weights and tile t + 1 are in
-        auto arrive = [&](int32_t t, int u) {
+        auto arrive = [&](int32_t t) {
             __builtin_amdgcn_sched_barrier(0);
             if (t + 2 < s.tile1) {
                 __builtin_amdgcn_s_waitcnt(0x0F70 | 9);
@@ -802,33 +644,16 @@ __global__ __launch_bounds__(256, 1) void paged_rows64_kernel(const TileArgs a) 
                 __builtin_amdgcn_s_waitcnt(0x0F70);
             }
             meet();
-            if (t + 3 < s.tile1) {
-                issue(t + 3, ring[(u + 3) & 3]);
-            }
-        };
-        // the largest score of row `lane` in the tile whose maxima are in `top`
-        auto largest = [&](const float (*top)[kRows64]) {
-            return lane < rows ? fmaxf(top[0][lane], top[1][lane]) : kNone;
-        };
-        auto follow = [&](float high, float* alpha) {
-            const float up = fmaxf(m, high);
-            *alpha = up == kNone ? 1.0f : __builtin_amdgcn_exp2f((m - up) * a.c);
-            m = up;
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const float mine = __shfl(up, 32 * rh + 16 * b + col);
-                ref[b] = mine == kNone ? 0.0f : mine * a.c;
-            }
         };
         if (s.tile0 < s.tile1) {
-            arrive(s.tile0 - 1, 3);
-            products(yes, ring[0], no, nullptr, nullptr, no);
+            arrive(s.tile0 - 1);
+            if (s.tile0 + 2 < s.tile1) {
+                issue(s.tile0 + 2, ring[2]);
+            }
+            products(yes, ring[0], no, nullptr, nullptr, false, nothing, nothing);
             mask(s.tile0);
-            pass(tops[0]);
-            meet();
-            float alpha;
-            follow(largest(tops[0]), &alpha);
-            weigh(weights[0], sum);
+            follow();
+            weigh(weights[0]);
             // tiles up to here are seen by all rows, and the next one too
             const int32_t full = min(s.tile1 - 1, (all_see + 1) / kTile - 1);
             int32_t t = s.tile0;
@@ -836,59 +661,82 @@ __global__ __launch_bounds__(256, 1) void paged_rows64_kernel(const TileArgs a) 
                 // A reference left behind, or a tile that rows may not see, is
                 // for the loop after this one: the sums are touched by products
                 // alone here, and stay in the registers that products use.
-                int late = 0;
-                float high = kNone;
-                for (; t + 4 <= full; t += 4) {
+                int stop = 0;
+                bool here_already = false;
+                while (stop == 0) {
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
-                        arrive(t + u, u);
-                        high = largest(tops[u & 1]);
-                        if (__builtin_expect(__any((high - m) * a.c > kSlack), 0)) {
-                            late = u + 1;
+                        if (t + u >= full) {
+                            stop = u + 1;
                             break;
                         }
-                        l[0] += sum[0];
-                        l[1] += sum[1];
-                        products(yes, ring[(u + 1) & 3], yes, ring[u], weights[u & 1], no);
-                        pass(tops[(u + 1) & 1]);
-                        weigh(weights[(u + 1) & 1], sum);
+                        arrive(t + u);
+                        if (__builtin_expect(late_flags[u] != 0, 0)) {
+                            stop = u + 1;
+                            here_already = true;
+                            break;
+                        }
+                        if (tid == 0) {
+                            late_flags[(u + 2) & 3] = 0;
+                        }
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) {
+                            l[b] += sum[b];
+                        }
+                        float over;
+                        products(
+                            yes, ring[(u + 1) & 3], yes, ring[u], weights[u & 1], false,
+                            [&] {
+                                if (t + u + 3 < s.tile1) {
+                                    issue(t + u + 3, ring[(u + 3) & 3]);
+                                }
+                            },
+                            [&] { over = weigh(weights[(u + 1) & 1]); });
+                        tell(over, (u + 1) & 3);
                     }
-                    if (late != 0) {
-                        break;
-                    }
+                    t += stop == 0 ? 4 : 0;
                 }
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    if (u + 1 >= late && t + u < s.tile1) {
-                        if (u + 1 != late) {
-                            arrive(t + u, u);
-                            high = largest(tops[u & 1]);
+                    if (u + 1 >= stop && t + u < s.tile1) {
+                        if (u + 1 != stop || !here_already) {
+                            arrive(t + u);
                         }
-                        if (__any((high - m) * a.c > kSlack)) {
-                            follow(high, &alpha);
+                        if (late_flags[u] != 0) {
+                            const float alpha = follow();
 #pragma unroll
-                            for (int rb = 0; rb < 2; ++rb) {
-                                const float f = __shfl(alpha, 32 * rb + col32);
+                            for (int b = 0; b < NB; ++b) {
+                                const float f = __shfl(alpha, kWide ? 32 * b + col32 : col);
 #pragma unroll
-                                for (int ct = 0; ct < 4; ++ct) {
-                                    o[rb][ct] *= f;
+                                for (int i = 0; i < NO / NB; ++i) {
+                                    o[NO / NB * b + i] *= f;
                                 }
                             }
-                            l[0] *= __shfl(alpha, 32 * rh + col);
-                            l[1] *= __shfl(alpha, 32 * rh + 16 + col);
-                            weigh(weights[u & 1], sum);
+#pragma unroll
+                            for (int b = 0; b < NB; ++b) {
+                                l[b] *= __shfl(alpha, 32 * rh + 16 * b + col);
+                            }
+                            weigh(weights[u & 1]);
                             meet();
                         }
-                        l[0] += sum[0];
-                        l[1] += sum[1];
+                        if (tid == 0) {
+                            late_flags[(u + 2) & 3] = 0;
+                        }
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) {
+                            l[b] += sum[b];
+                        }
+                        if (t + u + 3 < s.tile1) {
+                            issue(t + u + 3, ring[(u + 3) & 3]);
+                        }
                         if (t + u + 1 < s.tile1) {
-                            products(yes, ring[(u + 1) & 3], no, nullptr, nullptr, no);
+                            products(yes, ring[(u + 1) & 3], no, nullptr, nullptr, false, nothing, nothing);
                             mask(t + u + 1);
                         }
-                        products(no, nullptr, yes, ring[u], weights[u & 1], yes);
+                        products(no, nullptr, yes, ring[u], weights[u & 1], (t + u) * kTile + kTile - 1 > all_see, nothing,
+                                 nothing);
                         if (t + u + 1 < s.tile1) {
-                            pass(tops[(u + 1) & 1]);
-                            weigh(weights[(u + 1) & 1], sum);
+                            tell(weigh(weights[(u + 1) & 1]), (u + 1) & 3);
                         }
                     }
                 }
@@ -898,58 +746,48 @@ __global__ __launch_bounds__(256, 1) void paged_rows64_kernel(const TileArgs a) 
         // the totals: the rows' parts of both key halves meet in `tops`
         __syncthreads();
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < NB; ++b) {
             l[b] += __shfl_xor(l[b], 16);
             l[b] += __shfl_xor(l[b], 32);
             if (grp == 0) {
-                tops[0][kh][32 * rh + 16 * b + col] = l[b];
+                tops[kh][32 * rh + 16 * b + col] = l[b];
             }
         }
         __syncthreads();
         const bool whole = s.begins && s.ends;
-        const int slot = 2 * static_cast<int>(blockIdx.x) + (s.begins ? 1 : 0);
-        // o[rb][ct] register e: channel 128 wave + 32 ct + 8 (e / 4) + 4 half + e % 4 of row 32 rb + col32
+        const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (s.begins ? 1 : 0);
+        // o[4 rb + ct] register e: channel 128 wave + 32 ct + 8 (e / 4) + 4 half + e % 4
+        // of row 32 rb + col32 (M = 16: o[ct], channel 128 wave + 16 ct + 4 grp + e of row col)
 #pragma unroll
-        for (int rb = 0; rb < 2; ++rb) {
-            const int row = 32 * rb + col32;
+        for (int i = 0; i < NO; ++i) {
+            const int row = kWide ? 32 * (i / 4) + col32 : col;
             if (row < rows) {
-                if (whole) {
-                    const float inv = 1.0f / (tops[0][0][row] + tops[0][1][row]);
-                    E* const to = static_cast<E*>(a.out) + (row0 + row) * kRank + 128 * wave + 4 * half;
+                const float inv = whole ? 1.0f / (tops[0][row] + tops[1][row]) : 1.0f;
+                const int ch = 128 * wave + (kWide ? 32 * (i % 4) + 4 * half : 16 * i + 4 * grp);
 #pragma unroll
-                    for (int ct = 0; ct < 4; ++ct) {
+                for (int g = 0; g < (kWide ? 4 : 1); ++g) {
+                    if (whole) {
+                        vec4 out;
 #pragma unroll
-                        for (int g = 0; g < 4; ++g) {
-                            vec4 out;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                out[e] = static_cast<E>(o[rb][ct][4 * g + e] * inv);
-                            }
-                            *reinterpret_cast<vec4*>(to + 32 * ct + 8 * g) = out;
+                        for (int e = 0; e < 4; ++e) {
+                            out[e] = static_cast<E>(o[i][4 * g + e] * inv);
                         }
-                    }
-                } else {
-                    float* const to = a.parts.sums + (static_cast<int64_t>(slot) * kRows64 + row) * kRank + 128 * wave +
-                                      4 * half;
+                        *reinterpret_cast<vec4*>(static_cast<E*>(a.out) + (row0 + row) * kRank + ch + 8 * g) = out;
+                    } else {
+                        f32x4 out;
 #pragma unroll
-                    for (int ct = 0; ct < 4; ++ct) {
-#pragma unroll
-                        for (int g = 0; g < 4; ++g) {
-                            f32x4 out;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                out[e] = o[rb][ct][4 * g + e];
-                            }
-                            *reinterpret_cast<f32x4*>(to + 32 * ct + 8 * g) = out;
+                        for (int e = 0; e < 4; ++e) {
+                            out[e] = o[i][4 * g + e];
                         }
+                        *reinterpret_cast<f32x4*>(a.parts.sums + (slot * M + row) * kRank + ch + 8 * g) = out;
                     }
                 }
             }
         }
         if (!whole && tid < rows) {
-            float* const to = a.parts.stats + (static_cast<int64_t>(slot) * kRows64 + tid) * 2;
+            float* const to = a.parts.stats + (slot * M + tid) * 2;
             to[0] = m == kNone ? kNone : m * a.c;
-            to[1] = tops[0][0][tid] + tops[0][1][tid];
+            to[1] = tops[0][tid] + tops[1][tid];
         }
         if (s.begins && !s.ends && tid == 0) {
             a.parts.heads[blockIdx.x] = PartHead{row0, rows, s.parts_after};
@@ -957,15 +795,22 @@ __global__ __launch_bounds__(256, 1) void paged_rows64_kernel(const TileArgs a) 
     }
 }
 
-// The parts of cut blocks added up: workgroup (g, y) takes rows y, y + gridDim.y, ..
-// of the block that piece g began and did not end. 64 lanes hold 512 channels,
-// the four waves alternate parts.
+// The parts of cut blocks added up, a wave per row of the block that piece g
+// began and did not end; 64 lanes hold 512 channels. Few parts: each wave adds
+// those of its rows in order. Many (kMany and more: one long request, few rows):
+// the four waves of a workgroup share a row's, and add their sums.
+constexpr int kMany = 16;
+
 template <class E, int M>
 __global__ __launch_bounds__(256) void paged_join_kernel(const TileArgs a) {
     __shared__ float sums[4][kRank], totals[4];
-    const int g = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int g = blockIdx.x, lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
     const PartHead head = a.parts.heads[g];
-    for (int r = blockIdx.y; r < head.rows; r += gridDim.y) {
+    const bool many = head.after + 1 >= kMany;
+    const int rows_at_once = many ? 1 : 4;
+    for (int r0 = blockIdx.y * rows_at_once; r0 < head.rows; r0 += gridDim.y * rows_at_once) {
+        const int r = many ? r0 : min(r0 + wave, head.rows - 1);
         auto slot = [&](int k) { return static_cast<int64_t>(k == 0 ? 2 * g + 1 : 2 * (g + k)) * M + r; };
         float high = kNone;
         for (int k = lane; k <= head.after; k += 64) {
@@ -974,35 +819,55 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const TileArgs a) {
         for (int o = 32; o >= 1; o >>= 1) {
             high = fmaxf(high, __shfl_xor(high, o));
         }
-        float total = 0.0f, sum[8] = {};
-        for (int k = wave; k <= head.after; k += 4) {
-            const float top = a.parts.stats[slot(k) * 2];
-            if (top == kNone) {
-                // no score above -infinity here: a total that is not 0 is NaN
-                total += a.parts.stats[slot(k) * 2 + 1];
+        float total = 0.0f;
+        f32x4 sum[2] = {};
+        for (int k = many ? wave : 0; k <= head.after; k += many ? 4 : 1) {
+            const float* const stats = a.parts.stats + slot(k) * 2;
+            const float top = stats[0];
+            const f32x4* const from = reinterpret_cast<const f32x4*>(a.parts.sums + slot(k) * kRank) + lane;
+            const f32x4 v0 = from[0], v1 = from[64];
+            // no score above -infinity here: weighs 0 (NaN in the total or the sums stays)
+            const float w = top == kNone ? 0.0f : __builtin_amdgcn_exp2f(top - high);
+            total = __builtin_fmaf(w, stats[1], total);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                sum[0][e] = __builtin_fmaf(w, v0[e], sum[0][e]);
+                sum[1][e] = __builtin_fmaf(w, v1[e], sum[1][e]);
+            }
+        }
+        if (many) {
+            __syncthreads();
+            *reinterpret_cast<f32x4*>(&sums[wave][4 * lane]) = sum[0];
+            *reinterpret_cast<f32x4*>(&sums[wave][256 + 4 * lane]) = sum[1];
+            if (lane == 0) {
+                totals[wave] = total;
+            }
+            __syncthreads();
+            if (wave != 0) {
                 continue;
             }
-            const float w = __builtin_amdgcn_exp2f(top - high);
-            total = __builtin_fmaf(w, a.parts.stats[slot(k) * 2 + 1], total);
-            const float* const from = a.parts.sums + slot(k) * kRank + 8 * lane;
+            total = (totals[0] + totals[1]) + (totals[2] + totals[3]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                sum[i] = __builtin_fmaf(w, from[i], sum[i]);
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int ch = 256 * i + 4 * lane + e;
+                    sum[i][e] = (sums[0][ch] + sums[1][ch]) + (sums[2][ch] + sums[3][ch]);
+                }
             }
         }
-        __syncthreads();
+        if (many || r0 + wave < head.rows) {
+            const float inv = 1.0f / total;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            sums[wave][8 * lane + i] = sum[i];
-        }
-        if (lane == 0) {
-            totals[wave] = total;
-        }
-        __syncthreads();
-        total = (totals[0] + totals[1]) + (totals[2] + totals[3]);
-        E* const out = static_cast<E*>(a.out) + (head.row0 + r) * kRank;
-        for (int i = threadIdx.x; i < kRank; i += 256) {
-            out[i] = static_cast<E>(((sums[0][i] + sums[1][i]) + (sums[2][i] + sums[3][i])) / total);
+            for (int i = 0; i < 2; ++i) {
+                typename Half<E>::vec4 out;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    out[e] = static_cast<E>(sum[i][e] * inv);
+                }
+                *reinterpret_cast<typename Half<E>::vec4*>(static_cast<E*>(a.out) + (head.row0 + r) * kRank + 256 * i +
+                                                           4 * lane) = out;
+            }
         }
     }
 }
@@ -1127,19 +992,19 @@ hipError_t launch(const PagedAttention& a, void* workspace, hipStream_t s) {
     t.parts.stats = reinterpret_cast<float*>(w);
     w += round_up(sizeof(float) * 2 * kGrid * m * 2, 256);
     t.parts.sums = reinterpret_cast<float*>(w);
-    if (m == kRows16) {
-        hipLaunchKernelGGL(paged_rows16_kernel<E>, dim3(kGrid), dim3(256), 0, s, t);
+    if (m == 16) {
+        hipLaunchKernelGGL((paged_rows_kernel<E, 16>), dim3(kGrid), dim3(256), 0, s, t);
     } else {
-        hipLaunchKernelGGL(paged_rows64_kernel<E>, dim3(kGrid), dim3(256), 0, s, t);
+        hipLaunchKernelGGL((paged_rows_kernel<E, 64>), dim3(kGrid), dim3(256), 0, s, t);
     }
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) {
         return err;
     }
-    if (m == kRows16) {
-        hipLaunchKernelGGL((paged_join_kernel<E, kRows16>), dim3(kGrid, kRows16), dim3(256), 0, s, t);
+    if (m == 16) {
+        hipLaunchKernelGGL((paged_join_kernel<E, 16>), dim3(kGrid, 16), dim3(256), 0, s, t);
     } else {
-        hipLaunchKernelGGL((paged_join_kernel<E, kRows64>), dim3(kGrid, 16), dim3(256), 0, s, t);
+        hipLaunchKernelGGL((paged_join_kernel<E, 64>), dim3(kGrid, 16), dim3(256), 0, s, t);
     }
     return hipGetLastError();
 }
@@ -1149,7 +1014,7 @@ hipError_t launch(const PagedAttention& a, void* workspace, hipStream_t s) {
 bool paged_tiled(int32_t rank, int32_t rope) { return rank == kRank && rope == kRope; }
 
 int paged_block_rows(int32_t max_added, int32_t heads) {
-    return static_cast<int64_t>(max_added) * heads <= kRows16 ? kRows16 : kRows64;
+    return static_cast<int64_t>(max_added) * heads <= 16 ? 16 : 64;
 }
 
 int64_t paged_workspace_bytes(int rows) {
