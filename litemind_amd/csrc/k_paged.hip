@@ -41,7 +41,6 @@ typedef __attribute__((address_space(3))) short4v lds_short4;
 
 constexpr int kRank = 512, kRope = 64, kWidth = kRank + kRope;
 constexpr int kRowBytes = kWidth * 2;        // 1152
-constexpr int kUnits = kRowBytes / 16;       // 16-byte units of a row
 constexpr int kTile = 32;                    // keys of a tile
 constexpr int kTileBytes = kTile * kRowBytes;
 constexpr int kGrid = 256;                   // workgroups that share out the tiles: one per CU
@@ -103,8 +102,15 @@ struct Piece {
     int32_t request;  // that `begin` lies in
     int64_t base;     // cost of the requests before it
 };
+// Begin of piece g. (In doubles, as the cuts of blocks below: a 64-bit division
+// is 150 instructions. Neighbours form a border from the same numbers, so they
+// agree on it however it rounds.)
 __device__ inline int64_t border(int64_t total, int32_t parts, int32_t g) {
-    return total / parts * g + total % parts * g / parts;
+    return g >= parts ? total : static_cast<int64_t>(static_cast<double>(total) * g / parts);
+}
+// Tile of a block at which a border `x` past the block's begin cuts it.
+__device__ inline int32_t cut(int64_t x, int64_t cost, int32_t tiles) {
+    return min(tiles, static_cast<int32_t>(static_cast<double>(x) * tiles / static_cast<double>(cost)));
 }
 
 // Every thread of the 256-thread workgroup calls it. Threads take stretches of
@@ -205,15 +211,21 @@ struct Walk {
         const int32_t tiles = sh.tiles(req, block);
         s.begins = p.begin <= at;
         s.ends = p.end >= at + cost;
-        s.tile0 = s.begins ? 0 : static_cast<int32_t>((p.begin - at) * tiles / cost);
-        s.tile1 = s.ends ? tiles : static_cast<int32_t>((p.end - at) * tiles / cost);
+        s.tile0 = s.begins ? 0 : cut(p.begin - at, cost, tiles);
+        s.tile1 = s.ends ? tiles : cut(p.end - at, cost, tiles);
         s.parts_after = 0;
         if (s.begins && !s.ends) {
-            int32_t g = static_cast<int32_t>(blockIdx.x) + 1;
-            while (g < p.parts && border(p.total, p.parts, g) < at + cost) {
+            // the last piece that begins before the block's end, from its share of the line
+            const int32_t own = static_cast<int32_t>(blockIdx.x);
+            int32_t g = static_cast<int32_t>(static_cast<double>(at + cost) * p.parts / static_cast<double>(p.total));
+            g = max(own, min(g, p.parts - 1));
+            while (g + 1 < p.parts && border(p.total, p.parts, g + 1) < at + cost) {
                 ++g;
             }
-            s.parts_after = g - static_cast<int32_t>(blockIdx.x) - 1;
+            while (g > own && border(p.total, p.parts, g) >= at + cost) {
+                --g;
+            }
+            s.parts_after = g - own;
         }
         at += cost;
         ++block;
@@ -795,79 +807,133 @@ __global__ __launch_bounds__(256, 1) void paged_rows_kernel(const TileArgs a) {
     }
 }
 
-// The parts of cut blocks added up, a wave per row of the block that piece g
-// began and did not end; 64 lanes hold 512 channels. Few parts: each wave adds
-// those of its rows in order. Many (kMany and more: one long request, few rows):
-// the four waves of a workgroup share a row's, and add their sums.
+// The parts of cut blocks added up. An item of work is four rows of a block, a
+// wave each with 64 lanes for 512 channels; of a block in kMany parts or more (a
+// long request, few rows) it is 128 channels of one row, 32 lanes for them and
+// the parts dealt to the workgroup's eight half waves. The workgroups take
+// items in turn, so a step with one cut block uses as many as one with 256.
 constexpr int kMany = 16;
+constexpr int kJoinGrid = 1024;
 
 template <class E, int M>
 __global__ __launch_bounds__(256) void paged_join_kernel(const TileArgs a) {
-    __shared__ float sums[4][kRank], totals[4];
-    const int g = blockIdx.x, lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-    const PartHead head = a.parts.heads[g];
-    const bool many = head.after + 1 >= kMany;
-    const int rows_at_once = many ? 1 : 4;
-    for (int r0 = blockIdx.y * rows_at_once; r0 < head.rows; r0 += gridDim.y * rows_at_once) {
-        const int r = many ? r0 : min(r0 + wave, head.rows - 1);
-        auto slot = [&](int k) { return static_cast<int64_t>(k == 0 ? 2 * g + 1 : 2 * (g + k)) * M + r; };
-        float high = kNone;
-        for (int k = lane; k <= head.after; k += 64) {
-            high = fmaxf(high, a.parts.stats[slot(k) * 2]);
+    __shared__ int32_t first[kGrid], wave_items[4];
+    __shared__ float sums[8][128], totals[8], tops[8];
+    static_assert(kGrid == 256, "a piece per thread");
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const PartHead own = a.parts.heads[tid];
+    const int32_t items = own.rows == 0 ? 0 : own.after + 1 >= kMany ? own.rows * 4 : (own.rows + 3) / 4;
+    int32_t sum_items = items;
+    for (int o = 1; o < 64; o <<= 1) {
+        const int32_t up = __shfl_up(sum_items, o);
+        sum_items += lane >= o ? up : 0;
+    }
+    if (lane == 63) {
+        wave_items[wave] = sum_items;
+    }
+    __syncthreads();
+    int32_t total_items = 0;
+    for (int w = 0; w < 4; ++w) {
+        sum_items += w < wave ? wave_items[w] : 0;
+        total_items += wave_items[w];
+    }
+    first[tid] = sum_items - items;
+    __syncthreads();
+    for (int32_t item = blockIdx.x; item < total_items; item += gridDim.x) {
+        int g = 0;  // the last piece whose items start at or before this one
+        for (int step = 128; step >= 1; step >>= 1) {
+            g += first[g + step] <= item ? step : 0;
         }
+        const PartHead head = a.parts.heads[g];
+        const int32_t at = item - first[g];
+        auto slot = [&](int k, int r) { return static_cast<int64_t>(k == 0 ? 2 * g + 1 : 2 * (g + k)) * M + r; };
+        // parts k0, k0 + by, ..; four loads at a time, those past the last weigh 0
+        auto add = [&](int k0, int by, int r, int channel, float high, f32x4 (&sum)[2], bool second, float& total) {
+            for (int k = k0; k <= head.after; k += 4 * by) {
+                f32x4 v[4][2];
+                float st[4][2];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int64_t from = slot(min(k + i * by, head.after), r);
+                    st[i][0] = a.parts.stats[from * 2];
+                    st[i][1] = a.parts.stats[from * 2 + 1];
+                    v[i][0] = *reinterpret_cast<const f32x4*>(a.parts.sums + from * kRank + channel);
+                    if (second) {
+                        v[i][1] = *reinterpret_cast<const f32x4*>(a.parts.sums + from * kRank + channel + 256);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    // no score above -infinity: weighs 0 (NaN in the total or the sums stays)
+                    const float w = st[i][0] == kNone || k + i * by > head.after
+                                        ? 0.0f
+                                        : __builtin_amdgcn_exp2f(st[i][0] - high);
+                    total = __builtin_fmaf(w, st[i][1], total);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        sum[0][e] = __builtin_fmaf(w, v[i][0][e], sum[0][e]);
+                        if (second) {
+                            sum[1][e] = __builtin_fmaf(w, v[i][1][e], sum[1][e]);
+                        }
+                    }
+                }
+            }
+        };
+        auto highest = [&](int k0, int by, int r) {
+            float high = kNone;
+            for (int k = k0; k <= head.after; k += by) {
+                high = fmaxf(high, a.parts.stats[slot(k, r) * 2]);
+            }
+            return high;
+        };
+        auto store = [&](int r, int channel, const f32x4& sum, float total) {
+            const float inv = 1.0f / total;
+            typename Half<E>::vec4 out;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                out[e] = static_cast<E>(sum[e] * inv);
+            }
+            *reinterpret_cast<typename Half<E>::vec4*>(static_cast<E*>(a.out) + (head.row0 + r) * kRank + channel) = out;
+        };
+        f32x4 sum[2] = {};
+        float total = 0.0f;
+        if (head.after + 1 < kMany) {
+            const int r = min(4 * at + wave, head.rows - 1);  // (a wave past the last row repeats it)
+            add(0, 1, r, 4 * lane, highest(0, 1, r), sum, true, total);
+            store(r, 4 * lane, sum[0], total);
+            store(r, 256 + 4 * lane, sum[1], total);
+            continue;
+        }
+        const int r = at >> 2, channel = (at & 3) * 128 + (tid & 31) * 4, eighth = tid >> 5;
+        float high = highest(tid, 256, r);
         for (int o = 32; o >= 1; o >>= 1) {
             high = fmaxf(high, __shfl_xor(high, o));
         }
-        float total = 0.0f;
-        f32x4 sum[2] = {};
-        for (int k = many ? wave : 0; k <= head.after; k += many ? 4 : 1) {
-            const float* const stats = a.parts.stats + slot(k) * 2;
-            const float top = stats[0];
-            const f32x4* const from = reinterpret_cast<const f32x4*>(a.parts.sums + slot(k) * kRank) + lane;
-            const f32x4 v0 = from[0], v1 = from[64];
-            // no score above -infinity here: weighs 0 (NaN in the total or the sums stays)
-            const float w = top == kNone ? 0.0f : __builtin_amdgcn_exp2f(top - high);
-            total = __builtin_fmaf(w, stats[1], total);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                sum[0][e] = __builtin_fmaf(w, v0[e], sum[0][e]);
-                sum[1][e] = __builtin_fmaf(w, v1[e], sum[1][e]);
-            }
+        __syncthreads();  // the item before has been read
+        if (lane == 0) {
+            tops[wave] = high;
         }
-        if (many) {
-            __syncthreads();
-            *reinterpret_cast<f32x4*>(&sums[wave][4 * lane]) = sum[0];
-            *reinterpret_cast<f32x4*>(&sums[wave][256 + 4 * lane]) = sum[1];
-            if (lane == 0) {
-                totals[wave] = total;
-            }
-            __syncthreads();
-            if (wave != 0) {
-                continue;
-            }
-            total = (totals[0] + totals[1]) + (totals[2] + totals[3]);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
+        __syncthreads();
+        high = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+        add(eighth, 8, r, channel, high, sum, false, total);
+        *reinterpret_cast<f32x4*>(&sums[eighth][(tid & 31) * 4]) = sum[0];
+        if ((tid & 31) == 0) {
+            totals[eighth] = total;
+        }
+        __syncthreads();
+        if (tid < 32) {
+            sum[0] = f32x4{};
+            total = 0.0f;
+            for (int i = 0; i < 8; ++i) {
+                const f32x4 v = *reinterpret_cast<const f32x4*>(&sums[i][tid * 4]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int ch = 256 * i + 4 * lane + e;
-                    sum[i][e] = (sums[0][ch] + sums[1][ch]) + (sums[2][ch] + sums[3][ch]);
+                    sum[0][e] += v[e];
                 }
+                total += totals[i];
             }
-        }
-        if (many || r0 + wave < head.rows) {
-            const float inv = 1.0f / total;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                typename Half<E>::vec4 out;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    out[e] = static_cast<E>(sum[i][e] * inv);
-                }
-                *reinterpret_cast<typename Half<E>::vec4*>(static_cast<E*>(a.out) + (head.row0 + r) * kRank + 256 * i +
-                                                           4 * lane) = out;
-            }
+            store(r, channel, sum[0], total);
         }
     }
 }
@@ -1002,9 +1068,9 @@ hipError_t launch(const PagedAttention& a, void* workspace, hipStream_t s) {
         return err;
     }
     if (m == 16) {
-        hipLaunchKernelGGL((paged_join_kernel<E, 16>), dim3(kGrid, 16), dim3(256), 0, s, t);
+        hipLaunchKernelGGL((paged_join_kernel<E, 16>), dim3(kJoinGrid), dim3(256), 0, s, t);
     } else {
-        hipLaunchKernelGGL((paged_join_kernel<E, 64>), dim3(kGrid, 16), dim3(256), 0, s, t);
+        hipLaunchKernelGGL((paged_join_kernel<E, 64>), dim3(kJoinGrid), dim3(256), 0, s, t);
     }
     return hipGetLastError();
 }
