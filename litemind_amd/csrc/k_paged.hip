@@ -36,14 +36,16 @@ typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short short4v __attribute__((ext_vector_type(4)));
 typedef short short8v __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) short4v lds_short4;
+typedef __attribute__((address_space(3))) char lds_char;
 
 constexpr int kRank = 512, kRope = 64, kWidth = kRank + kRope;
 constexpr int kRowBytes = kWidth * 2;        // 1152
 constexpr int kTile = 32;                    // keys of a tile
 constexpr int kTileBytes = kTile * kRowBytes;
 constexpr int kGrid = 256;                   // workgroups that share out the tiles: one per CU
+constexpr int kWaves = 8;                    // of each, two per SIMD
+constexpr int kThreads = 64 * kWaves;
 constexpr float kNone = -__builtin_inff();
 
 template <class E>
@@ -55,9 +57,6 @@ struct Half<_Float16> {
     static __device__ f32x4 mfma16(vec8 a, vec8 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
     }
-    static __device__ f32x16 mfma32(vec8 a, vec8 b, f32x16 c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-    }
 };
 template <>
 struct Half<bf16> {
@@ -65,9 +64,6 @@ struct Half<bf16> {
     typedef bf16x4 vec4;
     static __device__ f32x4 mfma16(vec8 a, vec8 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-    }
-    static __device__ f32x16 mfma32(vec8 a, vec8 b, f32x16 c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
     }
 };
 
@@ -113,18 +109,20 @@ __device__ inline int32_t cut(int64_t x, int64_t cost, int32_t tiles) {
     return min(tiles, static_cast<int32_t>(static_cast<double>(x) * tiles / static_cast<double>(cost)));
 }
 
-// Every thread of the 256-thread workgroup calls it. Threads take stretches of
-// requests; `scratch` (8 + 3 words of 64 bits) passes the sums.
+// Every thread of the workgroup calls it. Threads take stretches of requests;
+// `scratch` (kWaves + 2 words of 64 bits) passes the sums.
 __device__ inline Piece find_piece(const PagedView& v, const Shares& sh, int32_t g, int64_t* scratch) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int32_t per = (v.requests + 255) / 256;
+    const int32_t per = (v.requests + kThreads - 1) / kThreads;
     const int32_t r0 = min(tid * per, v.requests), r1 = min(r0 + per, v.requests);
     int64_t own = 0;
+#pragma unroll 1
     for (int32_t r = r0; r < r1; ++r) {
         const PagedRequest q = paged_request(v, r);
         own += sh.cost(q, sh.blocks(q));
     }
     int64_t sum = own;
+#pragma unroll 1
     for (int o = 1; o < 64; o <<= 1) {
         const int64_t up = __shfl_up(sum, o);
         sum += lane >= o ? up : 0;
@@ -134,30 +132,31 @@ __device__ inline Piece find_piece(const PagedView& v, const Shares& sh, int32_t
     }
     __syncthreads();
     int64_t before = sum - own, total = 0;
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < kWaves; ++w) {
         before += w < wave ? scratch[w] : 0;
         total += scratch[w];
     }
     Piece p;
     p.total = total;
-    p.parts = static_cast<int32_t>(max(int64_t{1}, min(static_cast<int64_t>(kGrid), total / (int64_t{kLeast} * sh.heads))));
+    p.parts = static_cast<int32_t>(max(int64_t{1}, min(static_cast<int64_t>(kGrid), static_cast<int64_t>(static_cast<double>(total) / (kLeast * static_cast<double>(sh.heads))))));
     p.begin = g < p.parts ? border(total, p.parts, g) : total;
     p.end = g < p.parts ? border(total, p.parts, g + 1) : total;
     if (p.begin >= before && p.begin < before + own) {
+#pragma unroll 1
         for (int32_t r = r0; r < r1; ++r) {
             const PagedRequest q = paged_request(v, r);
             const int64_t c = sh.cost(q, sh.blocks(q));
             if (p.begin < before + c) {
-                scratch[4] = r;
-                scratch[5] = before;
+                scratch[kWaves] = r;
+                scratch[kWaves + 1] = before;
                 break;
             }
             before += c;
         }
     }
     __syncthreads();
-    p.request = static_cast<int32_t>(scratch[4]);
-    p.base = scratch[5];
+    p.request = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(scratch[kWaves]));
+    p.base = scratch[kWaves + 1];
     return p;
 }
 
@@ -183,6 +182,7 @@ struct Walk {
         blocks = sh.blocks(req);
         // the block that `begin` lies in: the last whose cost line starts at or before it
         int32_t lo = 0, hi = blocks;
+#pragma unroll 1
         while (hi - lo > 1) {
             const int32_t mid = lo + (hi - lo) / 2;
             if (p.base + sh.cost(req, mid) <= p.begin) {
@@ -219,9 +219,11 @@ struct Walk {
             const int32_t own = static_cast<int32_t>(blockIdx.x);
             int32_t g = static_cast<int32_t>(static_cast<double>(at + cost) * p.parts / static_cast<double>(p.total));
             g = max(own, min(g, p.parts - 1));
+#pragma unroll 1
             while (g + 1 < p.parts && border(p.total, p.parts, g + 1) < at + cost) {
                 ++g;
             }
+#pragma unroll 1
             while (g > own && border(p.total, p.parts, g) >= at + cost) {
                 --g;
             }
@@ -262,12 +264,14 @@ struct TileArgs {
 // A tile in LDS: per eight rows their 64 units of latent (16 bytes each), a row
 // after the other, then their eight units of rotary key. A load fills 64 units,
 // so a row's latent is one load and eight rotary keys are one. Units are XORed by
-// row so that LDS reads are free of bank conflicts: a 16-lane group of a key read
-// takes one unit of 16 rows; 32 lanes of a transposing read four neighbouring
+// row so that LDS reads are free of bank conflicts (16 units to a cycle). A key
+// read's cycles take 16 rows: 0 - 3 and 12 - 15 of one unit and 4 - 11 of the next,
+// or the other way round (measured: with the units of rows 4 - 11 not closed under
+// XOR 1, a third of the cycles were conflicts). A transposing read's take four
 // units of four rows, or two of eight. Bits 2 and 3 come from the row within
 // four, bits 0 and 1 from the fours; rotary rows are 8 units apart.
 constexpr int kEightBytes = 8 * kRowBytes;  // 9216
-__device__ inline int swizzle(int r) { return (r & 3) << 2 | (r >> 2 & 2) | (r >> 2 & 1); }
+__device__ inline int swizzle(int r) { return (r & 3) << 2 | ((r >> 2 ^ r >> 3) & 1) << 1 | (r >> 3 & 1); }
 __device__ inline int latent_at(int r, int u) {
     return (r >> 3) * kEightBytes + (r & 7) * 1024 + ((u ^ swizzle(r)) << 4);
 }
@@ -275,17 +279,18 @@ __device__ inline int rotary_at(int r, int u) {
     return (r >> 3) * kEightBytes + 8192 + (r & 7) * 128 + ((u ^ (r >> 1 & 7)) << 4);
 }
 
-// The pages of one request's keys, 64 table entries at a time in the lanes.
+// The pages of one request's keys, a step ahead of their loads: look(key) reads
+// the table entry, take() the pool row of that key (a multiple of 16; the 15 after
+// it lie in the same page). The entry is a scalar load: a vector load's wait would
+// be one for all tiles in flight.
+typedef __attribute__((address_space(4))) const int32_t scalar_int;
 struct PageWalk {
     const int32_t* row;  // the request's table row
-    int32_t base;        // first entry held; a multiple of 64, or -1
-    int32_t held;        // this lane's
+    int32_t id, in_page;
     __device__ void start(const PagedView& v, int32_t request) {
         row = v.table + static_cast<int64_t>(request) * v.table_width;
-        base = -1;
     }
-    // Pool row of key (a multiple of 16; the 15 after it lie in the same page).
-    __device__ int64_t at(const PagedView& v, uint32_t page_mul, int32_t key) {
+    __device__ void look(const PagedView& v, uint32_t page_mul, int32_t key) {
         const uint32_t d = static_cast<uint32_t>(v.page_size) / 16, n = static_cast<uint32_t>(key) / 16;
         uint32_t page = __umulhi(n, page_mul);
         if (d == 1) {
@@ -293,14 +298,11 @@ struct PageWalk {
         } else if (page * d > n) {
             --page;
         }
-        const int32_t from = static_cast<int32_t>(page & ~63u);
-        if (from != base) {
-            base = from;
-            const int32_t i = from + static_cast<int32_t>(threadIdx.x & 63);
-            held = row[min(i, v.table_width - 1)];
-        }
-        const int32_t id = __builtin_amdgcn_readlane(held, static_cast<int>(page & 63));
-        return checked_page(v, id) * v.page_size + static_cast<int64_t>(n - page * d) * 16;
+        id = ((scalar_int*)row)[page];
+        in_page = static_cast<int32_t>(n - page * d) * 16;
+    }
+    __device__ int64_t take(const PagedView& v) const {
+        return checked_page(v, id) * v.page_size + in_page;
     }
 };
 
@@ -310,20 +312,27 @@ __device__ inline int here(int v) {
     asm volatile("" : "+v"(v));
     return v;
 }
+__device__ inline int lds_address(const char* p) {
+    return static_cast<int>(reinterpret_cast<uintptr_t>((const lds_char*)p));
+}
 
 // ---- blocks of query rows ----
-// M = 64 rows, four waves. The waves share tiles of 32 keys, which come straight
-// to LDS four deep, and split each product differently:
-//   S^T   wave (kh, rh): keys 16 kh .. + 15 for rows 32 rh .. + 31; its queries
-//         stay in 144 registers, 36 products of 16 x 16 x 32 a tile
-//   out^T channels 128 w .. + 127 of wave w for all rows; 128 registers of sums,
-//         16 products of 32 x 32 x 16 a tile
-// (M = 16: keys 16 kh .. for all rows, on both rh; 32 registers, 8 products of
-// 16 x 16 x 32.) The weights pass through LDS. One barrier a tile: between two,
-// the waves run the scores of tile t + 1 and the context of tile t, which do not
-// depend on each other, and the weights of t + 1 beside the last of the context.
-// A wave with 32 rows and all channels would need no exchange, but 256 + 16
-// registers of sums, where the matrix cores' results go to 256.
+// M = 64 rows, eight waves, two per SIMD, so that one's products run beside the
+// other's loads, exponentials and addresses. The waves share tiles of 32 keys,
+// which come straight to LDS four deep, and split each product differently, in
+// products of 16 x 16 x 32:
+//   S^T   wave (kh, rq): keys 16 kh .. + 15 for rows 16 rq .. + 15, 18 products a
+//         tile; its queries stay in 72 registers
+//   out^T channels 64 w .. + 63 of wave w for all rows, 16 products a tile; 64
+//         registers of sums
+// (M = 16: keys 16 kh .. for all rows, on every rq; 4 products, 16 registers.)
+// The weights pass through LDS. One barrier a tile: between two, the waves run
+// the scores of tile t + 1 and the context of tile t, which do not depend on each
+// other. LDS reads are 208 KB a tile, 191 bytes per clock of the products' time
+// against the 254 that a CU reads; four waves of twice the work each would need
+// 110, but have no second wave to fill a SIMD, and were no faster. Products of
+// 32 x 32 x 16 take 19.4 ns on numbers as they come, two of 16 x 16 x 32 16.2
+// (the clock gives way to the power drawn; on zeros 13.4 and 14.4).
 //
 // The weights' reference m, one per row, has to be the same for all waves: it is
 // moved only where a row's scores pass it by more than kSlack (in powers of
@@ -346,27 +355,23 @@ __device__ inline short8v finite_or_zero(short8v v) {
 }
 
 template <class E, int M>
-__global__ __launch_bounds__(256, 1) void paged_rows_kernel(const TileArgs a) {
+__global__ __launch_bounds__(kThreads, 2) void paged_rows_kernel(const TileArgs a) {
     static_assert(M == 64 || M == 16);
     using H = Half<E>;
     typedef typename H::vec8 vec8;
     typedef typename H::vec4 vec4;
-    constexpr bool kWide = M == 64;
-    constexpr int NB = kWide ? 2 : 1;        // blocks of 16 rows in a wave's scores
-    constexpr int NO = 8;                    // sums: [2][4] of 32 x 32, or [8] of 16 x 16
-    using Sum = std::conditional_t<kWide, f32x16, f32x4>;
+    constexpr int RB = M / 16;  // blocks of 16 rows
     // one array per stage: the compiler tracks loads to LDS per array
     __shared__ __align__(16) char s0[kTileBytes], s1[kTileBytes], s2[kTileBytes], s3[kTileBytes];
     __shared__ __align__(16) char weights[2][M * kTile * 2];
     __shared__ float tops[2][M];
     __shared__ int late_flags[4];
-    __shared__ int64_t scratch[8];
+    __shared__ int64_t scratch[kWaves + 2];
     char* const ring[4] = {s0, s1, s2, s3};
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int kh = wave & 1, rh = kWide ? wave >> 1 : 0;
-    const int col = lane & 15, grp = lane >> 4;     // of 16 x 16 products
-    const int col32 = lane & 31, half = lane >> 5;  // of 32 x 32 products
+    const int kh = wave & 1, rq = M == 64 ? wave >> 1 : 0;
+    const int col = lane & 15, grp = lane >> 4;
     Walk walk;
     walk.sh = Shares{a.heads, M};
     walk.p = find_piece(a.view, walk.sh, blockIdx.x, scratch);
@@ -377,133 +382,133 @@ __global__ __launch_bounds__(256, 1) void paged_rows_kernel(const TileArgs a) {
         return;
     }
     walk.start(a.view);
-    // The wave loads rows 8 wave .. + 7 of a tile: eight latents, and their rotary
-    // keys in one load, of which this lane takes
-    const int rotary_from = (lane >> 3) * kRowBytes + 1024 + (((lane & 7) ^ ((8 * wave + (lane >> 3)) >> 1 & 7)) << 4);
+    // The wave loads rows 4 wave .. + 3 of a tile: a load for each latent, one of
+    // half a wave for their rotary keys, of which this lane takes
+    const int rotary_from = (lane >> 3) * kRowBytes + 1024 + (((lane & 7) ^ ((4 * wave + (lane >> 3)) >> 1 & 7)) << 4);
     // Where the lane's reads of a tile begin. The scores' k-step ks reads latent
     // unit 4 ks + grp, bits 2 and 3 of which the swizzle changes: ks & 3 is XORed
     // in, the rest is a constant offset; so are channel tiles below. A row of
     // weights is 64 bytes, its four units XORed by row / 4.
     const int key_at = latent_at(16 * kh + col, grp);
     const int rotary_key_at = rotary_at(16 * kh + col, grp);
-    int value_at[2], weight_from[NB], weight_to[NB];
+    int value_at[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        // the first or second four of the lane's eight keys
-        const int r = 8 * (kWide ? half : grp) + 4 * i + ((lane & 15) >> 2);
-        const int u = kWide ? 2 * (lane >> 4 & 1) + ((lane & 3) >> 1) : (lane & 3) >> 1;
-        value_at[i] = latent_at(r, u) + (lane & 1) * 8 + wave * 256;
+        // the first or second four of the lane's eight keys; the wave's 64 channels are eight units
+        const int r = 8 * grp + 4 * i + (col >> 2);
+        value_at[i] = latent_at(r, ((lane & 3) >> 1) + 8 * (wave & 1)) + (lane & 1) * 8 + (wave >> 1) * 256;
     }
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        const int row = kWide ? 32 * b + col32 : col, to = 32 * rh + 16 * b + col;
-        weight_from[b] = row * 64 + (((kWide ? half : grp) ^ (row >> 2 & 3)) << 4);
-        weight_to[b] = to * 64 + (((2 * kh + (grp >> 1)) ^ (to >> 2 & 3)) << 4) + (grp & 1) * 8;
-    }
+    const int weight_from = col * 64 + ((grp ^ (col >> 2 & 3)) << 4);
+    const int score_row = 16 * rq + col;  // this lane's row of the scores
+    const int weight_to = score_row * 64 + (((2 * kh + (grp >> 1)) ^ (score_row >> 2 & 3)) << 4) + (grp & 1) * 8;
+    auto meet = [] {
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // this wave's LDS accesses are done
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    };
     Segment s;
-    while (walk.next(a.view, s)) {
-        const int in_request = s.block * M;  // the block's first row
-        const int64_t row0 = static_cast<int64_t>(s.req.first) * a.heads + in_request;
-        const int rows = min(M, s.req.added * a.heads - in_request);
-        const int32_t last = s.req.cached + s.req.added - 1;
-        const int32_t all_see = s.req.cached + in_request / a.heads;
-        PageWalk pages;
-        pages.start(a.view, s.request);
-        auto issue = [&](int32_t t, char* to) {
-            const int32_t key = t * kTile + 16 * (wave >> 1);
-            const int32_t first = min(key, last & ~15);
-            const char* const base =
-                static_cast<const char*>(a.pool) + pages.at(a.view, a.page_mul, first) * kRowBytes;
-            const __amdgpu_buffer_rsrc_t res =
-                __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 16 * kRowBytes, kBufferWord3);
-            to += wave * kEightBytes;
-            const int eight = 8 * (wave & 1), of = here(lane * 16);
-            if (key + 15 <= last) {
-#pragma unroll
-                for (int r = 0; r < 8; ++r) {
-                    buffer_lds16(res, to + r * 1024, static_cast<unsigned>(of ^ (swizzle(r) | (wave & 1) << 1) << 4),
-                                 static_cast<unsigned>((eight + r) * kRowBytes));
-                }
-                buffer_lds16(res, to + 8192, static_cast<unsigned>(rotary_from),
-                             static_cast<unsigned>(eight * kRowBytes));
-            } else {  // rows past the last key: the last key's once more
-#pragma unroll
-                for (int r = 0; r < 8; ++r) {
-                    buffer_lds16(res, to + r * 1024, static_cast<unsigned>(of ^ (swizzle(r) | (wave & 1) << 1) << 4),
-                                 static_cast<unsigned>((min(key + eight + r, last) - first) * kRowBytes));
-                }
-                const int r = of >> 7;  // lane / 8
-                buffer_lds16(res, to + 8192,
-                             static_cast<unsigned>(rotary_from + (min(key + eight + r, last) - first - r) * kRowBytes),
-                             0);
-            }
-        };
-        auto meet = [] {
-            __builtin_amdgcn_sched_barrier(0);
-            __builtin_amdgcn_s_waitcnt(0xc07f);  // this wave's LDS writes are done
-            __builtin_amdgcn_s_barrier();
-            __builtin_amdgcn_sched_barrier(0);
-        };
-        __syncthreads();  // the block before is done with LDS
-        if (tid < 4) {
-            late_flags[tid] = 0;
+    PageWalk pages;
+    int32_t last = 0;  // key
+    // Tile t's loads in five parts, so that they can be spread between products: a
+    // queue that takes 16 cycles a load would hold up the wave. Of a tile past the
+    // segment's they read nothing.
+    struct Loads {
+        __amdgpu_buffer_rsrc_t res;
+        char* eight;
+        int from, past;
+    };
+    auto prepare = [&](int32_t t, char* to) {
+        const int32_t key = t * kTile + 16 * (wave >> 2);
+        const int32_t first = min(key, last & ~15);
+        // (tiles are prepared in order: the row looked up is this one's)
+        const char* const base = static_cast<const char*>(a.pool) + pages.take(a.view) * kRowBytes;
+        pages.look(a.view, a.page_mul, min(key + kTile, last & ~15));
+        Loads d;
+        d.res = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, t < s.tile1 ? 16 * kRowBytes : 0, kBufferWord3);
+        d.eight = to + (wave >> 1) * kEightBytes;
+        // rows past the last key: the last key's once more
+        d.from = key - first + 4 * (wave & 3);
+        d.past = last - first;
+        return d;
+    };
+    auto load = [&](const Loads& d, int part) {
+        if (part < 4) {
+            buffer_lds16(d.res, d.eight + ((wave & 1) * 4 + part) * 1024,
+                         static_cast<unsigned>(here(lane * 16) ^ swizzle(4 * (wave & 3) + part) << 4),
+                         static_cast<unsigned>(min(d.from + part, d.past) * kRowBytes));
+        } else if (lane < 32) {
+            const int r = lane >> 3;
+            buffer_lds16(d.res, d.eight + 8192 + (wave & 1) * 512,
+                         static_cast<unsigned>(rotary_from + (min(d.from + r, d.past) - r) * kRowBytes), 0);
         }
+    };
+    auto issue = [&](int32_t t, char* to) {
+        const Loads d = prepare(t, to);
+#pragma unroll
+        for (int part = 0; part < 5; ++part) {
+            load(d, part);
+        }
+    };
+    int in_request = 0, rows = 0;  // the block's first row in its request, and its rows
+    int64_t row0 = 0;              // and in the output
+    int32_t all_see = 0, sees = 0;
+    vec8 q[18];
+    // The next block's first tiles and queries.
+    auto open = [&] {
+        in_request = s.block * M;
+        row0 = static_cast<int64_t>(s.req.first) * a.heads + in_request;
+        rows = min(M, s.req.added * a.heads - in_request);
+        last = s.req.cached + s.req.added - 1;
+        pages.start(a.view, s.request);
+        pages.look(a.view, a.page_mul, min(s.tile0 * kTile + 16 * (wave >> 2), last & ~15));
         if (s.tile0 < s.tile1) {
             issue(s.tile0, ring[0]);
         }
         if (s.tile0 + 1 < s.tile1) {
             issue(s.tile0 + 1, ring[1]);
         }
-        int32_t sees[NB];
-        vec8 q[NB][18];
+        const int own = min(score_row, rows - 1);
+        const E* const from_q = static_cast<const E*>(a.q) + (row0 + own) * kWidth + 8 * grp;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const int own = min(32 * rh + 16 * b + col, rows - 1);
-            sees[b] = s.req.cached + (in_request + own) / a.heads;
-            const E* const from_q = static_cast<const E*>(a.q) + (row0 + own) * kWidth + 8 * grp;
-#pragma unroll
-            for (int ks = 0; ks < 18; ++ks) {
-                q[b][ks] = *reinterpret_cast<const vec8*>(from_q + 32 * ks);
-            }
+        for (int ks = 0; ks < 18; ++ks) {
+            q[ks] = *reinterpret_cast<const vec8*>(from_q + 32 * ks);
         }
+        all_see = s.req.cached + in_request / a.heads;
+        sees = s.req.cached + (in_request + own) / a.heads;
+    };
+    bool more = walk.next(a.view, s);
+    if (more) {
+        open();
+    }
+    if (tid < 4) {
+        late_flags[tid] = 0;
+    }
+    while (more) {
         if (a.negative) {
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-#pragma unroll
-                for (int ks = 0; ks < 18; ++ks) {
-                    q[b][ks] = -q[b][ks];
-                }
+            for (int ks = 0; ks < 18; ++ks) {
+                q[ks] = -q[ks];
             }
         }
-        Sum o[NO] = {};
-        f32x4 sc[NB];             // scores of the newest tile
+        f32x4 o[RB][4] = {};
+        f32x4 sc;                 // scores of the newest tile
         float m = kNone;          // reference of row `lane`, the same in every wave
-        float ref[NB], l[NB], sum[NB];  // of this lane's rows: reference times c, total, the newest tile's
+        float ref = kUnset;       // of this lane's row of the scores, times c
+        float l = 0.0f, sum = 0.0f;  // its total, and the newest tile's
+        // the newest tile's weights; tells the others where a score passes the reference
+        auto weigh = [&](char* wt, int u) {
+            vec4 p;
+            float w[4], over = kNone;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            ref[b] = kUnset;
-            l[b] = sum[b] = 0.0f;
-        }
-        // the newest tile's weights; tells whether a score passes the reference
-        auto weigh = [&](char* wt) {
-            float over = kNone;
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                vec4 p;
-                float w[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float x = __builtin_fmaf(sc[b][e], a.c, -ref[b]);
-                    over = fmaxf(over, x);
-                    w[e] = __builtin_amdgcn_exp2f(x);
-                    p[e] = static_cast<E>(w[e]);
-                }
-                sum[b] = (w[0] + w[1]) + (w[2] + w[3]);
-                *reinterpret_cast<vec4*>(wt + weight_to[b]) = p;
+            for (int e = 0; e < 4; ++e) {
+                const float x = __builtin_fmaf(sc[e], a.c, -ref);
+                over = fmaxf(over, x);
+                w[e] = __builtin_amdgcn_exp2f(x);
+                p[e] = static_cast<E>(w[e]);
             }
-            return over;
-        };
-        auto tell = [&](float over, int u) {
+            sum = (w[0] + w[1]) + (w[2] + w[3]);
+            *reinterpret_cast<vec4*>(wt + weight_to) = p;
             if (__builtin_expect(__any(over > kSlack), 0)) {
                 if (lane == 0) {
                     late_flags[u] = 1;
@@ -511,19 +516,16 @@ __global__ __launch_bounds__(256, 1) void paged_rows_kernel(const TileArgs a) {
             }
         };
         // The products of an interval: scores of the tile in `next` (S), context of
-        // the tile in `now` (C), each step's operands read during the one before.
-        // The scores take the first half, so that `weights_of` runs beside the
-        // second half of the context.
+        // the tile in `now` (C), in six steps, each step's operands read during the
+        // one before; `between(i)` runs ahead of step i's products.
         auto products = [&](auto with_scores, const char* next, auto with_context, const char* now, const char* wt,
-                            bool sanitize, auto middle, auto weights_of) {
+                            bool sanitize, auto between) {
             constexpr bool S = decltype(with_scores)::value, C = decltype(with_context)::value;
-            // step i: k-steps 3 i .. + 2 of the scores (i < 6), part `unit(i)` of the context
-            auto unit = [](int i) { return i < 5 ? i : i == 5 ? -1 : i - 1; };
-            vec8 kf[2][3], vf[2], pf[NB];
+            vec8 kf[2][3], vf[2], pf[RB];
             const int k_at = here(key_at), r_at = here(rotary_key_at);
             const int v_at[2] = {here(value_at[0]), here(value_at[1])};
             auto read = [&](int i) {
-                if (S && i < 6) {
+                if constexpr (S) {
 #pragma unroll
                     for (int k = 0; k < 3; ++k) {
                         const int ks = 3 * i + k;
@@ -531,129 +533,92 @@ __global__ __launch_bounds__(256, 1) void paged_rows_kernel(const TileArgs a) {
                             next + (ks < 16 ? (k_at ^ (ks & 3) << 6) + (ks >> 2) * 256 : r_at ^ (ks & 1) << 6));
                     }
                 }
-                const int n = unit(i);
-                if (C && n >= 0) {
-                    // M = 64: keys 16 st .. + 15, channels 32 ct ..; M = 16: all keys, channels 16 ct ..
-                    const int st = kWide ? n / 4 : 0, ct = kWide ? n % 4 : n;
+                if (C && i < 4) {  // channels 16 i ..
                     short8v v;
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        // a channel tile is four units (M = 16: two), a wave's channels 16
-                        const int from_here =
-                            kWide ? (v_at[k] ^ ct << 6) + st * 2 * kEightBytes : v_at[k] ^ ct << 5;
-                        const short4v part = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(now + from_here));
+                        const short4v part =
+                            __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(now + (v_at[k] ^ i << 5)));
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             v[4 * k + e] = part[e];
                         }
                     }
-                    vf[n & 1] = __builtin_bit_cast(vec8, v);
-                }
-            };
-            auto read_weights = [&](int st) {
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    pf[b] = *reinterpret_cast<const vec8*>(wt + (weight_from[b] ^ st * 32));
+                    vf[i & 1] = __builtin_bit_cast(vec8, v);
                 }
             };
             if constexpr (S) {
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    sc[b] = f32x4{};
-                }
+                sc = f32x4{};
             }
             if constexpr (C) {
-                read_weights(0);
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) {
+                    pf[rb] = *reinterpret_cast<const vec8*>(wt + weight_from + rb * 1024);
+                }
             }
             read(0);
-            middle();
 #pragma unroll
-            for (int i = 0; i < 9; ++i) {
-                if (i < 8) {
+            for (int i = 0; i < 6; ++i) {
+                if (i < 5) {
                     read(i + 1);
                 }
-                if (i <= 6) {
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-                const int n = unit(i);
-                if (C && n >= 0) {
-                    vec8 f = vf[n & 1];
+                between(i);
+                __builtin_amdgcn_sched_barrier(0);
+                if (C && i < 4) {
+                    vec8 f = vf[i & 1];
                     if (sanitize) {
                         f = __builtin_bit_cast(vec8, finite_or_zero<E>(__builtin_bit_cast(short8v, f)));
                     }
-                    if constexpr (kWide) {
-                        o[n % 4] = H::mfma32(f, pf[0], o[n % 4]);
-                        o[4 + n % 4] = H::mfma32(f, pf[NB - 1], o[4 + n % 4]);
-                    } else {
-                        o[n] = H::mfma16(f, pf[0], o[n]);
-                    }
-                    if (kWide && n == 3) {
-                        read_weights(1);
+#pragma unroll
+                    for (int rb = 0; rb < RB; ++rb) {
+                        o[rb][i] = H::mfma16(f, pf[rb], o[rb][i]);
                     }
                 }
-                if (S && i < 6) {
+                if constexpr (S) {
 #pragma unroll
                     for (int k = 0; k < 3; ++k) {
-#pragma unroll
-                        for (int b = 0; b < NB; ++b) {
-                            sc[b] = H::mfma16(kf[i & 1][k], q[b][3 * i + k], sc[b]);
-                        }
+                        sc = H::mfma16(kf[i & 1][k], q[3 * i + k], sc);
                     }
                 }
-                if (i < 6) {
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-                if (i == 6) {
-                    weights_of();
-                }
+                __builtin_amdgcn_sched_barrier(0);
             }
-            __builtin_amdgcn_sched_barrier(0);
         };
         const std::true_type yes;
         const std::false_type no;
-        const auto nothing = [] {};
+        const auto nothing = [](int) {};
         auto mask = [&](int32_t t) {
             if (t * kTile + kTile - 1 > all_see) {
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        sc[b][e] = t * kTile + 16 * kh + 4 * grp + e > sees[b] ? kNone : sc[b][e];
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    sc[e] = t * kTile + 16 * kh + 4 * grp + e > sees ? kNone : sc[e];
                 }
             }
         };
         // moves the reference to the rows' largest scores of the newest tile;
         // returns the factor of row `lane`'s sums so far
         auto follow = [&] {
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                float high = fmaxf(fmaxf(sc[b][0], sc[b][1]), fmaxf(sc[b][2], sc[b][3]));
-                high = fmaxf(high, __shfl_xor(high, 16));
-                high = fmaxf(high, __shfl_xor(high, 32));
-                if (grp == 0) {
-                    tops[kh][32 * rh + 16 * b + col] = high;
-                }
+            float high = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
+            high = fmaxf(high, __shfl_xor(high, 16));
+            high = fmaxf(high, __shfl_xor(high, 32));
+            if (grp == 0) {
+                tops[kh][score_row] = high;
             }
             meet();
             const int row = min(lane, rows - 1);  // (rows past the last are the last once more)
             const float up = fmaxf(m, fmaxf(tops[0][row], tops[1][row]));
             const float alpha = up == kNone ? 1.0f : __builtin_amdgcn_exp2f((m - up) * a.c);
             m = up;
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const float mine = __shfl(up, 32 * rh + 16 * b + col);
-                ref[b] = mine == kNone ? kUnset : mine * a.c;
-            }
+            const float mine = __shfl(up, score_row);
+            ref = mine == kNone ? kUnset : mine * a.c;
             return alpha;
         };
-        // tile t's weights and tile t + 1 are in
+        // tile t's weights and tile t + 1 are in: all but tile t + 2's loads have come
         auto arrive = [&](int32_t t) {
             __builtin_amdgcn_sched_barrier(0);
-            if (t + 2 < s.tile1) {
-                __builtin_amdgcn_s_waitcnt(0x0F70 | 9);
-            } else {
+            if (t + 2 >= s.tile1) {
                 __builtin_amdgcn_s_waitcnt(0x0F70);
+            } else {
+                __builtin_amdgcn_s_waitcnt(0x0F70 | 5);
             }
             meet();
         };
@@ -662,10 +627,10 @@ __global__ __launch_bounds__(256, 1) void paged_rows_kernel(const TileArgs a) {
             if (s.tile0 + 2 < s.tile1) {
                 issue(s.tile0 + 2, ring[2]);
             }
-            products(yes, ring[0], no, nullptr, nullptr, false, nothing, nothing);
+            products(yes, ring[0], no, nullptr, nullptr, false, nothing);
             mask(s.tile0);
             follow();
-            weigh(weights[0]);
+            weigh(weights[0], 0);
             // tiles up to here are seen by all rows, and the next one too
             const int32_t full = min(s.tile1 - 1, (all_see + 1) / kTile - 1);
             int32_t t = s.tile0;
@@ -674,7 +639,7 @@ __global__ __launch_bounds__(256, 1) void paged_rows_kernel(const TileArgs a) {
                 // for the loop after this one: the sums are touched by products
                 // alone here, and stay in the registers that products use.
                 int stop = 0;
-                bool here_already = false;
+                bool arrived = false;
                 while (stop == 0) {
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
@@ -683,126 +648,151 @@ __global__ __launch_bounds__(256, 1) void paged_rows_kernel(const TileArgs a) {
                             break;
                         }
                         arrive(t + u);
-                        if (__builtin_expect(late_flags[u] != 0, 0)) {
+                        if (__builtin_expect(__builtin_amdgcn_readfirstlane(late_flags[u]) != 0, 0)) {
                             stop = u + 1;
-                            here_already = true;
+                            arrived = true;
                             break;
                         }
                         if (tid == 0) {
                             late_flags[(u + 2) & 3] = 0;
                         }
-#pragma unroll
-                        for (int b = 0; b < NB; ++b) {
-                            l[b] += sum[b];
-                        }
-                        float over;
-                        products(
-                            yes, ring[(u + 1) & 3], yes, ring[u], weights[u & 1], false,
-                            [&] {
-                                if (t + u + 3 < s.tile1) {
-                                    issue(t + u + 3, ring[(u + 3) & 3]);
-                                }
-                            },
-                            [&] { over = weigh(weights[(u + 1) & 1]); });
-                        tell(over, (u + 1) & 3);
+                        l += sum;
+                        const Loads d = prepare(t + u + 3, ring[(u + 3) & 3]);
+                        products(yes, ring[(u + 1) & 3], yes, ring[u], weights[u & 1], false, [&](int i) {
+                            if (i > 0) {
+                                load(d, i - 1);
+                            }
+                        });
+                        weigh(weights[(u + 1) & 1], (u + 1) & 3);
                     }
                     t += stop == 0 ? 4 : 0;
                 }
+                // one copy of the code for all stages, to which the compiler's
+                // tracking does not reach: it waits for every load here
+#pragma unroll 1
+                for (int u = stop - 1; u < 4 && t + u < s.tile1; ++u) {
+                    if (!arrived) {
+                        arrive(t + u);
+                    }
+                    arrived = false;
+                    auto stage = [&](int i) {
+                        const int at = (i & 3) == 0   ? lds_address(s0)
+                                       : (i & 3) == 1 ? lds_address(s1)
+                                       : (i & 3) == 2 ? lds_address(s2)
+                                                      : lds_address(s3);
+                        return (const char*)(lds_char*)static_cast<uintptr_t>(here(at));
+                    };
+                    if (__builtin_amdgcn_readfirstlane(late_flags[u]) != 0) {
+                        const float alpha = follow();
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    if (u + 1 >= stop && t + u < s.tile1) {
-                        if (u + 1 != stop || !here_already) {
-                            arrive(t + u);
-                        }
-                        if (late_flags[u] != 0) {
-                            const float alpha = follow();
+                        for (int rb = 0; rb < RB; ++rb) {
+                            const float f = __shfl(alpha, 16 * rb + col);
 #pragma unroll
-                            for (int b = 0; b < NB; ++b) {
-                                const float f = __shfl(alpha, kWide ? 32 * b + col32 : col);
-#pragma unroll
-                                for (int i = 0; i < NO / NB; ++i) {
-                                    o[NO / NB * b + i] *= f;
-                                }
+                            for (int ct = 0; ct < 4; ++ct) {
+                                o[rb][ct] *= f;
                             }
-#pragma unroll
-                            for (int b = 0; b < NB; ++b) {
-                                l[b] *= __shfl(alpha, 32 * rh + 16 * b + col);
-                            }
-                            weigh(weights[u & 1]);
-                            meet();
                         }
-                        if (tid == 0) {
-                            late_flags[(u + 2) & 3] = 0;
+                        l *= __shfl(alpha, score_row);
+                        weigh(weights[u & 1], u);
+                        meet();
+                    }
+                    if (tid == 0) {
+                        late_flags[(u + 2) & 3] = 0;
+                    }
+                    l += sum;
+                    if (t + u + 3 < s.tile1) {
+                        if (u == 0) {
+                            issue(t + u + 3, ring[3]);
+                        } else if (u == 1) {
+                            issue(t + u + 3, ring[0]);
+                        } else if (u == 2) {
+                            issue(t + u + 3, ring[1]);
+                        } else {
+                            issue(t + u + 3, ring[2]);
                         }
-#pragma unroll
-                        for (int b = 0; b < NB; ++b) {
-                            l[b] += sum[b];
-                        }
-                        if (t + u + 3 < s.tile1) {
-                            issue(t + u + 3, ring[(u + 3) & 3]);
-                        }
-                        if (t + u + 1 < s.tile1) {
-                            products(yes, ring[(u + 1) & 3], no, nullptr, nullptr, false, nothing, nothing);
-                            mask(t + u + 1);
-                        }
-                        products(no, nullptr, yes, ring[u], weights[u & 1], (t + u) * kTile + kTile - 1 > all_see, nothing,
-                                 nothing);
-                        if (t + u + 1 < s.tile1) {
-                            tell(weigh(weights[(u + 1) & 1]), (u + 1) & 3);
-                        }
+                    }
+                    if (t + u + 1 < s.tile1) {
+                        products(yes, stage(u + 1), no, nullptr, nullptr, false, nothing);
+                        mask(t + u + 1);
+                    }
+                    products(no, nullptr, yes, stage(u), weights[u & 1], (t + u) * kTile + kTile - 1 > all_see, nothing);
+                    if (t + u + 1 < s.tile1) {
+                        weigh(weights[(u + 1) & 1], (u + 1) & 3);
                     }
                 }
                 t += 4;
             }
         }
-        // the totals: the rows' parts of both key halves meet in `tops`
-        __syncthreads();
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            l[b] += __shfl_xor(l[b], 16);
-            l[b] += __shfl_xor(l[b], 32);
-            if (grp == 0) {
-                tops[kh][32 * rh + 16 * b + col] = l[b];
-            }
+        // The totals: the rows' parts of both key halves meet in `tops`. The next
+        // block's loads start before this one's results go out.
+        meet();
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        if (grp == 0) {
+            tops[kh][score_row] = l;
         }
-        __syncthreads();
+        if (tid < 4) {
+            late_flags[tid] = 0;
+        }
         const bool whole = s.begins && s.ends;
+        const int32_t parts_after = s.begins && !s.ends ? s.parts_after : -1;
         const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (s.begins ? 1 : 0);
-        // o[4 rb + ct] register e: channel 128 wave + 32 ct + 8 (e / 4) + 4 half + e % 4
-        // of row 32 rb + col32 (M = 16: o[ct], channel 128 wave + 16 ct + 4 grp + e of row col)
+        const int64_t out_row = row0;
+        const int out_rows = rows;
+        more = walk.next(a.view, s);
+        if (more) {
+            open();
+        }
+        meet();
+        // o[rb][ct] register e: channel 64 wave + 16 ct + 4 grp + e of row 16 rb + col
+        if (whole) {
+            // through LDS (stages 2 and 3: the next block's first tiles are in 0 and
+            // 1), so that rows go out whole; units XORed by row
 #pragma unroll
-        for (int i = 0; i < NO; ++i) {
-            const int row = kWide ? 32 * (i / 4) + col32 : col;
-            if (row < rows) {
-                const float inv = whole ? 1.0f / (tops[0][row] + tops[1][row]) : 1.0f;
-                const int ch = 128 * wave + (kWide ? 32 * (i % 4) + 4 * half : 16 * i + 4 * grp);
+            for (int rb = 0; rb < RB; ++rb) {
+                const int row = min(16 * rb + col, out_rows - 1);
+                const float inv = 1.0f / (tops[0][row] + tops[1][row]);
+                char* const to = (rb < 2 ? s2 : s3) + (16 * (rb & 1) + col) * 1024;
 #pragma unroll
-                for (int g = 0; g < (kWide ? 4 : 1); ++g) {
-                    if (whole) {
-                        vec4 out;
+                for (int ct = 0; ct < 4; ++ct) {
+                    vec4 out;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            out[e] = static_cast<E>(o[i][4 * g + e] * inv);
-                        }
-                        *reinterpret_cast<vec4*>(static_cast<E*>(a.out) + (row0 + row) * kRank + ch + 8 * g) = out;
-                    } else {
-                        f32x4 out;
+                    for (int e = 0; e < 4; ++e) {
+                        out[e] = static_cast<E>(o[rb][ct][e] * inv);
+                    }
+                    *reinterpret_cast<vec4*>(to + (((8 * wave + 2 * ct + (grp >> 1)) ^ col) << 4) + (grp & 1) * 8) = out;
+                }
+            }
+            meet();
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            out[e] = o[i][4 * g + e];
-                        }
-                        *reinterpret_cast<f32x4*>(a.parts.sums + (slot * M + row) * kRank + ch + 8 * g) = out;
+            for (int i = 0; i < M / kWaves; ++i) {
+                const int row = M / kWaves * wave + i;
+                if (row < out_rows) {
+                    const char* const from = (row < 32 ? s2 : s3) + (row & 31) * 1024 + ((lane ^ (row & 15)) << 4);
+                    *reinterpret_cast<u32x4*>(static_cast<E*>(a.out) + (out_row + row) * kRank + 8 * lane) =
+                        *reinterpret_cast<const u32x4*>(from);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+                const int row = 16 * rb + col;
+                if (row < out_rows) {
+                    float* const to = a.parts.sums + (slot * M + row) * kRank + 64 * wave + 4 * grp;
+#pragma unroll
+                    for (int ct = 0; ct < 4; ++ct) {
+                        *reinterpret_cast<f32x4*>(to + 16 * ct) = o[rb][ct];
                     }
                 }
             }
-        }
-        if (!whole && tid < rows) {
-            float* const to = a.parts.stats + (slot * M + tid) * 2;
-            to[0] = m == kNone ? kNone : m * a.c;
-            to[1] = tops[0][tid] + tops[1][tid];
-        }
-        if (s.begins && !s.ends && tid == 0) {
-            a.parts.heads[blockIdx.x] = PartHead{row0, rows, s.parts_after};
+            if (tid < out_rows) {
+                float* const to = a.parts.stats + (slot * M + tid) * 2;
+                to[0] = m == kNone ? kNone : m * a.c;
+                to[1] = tops[0][tid] + tops[1][tid];
+            }
+            if (parts_after >= 0 && tid == 0) {
+                a.parts.heads[blockIdx.x] = PartHead{out_row, out_rows, parts_after};
+            }
         }
     }
 }
@@ -1059,9 +1049,9 @@ hipError_t launch(const PagedAttention& a, void* workspace, hipStream_t s) {
     w += round_up(sizeof(float) * 2 * kGrid * m * 2, 256);
     t.parts.sums = reinterpret_cast<float*>(w);
     if (m == 16) {
-        hipLaunchKernelGGL((paged_rows_kernel<E, 16>), dim3(kGrid), dim3(256), 0, s, t);
+        hipLaunchKernelGGL((paged_rows_kernel<E, 16>), dim3(kGrid), dim3(kThreads), 0, s, t);
     } else {
-        hipLaunchKernelGGL((paged_rows_kernel<E, 64>), dim3(kGrid), dim3(256), 0, s, t);
+        hipLaunchKernelGGL((paged_rows_kernel<E, 64>), dim3(kGrid), dim3(kThreads), 0, s, t);
     }
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) {

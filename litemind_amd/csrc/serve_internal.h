@@ -36,7 +36,7 @@ __device__ inline PagedRequest paged_request(const PagedView& v, int32_t r) {
 
 // A page id of the table: ids outside the pool read page 0 and set the error word.
 __device__ inline int64_t checked_page(const PagedView& v, int32_t page) {
-    if (static_cast<uint32_t>(page) >= static_cast<uint64_t>(v.pages)) {
+    if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(v.pages)) {
         __hip_atomic_store(v.error, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
         return 0;
     }
