@@ -8,9 +8,14 @@
 //   half a unit, 7e-15 of the largest.
 //
 // The kept tokens are a prefix of the order (logit down, index up), found
-// without a sort by descending through the bits of the logits, eight at a time:
-// counts per value of the eight bits give the k-th largest logit, sums of e the
-// one at which top-p is reached.  Equal logits at a cut are told apart by index.
+// without a sort.  A sweep counts the row, or adds up its e, by 2048 equal
+// stretches of the logits' range; the stretch in which the k-th token lies, or
+// top-p is reached, is listed in LDS and searched by the bits of its logits.
+// The kept tokens' e are then added up by stretches of the row's indices, and the
+// stretch that the random number falls into is cut up again until one is left.
+//
+// A row is a workgroup's; its sweeps after the first come from the caches. What
+// they cost is the e: 12 steps of 64-bit arithmetic, 16 cycles of a SIMD for 64.
 #include "serve_internal.h"
 
 namespace lm {
@@ -18,17 +23,19 @@ namespace {
 
 constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / 64;
-constexpr int kBins = 256;
+constexpr int kBins = 2048;  // two a thread where they are added up
+constexpr int kTable = 1024;
+constexpr int kList = 4096;
+constexpr float kMost = 3.4028234663852886e38f;
+constexpr int kSpan = 256;  // what a wave loads at once
 
-// 2^t in units of 2^-bits, to the nearest, for t <= 0: t split into n + f with
-// |f| <= 1/2, 2^f by its power series to the 11th power (cut off at 4e-15), and
-// the unit taken from the double's mantissa next to 2^52.
-__device__ inline uint64_t exp2_units(double t, int bits) {
-    if (!(t > -64.0)) {
-        return 0;
-    }
-    const double n = __builtin_rint(t);
-    const double f = (t - n) * 0.693147180559945309417;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));  // rows of any alignment
+
+// 2^(j / 1024) for 0 <= j < 1024: the root of it over 2^(1/2) by the power series
+// of exp to the 11th power (|f| <= 0.17: f^12 / 12! = 2e-18), squared.
+__device__ inline double exp2_entry(int j) {
+    const double f = (j - kTable / 2) * (0.693147180559945309417 / (2 * kTable));
     double p = 1.0 / 39916800.0;
     p = __builtin_fma(p, f, 1.0 / 3628800.0);
     p = __builtin_fma(p, f, 1.0 / 362880.0);
@@ -41,8 +48,7 @@ __device__ inline uint64_t exp2_units(double t, int bits) {
     p = __builtin_fma(p, f, 0.5);
     p = __builtin_fma(p, f, 1.0);
     p = __builtin_fma(p, f, 1.0);
-    const double scaled = __builtin_ldexp(p, static_cast<int>(n) + bits);
-    return static_cast<uint64_t>(__double_as_longlong(scaled + 0x1p52)) & 0xfffffffffffffull;
+    return j == 0 ? 1.0 : p * p * 1.41421356237309504880;
 }
 
 // Whole numbers in the order of the floats; NaN below -infinity.
@@ -53,246 +59,564 @@ __device__ inline uint32_t order_key(float x) {
     const uint32_t b = __float_as_uint(x + 0.0f);  // -0 as +0
     return (b & 0x80000000u) != 0 ? ~b : b | 0x80000000u;
 }
+__device__ inline float key_float(uint32_t k) { return __uint_as_float((k & 0x80000000u) != 0 ? k & 0x7fffffffu : ~k); }
 constexpr uint32_t kKeyMinusInf = 0x007fffffu;
 
-// What a row's passes share.
-struct Row {
-    const float* x;
-    int32_t n;
-    double top, rate;  // largest logit, log2(e) / temperature
-    int bits;
-    bool top_inf;
-    __device__ uint64_t units(float v) const {
-        if (!(v > -__builtin_inff())) {
-            return 0;
-        }
-        if (top_inf) {
-            return v == __builtin_inff() ? 1ull << bits : 0;
-        }
-        return exp2_units((static_cast<double>(v) - top) * rate, bits);
-    }
+struct Shared {
+    double table[kTable];  // 2^(bits + j / 1024)
+    uint64_t bins[kBins];
+    uint32_t list_key[kList];
+    int32_t list_at[kList];
+    uint64_t part[kWaves];
+    uint64_t found[3];
+    uint32_t key_part[kWaves], key_part2[kWaves];
+    int32_t at_part[kWaves];
+    uint32_t listed;
 };
 
 template <class T, class F>
-__device__ inline T block_reduce(T v, T* part, F f) {
+__device__ inline T wave_reduce(T v, F f) {
     for (int o = 32; o >= 1; o >>= 1) {
         v = f(v, __shfl_xor(v, o));
     }
+    return v;
+}
+template <class T, class F>
+__device__ inline T block_reduce(T v, T* part, F f) {
+    v = wave_reduce(v, f);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) {
         part[threadIdx.x >> 6] = v;
     }
     __syncthreads();
     v = part[0];
+#pragma unroll
     for (int w = 1; w < kWaves; ++w) {
         v = f(v, part[w]);
     }
     return v;
 }
-
-__device__ inline uint64_t block_sum(uint64_t v, uint64_t* part) {
-    return block_reduce(v, part, [](uint64_t a, uint64_t b) { return a + b; });
-}
-
-// The exclusive prefix of v over the workgroup's threads.
-__device__ inline uint64_t block_before(uint64_t v, uint64_t* part) {
+struct Add {
+    __device__ uint64_t operator()(uint64_t a, uint64_t b) const { return a + b; }
+};
+// The exclusive prefix of v over the wave's lanes.
+__device__ inline uint64_t wave_before(uint64_t v) {
     uint64_t sum = v;
     for (int o = 1; o < 64; o <<= 1) {
         const uint64_t up = __shfl_up(sum, o);
-        if ((threadIdx.x & 63) >= static_cast<unsigned>(o)) {
-            sum += up;
-        }
+        sum += (threadIdx.x & 63) >= static_cast<unsigned>(o) ? up : 0;
     }
-    __syncthreads();
-    if ((threadIdx.x & 63) == 63) {
-        part[threadIdx.x >> 6] = sum;
-    }
-    __syncthreads();
-    uint64_t base = 0;
-    for (int w = 0; w < static_cast<int>(threadIdx.x >> 6); ++w) {
-        base += part[w];
-    }
-    return base + sum - v;
+    return sum - v;
 }
 
-// A prefix of the order: keys above `key`, and of those equal to it the
-// `equal` of lowest index.
-struct Cut {
-    uint32_t key;
-    uint64_t equal;
+// What a row's sweeps share.
+struct Row {
+    const float* x;
+    int32_t n;
+    double top, rate;  // largest logit, 1024 log2(e) / temperature
+    float top_f, scale;  // stretches per logit
+    uint64_t one;      // e = 1
+    bool top_inf;
+    const double* table;
+
+    // e in units, to the nearest: t = 1024 log2 e = j + f with |f| <= 1/2; 2^f/1024 by
+    // its power series (cut off at 6e-16), 2^(j / 1024) from the table and the
+    // exponent, the whole number from the mantissa next to 2^52.
+    __device__ uint64_t units_of(double d) const {
+        constexpr double kC1 = 0.693147180559945309417 / kTable, kC2 = kC1 * kC1 / 2, kC3 = kC1 * kC1 * kC1 / 6;
+        const double t = d * rate;
+        const double z = t + 0x1.8p52;
+        const double f = t - (z - 0x1.8p52);
+        const int32_t j = static_cast<int32_t>(__double_as_longlong(z));
+        const double p = f * __builtin_fma(f, __builtin_fma(f, kC3, kC2), kC1);
+        const int64_t whole = __double_as_longlong(table[j & (kTable - 1)]) + (static_cast<int64_t>(j >> 10) << 52);
+        const double e = __longlong_as_double(whole);
+        const uint64_t u = static_cast<uint64_t>(__double_as_longlong(__builtin_fma(e, p, e) + 0x1p52)) & 0xfffffffffffffull;
+        return t > -64.0 * kTable ? u : 0;
+    }
+    __device__ uint64_t units(float v) const {
+        if (top_inf) {
+            return v == __builtin_inff() ? one : 0;
+        }
+        return units_of(static_cast<double>(v) - top);
+    }
+    // The stretch of the range: kBins - 1 at the largest; 0 has no weight at all.
+    __device__ int bin(float v) const {
+        const float d = fminf(fminf(top_f - v, kMost) * scale, static_cast<float>(kBins - 1));
+        return v >= top_f ? kBins - 1 : kBins - 1 - static_cast<int>(d);
+    }
 };
 
-// Descends to the key at which the weight of the keys above it, within
-// `outer`, reaches `want`: the largest key with weight(keys > key) < want <=
-// weight(keys >= key).  Weights: 1 each, or units.  *above: weight(keys > key).
-template <bool MASS>
-__device__ uint32_t descend(const Row& r, uint32_t floor_key, uint64_t want, uint64_t* bins, uint64_t* part,
-                            uint64_t* above) {
-    uint32_t prefix = 0;
-    uint64_t before = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        __syncthreads();
-        for (int b = threadIdx.x; b < kBins; b += kThreads) {
-            bins[b] = 0;
+// f(index, four logits) for the wave's share [from, to) of a row: whole spans
+// but at the row's end, where the missing ones are NaN.
+template <class F>
+__device__ inline void sweep(const Row& r, int32_t from, int32_t to, F f) {
+    const int lane = threadIdx.x & 63;
+    if (r.n < 4) {
+        if (from < to) {
+            f32x4 v = __builtin_nanf("");
+            for (int j = 0; j < r.n; ++j) {
+                v[j] = lane == 0 ? r.x[j] : v[j];
+            }
+            f(4 * lane, v);
         }
-        __syncthreads();
-        for (int32_t i = threadIdx.x; i < r.n; i += kThreads) {
-            const uint32_t key = order_key(r.x[i]);
-            if (key >= floor_key && key > kKeyMinusInf &&
-                (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8)))) {
-                const uint64_t w = MASS ? r.units(r.x[i]) : 1;
-                if (w != 0) {
-                    atomicAdd(reinterpret_cast<unsigned long long*>(&bins[(key >> shift) & 255]), w);
+        return;
+    }
+#pragma unroll 1
+    for (int32_t base = from; base < to; base += 4 * kSpan) {
+        f32x4 v[4];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int32_t i = min(base + g * kSpan + 4 * lane, r.n - 4);
+            v[g] = *reinterpret_cast<const f32x4_any*>(r.x + i);
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int32_t first = base + g * kSpan, i = first + 4 * lane;
+            if (first >= to) {
+                break;
+            }
+            if (first + kSpan > r.n && i > r.n - 4) {
+                // loaded from n - 4: the row's last i .. n - 1 moved down
+                const f32x4 w = v[g];
+                const int past = i - (r.n - 4);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float u = __builtin_nanf("");
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        u = j + past == k ? w[k] : u;
+                    }
+                    v[g][j] = u;
                 }
             }
+            f(i, v[g]);
         }
-        __syncthreads();
-        // the highest bin whose sum from above reaches want
-        const int b = 255 - static_cast<int>(threadIdx.x & 255);
-        const uint64_t own = threadIdx.x < kBins ? bins[b] : 0;
-        const uint64_t ahead = block_before(own, part) + before;
-        __syncthreads();
-        if (threadIdx.x < kBins && ahead < want && ahead + own >= want) {
-            part[kWaves] = static_cast<uint64_t>(b);
-            part[kWaves + 1] = ahead;
-        }
-        __syncthreads();
-        prefix |= static_cast<uint32_t>(part[kWaves]) << shift;
-        before = part[kWaves + 1];
     }
-    *above = before;
-    return prefix;
+}
+// The wave's share of [from, to), whole spans.
+__device__ inline int32_t share_of(int32_t from, int32_t to) {
+    return ((to - from + kWaves - 1) / kWaves + kSpan - 1) / kSpan * kSpan;
+}
+template <class F>
+__device__ inline void sweep_row(const Row& r, F f) {
+    const int32_t share = share_of(0, r.n), from = static_cast<int32_t>(threadIdx.x >> 6) * share;
+    sweep(r, from, min(from + share, r.n), f);
 }
 
+// The bin, from the highest down, at which the bins' sum reaches want.
+struct Found {
+    int bin;
+    uint64_t above, own;  // the sums of the bins above it and of itself
+};
+__device__ inline Found find_bin(Shared& sh, uint64_t want) {
+    __syncthreads();
+    const int b = kBins - 1 - 2 * static_cast<int>(threadIdx.x);
+    const uint64_t hi = sh.bins[b], lo = sh.bins[b - 1], own = hi + lo;
+    uint64_t ahead = wave_before(own);
+    if ((threadIdx.x & 63) == 63) {
+        sh.part[threadIdx.x >> 6] = ahead + own;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        ahead += w < static_cast<int>(threadIdx.x >> 6) ? sh.part[w] : 0;
+    }
+    if (ahead < want && ahead + own >= want) {
+        const bool second = ahead + hi < want;
+        sh.found[0] = static_cast<uint64_t>(second ? b - 1 : b);
+        sh.found[1] = second ? ahead + hi : ahead;
+        sh.found[2] = second ? lo : hi;
+    }
+    __syncthreads();
+    return Found{static_cast<int>(sh.found[0]), sh.found[1], sh.found[2]};
+}
+__device__ inline void clear_bins(Shared& sh) {
+    __syncthreads();
+    sh.bins[threadIdx.x] = sh.bins[threadIdx.x + kThreads] = 0;
+    __syncthreads();
+}
+__device__ inline void add_bin(Shared& sh, int b, uint64_t w) {
+    atomicAdd(reinterpret_cast<unsigned long long*>(&sh.bins[b]), static_cast<unsigned long long>(w));
+}
+
+// The key at which the weight of the keys from the highest down reaches want;
+// each(f) calls f(key, weight) for all, lo and hi are bounds of the keys.
+struct Selected {
+    uint32_t key;
+    uint64_t above, own;  // the weights of the keys above it and of itself
+};
+template <class Each>
+__device__ Selected select(Shared& sh, uint32_t lo, uint32_t hi, uint64_t want, Each each) {
+    int bits = max(32 - __clz(static_cast<int>(lo ^ hi)), 1);
+    uint32_t prefix = bits == 32 ? 0 : hi >> bits << bits;
+    Selected s{hi, 0, 0};
+#pragma unroll 1
+    while (bits > 0) {
+        const int shift = max(bits - 11, 0);
+        clear_bins(sh);
+        each([&](uint32_t key, auto weight) {
+            if (static_cast<uint64_t>(key ^ prefix) >> bits == 0) {
+                add_bin(sh, static_cast<int>(key >> shift & (kBins - 1) & ((1u << (bits - shift)) - 1)), weight());
+            }
+        });
+        const Found f = find_bin(sh, want - s.above);
+        prefix |= static_cast<uint32_t>(f.bin) << shift;
+        s.above += f.above;
+        s.own = f.own;
+        bits = shift;
+    }
+    s.key = prefix;
+    return s;
+}
+
+// The first index up to which the weights add up to more than target, of
+// weights that do in the end.  weigh(index, four logits, four weights) gives them.
+struct Located {
+    int32_t at;
+    uint64_t weight;
+};
+template <class Weigh, class Target>
+__device__ Located locate(Shared& sh, const Row& r, Weigh weigh, Target target_of) {
+    const int wave = threadIdx.x >> 6;
+    int32_t from = 0, to = r.n;
+    uint64_t target = 0;
+    bool first = true;
+    while (first || to - from > kSpan) {
+        const int32_t share = share_of(from, to), mine = from + wave * share;
+        uint64_t sum = 0;
+        sweep(r, min(mine, to), min(mine + share, to), [&](int32_t i, f32x4 v) {
+            uint64_t w[4];
+            weigh(i, v, w);
+            sum += w[0] + w[1] + w[2] + w[3];
+        });
+        sum = wave_reduce(sum, Add());
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) {
+            sh.part[wave] = sum;
+        }
+        __syncthreads();
+        if (first) {
+            uint64_t total = 0;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                total += sh.part[w];
+            }
+            target = target_of(total);
+            first = false;
+        }
+        int w = 0;
+        while (w < kWaves - 1 && target >= sh.part[w]) {
+            target -= sh.part[w];
+            ++w;
+        }
+        from = min(from + w * share, to);
+        to = min(from + share, to);
+    }
+    __syncthreads();
+    if (wave == 0) {
+        sweep(r, from, to, [&](int32_t i, f32x4 v) {
+            uint64_t w[4];
+            weigh(i, v, w);
+            const uint64_t own = w[0] + w[1] + w[2] + w[3];
+            uint64_t before = wave_before(own);
+            if (target >= before && target - before < own) {
+                int at = 0;
+                uint64_t weight = w[0];
+#pragma unroll
+                for (int j = 0; j < 3; ++j) {
+                    if (at == j && target - before >= w[j]) {
+                        before += w[j];
+                        at = j + 1;
+                        weight = w[j + 1];
+                    }
+                }
+                sh.found[0] = static_cast<uint64_t>(i + at);
+                sh.found[1] = weight;
+            }
+        });
+    }
+    __syncthreads();
+    return Located{static_cast<int32_t>(sh.found[0]), sh.found[1]};
+}
+
+// A prefix of the order: keys above `key`, and of those equal to it the ones up
+// to index `last`.
+struct Cut {
+    uint32_t key;
+    int32_t last;
+    __device__ bool keeps(uint32_t k, int32_t i) const { return k > key || (k == key && i <= last); }
+};
+
 __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a, int bits) {
-    __shared__ uint64_t bins[kBins], part[kWaves + 2];
-    __shared__ uint32_t keys[kWaves];
+    __shared__ Shared sh;
     const int64_t row = blockIdx.x;
     const lm_sampling set = a.settings[row];
     Row r;
     r.x = a.logits + row * a.stride;
     r.n = static_cast<int32_t>(a.vocab);
-    r.bits = bits;
-    uint32_t best = 0;
-    for (int32_t i = threadIdx.x; i < r.n; i += kThreads) {
-        best = max(best, order_key(r.x[i]));
-    }
-    best = block_reduce(best, keys, [](uint32_t x, uint32_t y) { return max(x, y); });
-    if (best <= kKeyMinusInf) {
+    r.table = sh.table;
+    r.one = 1ull << bits;
+    sh.table[threadIdx.x] = __builtin_ldexp(exp2_entry(threadIdx.x), bits);
+    // the first of the largest logits, and the least above -infinity
+    float top = -__builtin_inff(), least = __builtin_inff();
+    int32_t top_at = 0x7fffffff;
+    sweep_row(r, [&](int32_t i, f32x4 v) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            top_at = v[j] > top ? i + j : top_at;
+            top = v[j] > top ? v[j] : top;
+            least = v[j] > -__builtin_inff() && v[j] < least ? v[j] : least;
+        }
+    });
+    const float own_top = top;
+    auto larger = [](uint32_t x, uint32_t y) { return max(x, y); };
+    auto smaller = [](uint32_t x, uint32_t y) { return min(x, y); };
+    const uint32_t best = block_reduce(order_key(top), sh.key_part, larger);
+    least = key_float(block_reduce(order_key(least), sh.key_part2, smaller));
+    top = key_float(best);
+    top_at = block_reduce(own_top == top ? top_at : 0x7fffffff, sh.at_part, [](int32_t x, int32_t y) { return min(x, y); });
+    if (best <= kKeyMinusInf || !(set.temperature > 0.0f) || set.min_p > 1.0f) {
         if (threadIdx.x == 0) {
-            a.token[row] = -1;
+            a.token[row] = best <= kKeyMinusInf ? -1 : top_at;
             if (a.probability != nullptr) {
-                a.probability[row] = 0.0f;
+                a.probability[row] = best <= kKeyMinusInf ? 0.0f : 1.0f;
             }
         }
         return;
     }
-    const float top = __uint_as_float((best & 0x80000000u) != 0 ? best & 0x7fffffffu : ~best);
-    const bool greedy = !(set.temperature > 0.0f);
+    const double temperature = static_cast<double>(set.temperature);
     r.top = static_cast<double>(top);
+    r.top_f = top;
     r.top_inf = top == __builtin_inff();
-    r.rate = greedy ? 0.0 : 1.4426950408889634074 / static_cast<double>(set.temperature);
-    // the cut of top-k, then of top-p within it
-    const uint64_t all = ~0ull;
-    Cut cut{kKeyMinusInf + 1, all};
-    if (greedy) {
-        cut = Cut{best, 1};
-    } else {
-        if (set.top_k > 0 && set.top_k < r.n) {
-            uint64_t candidates = 0;
-            for (int32_t i = threadIdx.x; i < r.n; i += kThreads) {
-                candidates += order_key(r.x[i]) > kKeyMinusInf ? 1 : 0;
-            }
-            candidates = block_sum(candidates, part);
-            if (static_cast<uint64_t>(set.top_k) < candidates) {
-                uint64_t above = 0;
-                const uint32_t key = descend<false>(r, 0, static_cast<uint64_t>(set.top_k), bins, part, &above);
-                cut = Cut{key, static_cast<uint64_t>(set.top_k) - above};
-            }
+    r.rate = kTable * 1.4426950408889634074 / temperature;
+    // Logits that lie 48 powers of two under the largest weigh nothing. Up to there,
+    // or to the least one, the range is cut into stretches kBins - 1 .. 1; what lies
+    // further below is in stretch 0.
+    r.scale = fminf((kBins - 2) / fminf(static_cast<float>(48 * 0.6931471805599453 * temperature), top - least), kMost);
+
+    Cut cut{kKeyMinusInf + 1, 0x7fffffff};
+    bool whole = false;  // the list holds all that the cut keeps
+    // listed: those kept that f(stretch) picks
+    auto gather = [&](auto f) {
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            sh.listed = 0;
         }
-        if (set.top_p < 1.0f) {
-            // mass of the prefix: keys above the cut, and `equal` times the cut's
-            uint64_t mass = 0, ties = 0;
-            for (int32_t i = threadIdx.x; i < r.n; i += kThreads) {
-                const uint32_t key = order_key(r.x[i]);
-                mass += key > cut.key ? r.units(r.x[i]) : 0;
-                ties += key == cut.key ? 1 : 0;
-            }
-            mass = block_sum(mass, part);
-            ties = block_sum(ties, part);
-            const uint32_t k = cut.key;
-            const uint64_t each = r.units(__uint_as_float((k & 0x80000000u) != 0 ? k & 0x7fffffffu : ~k));
-            const uint64_t tied = min(cut.equal, ties);
-            const uint64_t total = mass + tied * each;
-            // a token is kept while the mass before it is under top_p of the total
-            const double share = fmax(static_cast<double>(set.top_p), 0.0) * static_cast<double>(total);
-            const uint64_t want = max(static_cast<uint64_t>(__builtin_ceil(share)), uint64_t{1});
-            if (want <= mass) {
-                uint64_t above = 0;
-                const uint32_t key = descend<true>(r, 0, want, bins, part, &above);
-                const uint64_t unit = r.units(__uint_as_float((key & 0x80000000u) != 0 ? key & 0x7fffffffu : ~key));
-                cut = Cut{key, (want - above + unit - 1) / unit};
-            } else if (want <= total) {
-                cut = Cut{cut.key, (want - mass + each - 1) / each};
-            }
-        }
-        if (set.min_p > 1.0f) {
-            cut = Cut{best, 1};
-        } else if (set.min_p > 0.0f) {
-            // the lowest key whose e is at least min_p; the largest logit's always
-            uint32_t lowest = best;
-            for (int32_t i = threadIdx.x; i < r.n; i += kThreads) {
-                const uint32_t key = order_key(r.x[i]);
-                if (key >= cut.key && key > kKeyMinusInf && !r.top_inf &&
-                    exp((static_cast<double>(r.x[i]) - r.top) / static_cast<double>(set.temperature)) >=
-                        static_cast<double>(set.min_p)) {
-                    lowest = min(lowest, key);
+        __syncthreads();
+        sweep_row(r, [&](int32_t i, f32x4 v) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (v[j] > -__builtin_inff() && f(r.bin(v[j]))) {
+                    const uint32_t key = order_key(v[j]);
+                    if (cut.keeps(key, i + j)) {
+                        const uint32_t at = atomicAdd(&sh.listed, 1u);
+                        if (at < kList) {
+                            sh.list_key[at] = key;
+                            sh.list_at[at] = i + j;
+                        }
+                    }
                 }
             }
-            lowest = block_reduce(lowest, keys, [](uint32_t x, uint32_t y) { return min(x, y); });
-            if (lowest > cut.key) {
-                cut = Cut{lowest, all};
-            }
-        }
-    }
-    // the kept tokens in index order, a stretch of the row per thread
-    const int32_t per = (r.n + kThreads - 1) / kThreads;
-    const int32_t i0 = min(static_cast<int32_t>(threadIdx.x) * per, r.n), i1 = min(i0 + per, r.n);
-    uint64_t ties = 0;
-    for (int32_t i = i0; i < i1; ++i) {
-        ties += order_key(r.x[i]) == cut.key ? 1 : 0;
-    }
-    const uint64_t ties_before = block_before(ties, part);
-    auto weight = [&](int32_t i, uint64_t& seen) -> uint64_t {
-        const uint32_t key = order_key(r.x[i]);
-        const bool kept = key > cut.key || (key == cut.key && seen < cut.equal);
-        seen += key == cut.key ? 1 : 0;
-        return kept ? r.units(r.x[i]) : 0;
+        });
+        __syncthreads();
     };
-    uint64_t sum = 0, seen = ties_before;
-    for (int32_t i = i0; i < i1; ++i) {
-        sum += weight(i, seen);
-    }
-    const uint64_t before = block_before(sum, part);
-    const uint64_t total = block_sum(sum, part);
-    // running > u total: over the whole number below it
-    const float u = a.uniform[row];
-    const double at = (u > 0.0f ? static_cast<double>(u) : 0.0) * static_cast<double>(total);
-    const uint64_t target = min(static_cast<uint64_t>(at), total - 1);
-    __syncthreads();
-    if (target >= before && target - before < sum) {
-        uint64_t running = before;
-        seen = ties_before;
-        for (int32_t i = i0; i < i1; ++i) {
-            const uint64_t w = weight(i, seen);
-            running += w;
-            if (running > target) {
-                a.token[row] = i;
-                if (a.probability != nullptr) {
-                    a.probability[row] = static_cast<float>(static_cast<double>(w) / static_cast<double>(total));
+    auto each_listed = [&](auto f) {
+        for (uint32_t t = threadIdx.x; t < sh.listed; t += kThreads) {
+            f(sh.list_key[t], sh.list_at[t]);
+        }
+    };
+    auto listed_bounds = [&](uint32_t& lo, uint32_t& hi) {
+        lo = 0xffffffffu;
+        hi = 0;
+        each_listed([&](uint32_t key, int32_t) {
+            lo = min(lo, key);
+            hi = max(hi, key);
+        });
+        lo = block_reduce(lo, sh.key_part, smaller);
+        hi = block_reduce(hi, sh.key_part2, larger);
+    };
+    // the index of the equal-th of the row's (the list's) logits of that key
+    auto last_listed = [&](uint32_t key, uint64_t equal) {
+        return static_cast<int32_t>(~select(sh, ~static_cast<uint32_t>(r.n), ~0u, equal, [&](auto f) {
+            each_listed([&](uint32_t k, int32_t i) {
+                if (k == key) {
+                    f(~static_cast<uint32_t>(i), [] { return uint64_t{1}; });
                 }
-                break;
+            });
+        }).key);
+    };
+    auto last_in_row = [&](uint32_t key, uint64_t equal) {
+        return locate(sh, r, [&](int32_t, f32x4 v, uint64_t* w) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                w[j] = order_key(v[j]) == key ? 1 : 0;
             }
+        }, [&](uint64_t) { return equal - 1; }).at;
+    };
+
+    if (set.top_k > 0 && set.top_k < r.n) {
+        const uint64_t k = static_cast<uint64_t>(set.top_k);
+        clear_bins(sh);
+        sweep_row(r, [&](int32_t, f32x4 v) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (v[j] > -__builtin_inff()) {
+                    add_bin(sh, r.bin(v[j]), 1);
+                }
+            }
+        });
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            // those of stretch 0 weigh nothing: as well all kept as none
+            sh.bins[0] = 1ull << 40;
+        }
+        const Found f = find_bin(sh, k);
+        if (f.bin > 0) {
+            auto one = [] { return uint64_t{1}; };
+            uint32_t lo, hi;
+            whole = f.above + f.own <= kList;
+            if (f.own <= kList) {
+                gather([&](int b) { return whole ? b >= f.bin : b == f.bin; });
+                listed_bounds(lo, hi);
+                const uint64_t want = whole ? k : k - f.above;
+                const Selected s = select(sh, lo, hi, want, [&](auto add) {
+                    each_listed([&](uint32_t key, int32_t) { add(key, one); });
+                });
+                cut.key = s.key;
+                if (want - s.above < s.own) {
+                    cut.last = last_listed(s.key, want - s.above);
+                }
+            } else {
+                const Selected s = select(sh, kKeyMinusInf + 1, best, k - f.above, [&](auto add) {
+                    sweep_row(r, [&](int32_t, f32x4 v) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            if (v[j] > -__builtin_inff() && r.bin(v[j]) == f.bin) {
+                                add(order_key(v[j]), one);
+                            }
+                        }
+                    });
+                });
+                cut.key = s.key;
+                if (k - f.above - s.above < s.own) {
+                    cut.last = last_in_row(s.key, k - f.above - s.above);
+                }
+            }
+        }
+    }
+    if (set.top_p < 1.0f) {
+        // a token is kept while the e before it are under top_p of the total
+        auto wanted = [&](uint64_t total) {
+            const double part = fmax(static_cast<double>(set.top_p), 0.0) * static_cast<double>(total);
+            return max(static_cast<uint64_t>(__builtin_ceil(part)), uint64_t{1});
+        };
+        auto narrow = [&](const Selected& s, uint64_t want, bool listed) {
+            const uint64_t unit = r.units(key_float(s.key)), equal = (want - s.above + unit - 1) / unit;
+            if (s.key > cut.key) {
+                cut.last = 0x7fffffff;
+            }
+            cut.key = s.key;
+            if (equal * unit < s.own) {
+                cut.last = listed ? last_listed(s.key, equal) : last_in_row(s.key, equal);
+            }
+        };
+        auto listed_mass = [&](auto add) {
+            each_listed([&](uint32_t key, int32_t i) {
+                if (cut.keeps(key, i)) {
+                    add(key, [&] { return r.units(key_float(key)); });
+                }
+            });
+        };
+        uint32_t lo, hi;
+        if (whole) {
+            uint64_t total = 0;
+            listed_mass([&](uint32_t, auto weight) { total += weight(); });
+            total = block_reduce(total, sh.part, Add());
+            const uint64_t want = wanted(total);
+            listed_bounds(lo, hi);
+            const Selected s = select(sh, lo, hi, want, listed_mass);
+            narrow(s, want, true);
+        } else {
+            clear_bins(sh);
+            uint64_t total = 0;
+            sweep_row(r, [&](int32_t i, f32x4 v) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (cut.keeps(order_key(v[j]), i + j)) {
+                        const uint64_t e = r.units(v[j]);
+                        total += e;
+                        if (e != 0) {
+                            add_bin(sh, r.bin(v[j]), e);
+                        }
+                    }
+                }
+            });
+            total = block_reduce(total, sh.part, Add());
+            const uint64_t want = wanted(total);
+            const Found f = find_bin(sh, want);
+            gather([&](int b) { return b == f.bin; });
+            if (sh.listed <= kList) {
+                listed_bounds(lo, hi);
+                const Selected s = select(sh, lo, hi, want - f.above, listed_mass);
+                narrow(s, want - f.above, true);
+            } else {
+                const Selected s = select(sh, cut.key, best, want - f.above, [&](auto add) {
+                    sweep_row(r, [&](int32_t i, f32x4 v) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint32_t key = order_key(v[j]);
+                            if (cut.keeps(key, i + j) && r.bin(v[j]) == f.bin) {
+                                add(key, [&] { return r.units(v[j]); });
+                            }
+                        }
+                    });
+                });
+                narrow(s, want - f.above, false);
+            }
+        }
+    }
+    if (set.min_p > 0.0f) {
+        // the lowest key whose e is at least min_p, between one whose is not and
+        // the largest's, by as many probes as there are threads
+        uint32_t under = kKeyMinusInf, least_kept = best;
+        while (!r.top_inf && least_kept - under > 1) {
+            const uint32_t step = (least_kept - under + kThreads - 1) / kThreads;
+            const uint64_t probe = under + static_cast<uint64_t>(threadIdx.x + 1) * step;
+            const double x = static_cast<double>(key_float(static_cast<uint32_t>(min(probe, static_cast<uint64_t>(least_kept)))));
+            const int fewer = __syncthreads_count(probe < least_kept && !(exp((x - r.top) / temperature) >= static_cast<double>(set.min_p)));
+            under += static_cast<uint32_t>(fewer) * step;
+            least_kept = static_cast<uint32_t>(min(under + static_cast<uint64_t>(step), static_cast<uint64_t>(least_kept)));
+        }
+        if (least_kept > cut.key) {
+            cut = Cut{least_kept, 0x7fffffff};
+        }
+    }
+    uint64_t total = 0;
+    const float least_f = key_float(cut.key);
+    const Located l = locate(sh, r, [&](int32_t i, f32x4 v, uint64_t* w) {
+        bool kept[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            kept[j] = v[j] > least_f || (v[j] == least_f && i + j <= cut.last);
+            w[j] = 0;
+        }
+        if (kept[0] || kept[1] || kept[2] || kept[3]) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                w[j] = kept[j] ? r.units(v[j]) : 0;
+            }
+        }
+    }, [&](uint64_t all) {
+        // running > u total: over the whole number below it
+        const float u = a.uniform[row];
+        total = all;
+        return min(static_cast<uint64_t>((u > 0.0f ? static_cast<double>(u) : 0.0) * static_cast<double>(all)), all - 1);
+    });
+    if (threadIdx.x == 0) {
+        a.token[row] = l.at;
+        if (a.probability != nullptr) {
+            a.probability[row] = static_cast<float>(static_cast<double>(l.weight) / static_cast<double>(total));
         }
     }
 }
