@@ -117,7 +117,7 @@ struct Row {
     float top_f, scale;  // stretches per logit
     uint64_t one;      // e = 1
     bool top_inf;
-    const double* table;
+    const double* table;  // in LDS
 
     // e in units, to the nearest: t = 1024 log2 e = j + f with |f| <= 1/2; 2^f/1024 by
     // its power series (cut off at 6e-16), 2^(j / 1024) from the table and the
@@ -147,50 +147,43 @@ struct Row {
     }
 };
 
-// f(index, four logits) for the wave's share [from, to) of a row: whole spans
-// but at the row's end, where the missing ones are NaN.
-template <class F>
-__device__ inline void sweep(const Row& r, int32_t from, int32_t to, F f) {
-    const int lane = threadIdx.x & 63;
-    if (r.n < 4) {
-        if (from < to) {
-            f32x4 v = __builtin_nanf("");
-            for (int j = 0; j < r.n; ++j) {
-                v[j] = lane == 0 ? r.x[j] : v[j];
+// f(index, four logits) for the wave's share [from, to) of a row: whole spans but
+// at the row's end, past which the logits are NaN.
+__device__ __forceinline__ f32x4 load4(const Row& r, int32_t first, int32_t i) {
+    f32x4 v = __builtin_nanf("");
+    if (first + kSpan <= r.n) {
+        v = *reinterpret_cast<const f32x4_any*>(r.x + i);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (i + j < r.n) {
+                v[j] = r.x[i + j];
             }
-            f(4 * lane, v);
         }
-        return;
     }
+    return v;
+}
+template <class F>
+__device__ __forceinline__ void sweep(const Row& r, int32_t from, int32_t to, F f) {
+    const int lane = threadIdx.x & 63;
+    from = __builtin_amdgcn_readfirstlane(from);
+    to = __builtin_amdgcn_readfirstlane(to);
 #pragma unroll 1
     for (int32_t base = from; base < to; base += 4 * kSpan) {
         f32x4 v[4];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            const int32_t i = min(base + g * kSpan + 4 * lane, r.n - 4);
-            v[g] = *reinterpret_cast<const f32x4_any*>(r.x + i);
+            const int32_t first = base + g * kSpan;
+            if (first < to) {
+                v[g] = load4(r, first, first + 4 * lane);
+            }
         }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            const int32_t first = base + g * kSpan, i = first + 4 * lane;
-            if (first >= to) {
-                break;
+            const int32_t first = base + g * kSpan;
+            if (first < to) {
+                f(first + 4 * lane, v[g]);
             }
-            if (first + kSpan > r.n && i > r.n - 4) {
-                // loaded from n - 4: the row's last i .. n - 1 moved down
-                const f32x4 w = v[g];
-                const int past = i - (r.n - 4);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float u = __builtin_nanf("");
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        u = j + past == k ? w[k] : u;
-                    }
-                    v[g][j] = u;
-                }
-            }
-            f(i, v[g]);
         }
     }
 }
@@ -199,7 +192,7 @@ __device__ inline int32_t share_of(int32_t from, int32_t to) {
     return ((to - from + kWaves - 1) / kWaves + kSpan - 1) / kSpan * kSpan;
 }
 template <class F>
-__device__ inline void sweep_row(const Row& r, F f) {
+__device__ __forceinline__ void sweep_row(const Row& r, F f) {
     const int32_t share = share_of(0, r.n), from = static_cast<int32_t>(threadIdx.x >> 6) * share;
     sweep(r, from, min(from + share, r.n), f);
 }
@@ -240,33 +233,32 @@ __device__ inline void add_bin(Shared& sh, int b, uint64_t w) {
     atomicAdd(reinterpret_cast<unsigned long long*>(&sh.bins[b]), static_cast<unsigned long long>(w));
 }
 
-// The key at which the weight of the keys from the highest down reaches want;
-// each(f) calls f(key, weight) for all, lo and hi are bounds of the keys.
+// The key at which the weight of the keys from the highest down reaches want, by
+// eleven bits at a time; each(f) calls f(key, weight) for all, lo and hi are bounds
+// of the keys.
 struct Selected {
     uint32_t key;
     uint64_t above, own;  // the weights of the keys above it and of itself
 };
 template <class Each>
-__device__ Selected select(Shared& sh, uint32_t lo, uint32_t hi, uint64_t want, Each each) {
+__device__ __forceinline__ Selected select(Shared& sh, uint32_t lo, uint32_t hi, uint64_t want, Each each) {
     int bits = max(32 - __clz(static_cast<int>(lo ^ hi)), 1);
-    uint32_t prefix = bits == 32 ? 0 : hi >> bits << bits;
-    Selected s{hi, 0, 0};
+    Selected s{bits == 32 ? 0 : hi >> bits << bits, 0, 0};
 #pragma unroll 1
     while (bits > 0) {
         const int shift = max(bits - 11, 0);
         clear_bins(sh);
-        each([&](uint32_t key, auto weight) {
-            if (static_cast<uint64_t>(key ^ prefix) >> bits == 0) {
-                add_bin(sh, static_cast<int>(key >> shift & (kBins - 1) & ((1u << (bits - shift)) - 1)), weight());
+        each([&](uint32_t key, uint64_t weight) {
+            if (static_cast<uint64_t>(key ^ s.key) >> bits == 0) {
+                add_bin(sh, static_cast<int>((key ^ s.key) >> shift), weight);
             }
         });
         const Found f = find_bin(sh, want - s.above);
-        prefix |= static_cast<uint32_t>(f.bin) << shift;
+        s.key |= static_cast<uint32_t>(f.bin) << shift;
         s.above += f.above;
         s.own = f.own;
         bits = shift;
     }
-    s.key = prefix;
     return s;
 }
 
@@ -277,7 +269,7 @@ struct Located {
     uint64_t weight;
 };
 template <class Weigh, class Target>
-__device__ Located locate(Shared& sh, const Row& r, Weigh weigh, Target target_of) {
+__device__ __forceinline__ Located locate(Shared& sh, const Row& r, Weigh weigh, Target target_of) {
     const int wave = threadIdx.x >> 6;
     int32_t from = 0, to = r.n;
     uint64_t target = 0;
@@ -315,26 +307,25 @@ __device__ Located locate(Shared& sh, const Row& r, Weigh weigh, Target target_o
     }
     __syncthreads();
     if (wave == 0) {
-        sweep(r, from, to, [&](int32_t i, f32x4 v) {
-            uint64_t w[4];
-            weigh(i, v, w);
-            const uint64_t own = w[0] + w[1] + w[2] + w[3];
-            uint64_t before = wave_before(own);
-            if (target >= before && target - before < own) {
-                int at = 0;
-                uint64_t weight = w[0];
+        const int32_t i = from + 4 * static_cast<int32_t>(threadIdx.x);
+        uint64_t w[4];
+        weigh(i, load4(r, from, i), w);
+        const uint64_t own = w[0] + w[1] + w[2] + w[3];
+        uint64_t before = wave_before(own);
+        if (target >= before && target - before < own) {
+            int at = 0;
+            uint64_t weight = w[0];
 #pragma unroll
-                for (int j = 0; j < 3; ++j) {
-                    if (at == j && target - before >= w[j]) {
-                        before += w[j];
-                        at = j + 1;
-                        weight = w[j + 1];
-                    }
+            for (int j = 0; j < 3; ++j) {
+                if (at == j && target - before >= w[j]) {
+                    before += w[j];
+                    at = j + 1;
+                    weight = w[j + 1];
                 }
-                sh.found[0] = static_cast<uint64_t>(i + at);
-                sh.found[1] = weight;
             }
-        });
+            sh.found[0] = static_cast<uint64_t>(i + at);
+            sh.found[1] = weight;
+        }
     }
     __syncthreads();
     return Located{static_cast<int32_t>(sh.found[0]), sh.found[1]};
@@ -395,185 +386,118 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a, in
     // further below is in stretch 0.
     r.scale = fminf((kBins - 2) / fminf(static_cast<float>(48 * 0.6931471805599453 * temperature), top - least), kMost);
 
+    // The cut of top-k by counts, then that of top-p by sums of e within it.
     Cut cut{kKeyMinusInf + 1, 0x7fffffff};
     bool whole = false;  // the list holds all that the cut keeps
-    // listed: those kept that f(stretch) picks
-    auto gather = [&](auto f) {
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            sh.listed = 0;
+#pragma unroll 1
+    for (int step = 0; step < 2; ++step) {
+        const bool mass = step == 1;
+        if (mass ? !(set.top_p < 1.0f) : set.top_k <= 0 || set.top_k >= r.n) {
+            continue;
         }
-        __syncthreads();
-        sweep_row(r, [&](int32_t i, f32x4 v) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (v[j] > -__builtin_inff() && f(r.bin(v[j]))) {
-                    const uint32_t key = order_key(v[j]);
-                    if (cut.keeps(key, i + j)) {
-                        const uint32_t at = atomicAdd(&sh.listed, 1u);
-                        if (at < kList) {
-                            sh.list_key[at] = key;
-                            sh.list_at[at] = i + j;
-                        }
-                    }
-                }
-            }
-        });
-        __syncthreads();
-    };
-    auto each_listed = [&](auto f) {
-        for (uint32_t t = threadIdx.x; t < sh.listed; t += kThreads) {
-            f(sh.list_key[t], sh.list_at[t]);
-        }
-    };
-    auto listed_bounds = [&](uint32_t& lo, uint32_t& hi) {
-        lo = 0xffffffffu;
-        hi = 0;
-        each_listed([&](uint32_t key, int32_t) {
-            lo = min(lo, key);
-            hi = max(hi, key);
-        });
-        lo = block_reduce(lo, sh.key_part, smaller);
-        hi = block_reduce(hi, sh.key_part2, larger);
-    };
-    // the index of the equal-th of the row's (the list's) logits of that key
-    auto last_listed = [&](uint32_t key, uint64_t equal) {
-        return static_cast<int32_t>(~select(sh, ~static_cast<uint32_t>(r.n), ~0u, equal, [&](auto f) {
-            each_listed([&](uint32_t k, int32_t i) {
-                if (k == key) {
-                    f(~static_cast<uint32_t>(i), [] { return uint64_t{1}; });
-                }
-            });
-        }).key);
-    };
-    auto last_in_row = [&](uint32_t key, uint64_t equal) {
-        return locate(sh, r, [&](int32_t, f32x4 v, uint64_t* w) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                w[j] = order_key(v[j]) == key ? 1 : 0;
-            }
-        }, [&](uint64_t) { return equal - 1; }).at;
-    };
-
-    if (set.top_k > 0 && set.top_k < r.n) {
-        const uint64_t k = static_cast<uint64_t>(set.top_k);
-        clear_bins(sh);
-        sweep_row(r, [&](int32_t, f32x4 v) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (v[j] > -__builtin_inff()) {
-                    add_bin(sh, r.bin(v[j]), 1);
-                }
-            }
-        });
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            // those of stretch 0 weigh nothing: as well all kept as none
-            sh.bins[0] = 1ull << 40;
-        }
-        const Found f = find_bin(sh, k);
-        if (f.bin > 0) {
-            auto one = [] { return uint64_t{1}; };
-            uint32_t lo, hi;
-            whole = f.above + f.own <= kList;
-            if (f.own <= kList) {
-                gather([&](int b) { return whole ? b >= f.bin : b == f.bin; });
-                listed_bounds(lo, hi);
-                const uint64_t want = whole ? k : k - f.above;
-                const Selected s = select(sh, lo, hi, want, [&](auto add) {
-                    each_listed([&](uint32_t key, int32_t) { add(key, one); });
-                });
-                cut.key = s.key;
-                if (want - s.above < s.own) {
-                    cut.last = last_listed(s.key, want - s.above);
-                }
-            } else {
-                const Selected s = select(sh, kKeyMinusInf + 1, best, k - f.above, [&](auto add) {
-                    sweep_row(r, [&](int32_t, f32x4 v) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            if (v[j] > -__builtin_inff() && r.bin(v[j]) == f.bin) {
-                                add(order_key(v[j]), one);
-                            }
-                        }
-                    });
-                });
-                cut.key = s.key;
-                if (k - f.above - s.above < s.own) {
-                    cut.last = last_in_row(s.key, k - f.above - s.above);
-                }
-            }
-        }
-    }
-    if (set.top_p < 1.0f) {
-        // a token is kept while the e before it are under top_p of the total
-        auto wanted = [&](uint64_t total) {
-            const double part = fmax(static_cast<double>(set.top_p), 0.0) * static_cast<double>(total);
-            return max(static_cast<uint64_t>(__builtin_ceil(part)), uint64_t{1});
-        };
-        auto narrow = [&](const Selected& s, uint64_t want, bool listed) {
-            const uint64_t unit = r.units(key_float(s.key)), equal = (want - s.above + unit - 1) / unit;
-            if (s.key > cut.key) {
-                cut.last = 0x7fffffff;
-            }
-            cut.key = s.key;
-            if (equal * unit < s.own) {
-                cut.last = listed ? last_listed(s.key, equal) : last_in_row(s.key, equal);
-            }
-        };
-        auto listed_mass = [&](auto add) {
-            each_listed([&](uint32_t key, int32_t i) {
-                if (cut.keeps(key, i)) {
-                    add(key, [&] { return r.units(key_float(key)); });
-                }
-            });
-        };
-        uint32_t lo, hi;
+        auto weight = [&](float v) { return mass ? r.units(v) : uint64_t{1}; };
+        uint64_t total = 0, above = 0;
+        int stretch = 0;
         if (whole) {
-            uint64_t total = 0;
-            listed_mass([&](uint32_t, auto weight) { total += weight(); });
-            total = block_reduce(total, sh.part, Add());
-            const uint64_t want = wanted(total);
-            listed_bounds(lo, hi);
-            const Selected s = select(sh, lo, hi, want, listed_mass);
-            narrow(s, want, true);
+            for (uint32_t t = threadIdx.x; t < sh.listed; t += kThreads) {
+                total += cut.keeps(sh.list_key[t], sh.list_at[t]) ? weight(key_float(sh.list_key[t])) : 0;
+            }
         } else {
             clear_bins(sh);
-            uint64_t total = 0;
+            const float least_f = key_float(cut.key);
             sweep_row(r, [&](int32_t i, f32x4 v) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    if (cut.keeps(order_key(v[j]), i + j)) {
-                        const uint64_t e = r.units(v[j]);
-                        total += e;
-                        if (e != 0) {
-                            add_bin(sh, r.bin(v[j]), e);
+                    if (v[j] > least_f || (v[j] == least_f && i + j <= cut.last)) {
+                        const uint64_t w = weight(v[j]);
+                        total += w;
+                        if (w != 0) {
+                            add_bin(sh, r.bin(v[j]), w);
                         }
                     }
                 }
             });
-            total = block_reduce(total, sh.part, Add());
-            const uint64_t want = wanted(total);
+        }
+        total = block_reduce(total, sh.part, Add());
+        // a token is kept while the e before it are under top_p of the total
+        const uint64_t want =
+            mass ? max(static_cast<uint64_t>(__builtin_ceil(fmax(static_cast<double>(set.top_p), 0.0) * static_cast<double>(total))), uint64_t{1})
+                 : static_cast<uint64_t>(set.top_k);
+        if (want > total) {
+            continue;
+        }
+        if (!whole) {
             const Found f = find_bin(sh, want);
-            gather([&](int b) { return b == f.bin; });
-            if (sh.listed <= kList) {
-                listed_bounds(lo, hi);
-                const Selected s = select(sh, lo, hi, want - f.above, listed_mass);
-                narrow(s, want - f.above, true);
-            } else {
-                const Selected s = select(sh, cut.key, best, want - f.above, [&](auto add) {
-                    sweep_row(r, [&](int32_t i, f32x4 v) {
+            if (f.bin == 0) {
+                continue;  // those of stretch 0 weigh nothing: as well all kept as none
+            }
+            stretch = f.bin;
+            whole = !mass && f.above + f.own <= kList;
+            above = whole ? 0 : f.above;
+            if (threadIdx.x == 0) {
+                sh.listed = 0;
+            }
+            __syncthreads();
+            sweep_row(r, [&](int32_t i, f32x4 v) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const uint32_t key = order_key(v[j]);
-                            if (cut.keeps(key, i + j) && r.bin(v[j]) == f.bin) {
-                                add(key, [&] { return r.units(v[j]); });
+                for (int j = 0; j < 4; ++j) {
+                    const int b = v[j] > -__builtin_inff() ? r.bin(v[j]) : 0;
+                    if (b == stretch || (whole && b > stretch)) {
+                        const uint32_t key = order_key(v[j]);
+                        if (cut.keeps(key, i + j)) {
+                            const uint32_t at = atomicAdd(&sh.listed, 1u);
+                            if (at < kList) {
+                                sh.list_key[at] = key;
+                                sh.list_at[at] = i + j;
                             }
                         }
-                    });
-                });
-                narrow(s, want - f.above, false);
+                    }
+                }
+            });
+            __syncthreads();
+        }
+        // a stretch of more is read from the row again
+        const bool listed = sh.listed <= kList;
+        uint32_t lo = 0xffffffffu, hi = 0;
+        for (uint32_t t = threadIdx.x; listed && t < sh.listed; t += kThreads) {
+            lo = min(lo, sh.list_key[t]);
+            hi = max(hi, sh.list_key[t]);
+        }
+        lo = listed ? block_reduce(lo, sh.key_part, smaller) : cut.key;
+        hi = listed ? block_reduce(hi, sh.key_part2, larger) : best;
+        // the key at the cut, then, where only some of it are kept, the last one's index
+        uint64_t goal = want - above;
+        uint32_t key = 0;
+#pragma unroll 1
+        for (bool by_index = false;; by_index = true) {
+            const Selected s = select(sh, lo, hi, goal, [&](auto add) {
+                auto one = [&](uint32_t k, int32_t i) {
+                    if (cut.keeps(k, i) && (!by_index || k == key)) {
+                        add(by_index ? ~static_cast<uint32_t>(i) : k, by_index ? uint64_t{1} : weight(key_float(k)));
+                    }
+                };
+                const int32_t many = listed ? static_cast<int32_t>(sh.listed) : r.n;
+                for (int32_t t = threadIdx.x; t < many; t += kThreads) {
+                    if (listed) {
+                        one(sh.list_key[t], sh.list_at[t]);
+                    } else if (r.x[t] > -__builtin_inff() && r.bin(r.x[t]) == stretch) {
+                        one(order_key(r.x[t]), t);
+                    }
+                }
+            });
+            if (by_index) {
+                cut = Cut{key, static_cast<int32_t>(~s.key)};
+                break;
             }
+            key = s.key;
+            const uint64_t unit = weight(key_float(key)), equal = (goal - s.above + unit - 1) / unit;
+            if (equal * unit >= s.own) {
+                cut = Cut{key, key > cut.key ? 0x7fffffff : cut.last};
+                break;
+            }
+            goal = equal;
+            lo = ~static_cast<uint32_t>(r.n);
+            hi = ~0u;
         }
     }
     if (set.min_p > 0.0f) {
