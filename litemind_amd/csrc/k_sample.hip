@@ -27,6 +27,7 @@ constexpr int kBins = 2048;  // two a thread where they are added up
 constexpr int kTable = 1024;
 constexpr int kList = 4096;
 constexpr float kMost = 3.4028234663852886e38f;
+constexpr uint64_t kRaw = 0x4330000000000000ull;  // the bits of 2^52
 constexpr int kSpan = 256;  // what a wave loads at once
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -119,26 +120,38 @@ struct Row {
     bool top_inf;
     const double* table;  // in LDS
 
-    // e in units, to the nearest: t = 1024 log2 e = j + f with |f| <= 1/2; 2^f/1024 by
-    // its power series (cut off at 6e-16), 2^(j / 1024) from the table and the
-    // exponent, the whole number from the mantissa next to 2^52.
-    __device__ uint64_t units_of(double d) const {
+    // e in units, to the nearest, as the bits of e + 2^52: t = 1024 log2 e = j + f with
+    // |f| <= 1/2; 2^(f / 1024) by its power series (cut off at 6e-16), 2^(j / 1024) from
+    // the table and the exponent. Under 2^-64, and for NaN, it is 2^52.
+    __device__ __forceinline__ uint64_t raw(float v) const {
         constexpr double kC1 = 0.693147180559945309417 / kTable, kC2 = kC1 * kC1 / 2, kC3 = kC1 * kC1 * kC1 / 6;
-        const double t = d * rate;
+        const double t = fmax((static_cast<double>(v) - top) * rate, -64.0 * kTable);
         const double z = t + 0x1.8p52;
         const double f = t - (z - 0x1.8p52);
         const int32_t j = static_cast<int32_t>(__double_as_longlong(z));
         const double p = f * __builtin_fma(f, __builtin_fma(f, kC3, kC2), kC1);
         const int64_t whole = __double_as_longlong(table[j & (kTable - 1)]) + (static_cast<int64_t>(j >> 10) << 52);
         const double e = __longlong_as_double(whole);
-        const uint64_t u = static_cast<uint64_t>(__double_as_longlong(__builtin_fma(e, p, e) + 0x1p52)) & 0xfffffffffffffull;
-        return t > -64.0 * kTable ? u : 0;
+        return static_cast<uint64_t>(__double_as_longlong(__builtin_fma(e, p, e) + 0x1p52));
     }
-    __device__ uint64_t units(float v) const {
+    __device__ __forceinline__ uint64_t units(float v) const {
         if (top_inf) {
             return v == __builtin_inff() ? one : 0;
         }
-        return units_of(static_cast<double>(v) - top);
+        return raw(v) - kRaw;
+    }
+    __device__ __forceinline__ void units(f32x4 v, uint64_t* w) const {
+        if (top_inf) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                w[j] = v[j] == __builtin_inff() ? one : 0;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                w[j] = raw(v[j]) - kRaw;
+            }
+        }
     }
     // The stretch of the range: kBins - 1 at the largest; 0 has no weight at all.
     __device__ int bin(float v) const {
@@ -349,27 +362,33 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a, in
     r.table = sh.table;
     r.one = 1ull << bits;
     sh.table[threadIdx.x] = __builtin_ldexp(exp2_entry(threadIdx.x), bits);
-    // the first of the largest logits, and the least above -infinity
-    float top = -__builtin_inff(), least = __builtin_inff();
-    int32_t top_at = 0x7fffffff;
-    sweep_row(r, [&](int32_t i, f32x4 v) {
+    // the largest logit and the least; -infinity, where there is one, and NaN are not
+    // told from each other
+    float own = -__builtin_inff(), least = __builtin_inff();
+    sweep_row(r, [&](int32_t, f32x4 v) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            top_at = v[j] > top ? i + j : top_at;
-            top = v[j] > top ? v[j] : top;
-            least = v[j] > -__builtin_inff() && v[j] < least ? v[j] : least;
+            own = v[j] > own ? v[j] : own;
+            least = v[j] < least ? v[j] : least;
         }
     });
-    const float own_top = top;
     auto larger = [](uint32_t x, uint32_t y) { return max(x, y); };
     auto smaller = [](uint32_t x, uint32_t y) { return min(x, y); };
-    const uint32_t best = block_reduce(order_key(top), sh.key_part, larger);
+    const uint32_t best = block_reduce(order_key(own), sh.key_part, larger);
     least = key_float(block_reduce(order_key(least), sh.key_part2, smaller));
-    top = key_float(best);
-    top_at = block_reduce(own_top == top ? top_at : 0x7fffffff, sh.at_part, [](int32_t x, int32_t y) { return min(x, y); });
+    const float top = key_float(best);
     if (best <= kKeyMinusInf || !(set.temperature > 0.0f) || set.min_p > 1.0f) {
+        int32_t at = 0x7fffffff;
+        if (best > kKeyMinusInf) {
+            sweep_row(r, [&](int32_t i, f32x4 v) {
+                if (v[0] == top || v[1] == top || v[2] == top || v[3] == top) {
+                    at = min(at, i + (v[0] == top ? 0 : v[1] == top ? 1 : v[2] == top ? 2 : 3));
+                }
+            });
+            at = block_reduce(at, sh.at_part, [](int32_t x, int32_t y) { return min(x, y); });
+        }
         if (threadIdx.x == 0) {
-            a.token[row] = best <= kKeyMinusInf ? -1 : top_at;
+            a.token[row] = best <= kKeyMinusInf ? -1 : at;
             if (a.probability != nullptr) {
                 a.probability[row] = best <= kKeyMinusInf ? 0.0f : 1.0f;
             }
@@ -384,11 +403,64 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a, in
     // Logits that lie 48 powers of two under the largest weigh nothing. Up to there,
     // or to the least one, the range is cut into stretches kBins - 1 .. 1; what lies
     // further below is in stretch 0.
-    r.scale = fminf((kBins - 2) / fminf(static_cast<float>(48 * 0.6931471805599453 * temperature), top - least), kMost);
+    r.scale = static_cast<float>(48 * 0.6931471805599453 * temperature);
+    r.scale = fminf((kBins - 2) / (least > -__builtin_inff() ? fminf(r.scale, top - least) : r.scale), kMost);
 
-    // The cut of top-k by counts, then that of top-p by sums of e within it.
     Cut cut{kKeyMinusInf + 1, 0x7fffffff};
-    bool whole = false;  // the list holds all that the cut keeps
+    // Lists the kept ones of a stretch, or of it and those above it; false: too many.
+    auto gather = [&](int stretch, bool upwards) {
+        // a logit under all of them, without their stretches: one stretch more, and
+        // two steps for the roundings
+        const uint32_t under = order_key(top - (kBins + 1 - stretch) / r.scale);
+        const float loose = r.top_inf || stretch == 0 ? -kMost : key_float(max(under, kKeyMinusInf + 3) - 2);
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            sh.listed = 0;
+        }
+        __syncthreads();
+        sweep_row(r, [&](int32_t i, f32x4 v) {
+            if (v[0] >= loose || v[1] >= loose || v[2] >= loose || v[3] >= loose) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t key = order_key(v[j]);
+                    if (cut.keeps(key, i + j)) {
+                        const int b = r.bin(v[j]);
+                        if (b == stretch || (upwards && b > stretch)) {
+                            const uint32_t at = atomicAdd(&sh.listed, 1u);
+                            if (at < kList) {
+                                sh.list_key[at] = key;
+                                sh.list_at[at] = i + j;
+                            }
+                        }
+                    }
+                }
+            }
+        });
+        __syncthreads();
+        return sh.listed <= kList;
+    };
+    auto listed_share = [&](auto f) {
+#pragma unroll 1
+        for (uint32_t t = threadIdx.x; t < sh.listed; t += kThreads) {
+            f(sh.list_key[t], sh.list_at[t]);
+        }
+    };
+    // The list holds all that the cut keeps. For a short row that is any cut; for
+    // top-k of fewer than there are threads, each thread's largest logit bounds the
+    // k-th largest from below.
+    bool whole = r.n <= kList && (set.top_k > 0 || set.top_p < 1.0f);
+    if (whole) {
+        gather(0, true);
+    } else if (set.top_k > 0 && set.top_k <= kThreads) {
+        clear_bins(sh);
+        if (own > -__builtin_inff()) {
+            add_bin(sh, r.bin(own), 1);
+        }
+        if (__syncthreads_count(own > -__builtin_inff()) >= set.top_k) {
+            whole = gather(find_bin(sh, static_cast<uint64_t>(set.top_k)).bin, true);
+        }
+    }
+    // The cut of top-k by counts, then that of top-p by sums of e within it.
 #pragma unroll 1
     for (int step = 0; step < 2; ++step) {
         const bool mass = step == 1;
@@ -399,21 +471,20 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a, in
         uint64_t total = 0, above = 0;
         int stretch = 0;
         if (whole) {
-            for (uint32_t t = threadIdx.x; t < sh.listed; t += kThreads) {
-                total += cut.keeps(sh.list_key[t], sh.list_at[t]) ? weight(key_float(sh.list_key[t])) : 0;
-            }
+            listed_share([&](uint32_t key, int32_t i) { total += cut.keeps(key, i) ? weight(key_float(key)) : 0; });
         } else {
             clear_bins(sh);
             const float least_f = key_float(cut.key);
             sweep_row(r, [&](int32_t i, f32x4 v) {
+                uint64_t w[4] = {1, 1, 1, 1};
+                if (mass) {
+                    r.units(v, w);
+                }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    if (v[j] > least_f || (v[j] == least_f && i + j <= cut.last)) {
-                        const uint64_t w = weight(v[j]);
-                        total += w;
-                        if (w != 0) {
-                            add_bin(sh, r.bin(v[j]), w);
-                        }
+                    if ((v[j] > least_f || (v[j] == least_f && i + j <= cut.last)) && w[j] != 0) {
+                        total += w[j];
+                        add_bin(sh, r.bin(v[j]), w[j]);
                     }
                 }
             });
@@ -426,43 +497,27 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a, in
         if (want > total) {
             continue;
         }
+        bool listed = true;
         if (!whole) {
             const Found f = find_bin(sh, want);
             if (f.bin == 0) {
                 continue;  // those of stretch 0 weigh nothing: as well all kept as none
             }
             stretch = f.bin;
-            whole = !mass && f.above + f.own <= kList;
-            above = whole ? 0 : f.above;
-            if (threadIdx.x == 0) {
-                sh.listed = 0;
+            whole = gather(stretch, true);
+            if (!whole) {
+                above = f.above;
+                listed = gather(stretch, false);
             }
-            __syncthreads();
-            sweep_row(r, [&](int32_t i, f32x4 v) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int b = v[j] > -__builtin_inff() ? r.bin(v[j]) : 0;
-                    if (b == stretch || (whole && b > stretch)) {
-                        const uint32_t key = order_key(v[j]);
-                        if (cut.keeps(key, i + j)) {
-                            const uint32_t at = atomicAdd(&sh.listed, 1u);
-                            if (at < kList) {
-                                sh.list_key[at] = key;
-                                sh.list_at[at] = i + j;
-                            }
-                        }
-                    }
-                }
-            });
-            __syncthreads();
         }
-        // a stretch of more is read from the row again
-        const bool listed = sh.listed <= kList;
         uint32_t lo = 0xffffffffu, hi = 0;
-        for (uint32_t t = threadIdx.x; listed && t < sh.listed; t += kThreads) {
-            lo = min(lo, sh.list_key[t]);
-            hi = max(hi, sh.list_key[t]);
+        if (listed) {
+            listed_share([&](uint32_t key, int32_t) {
+                lo = min(lo, key);
+                hi = max(hi, key);
+            });
         }
+        // a stretch of too many is read from the row again
         lo = listed ? block_reduce(lo, sh.key_part, smaller) : cut.key;
         hi = listed ? block_reduce(hi, sh.key_part2, larger) : best;
         // the key at the cut, then, where only some of it are kept, the last one's index
@@ -477,6 +532,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a, in
                     }
                 };
                 const int32_t many = listed ? static_cast<int32_t>(sh.listed) : r.n;
+#pragma unroll 1
                 for (int32_t t = threadIdx.x; t < many; t += kThreads) {
                     if (listed) {
                         one(sh.list_key[t], sh.list_at[t]);
@@ -504,6 +560,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a, in
         // the lowest key whose e is at least min_p, between one whose is not and
         // the largest's, by as many probes as there are threads
         uint32_t under = kKeyMinusInf, least_kept = best;
+#pragma unroll 1
         while (!r.top_inf && least_kept - under > 1) {
             const uint32_t step = (least_kept - under + kThreads - 1) / kThreads;
             const uint64_t probe = under + static_cast<uint64_t>(threadIdx.x + 1) * step;
@@ -514,33 +571,60 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a, in
         }
         if (least_kept > cut.key) {
             cut = Cut{least_kept, 0x7fffffff};
+            whole = whole || gather(r.bin(key_float(least_kept)), true);
         }
     }
+    // running > u total: over the whole number below it
+    auto target_of = [&](uint64_t total) {
+        const float u = a.uniform[row];
+        return min(static_cast<uint64_t>((u > 0.0f ? static_cast<double>(u) : 0.0) * static_cast<double>(total)), total - 1);
+    };
+    Located drawn;
     uint64_t total = 0;
-    const float least_f = key_float(cut.key);
-    const Located l = locate(sh, r, [&](int32_t i, f32x4 v, uint64_t* w) {
-        bool kept[4];
+    if (whole) {
+        listed_share([&](uint32_t key, int32_t i) { total += cut.keeps(key, i) ? r.units(key_float(key)) : 0; });
+        total = block_reduce(total, sh.part, Add());
+        const Selected s = select(sh, ~static_cast<uint32_t>(r.n), ~0u, target_of(total) + 1, [&](auto add) {
+            listed_share([&](uint32_t key, int32_t i) {
+                if (cut.keeps(key, i)) {
+                    add(~static_cast<uint32_t>(i), r.units(key_float(key)));
+                }
+            });
+        });
+        drawn = Located{static_cast<int32_t>(~s.key), s.own};
+    } else {
+        const float least_f = key_float(cut.key), next_f = key_float(cut.key + 1);
+        drawn = locate(sh, r, [&](int32_t i, f32x4 v, uint64_t* w) {
+            // (a span before the last kept index, after it, or both)
+            const int32_t first = __builtin_amdgcn_readfirstlane(i);
+            const float from = first <= cut.last ? least_f : next_f;
+            if (first <= cut.last && cut.last - first < kSpan) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            kept[j] = v[j] > least_f || (v[j] == least_f && i + j <= cut.last);
-            w[j] = 0;
-        }
-        if (kept[0] || kept[1] || kept[2] || kept[3]) {
+                for (int j = 0; j < 4; ++j) {
+                    v[j] = v[j] == least_f && i + j > cut.last ? __builtin_nanf("") : v[j];
+                }
+            }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                w[j] = kept[j] ? r.units(v[j]) : 0;
+                w[j] = 0;
             }
-        }
-    }, [&](uint64_t all) {
-        // running > u total: over the whole number below it
-        const float u = a.uniform[row];
-        total = all;
-        return min(static_cast<uint64_t>((u > 0.0f ? static_cast<double>(u) : 0.0) * static_cast<double>(all)), all - 1);
-    });
+            const bool kept[4] = {v[0] >= from, v[1] >= from, v[2] >= from, v[3] >= from};
+            if (kept[0] || kept[1] || kept[2] || kept[3]) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    v[j] = kept[j] ? v[j] : __builtin_nanf("");
+                }
+                r.units(v, w);
+            }
+        }, [&](uint64_t all) {
+            total = all;
+            return target_of(all);
+        });
+    }
     if (threadIdx.x == 0) {
-        a.token[row] = l.at;
+        a.token[row] = drawn.at;
         if (a.probability != nullptr) {
-            a.probability[row] = static_cast<float>(static_cast<double>(l.weight) / static_cast<double>(total));
+            a.probability[row] = static_cast<float>(static_cast<double>(drawn.weight) / static_cast<double>(total));
         }
     }
 }
