@@ -504,7 +504,10 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a, in
                 continue;  // those of stretch 0 weigh nothing: as well all kept as none
             }
             stretch = f.bin;
-            whole = gather(stretch, true);
+            // Of 4096 logits in or above it thrown at 1024 threads, 19 threads would get
+            // none; with fewer such threads the list would not hold them.
+            const bool reaches = own > -__builtin_inff() && r.bin(own) >= stretch;
+            whole = __syncthreads_count(reaches) <= kThreads - 19 && gather(stretch, true);
             if (!whole) {
                 above = f.above;
                 listed = gather(stretch, false);
