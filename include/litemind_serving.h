@@ -15,7 +15,8 @@
  * kind on the context, and may be captured into a HIP graph on the context's
  * stream after that (before it, a call under capture is LM_EINVAL).  Replays
  * share the context's scratch: they run on the context's stream, or on another
- * one that waits for it and that it waits for.
+ * one that waits for it and that it waits for.  lm_paged_forward and
+ * lm_paged_decoder_forward refuse capture (LM_EINVAL).
  */
 #ifndef LITEMIND_SERVING_H
 #define LITEMIND_SERVING_H
@@ -89,6 +90,37 @@ int lm_page_plan(lm_context* ctx, const lm_paged_step* step);
  * and the next lm_synchronize or lm_copy_d2h returns LM_EKERNEL.  Asynchronous. */
 int lm_paged_attention(lm_context* ctx, const lm_paged_step* step, const void* q_dev, const void* pool_dev,
                        int32_t dtype, int32_t heads, int32_t rank, int32_t rope, float scale, void* out_dev);
+
+/* ---- the model's layers over the pages ----
+ * Gives every layer of the context a pool of `pages` pages of page_size tokens
+ * in HBM (fp16, 2 (kv_lora_rank + qk_rope) bytes per token and layer: 1152 on
+ * DeepSeek-V2, where lm_attention_configure's cache takes 16640 on V2-Lite).
+ * After lm_attention_configure, once per context.  Needs kv_lora_rank (up to
+ * 1024), qk_nope, hidden_size, q_lora_rank and heads * v_head_dim in multiples of
+ * 32, v_head_dim of 16 and qk_rope of 8.  The pages start as zeros. */
+int lm_paged_configure(lm_context* ctx, int64_t pages, int32_t page_size);
+/* A layer's pool [pages][page_size][kv_lora_rank + qk_rope] fp16, to read or
+ * fill pages (a row: the normalised latent, then the rotated key). */
+int lm_paged_pool(lm_context* ctx, int32_t layer, void** out_dev);
+
+/* lm_attention_forward for the new tokens of all requests of a planned step:
+ * x_dev [tokens, hidden] at the step's positions, their latents stored in the
+ * step's slots of the layer's pool, attention over each request's pages, and
+ * out_dev [tokens, hidden] = o_proj . context, or added to it (accumulate = 1).
+ * The step's pages and page_size are those of lm_paged_configure; max_added,
+ * positions and slots are read too.  Rows past the last new token are computed
+ * from what x_dev holds there, without a store or attention: they neither reach
+ * other rows nor mean anything.  Positions at or past context_length are not
+ * rotated, as lm_attention_forward's.  kv_b_proj is absorbed into the query and
+ * the output; queries, latents and weights round to fp16, within the MFMA
+ * path's tolerance.  out_dev must not overlap x_dev.  Asynchronous. */
+int lm_paged_forward(lm_context* ctx, int32_t layer, const lm_paged_step* step, const float* x_dev, float* out_dev,
+                     int32_t accumulate);
+/* lm_decoder_forward's layer loop with lm_paged_forward as the attention:
+ * hidden_dev [tokens, H] in place.  Rows past the last new token are taken as
+ * zeros; what they come out as means nothing.  `path` as there. */
+int lm_paged_decoder_forward(lm_context* ctx, int32_t first_layer, int32_t last_layer, const lm_paged_step* step,
+                             float* hidden_dev, int32_t path);
 
 /* ---- sampled tokens, beside lm_head_forward's greedy ones ----
  * The settings of one row of logits. */

@@ -193,6 +193,10 @@ PROTOTYPES = {
     "lm_decoder_forward": [_P, _I32, _I32, _P, _I64, _I64, _I32],
     "lm_page_plan": [_P, _P],
     "lm_paged_attention": [_P, _P, _P, _P, _I32, _I32, _I32, _I32, _F, _P],
+    "lm_paged_configure": [_P, _I64, _I32],
+    "lm_paged_pool": [_P, _I32, _P],
+    "lm_paged_forward": [_P, _I32, _P, _P, _P, _I32],
+    "lm_paged_decoder_forward": [_P, _I32, _I32, _P, _P, _I32],
     "lm_sample": [_P, _P, _I64, _I64, _I64, _P, _P, _P, _P],
 }
 _RESTYPE = {"lm_last_error": C.c_char_p}
@@ -549,6 +553,24 @@ class Context:
         """Latent attention of the step's tokens over their requests' pages (lm_paged_attention)."""
         self._check(self.lib.lm_paged_attention(self.handle, C.byref(step), _ptr(q), _ptr(pool), dtype, heads, rank,
                                                 rope, scale, _ptr(out)))
+
+    def paged_configure(self, pages: int, page_size: int = 64) -> None:
+        """A pool of latent pages for every layer of the context (lm_paged_configure)."""
+        self._check(self.lib.lm_paged_configure(self.handle, pages, page_size))
+
+    def paged_pool(self, layer: int) -> int:
+        """Device address of a layer's pool [pages][page_size][kv_lora_rank + qk_rope] fp16 (lm_paged_pool)."""
+        out = C.c_void_p()
+        self._check(self.lib.lm_paged_pool(self.handle, layer, C.byref(out)))
+        return out.value
+
+    def paged_forward(self, layer: int, step: PagedStep, x, out, accumulate: bool = False) -> None:
+        """A layer's attention for the new tokens of a planned step's requests (lm_paged_forward)."""
+        self._check(self.lib.lm_paged_forward(self.handle, layer, C.byref(step), _ptr(x), _ptr(out), int(accumulate)))
+
+    def paged_decoder_forward(self, first: int, last: int, step: PagedStep, hidden, path: int = PATH_AUTO) -> None:
+        """The layer loop for the new tokens of a planned step's requests (lm_paged_decoder_forward)."""
+        self._check(self.lib.lm_paged_decoder_forward(self.handle, first, last, C.byref(step), _ptr(hidden), path))
 
     def sample(self, logits, rows: int, vocab: int, settings, uniform, token, probability=None,
                row_stride: int = 0) -> None:

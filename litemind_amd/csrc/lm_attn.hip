@@ -28,9 +28,13 @@
 // (lm_attention_set_score_budget, default 1 GiB) for the scores (and the MFMA
 // core's fp16 copies), so a long cache takes smaller groups instead of failing
 // to allocate.
+//
+// lm_paged_forward and lm_paged_decoder_forward (litemind_serving.h) run the same
+// weights for many requests over pages of latents: the projections of k_proj.hip,
+// kv_b_proj absorbed and the latents stored by k_latent.hip, k_paged.hip's core.
 #include "litemind_attention.h"
 #include "lm_error.h"
-#include "lm_internal.h"
+#include "serve_internal.h"
 
 #include <algorithm>
 #include <cmath>
@@ -68,6 +72,7 @@ struct AttnLayer {
     float* input_norm = nullptr;  // [H], lm_decoder_forward
     KvCacheDev cache;
     int64_t count = 0;  // KvCache::token_count
+    _Float16* absorbed = nullptr;  // kv_b's key halves for the pages, panels [heads rank][nope]
 };
 
 // Projections in the order of AttnLayer::table16.
@@ -90,6 +95,9 @@ struct AttnState {
     float* xn = nullptr;      // lm_decoder_forward: normalised rows [T, H]
     size_t xn_floats = 0;
     int64_t score_budget = 0; // bytes of the attention core's scratch (0: the default)
+    _Float16* pools = nullptr; // lm_paged_configure: [layers][pages][page_size][rank + rope]
+    int64_t pages = 0;
+    int32_t page_size = 0;
 };
 
 void attention_release(AttnState* st) {
@@ -100,7 +108,9 @@ void attention_release(AttnState* st) {
         (void)hipFree(L.slab);
         (void)hipFree(L.slab16);
         (void)hipFree(L.input_norm);
+        (void)hipFree(L.absorbed);
     }
+    (void)hipFree(st->pools);
     if (st->fork != nullptr) {
         (void)hipEventDestroy(st->fork);
     }
@@ -628,6 +638,214 @@ int attention_tokens(AttnState* st, hipStream_t stream, int32_t layer, const flo
     return LM_OK;
 }
 
+// The layer's kv_b_proj taken apart for the pages, once per upload.
+int absorb(AttnState* st, AttnLayer& L, int32_t layer, hipStream_t stream) {
+    if (L.kv_a == nullptr) {
+        return fail(LM_ENOTRES, "layer " + std::to_string(layer) + " has no attention weights (lm_upload_attention)");
+    }
+    if (L.table16 == nullptr) {
+        return fail(LM_EINVAL, "layer " + std::to_string(layer) + ": a weight outside fp16's range, or a width that is "
+                                   "not a multiple of 32, keeps it from the pages");
+    }
+    if (L.absorbed != nullptr) {
+        return LM_OK;
+    }
+    const lm_mla_config& c = st->cfg;
+    const size_t bytes = sizeof(_Float16) * c.num_heads * c.qk_nope_head_dim * static_cast<size_t>(c.kv_lora_rank);
+    if (hipMalloc(reinterpret_cast<void**>(&L.absorbed), bytes) != hipSuccess) {
+        (void)hipGetLastError();
+        L.absorbed = nullptr;
+        return fail(LM_ENOMEM, "absorbed weights of layer " + std::to_string(layer));
+    }
+    LM_ATT_HIP(lm::launch_absorb(L.w16[lm::kProjKvb], L.absorbed, c.num_heads, c.qk_nope_head_dim, c.v_head_dim,
+                                 c.kv_lora_rank, stream));
+    return LM_OK;
+}
+
+// What both paged entry points need of the context and the step.
+int check_paged(lm_context* ctx, const lm_paged_step* step, AttnState** out) {
+    int rc = lm::check_step_sizes(step);
+    if (rc == LM_OK) {
+        rc = get_state(ctx, out);
+    }
+    if (rc != LM_OK) {
+        return rc;
+    }
+    const AttnState* st = *out;
+    if (st->pools == nullptr) {
+        return fail(LM_EINVAL, "the pages are not configured (lm_paged_configure)");
+    }
+    if (step->pages != st->pages || step->page_size != st->page_size) {
+        return fail(LM_EINVAL, "the step's pages differ from the " + std::to_string(st->pages) + " of " +
+                                   std::to_string(st->page_size) + " tokens of lm_paged_configure");
+    }
+    const lm_mla_config& c = st->cfg;
+    const int64_t widest = std::max({static_cast<int64_t>(c.hidden_size), static_cast<int64_t>(c.q_lora_rank),
+                                     static_cast<int64_t>(c.num_heads) * c.v_head_dim});
+    if (step->tokens * widest > INT32_MAX / 2 || step->tokens * c.num_heads > INT32_MAX) {
+        return fail(LM_EINVAL, "too many tokens in one step");
+    }
+    if (step->tokens == 0) {
+        return LM_OK;
+    }
+    for (const int32_t* p : {static_cast<const int32_t*>(step->table), static_cast<const int32_t*>(step->lengths),
+                             static_cast<const int32_t*>(step->starts), static_cast<const int32_t*>(step->positions),
+                             static_cast<const int32_t*>(step->slots)}) {
+        if (p == nullptr || reinterpret_cast<uintptr_t>(p) % 4 != 0) {
+            return fail(LM_EINVAL, "a null or misaligned array of the step");
+        }
+    }
+    const lm::ContextInfo info = lm::context_info(ctx);
+    LM_ATT_HIP(hipSetDevice(info.device));
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    LM_ATT_HIP(hipStreamIsCapturing(info.stream, &capture));
+    if (capture != hipStreamCaptureStatusNone) {
+        return fail(LM_EINVAL, "the model's layers over pages cannot be captured");
+    }
+    return LM_OK;
+}
+
+// A layer's attention for a step's tokens over its pages; as attention_tokens, x
+// may be `out` with in_norm.
+int attention_paged(lm_context* ctx, AttnState* st, int32_t layer, const lm_paged_step& step, const float* x,
+                    float* out, int32_t accumulate, const float* in_norm) {
+    const lm::ContextInfo info = lm::context_info(ctx);
+    const hipStream_t stream = info.stream;
+    const lm_mla_config& c = st->cfg;
+    const lm::AttnShape& a = st->shape;
+    AttnLayer& L = st->layers[static_cast<size_t>(layer)];
+    int rc = absorb(st, L, layer, stream);
+    if (rc != LM_OK) {
+        return rc;
+    }
+    const int64_t T = step.tokens, H = c.hidden_size, heads = c.num_heads, nope = c.qk_nope_head_dim,
+                  rope = c.qk_rope_head_dim, qk = nope + rope, rank = c.kv_lora_rank, vh = c.v_head_dim,
+                  ql = c.q_lora_rank;
+    size_t total_f = 0;
+    auto region = [&](int64_t floats) {
+        const size_t at = total_f;
+        total_f += static_cast<size_t>((floats + 63) / 64 * 64);
+        return at;
+    };
+    auto halves = [](int64_t n) { return (n + 1) / 2; };
+    const size_t x16_at = region(halves(T * H));
+    const size_t q_at = region(T * heads * qk);
+    const size_t ql_at = region(T * ql);
+    const size_t ql16_at = region(halves(T * ql));
+    const size_t lat_at = region(T * (rank + rope));
+    const size_t q16_at = region(halves(T * heads * (rank + rope)));
+    const size_t ctx16_at = region(halves(T * heads * rank));
+    const size_t v16_at = region(halves(T * heads * vh));
+    rc = ensure_buffer(&st->ws, &st->ws_floats, stream, total_f);
+    if (rc != LM_OK) {
+        return rc;
+    }
+    float* const ws = st->ws;
+    auto h16 = [&](size_t at) { return reinterpret_cast<_Float16*>(ws + at); };
+    lm::ProjArgs p;
+    p.tokens = T;
+    p.heads = a.heads;
+    auto segment = [&](int proj, int64_t rows, float* to, int32_t add) {
+        lm::ProjSegment seg;
+        seg.w = L.w16[proj];
+        seg.rows = static_cast<int32_t>(rows);
+        seg.kind = lm::kProjPlain;
+        seg.out = to;
+        seg.accumulate = add;
+        return seg;
+    };
+    if (in_norm != nullptr) {
+        LM_ATT_HIP(lm::launch_norm16(x, in_norm, h16(x16_at), T, static_cast<int32_t>(H), c.rms_norm_eps, stream));
+    } else {
+        LM_ATT_HIP(lm::launch_to_f16_rows(x, h16(x16_at), T, static_cast<int32_t>(H), static_cast<int32_t>(H),
+                                          stream));
+    }
+    // queries (src/Attention.cpp:33-48) and the compressed keys and values (:50-56)
+    p.x16 = h16(x16_at);
+    p.width = static_cast<int32_t>(H);
+    p.seg[0] = ql == 0 ? segment(lm::kProjQ, heads * qk, ws + q_at, 0) : segment(lm::kProjQa, ql, ws + ql_at, 0);
+    p.seg[1] = segment(lm::kProjKva, rank + rope, ws + lat_at, 0);
+    LM_ATT_HIP(lm::launch_proj(p, stream));
+    p.seg[1] = lm::ProjSegment{};
+    if (ql != 0) {
+        LM_ATT_HIP(lm::launch_norm16(ws + ql_at, L.q_a_norm, h16(ql16_at), T, static_cast<int32_t>(ql),
+                                     c.rms_norm_eps, stream));
+        p.x16 = h16(ql16_at);
+        p.width = static_cast<int32_t>(ql);
+        p.seg[0] = segment(lm::kProjQb, heads * qk, ws + q_at, 0);
+        LM_ATT_HIP(lm::launch_proj(p, stream));
+    }
+    // the latents into their slots (:57-75), the queries' rotary part, and the rest
+    // through kv_b's key halves
+    const int32_t* const live = step.starts + step.requests;
+    _Float16* const pool = st->pools + static_cast<int64_t>(layer) * st->pages * st->page_size * (rank + rope);
+    lm::LatentArgs r;
+    r.tokens = T;
+    r.heads = a.heads;
+    r.nope = a.nope;
+    r.rope = a.rope;
+    r.rank = static_cast<int32_t>(rank);
+    r.q = ws + q_at;
+    r.lat = ws + lat_at;
+    r.norm = L.kv_a_norm;
+    r.eps = c.rms_norm_eps;
+    r.positions = step.positions;
+    r.slots = step.slots;
+    r.live = live;
+    r.max_positions = a.max_positions;
+    r.cos_t = a.cos_t;
+    r.sin_t = a.sin_t;
+    r.pool = pool;
+    r.pool_rows = st->pages * st->page_size;
+    r.q16 = h16(q16_at);
+    LM_ATT_HIP(lm::launch_latent_rows(r, stream));
+    lm::HeadsArgs g;
+    g.tokens = T;
+    g.heads = a.heads;
+    g.K = a.nope;
+    g.N = static_cast<int32_t>(rank);
+    g.x = ws + q_at;
+    g.x_f32 = 1;
+    g.x_token = heads * qk;
+    g.x_head = qk;
+    g.w = L.absorbed;
+    g.w_rows = heads * rank;
+    g.w_head = static_cast<int32_t>(rank);
+    g.w_first = 0;
+    g.out = h16(q16_at);
+    g.out_panels = 0;
+    g.out_token = heads * (rank + rope);
+    g.out_head = rank + rope;
+    g.live = nullptr;
+    LM_ATT_HIP(lm::launch_heads(g, stream));
+    // causal attention over the pages (:77-98), kv_b's value halves
+    rc = lm_paged_attention(ctx, &step, h16(q16_at), pool, LM_DT_F16, a.heads, static_cast<int32_t>(rank), a.rope,
+                            st->scale, h16(ctx16_at));
+    if (rc != LM_OK) {
+        return rc;
+    }
+    g.K = static_cast<int32_t>(rank);
+    g.N = a.vh;
+    g.x = h16(ctx16_at);
+    g.x_f32 = 0;
+    g.x_token = heads * rank;
+    g.x_head = rank;
+    g.w = L.w16[lm::kProjKvb];
+    g.w_rows = heads * (nope + vh);
+    g.w_head = static_cast<int32_t>(nope + vh);
+    g.w_first = a.nope;
+    g.out = h16(v16_at);
+    g.out_panels = 1;
+    g.live = live;
+    LM_ATT_HIP(lm::launch_heads(g, stream));
+    // output projection (:100-101)
+    p.x16 = h16(v16_at);
+    p.width = static_cast<int32_t>(heads * vh);
+    p.seg[0] = segment(lm::kProjO, H, out, accumulate);
+    LM_ATT_HIP(lm::launch_proj(p, stream));
+    return LM_OK;
+}
+
 int upload(hipStream_t stream, void* dst, const void* src, size_t bytes) {
     LM_ATT_HIP(hipMemcpyAsync(dst, src, bytes, hipMemcpyHostToDevice, stream));
     return LM_OK;
@@ -922,6 +1140,8 @@ int lm_upload_attention(lm_context* ctx, int32_t layer, const uint16_t* q_proj_h
     (void)hipFree(L.slab);
     L.slab = nullptr;
     L.kv_a = nullptr;
+    (void)hipFree(L.absorbed);
+    L.absorbed = nullptr;
     hipError_t err = hipMalloc(&L.slab, static_cast<size_t>(total));
     if (err != hipSuccess) {
         return fail(LM_ENOMEM, "attention weights of layer " + std::to_string(layer) + ": " + hipGetErrorString(err));
@@ -1282,6 +1502,143 @@ int lm_decoder_forward(lm_context* ctx, int32_t first_layer, int32_t last_layer,
             return fail(LM_EFULL, "the KV cache is full (" + std::to_string(st->cfg.context_length) + " tokens)");
         }
         return LM_OK;
+    } catch (const std::bad_alloc&) {
+        return fail(LM_ENOMEM, "host allocation failed");
+    }
+}
+
+int lm_paged_configure(lm_context* ctx, int64_t pages, int32_t page_size) {
+    if (page_size < 16 || page_size > 4096 || page_size % 16 != 0) {
+        return fail(LM_EINVAL, "page_size must be a multiple of 16 up to 4096");
+    }
+    if (pages < 1 || pages > INT32_MAX || pages * page_size > INT32_MAX) {
+        return fail(LM_EINVAL, "the pool must hold 1 page at least and 2^31 - 1 tokens at most");
+    }
+    AttnState* st = nullptr;
+    const int rc = get_state(ctx, &st);
+    if (rc != LM_OK) {
+        return rc;
+    }
+    const lm_mla_config& c = st->cfg;
+    if (c.kv_lora_rank % 32 != 0 || c.kv_lora_rank > 1024 || c.qk_nope_head_dim < 32 || c.qk_nope_head_dim % 32 != 0 ||
+        c.v_head_dim % 16 != 0 || c.qk_rope_head_dim % 8 != 0 || c.hidden_size % 32 != 0 || c.q_lora_rank % 32 != 0 ||
+        c.num_heads * c.v_head_dim % 32 != 0) {
+        return fail(LM_EINVAL, "pages need kv_lora_rank (up to 1024), qk_nope, hidden_size, q_lora_rank and heads * "
+                               "v_head_dim in multiples of 32, v_head_dim of 16, qk_rope of 8");
+    }
+    if (st->pools != nullptr) {
+        return fail(LM_EINVAL, "the pages are already configured for this context");
+    }
+    const lm::ContextInfo info = lm::context_info(ctx);
+    LM_ATT_HIP(hipSetDevice(info.device));
+    const size_t bytes = sizeof(_Float16) * static_cast<size_t>(info.layers) * static_cast<size_t>(pages * page_size) *
+                         static_cast<size_t>(c.kv_lora_rank + c.qk_rope_head_dim);
+    hipError_t err = hipMalloc(reinterpret_cast<void**>(&st->pools), bytes);
+    if (err != hipSuccess) {
+        (void)hipGetLastError();
+        st->pools = nullptr;
+        return fail(LM_ENOMEM, "pages (" + std::to_string(bytes) + " bytes): " + hipGetErrorString(err));
+    }
+    err = hipMemset(st->pools, 0, bytes);
+    if (err == hipSuccess) {
+        err = hipDeviceSynchronize();
+    }
+    if (err != hipSuccess) {
+        (void)hipFree(st->pools);
+        st->pools = nullptr;
+        return fail(LM_EHIP, std::string("pages: ") + hipGetErrorString(err));
+    }
+    st->pages = pages;
+    st->page_size = page_size;
+    return LM_OK;
+}
+
+int lm_paged_pool(lm_context* ctx, int32_t layer, void** out_dev) {
+    if (out_dev == nullptr) {
+        return fail(LM_EINVAL, "null output");
+    }
+    AttnState* st = nullptr;
+    int rc = get_state(ctx, &st);
+    if (rc == LM_OK) {
+        rc = check_attn_layer(st, layer);
+    }
+    if (rc != LM_OK) {
+        return rc;
+    }
+    if (st->pools == nullptr) {
+        return fail(LM_EINVAL, "the pages are not configured (lm_paged_configure)");
+    }
+    *out_dev = st->pools + static_cast<int64_t>(layer) * st->pages * st->page_size *
+                               (st->cfg.kv_lora_rank + st->cfg.qk_rope_head_dim);
+    return LM_OK;
+}
+
+int lm_paged_forward(lm_context* ctx, int32_t layer, const lm_paged_step* step, const float* x_dev, float* out_dev,
+                     int32_t accumulate) {
+    try {
+        AttnState* st = nullptr;
+        int rc = check_paged(ctx, step, &st);
+        if (rc == LM_OK) {
+            rc = check_attn_layer(st, layer);
+        }
+        if (rc != LM_OK || step->tokens == 0) {
+            return rc;
+        }
+        if (x_dev == nullptr || out_dev == nullptr) {
+            return fail(LM_EINVAL, "null input or output");
+        }
+        const size_t row_bytes = sizeof(float) * static_cast<size_t>(st->cfg.hidden_size) * static_cast<size_t>(step->tokens);
+        const char* xb = reinterpret_cast<const char*>(x_dev);
+        const char* ob = reinterpret_cast<const char*>(out_dev);
+        if (xb < ob + row_bytes && ob < xb + row_bytes) {
+            return fail(LM_EINVAL, "out_dev overlaps x_dev");
+        }
+        return attention_paged(ctx, st, layer, *step, x_dev, out_dev, accumulate, nullptr);
+    } catch (const std::bad_alloc&) {
+        return fail(LM_ENOMEM, "host allocation failed");
+    }
+}
+
+int lm_paged_decoder_forward(lm_context* ctx, int32_t first_layer, int32_t last_layer, const lm_paged_step* step,
+                             float* hidden_dev, int32_t path) {
+    try {
+        AttnState* st = nullptr;
+        int rc = check_paged(ctx, step, &st);
+        if (rc == LM_OK) {
+            rc = check_attn_layer(st, first_layer);
+        }
+        if (rc == LM_OK) {
+            rc = check_attn_layer(st, last_layer);
+        }
+        if (rc != LM_OK) {
+            return rc;
+        }
+        if (first_layer > last_layer) {
+            return fail(LM_EINVAL, "first_layer > last_layer");
+        }
+        if (step->tokens == 0) {
+            return LM_OK;
+        }
+        if (hidden_dev == nullptr) {
+            return fail(LM_EINVAL, "null hidden state");
+        }
+        for (int32_t l = first_layer; l <= last_layer; ++l) {
+            const AttnLayer& L = st->layers[static_cast<size_t>(l)];
+            if (L.input_norm == nullptr || L.kv_a == nullptr) {
+                return fail(LM_ENOTRES, "layer " + std::to_string(l) + " has no attention weights or input norm");
+            }
+        }
+        // what the caller left in rows past the last new token must not steer the experts
+        const lm::ContextInfo info = lm::context_info(ctx);
+        LM_ATT_HIP(lm::launch_clear_rows(hidden_dev, step->starts + step->requests, step->tokens, info.hidden,
+                                         info.stream));
+        for (int32_t l = first_layer; l <= last_layer && rc == LM_OK; ++l) {
+            rc = attention_paged(ctx, st, l, *step, hidden_dev, hidden_dev, 1, st->layers[l].input_norm);
+            if (rc == LM_OK) {
+                rc = lm::ffn_sublayer(ctx, l, hidden_dev, step->tokens, path);
+            }
+        }
+        return rc;
     } catch (const std::bad_alloc&) {
         return fail(LM_ENOMEM, "host allocation failed");
     }

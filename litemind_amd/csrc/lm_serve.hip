@@ -106,8 +106,9 @@ int serve_state(lm_context* ctx, int rows, lm::ServeState** out, void** parts) {
     return LM_OK;
 }
 
-// The sizes that every use of a step relies on.
-int check_sizes(const lm_paged_step* s) {
+}  // namespace
+
+int lm::check_step_sizes(const lm_paged_step* s) {
     if (s == nullptr) {
         return fail(LM_EINVAL, "null step");
     }
@@ -129,12 +130,10 @@ int check_sizes(const lm_paged_step* s) {
     return LM_OK;
 }
 
-}  // namespace
-
 extern "C" {
 
 int lm_page_plan(lm_context* ctx, const lm_paged_step* step) {
-    const int rc = check_sizes(step);
+    const int rc = lm::check_step_sizes(step);
     if (rc != LM_OK) {
         return rc;
     }
@@ -164,7 +163,7 @@ int lm_page_plan(lm_context* ctx, const lm_paged_step* step) {
 int lm_paged_attention(lm_context* ctx, const lm_paged_step* step, const void* q_dev, const void* pool_dev,
                        int32_t dtype, int32_t heads, int32_t rank, int32_t rope, float scale, void* out_dev) {
     try {
-        int rc = check_sizes(step);
+        int rc = lm::check_step_sizes(step);
         if (rc != LM_OK) {
             return rc;
         }

@@ -75,7 +75,49 @@ struct SampleArgs {
 };
 hipError_t launch_sample(const SampleArgs& a, hipStream_t s);
 
+// ---- the model's layers over pages (k_latent.hip) ----
+struct LatentArgs {
+    int64_t tokens;
+    int32_t heads, nope, rope, rank;
+    const float* q;    // [tokens][heads][nope + rope]
+    const float* lat;  // [tokens][rank + rope]
+    const float* norm; // [rank]
+    float eps;
+    const int32_t* positions;
+    const int32_t* slots;
+    const int32_t* live;  // the number of new tokens
+    int64_t max_positions;
+    const float* cos_t;
+    const float* sin_t;
+    _Float16* pool;
+    int64_t pool_rows;
+    _Float16* q16;  // [tokens][heads][rank + rope]: the rope part is written
+};
+hipError_t launch_latent_rows(const LatentArgs& a, hipStream_t s);
+// Zeros into the rows of [tokens][width] from live[0] on.
+hipError_t launch_clear_rows(float* rows, const int32_t* live, int64_t tokens, int32_t width, hipStream_t s);
+hipError_t launch_absorb(const _Float16* kvb, _Float16* out, int32_t heads, int32_t nope, int32_t vh, int32_t rank,
+                         hipStream_t s);
+// out[t][h][n] = sum_k x[t][h][k] w[h w_head + w_first + n][k], K % 32 == 0, N % 16 == 0
+struct HeadsArgs {
+    int64_t tokens;
+    int32_t heads, K, N;
+    const void* x;  // fp32 or fp16
+    int32_t x_f32;
+    int64_t x_token, x_head;
+    const _Float16* w;  // panels [w_rows][K]
+    int64_t w_rows;
+    int32_t w_head, w_first;
+    _Float16* out;
+    int32_t out_panels;  // panels [tokens][heads N], or rows:
+    int64_t out_token, out_head;
+    const int32_t* live;  // rows from here on give zeros (null: none)
+};
+hipError_t launch_heads(const HeadsArgs& a, hipStream_t s);
+
 // ---- services of lm_serve.hip ----
+// LM_OK where a step's sizes can be relied on.
+int check_step_sizes(const lm_paged_step* step);
 struct ServeState;
 ServeState*& context_serve(lm_context* ctx);
 void serve_release(ServeState* st);
