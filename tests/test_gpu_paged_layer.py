@@ -192,21 +192,22 @@ def run_decoder(d, path, layers, prompts, follow):
                 rows.append(dh.download())
                 at += added[r]
             alone.append(rows)
-    return together, alone
+    return together, alone, states
 
 
 @pytest.mark.parametrize("path", [lm.PATH_AUTO, lm.PATH_MFMA])
 def test_decoder_together_as_alone(path):
     announce(f"paged decoder: path {path}")
     d = dataclasses.replace(SMALL, max_positions=256)
-    together, alone = run_decoder(d, path, 2, [37, 1, 64, 18], [1, 1, 3])
+    together, alone, states = run_decoder(d, path, 2, [37, 1, 64, 18], [1, 1, 3])
     for n, rows in enumerate(together):
         for r, y in enumerate(rows):
             want = alone[r][n]
-            rel = np.abs(y - want).sum() / np.abs(want).sum()
-            print(f"step {n} request {r}: mean_rel={rel:.3e}")
-            # two layers' attention, each within its bar of an output that is added to the state
-            assert np.isfinite(y).all() and rel <= 2 * MEAN_REL
+            change = np.abs(want - states[n][r])
+            rel = np.abs(y - want).sum() / change.sum()
+            print(f"step {n} request {r}: mean_rel={rel:.3e} of the change")
+            # what two layers add: their attention each within its bar on both sides, and experts of 1e-3
+            assert np.isfinite(y).all() and rel <= 2 * (2 * MEAN_REL + 1e-3)
 
 
 def test_refusals():
