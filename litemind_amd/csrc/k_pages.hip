@@ -5,9 +5,9 @@
 //   ceil(length / P) - ceil(cached / P), their place in the ring the sum of
 //   those before;  slot of position p = table[p / P] P + p % P
 //
-// Three sums over the requests, and per token, taken page and returned page one
-// search in them.  Latency bound: a decode step of 48 requests reads and writes
-// 2 KB.  One workgroup; requests in chunks of one per thread.
+// Three sums over the requests; per four tokens, and per taken and returned page,
+// one search in them.  Latency bound: a decode step of 48 requests reads and
+// writes 2 KB.  One workgroup; requests in chunks of one per thread.
 #include "serve_internal.h"
 
 namespace lm {
@@ -78,6 +78,9 @@ __global__ __launch_bounds__(kThreads) void page_plan_kernel(const lm_paged_step
     const int64_t pages = s.pages;
     const int64_t head = ((s.queue_in[0] % pages) + pages) % pages;
     const int32_t count = s.queue_in[1];
+    // places in the ring in 32 bits: a division of 64 takes 150 instructions
+    const uint32_t ring = static_cast<uint32_t>(pages), front = static_cast<uint32_t>(head),
+                   behind = static_cast<uint32_t>((head + max(count, 0)) % pages);
     // can the step be served: totals in 64 bits
     if (tid < 2) {
         flags[tid] = 0;
@@ -153,22 +156,36 @@ __global__ __launch_bounds__(kThreads) void page_plan_kernel(const lm_paged_step
             const Sums from{starts[0], firsts[0], backs[0]};
             for (int32_t i = from.taken + tid; i < before.taken; i += kThreads) {
                 const int k = find(firsts, n, i);
-                s.table[(r0 + k) * s.table_width + had[k] + i - firsts[k]] = s.ring[(head + i) % pages];
+                s.table[(r0 + k) * s.table_width + had[k] + i - firsts[k]] = s.ring[(front + i) % ring];
             }
             for (int32_t i = from.back + tid; i < before.back; i += kThreads) {
                 const int k = find(backs, n, i);
-                s.ring[(head + count + i) % pages] = s.table[(r0 + k) * s.table_width + i - backs[k]];
+                s.ring[(behind + i) % ring] = s.table[(r0 + k) * s.table_width + i - backs[k]];
             }
-            for (int32_t t = from.tokens + tid; t < before.tokens; t += kThreads) {
-                const int k = find(starts, n, t);
-                const int32_t p = cached[k] + t - starts[k];
-                const int32_t column = p / s.page_size;
-                const int32_t page = column < had[k] ? s.table[(r0 + k) * s.table_width + column]
-                                                     : s.ring[(head + firsts[k] + column - had[k]) % pages];
-                s.positions[t] = p;
-                s.slots[t] = static_cast<uint32_t>(page) < static_cast<uint64_t>(pages)
-                                 ? page * s.page_size + p % s.page_size
-                                 : -1;
+            for (int32_t t = from.tokens + 4 * tid; t < before.tokens; t += 4 * kThreads) {
+                int k = find(starts, n, t);
+                int32_t page[4], place[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (t + j < before.tokens) {
+                        while (k + 1 < n && starts[k + 1] <= t + j) {
+                            ++k;
+                        }
+                        place[j] = cached[k] + t + j - starts[k];
+                        const int32_t column = place[j] / s.page_size;
+                        page[j] = column < had[k] ? s.table[(r0 + k) * s.table_width + column]
+                                                  : s.ring[(front + static_cast<uint32_t>(firsts[k] + column - had[k])) % ring];
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (t + j < before.tokens) {
+                        s.positions[t + j] = place[j];
+                        s.slots[t + j] = static_cast<uint32_t>(page[j]) < ring
+                                             ? page[j] * s.page_size + place[j] % s.page_size
+                                             : -1;
+                    }
+                }
             }
         }
     } else {
