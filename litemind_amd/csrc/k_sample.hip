@@ -115,7 +115,7 @@ struct Row {
     const float* x;
     int32_t n;
     double top, rate;  // largest logit, 1024 log2(e) / temperature
-    float top_f, scale;  // stretches per logit
+    float top_f, scale, offset;  // stretches per logit, and where the largest lies
     uint64_t one;      // e = 1
     bool top_inf;
     const double* table;  // in LDS
@@ -153,10 +153,22 @@ struct Row {
             }
         }
     }
-    // The stretch of the range: kBins - 1 at the largest; 0 has no weight at all.
+    // The stretch of the range, kBins - 1 at the largest: one rounding and a cut, so
+    // that a larger logit is never in a lower one, whatever the range.
     __device__ int bin(float v) const {
-        const float d = fminf(fminf(top_f - v, kMost) * scale, static_cast<float>(kBins - 1));
-        return v >= top_f ? kBins - 1 : kBins - 1 - static_cast<int>(d);
+        return static_cast<int>(__builtin_amdgcn_fmed3f(__builtin_fmaf(v, scale, offset), 0.0f, static_cast<float>(kBins - 1)));
+    }
+    // A logit that no logit of the stretch lies under, and one that none lies over: a
+    // stretch more, and two steps for the roundings.
+    __device__ float under(int stretch) const {
+        return near((static_cast<float>(stretch) - 1.0f - offset) / scale, -1, stretch == 0);
+    }
+    __device__ float over(int stretch) const { return near((static_cast<float>(stretch) + 2.0f - offset) / scale, 1, false); }
+    __device__ static float near(float v, int way, bool all) {
+        if (all || !(v > -kMost && v < kMost)) {
+            return way < 0 ? -kMost : kMost;
+        }
+        return key_float(order_key(v) + 2 * way);
     }
 };
 
@@ -404,15 +416,14 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a, in
     // or to the least one, the range is cut into stretches kBins - 1 .. 1; what lies
     // further below is in stretch 0.
     r.scale = static_cast<float>(48 * 0.6931471805599453 * temperature);
-    r.scale = fminf((kBins - 2) / (least > -__builtin_inff() ? fminf(r.scale, top - least) : r.scale), kMost);
+    r.scale = (kBins - 2) / (least > -__builtin_inff() ? fminf(r.scale, top - least) : r.scale);
+    r.scale = fminf(r.scale, 1e30f / fmaxf(fabsf(r.top_inf ? 0.0f : top), 1.0f));
+    r.offset = static_cast<float>(kBins) - 0.5f - (r.top_inf ? 0.0f : top) * r.scale;
 
     Cut cut{kKeyMinusInf + 1, 0x7fffffff};
     // Lists the kept ones of a stretch, or of it and those above it; false: too many.
-    auto gather = [&](int stretch, bool upwards) {
-        // a logit under all of them, without their stretches: one stretch more, and
-        // two steps for the roundings
-        const uint32_t under = order_key(top - (kBins + 1 - stretch) / r.scale);
-        const float loose = r.top_inf || stretch == 0 ? -kMost : key_float(max(under, kKeyMinusInf + 3) - 2);
+    auto gather = [&](int stretch, bool upwards) __attribute__((always_inline)) {
+        const float loose = r.under(stretch);
         __syncthreads();
         if (threadIdx.x == 0) {
             sh.listed = 0;
@@ -468,7 +479,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a, in
             continue;
         }
         auto weight = [&](float v) { return mass ? r.units(v) : uint64_t{1}; };
-        uint64_t total = 0, above = 0;
+        uint64_t total = 0, above = 0;  // (total: this thread's share of it)
         int stretch = 0;
         if (whole) {
             listed_share([&](uint32_t key, int32_t i) { total += cut.keeps(key, i) ? weight(key_float(key)) : 0; });
@@ -482,12 +493,13 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a, in
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    if ((v[j] > least_f || (v[j] == least_f && i + j <= cut.last)) && w[j] != 0) {
-                        total += w[j];
+                    if (v[j] > least_f || (v[j] == least_f && i + j <= cut.last)) {
                         add_bin(sh, r.bin(v[j]), w[j]);
                     }
                 }
             });
+            __syncthreads();
+            total = sh.bins[threadIdx.x] + sh.bins[threadIdx.x + kThreads];
         }
         total = block_reduce(total, sh.part, Add());
         // a token is kept while the e before it are under top_p of the total
@@ -500,8 +512,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a, in
         bool listed = true;
         if (!whole) {
             const Found f = find_bin(sh, want);
-            if (f.bin == 0) {
-                continue;  // those of stretch 0 weigh nothing: as well all kept as none
+            if (f.bin == 0 && !mass && r.over(0) < top && r.units(r.over(0)) == 0) {
+                continue;  // a cut among those that weigh nothing
             }
             stretch = f.bin;
             // Of 4096 logits in or above it thrown at 1024 threads, 19 threads would get
@@ -561,14 +573,26 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a, in
     }
     if (set.min_p > 0.0f) {
         // the lowest key whose e is at least min_p, between one whose is not and
-        // the largest's, by as many probes as there are threads
+        // the largest's, by as many probes as there are threads; close to where the
+        // logarithm has it, if that is borne out
+        auto kept = [&](double x) { return exp((x - r.top) / temperature) >= static_cast<double>(set.min_p); };
         uint32_t under = kKeyMinusInf, least_kept = best;
+        const double guess = r.top + temperature * log(static_cast<double>(set.min_p));
+        const double room = 1e-13 * (fabs(r.top) + fabs(guess));
+        const float below = static_cast<float>(guess - room), above = static_cast<float>(guess + room);
+        if (!r.top_inf && below > -kMost && above < top) {
+            const uint32_t low = order_key(below) - 1, high = order_key(above) + 1;
+            if (!kept(static_cast<double>(key_float(low))) && kept(static_cast<double>(key_float(high)))) {
+                under = low;
+                least_kept = high;
+            }
+        }
 #pragma unroll 1
         while (!r.top_inf && least_kept - under > 1) {
             const uint32_t step = (least_kept - under + kThreads - 1) / kThreads;
             const uint64_t probe = under + static_cast<uint64_t>(threadIdx.x + 1) * step;
             const double x = static_cast<double>(key_float(static_cast<uint32_t>(min(probe, static_cast<uint64_t>(least_kept)))));
-            const int fewer = __syncthreads_count(probe < least_kept && !(exp((x - r.top) / temperature) >= static_cast<double>(set.min_p)));
+            const int fewer = __syncthreads_count(probe < least_kept && !kept(x));
             under += static_cast<uint32_t>(fewer) * step;
             least_kept = static_cast<uint32_t>(min(under + static_cast<uint64_t>(step), static_cast<uint64_t>(least_kept)));
         }
