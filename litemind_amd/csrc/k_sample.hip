@@ -430,18 +430,16 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a, in
         }
         __syncthreads();
         sweep_row(r, [&](int32_t i, f32x4 v) {
-            if (v[0] >= loose || v[1] >= loose || v[2] >= loose || v[3] >= loose) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < 4; ++j) {
+                if (v[j] >= loose) {
+                    const int b = r.bin(v[j]);
                     const uint32_t key = order_key(v[j]);
-                    if (cut.keeps(key, i + j)) {
-                        const int b = r.bin(v[j]);
-                        if (b == stretch || (upwards && b > stretch)) {
-                            const uint32_t at = atomicAdd(&sh.listed, 1u);
-                            if (at < kList) {
-                                sh.list_key[at] = key;
-                                sh.list_at[at] = i + j;
-                            }
+                    if ((b == stretch || (upwards && b > stretch)) && cut.keeps(key, i + j)) {
+                        const uint32_t at = atomicAdd(&sh.listed, 1u);
+                        if (at < kList) {
+                            sh.list_key[at] = key;
+                            sh.list_at[at] = i + j;
                         }
                     }
                 }
