@@ -34,8 +34,8 @@ __device__ inline void rotate_to(const LatentArgs& a, const float* from, int i, 
 
 // A workgroup per token: its normalised latent and rotated key into its slot of
 // the pool, its heads' rotated query channels behind the absorbed ones. Rows
-// without a slot in the pool store nothing there. Bound by its launch: 9 KB read
-// and 3 KB written a token (16 heads).
+// without a slot in the pool store nothing there. Bound by its launch: 14 KB read
+// and 3 KB written a token (16 heads; one token 4.6 us, 2048 10 us).
 __global__ __launch_bounds__(256) void latent_rows_kernel(const LatentArgs a) {
     __shared__ double part[4];
     const int64_t t = blockIdx.x;
@@ -103,7 +103,10 @@ __device__ inline half8 load8(const _Float16* p) { return *reinterpret_cast<cons
 // Per head: out[t][n] = sum_k x[t][k] w[n][k]. A wave takes B x B of a head, as
 // products of 16 x 16 x 32 whose operands come straight from memory: the weights of
 // all heads (2 MB a side on V2-Lite) stay in each L2, and K is 128 or 512, so there
-// is no loop long enough to pay for staging in LDS.
+// is no loop long enough to pay for staging in LDS. Row m of a product's weights is
+// row B / 4 (m / 4) + 4 j + m % 4 of the tile, so that a lane's sums of all products
+// are B / 4 successive channels of a token (queries of 2048 tokens: 33.1 -> 31.4 us).
+// Bound by those loads: 200 MB from the caches for that call, 4.3 GFLOP.
 template <class X, int B>
 __global__ __launch_bounds__(256) void heads_kernel(const HeadsArgs a) {
     constexpr int S = B / 16;
@@ -123,7 +126,7 @@ __global__ __launch_bounds__(256) void heads_kernel(const HeadsArgs a) {
 #pragma unroll
     for (int i = 0; i < S; ++i) {
         x[i] = static_cast<const X*>(a.x) + min(t0 + 16 * i + low, a.tokens - 1) * a.x_token + h * a.x_head + 8 * grp;
-        w[i] = a.w + panel_index(static_cast<int64_t>(h) * a.w_head + a.w_first + n0 + 16 * i + low, 8 * grp, a.w_rows);
+        w[i] = a.w + panel_index(static_cast<int64_t>(h) * a.w_head + a.w_first + n0 + B / 4 * (low >> 2) + 4 * i + (low & 3), 8 * grp, a.w_rows);
     }
     f32x4 sums[S][S] = {};
 #pragma unroll 4
@@ -149,7 +152,7 @@ __global__ __launch_bounds__(256) void heads_kernel(const HeadsArgs a) {
         if (t < a.tokens) {
 #pragma unroll
             for (int j = 0; j < S; ++j) {
-                const int n = n0 + 16 * j + 4 * grp;
+                const int n = n0 + B / 4 * grp + 4 * j;
                 half4 v;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -190,7 +193,10 @@ hipError_t launch_absorb(const _Float16* kvb, _Float16* out, int32_t heads, int3
     return hipGetLastError();
 }
 
-// The largest tiles that still give every SIMD one.
+// The largest tiles that still give every SIMD one. V2-Lite's queries and outputs
+// with B = 16, 32, 64 (us): 32 tokens 4.2, 5.5, 7.9 and 7.4, 8.6, 12.4; 128 tokens
+// 7.7, 5.9, 9.4 and 7.2, 8.5, 15.0; 512 tokens 23.4, 14.2, 10.5 and 13.9, 9.0, 15.4;
+// 2048 tokens 84.7, 47.2, 33.1 and 49.8, 27.6, 18.9.
 hipError_t launch_heads(const HeadsArgs& a, hipStream_t s) {
     const auto tiles = [&](int b) { return a.N % b == 0 ? (a.tokens + b - 1) / b * (a.N / b) * a.heads : 0; };
     const int b = tiles(64) >= 1024 ? 64 : tiles(32) >= 1024 ? 32 : 16;
