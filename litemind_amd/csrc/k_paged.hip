@@ -498,10 +498,12 @@ __global__ __launch_bounds__(kThreads, 2) void paged_rows_kernel(const TileArgs 
         float m = kNone;          // reference of row `lane`, the same in every wave
         float ref = kUnset;       // of this lane's row of the scores, times c
         float l = 0.0f, sum = 0.0f;  // its total, and the newest tile's
-        // the newest tile's weights; tells the others where a score passes the reference
-        auto weigh = [&](char* wt, int u) {
+        // the newest tile's weights
+        float over = kNone;
+        auto exps = [&](char* wt) {
             vec4 p;
-            float w[4], over = kNone;
+            float w[4];
+            over = kNone;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float x = __builtin_fmaf(sc[e], a.c, -ref);
@@ -511,36 +513,49 @@ __global__ __launch_bounds__(kThreads, 2) void paged_rows_kernel(const TileArgs 
             }
             sum = (w[0] + w[1]) + (w[2] + w[3]);
             *reinterpret_cast<vec4*>(wt + weight_to) = p;
+        };
+        // tells the others where a score passed the reference
+        auto tell = [&](int u) {
             if (__builtin_expect(__any(over > kSlack), 0)) {
                 if (lane == 0) {
                     late_flags[u] = 1;
                 }
             }
         };
-        // The products of an interval: scores of the tile in `next` (S), context of
-        // the tile in `now` (C), in six steps, each step's operands read during the
-        // one before; `between(i)` runs ahead of step i's products.
+        auto weigh = [&](char* wt, int u) {
+            exps(wt);
+            tell(u);
+        };
+        // The products of an interval: scores of the tile in `next` (S) in six steps,
+        // then context of the tile in `now` (C) in four, each step's operands read
+        // during the one before; `between(i)` runs ahead of step i's products.
         auto products = [&](auto with_scores, const char* next, auto with_context, const char* now, const char* wt,
                             bool sanitize, auto between) {
             constexpr bool S = decltype(with_scores)::value, C = decltype(with_context)::value;
+            constexpr int kFrom = S ? 0 : 6, kTo = C ? 10 : 6;
             vec8 kf[2][3], vf[2], pf[RB];
             const int k_at = here(key_at), r_at = here(rotary_key_at);
             const int v_at[2] = {here(value_at[0]), here(value_at[1])};
             auto read = [&](int i) {
-                if constexpr (S) {
+                if (i < 6) {
 #pragma unroll
                     for (int k = 0; k < 3; ++k) {
                         const int ks = 3 * i + k;
                         kf[i & 1][k] = *reinterpret_cast<const vec8*>(
                             next + (ks < 16 ? (k_at ^ (ks & 3) << 6) + (ks >> 2) * 256 : r_at ^ (ks & 1) << 6));
                     }
-                }
-                if (C && i < 4) {  // channels 16 i ..
+                } else {  // channels 16 (i - 6) ..
+                    if (i == 6) {
+#pragma unroll
+                        for (int rb = 0; rb < RB; ++rb) {
+                            pf[rb] = *reinterpret_cast<const vec8*>(wt + weight_from + rb * 1024);
+                        }
+                    }
                     short8v v;
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
                         const short4v part =
-                            __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(now + (v_at[k] ^ i << 5)));
+                            __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(now + (v_at[k] ^ (i - 6) << 5)));
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             v[4 * k + e] = part[e];
@@ -549,37 +564,35 @@ __global__ __launch_bounds__(kThreads, 2) void paged_rows_kernel(const TileArgs 
                     vf[i & 1] = __builtin_bit_cast(vec8, v);
                 }
             };
+            f32x4 odd{};
             if constexpr (S) {
                 sc = f32x4{};
             }
-            if constexpr (C) {
+            read(kFrom);
 #pragma unroll
-                for (int rb = 0; rb < RB; ++rb) {
-                    pf[rb] = *reinterpret_cast<const vec8*>(wt + weight_from + rb * 1024);
-                }
-            }
-            read(0);
-#pragma unroll
-            for (int i = 0; i < 6; ++i) {
-                if (i < 5) {
+            for (int i = kFrom; i < kTo; ++i) {
+                if (i + 1 < kTo) {
                     read(i + 1);
                 }
                 between(i);
                 __builtin_amdgcn_sched_barrier(0);
-                if (C && i < 4) {
+                if (i >= 6) {
                     vec8 f = vf[i & 1];
                     if (sanitize) {
                         f = __builtin_bit_cast(vec8, finite_or_zero<E>(__builtin_bit_cast(short8v, f)));
                     }
 #pragma unroll
                     for (int rb = 0; rb < RB; ++rb) {
-                        o[rb][i] = H::mfma16(f, pf[rb], o[rb][i]);
+                        o[rb][i - 6] = H::mfma16(f, pf[rb], o[rb][i - 6]);
                     }
-                }
-                if constexpr (S) {
+                } else {
 #pragma unroll
                     for (int k = 0; k < 3; ++k) {
-                        sc = H::mfma16(kf[i & 1][k], q[3 * i + k], sc);
+                        f32x4& to = (3 * i + k) % 2 == 0 ? sc : odd;
+                        to = H::mfma16(kf[i & 1][k], q[3 * i + k], to);
+                    }
+                    if (i == 5) {
+                        sc += odd;
                     }
                 }
                 __builtin_amdgcn_sched_barrier(0);
@@ -661,11 +674,14 @@ __global__ __launch_bounds__(kThreads, 2) void paged_rows_kernel(const TileArgs 
                         l += sum;
                         const Loads d = prepare(t + u + 3, ring[(u + 3) & 3]);
                         products(yes, ring[(u + 1) & 3], yes, ring[u], weights[u & 1], false, [&](int i) {
-                            if (i > 0) {
+                            if (i > 0 && i < 6) {
                                 load(d, i - 1);
                             }
+                            if (i == 7) {
+                                exps(weights[(u + 1) & 1]);
+                            }
                         });
-                        weigh(weights[(u + 1) & 1], (u + 1) & 3);
+                        tell((u + 1) & 3);
                     }
                     t += stop == 0 ? 4 : 0;
                 }
