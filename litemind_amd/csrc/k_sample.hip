@@ -15,7 +15,11 @@
 // stretch that the random number falls into is cut up again until one is left.
 //
 // A row is a workgroup's; its sweeps after the first come from the caches. What
-// they cost is the e: 12 steps of 64-bit arithmetic, 16 cycles of a SIMD for 64.
+// they cost is the e: 11 steps of 64-bit arithmetic and as many others, 22 us for
+// 102400 on one CU. By temperature alone a row has one such sweep (35 us by
+// itself, 256 rows 50 us), by top-k none (28 us), by top-p two (100 us). Sharing a
+// row among workgroups, a kernel for each sweep, was no faster: 40 us for top-k
+// and 76 for 32 rows of any settings, where this takes 72.
 #include "serve_internal.h"
 
 namespace lm {
