@@ -45,7 +45,7 @@ typedef struct lm_paged_step {
     int32_t* ring;            /* [pages] the free pages, a ring: entries head .. head + count - 1, modulo pages */
     const int32_t* queue_in;  /* [2] head and count of the ring before the step */
     int32_t* queue_out;       /* [2] after it; may equal queue_in */
-    int32_t* lengths;         /* [requests] tokens in the cache with the step's; 0 of a request that is over */
+    int32_t* lengths;         /* [requests] tokens in the cache with the step's, 0 of a request that is over; may equal cached */
     int32_t* starts;          /* [requests + 1] first row of each request's new tokens */
     int32_t* positions;       /* [tokens] position of each new token; 0 past the last */
     int32_t* slots;           /* [tokens] slot of each new token; -1 past the last */
@@ -56,17 +56,21 @@ typedef struct lm_paged_step {
 #define LM_STEP_LENGTH 1  /* a negative cached length, or a request longer than its table row */
 #define LM_STEP_TOKENS 2  /* the new tokens exceed `tokens`, or a request's exceed max_added */
 #define LM_STEP_PAGES 3   /* the ring holds fewer pages than the step needs */
+#define LM_STEP_RING 4    /* a negative count, or more free pages after the step than the pool has */
 
 /* Plans a step from cached and added: writes lengths, starts, positions, slots,
  * queue_out and info.  A request takes the pages that its new tokens start from
  * the ring's head, requests in order, and enters them in its table row; the
  * pages of a request that is over go behind the ring's last free page, in
- * request and column order.  queue_in apart, no input is changed that the plan
- * reads, so planning the same step again gives the same.  A step that cannot be
+ * request and column order.  No input is changed that the plan reads, but where
+ * queue_out or lengths are queue_in or cached themselves, so planning the same
+ * step again gives the same.  A step that cannot be
  * served (info[0] is the first LM_STEP_* that applies, in their order) takes and
  * gives back nothing: starts are 0, slots -1, lengths the cached ones, the table
  * and the ring as they were.  A page id outside the pool makes the slots of its
- * tokens -1.  Asynchronous. */
+ * tokens -1.  A page is one request's or the ring's: one that two requests name
+ * (attention may read it for both) comes back once for each that is over, so the
+ * caller takes it out of one row first.  Asynchronous. */
 int lm_page_plan(lm_context* ctx, const lm_paged_step* step);
 
 /* Attention of the step's new tokens over the pages, in the latent space that
@@ -82,6 +86,8 @@ int lm_page_plan(lm_context* ctx, const lm_paged_step* step);
  *   out_dev  [tokens][heads][rank], all of `dtype` (LM_DT_F16 or LM_DT_BF16),
  *            16-byte aligned; out_dev overlaps neither of the others
  *   rank     a multiple of 8 up to 1024, rope a multiple of 8 up to 256
+ *   heads    tokens * heads under 2^30, and (tokens * heads / 16 + tokens) blocks
+ *            of heads times the tokens of a table row under 2^62
  * Products have the inputs' 16 bits, sums 32; the softmax weights round to 16
  * bits before the second product, the output once at the end.  Rows past the
  * last request's are not written.  What lies in a page past a request's length,
@@ -113,7 +119,9 @@ int lm_paged_pool(lm_context* ctx, int32_t layer, void** out_dev);
  * other rows nor mean anything.  Positions at or past context_length are not
  * rotated, as lm_attention_forward's.  kv_b_proj is absorbed into the query and
  * the output; queries, latents and weights round to fp16, within the MFMA
- * path's tolerance.  out_dev must not overlap x_dev.  Asynchronous. */
+ * path's tolerance.  out_dev must not overlap x_dev.  tokens * heads at most
+ * 2^24, and tokens times the widest of hidden_size, q_lora_rank and heads *
+ * v_head_dim 2^30.  Asynchronous. */
 int lm_paged_forward(lm_context* ctx, int32_t layer, const lm_paged_step* step, const float* x_dev, float* out_dev,
                      int32_t accumulate);
 /* lm_decoder_forward's layer loop with lm_paged_forward as the attention:

@@ -104,7 +104,7 @@ class PagedStep(C.Structure):
     ]
 
 
-STEP_OK, STEP_LENGTH, STEP_TOKENS, STEP_PAGES = range(4)  # LM_STEP_*: PagedStep.info[0] after a plan
+STEP_OK, STEP_LENGTH, STEP_TOKENS, STEP_PAGES, STEP_RING = range(5)  # LM_STEP_*: PagedStep.info[0] after a plan
 # lm_sampling: one row's settings, as a numpy structured type
 SAMPLING = np.dtype([("temperature", np.float32), ("top_k", np.int32), ("top_p", np.float32), ("min_p", np.float32)])
 

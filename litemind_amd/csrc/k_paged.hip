@@ -958,7 +958,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const TileArgs a) {
 }
 
 // ---- any widths ----
-// One workgroup per token and head, its four waves on alternate keys, a lane on
+// A workgroup per token and head (in turn, past 2^20 of them), its four waves on alternate keys, a lane on
 // channels lane + 64 i; running maximum and sum per wave, joined at the end.
 constexpr int kMaxRank = 1024, kMaxRope = 256;
 
@@ -967,97 +967,101 @@ __global__ __launch_bounds__(256) void paged_any_kernel(const PagedAttention a) 
     constexpr int kC = kMaxRank / 64, kR = kMaxRope / 64;
     __shared__ float part[4][kMaxRank], stats[4][2];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int32_t t = static_cast<int32_t>(blockIdx.x / a.heads), h = static_cast<int32_t>(blockIdx.x % a.heads);
-    const PagedView& v = a.view;
-    // the token's request: the last whose rows start at or before it
-    int32_t lo = 0, hi = v.requests;
-    while (hi - lo > 1) {
-        const int32_t mid = lo + (hi - lo) / 2;
-        if (v.starts[mid] <= t) {
-            lo = mid;
-        } else {
-            hi = mid;
+    const int64_t rows = static_cast<int64_t>(a.view.tokens) * a.heads;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const int32_t t = static_cast<int32_t>(row / a.heads), h = static_cast<int32_t>(row % a.heads);
+        const PagedView& v = a.view;
+        // the token's request: the last whose rows start at or before it
+        int32_t lo = 0, hi = v.requests;
+        while (hi - lo > 1) {
+            const int32_t mid = lo + (hi - lo) / 2;
+            if (v.starts[mid] <= t) {
+                lo = mid;
+            } else {
+                hi = mid;
+            }
         }
-    }
-    const PagedRequest r = paged_request(v, lo);
-    if (t < r.first || t >= r.first + r.added) {
-        return;  // past the last request's rows
-    }
-    const int width = a.rank + a.rope;
-    const E* const q = static_cast<const E*>(a.q) + (static_cast<int64_t>(t) * a.heads + h) * width;
-    float qc[kC], qr[kR], o[kC];
-#pragma unroll
-    for (int i = 0; i < kC; ++i) {
-        qc[i] = lane + 64 * i < a.rank ? static_cast<float>(q[lane + 64 * i]) : 0.0f;
-        o[i] = 0.0f;
-    }
-#pragma unroll
-    for (int i = 0; i < kR; ++i) {
-        qr[i] = lane + 64 * i < a.rope ? static_cast<float>(q[a.rank + lane + 64 * i]) : 0.0f;
-    }
-    float m = kNone, l = 0.0f;
-    const int32_t keys = r.cached + t - r.first + 1;
-    for (int32_t j = wave; j < keys; j += 4) {
-        const int64_t page = checked_page(v, v.table[static_cast<int64_t>(lo) * v.table_width + j / v.page_size]);
-        const E* const row = static_cast<const E*>(a.pool) + (page * v.page_size + j % v.page_size) * width;
-        float c[kC], s = 0.0f;
+        const PagedRequest r = paged_request(v, lo);
+        if (t < r.first || t >= r.first + r.added) {
+            continue;  // past the last request's rows
+        }
+        const int width = a.rank + a.rope;
+        const E* const q = static_cast<const E*>(a.q) + (static_cast<int64_t>(t) * a.heads + h) * width;
+        float qc[kC], qr[kR], o[kC];
 #pragma unroll
         for (int i = 0; i < kC; ++i) {
-            c[i] = lane + 64 * i < a.rank ? static_cast<float>(row[lane + 64 * i]) : 0.0f;
-            s = __builtin_fmaf(qc[i], c[i], s);
+            qc[i] = lane + 64 * i < a.rank ? static_cast<float>(q[lane + 64 * i]) : 0.0f;
+            o[i] = 0.0f;
         }
 #pragma unroll
         for (int i = 0; i < kR; ++i) {
-            s = __builtin_fmaf(qr[i], lane + 64 * i < a.rope ? static_cast<float>(row[a.rank + lane + 64 * i]) : 0.0f,
-                               s);
+            qr[i] = lane + 64 * i < a.rope ? static_cast<float>(q[a.rank + lane + 64 * i]) : 0.0f;
         }
-        for (int w = 32; w >= 1; w >>= 1) {
-            s += __shfl_xor(s, w);
+        float m = kNone, l = 0.0f;
+        const int32_t keys = r.cached + t - r.first + 1;
+        for (int32_t j = wave; j < keys; j += 4) {
+            const int64_t page = checked_page(v, v.table[static_cast<int64_t>(lo) * v.table_width + j / v.page_size]);
+            const E* const key = static_cast<const E*>(a.pool) + (page * v.page_size + j % v.page_size) * width;
+            float c[kC], s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kC; ++i) {
+                c[i] = lane + 64 * i < a.rank ? static_cast<float>(key[lane + 64 * i]) : 0.0f;
+                s = __builtin_fmaf(qc[i], c[i], s);
+            }
+#pragma unroll
+            for (int i = 0; i < kR; ++i) {
+                s = __builtin_fmaf(qr[i], lane + 64 * i < a.rope ? static_cast<float>(key[a.rank + lane + 64 * i]) : 0.0f,
+                                   s);
+            }
+            for (int w = 32; w >= 1; w >>= 1) {
+                s += __shfl_xor(s, w);
+            }
+            s *= a.scale;
+            const float top = fmaxf(m, s);
+            // no score above -infinity yet: nothing to rescale, and no weight
+            const float alpha = m == kNone ? 1.0f : __expf(m - top);
+            const float p = s == kNone ? 0.0f : __expf(s - top);
+            l = __builtin_fmaf(l, alpha, p);
+#pragma unroll
+            for (int i = 0; i < kC; ++i) {
+                o[i] = __builtin_fmaf(o[i], alpha, p * c[i]);
+            }
+            m = top;
         }
-        s *= a.scale;
-        const float top = fmaxf(m, s);
-        // no score above -infinity yet: nothing to rescale, and no weight
-        const float alpha = m == kNone ? 1.0f : __expf(m - top);
-        const float p = s == kNone ? 0.0f : __expf(s - top);
-        l = __builtin_fmaf(l, alpha, p);
 #pragma unroll
         for (int i = 0; i < kC; ++i) {
-            o[i] = __builtin_fmaf(o[i], alpha, p * c[i]);
+            part[wave][lane + 64 * i] = o[i];
         }
-        m = top;
-    }
-#pragma unroll
-    for (int i = 0; i < kC; ++i) {
-        part[wave][lane + 64 * i] = o[i];
-    }
-    if (lane == 0) {
-        stats[wave][0] = m;
-        stats[wave][1] = l;
-    }
-    __syncthreads();
-    float top = kNone, total = 0.0f, w[4];
-    for (int i = 0; i < 4; ++i) {
-        top = fmaxf(top, stats[i][0]);
-    }
-    for (int i = 0; i < 4; ++i) {
-        w[i] = stats[i][0] == kNone ? 0.0f : __expf(stats[i][0] - top);
-        total = __builtin_fmaf(w[i], stats[i][1], total);
-    }
-    E* const out = static_cast<E*>(a.out) + (static_cast<int64_t>(t) * a.heads + h) * a.rank;
-    for (int i = threadIdx.x; i < a.rank; i += 256) {
-        float sum = 0.0f;
-        for (int k = 0; k < 4; ++k) {
-            sum = __builtin_fmaf(w[k], part[k][i], sum);
+        if (lane == 0) {
+            stats[wave][0] = m;
+            stats[wave][1] = l;
         }
-        out[i] = static_cast<E>(sum / total);
+        __syncthreads();
+        float top = kNone, total = 0.0f, w[4];
+        for (int i = 0; i < 4; ++i) {
+            top = fmaxf(top, stats[i][0]);
+        }
+        for (int i = 0; i < 4; ++i) {
+            w[i] = stats[i][0] == kNone ? 0.0f : __expf(stats[i][0] - top);
+            total = __builtin_fmaf(w[i], stats[i][1], total);
+        }
+        E* const out = static_cast<E*>(a.out) + (static_cast<int64_t>(t) * a.heads + h) * a.rank;
+        for (int i = threadIdx.x; i < a.rank; i += 256) {
+            float sum = 0.0f;
+            for (int k = 0; k < 4; ++k) {
+                sum = __builtin_fmaf(w[k], part[k][i], sum);
+            }
+            out[i] = static_cast<E>(sum / total);
+        }
+        __syncthreads();  // `part` is free again
     }
 }
 
 template <class E>
 hipError_t launch(const PagedAttention& a, void* workspace, hipStream_t s) {
     if (!paged_tiled(a.rank, a.rope)) {
-        hipLaunchKernelGGL(paged_any_kernel<E>, dim3(static_cast<unsigned>(a.view.tokens * a.heads)), dim3(256), 0, s,
-                           a);
+        hipLaunchKernelGGL(paged_any_kernel<E>, dim3(static_cast<unsigned>(std::min(static_cast<int64_t>(a.view.tokens) * a.heads, int64_t{1} << 20))),
+                           dim3(256), 0, s, a);
         return hipGetLastError();
     }
     TileArgs t;
@@ -1097,6 +1101,11 @@ hipError_t launch(const PagedAttention& a, void* workspace, hipStream_t s) {
 }  // namespace
 
 bool paged_tiled(int32_t rank, int32_t rope) { return rank == kRank && rope == kRope; }
+
+bool paged_shares_out(int64_t tokens, int32_t heads, int64_t room) {
+    const double rows = static_cast<double>(tokens) * heads;
+    return (rows / 16 + static_cast<double>(tokens)) * ((static_cast<double>(room) + kExtra) * heads + rows + 64) < 0x1p62;
+}
 
 int paged_block_rows(int32_t max_added, int32_t heads) {
     return static_cast<int64_t>(max_added) * heads <= 16 ? 16 : 64;

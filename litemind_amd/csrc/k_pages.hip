@@ -72,7 +72,7 @@ __device__ inline int find(const int32_t* at, int n, int32_t i) {
 __global__ __launch_bounds__(kThreads) void page_plan_kernel(const lm_paged_step s) {
     __shared__ int32_t starts[kThreads], firsts[kThreads], backs[kThreads], had[kThreads], cached[kThreads];
     __shared__ Sums wave_sums[kWaves];
-    __shared__ int64_t wave_tokens[kWaves], wave_taken[kWaves];
+    __shared__ int64_t wave_tokens[kWaves], wave_taken[kWaves], wave_back[kWaves];
     __shared__ int32_t flags[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t pages = s.pages;
@@ -86,7 +86,7 @@ __global__ __launch_bounds__(kThreads) void page_plan_kernel(const lm_paged_step
         flags[tid] = 0;
     }
     __syncthreads();
-    int64_t tokens = 0, taken = 0;
+    int64_t tokens = 0, taken = 0, back = 0;
     for (int64_t r = tid; r < s.requests; r += kThreads) {
         const Request q = load_request(s, r);
         if (q.bad_length) {
@@ -97,25 +97,30 @@ __global__ __launch_bounds__(kThreads) void page_plan_kernel(const lm_paged_step
         }
         tokens += q.added;
         taken += q.taken;
+        back += q.over ? q.had : 0;
     }
     for (int o = 32; o >= 1; o >>= 1) {
         tokens += __shfl_xor(tokens, o);
         taken += __shfl_xor(taken, o);
+        back += __shfl_xor(back, o);
     }
     if (lane == 0) {
         wave_tokens[wave] = tokens;
         wave_taken[wave] = taken;
+        wave_back[wave] = back;
     }
     __syncthreads();
-    tokens = taken = 0;
+    tokens = taken = back = 0;
     for (int w = 0; w < kWaves; ++w) {
         tokens += wave_tokens[w];
         taken += wave_taken[w];
+        back += wave_back[w];
     }
     const int32_t status = flags[0] != 0                             ? LM_STEP_LENGTH
                            : flags[1] != 0 || tokens > s.tokens      ? LM_STEP_TOKENS
                            : taken > max(static_cast<int64_t>(count), int64_t{0}) ? LM_STEP_PAGES
-                                                                     : LM_STEP_OK;
+                           : count < 0 || count - taken + back > pages ? LM_STEP_RING
+                                                                       : LM_STEP_OK;
     Sums before{};  // of the requests in earlier chunks
     if (status == LM_STEP_OK) {
         for (int64_t r0 = 0; r0 < s.requests; r0 += kThreads) {

@@ -22,10 +22,13 @@
 // and 76 for 32 rows of any settings, where this takes 72.
 #include "serve_internal.h"
 
+#include <algorithm>
+
 namespace lm {
 namespace {
 
 constexpr int kThreads = 1024;
+constexpr int64_t kMostRows = int64_t{1} << 21;
 constexpr int kWaves = kThreads / 64;
 constexpr int kBins = 2048;  // two a thread where they are added up
 constexpr int kTable = 1024;
@@ -368,9 +371,9 @@ struct Cut {
     __device__ bool keeps(uint32_t k, int32_t i) const { return k > key || (k == key && i <= last); }
 };
 
-__global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a, int bits) {
+__global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a, int64_t row0, int bits) {
     __shared__ Shared sh;
-    const int64_t row = blockIdx.x;
+    const int64_t row = row0 + blockIdx.x;
     const lm_sampling set = a.settings[row];
     Row r;
     r.x = a.logits + row * a.stride;
@@ -665,8 +668,14 @@ hipError_t launch_sample(const SampleArgs& a, hipStream_t s) {
     while (a.vocab > int64_t{1} << (63 - bits)) {
         --bits;
     }
-    hipLaunchKernelGGL(sample_kernel, dim3(static_cast<unsigned>(a.rows)), dim3(kThreads), 0, s, a, bits);
-    return hipGetLastError();
+    // (a launch takes less than 2^32 threads)
+    hipError_t err = hipSuccess;
+    for (int64_t row0 = 0; row0 < a.rows && err == hipSuccess; row0 += kMostRows) {
+        hipLaunchKernelGGL(sample_kernel, dim3(static_cast<unsigned>(std::min(a.rows - row0, kMostRows))), dim3(kThreads), 0, s,
+                           a, row0, bits);
+        err = hipGetLastError();
+    }
+    return err;
 }
 
 }  // namespace lm

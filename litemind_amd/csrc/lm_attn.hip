@@ -657,8 +657,13 @@ int absorb(AttnState* st, AttnLayer& L, int32_t layer, hipStream_t stream) {
         L.absorbed = nullptr;
         return fail(LM_ENOMEM, "absorbed weights of layer " + std::to_string(layer));
     }
-    LM_ATT_HIP(lm::launch_absorb(L.w16[lm::kProjKvb], L.absorbed, c.num_heads, c.qk_nope_head_dim, c.v_head_dim,
-                                 c.kv_lora_rank, stream));
+    const hipError_t err = lm::launch_absorb(L.w16[lm::kProjKvb], L.absorbed, c.num_heads, c.qk_nope_head_dim,
+                                             c.v_head_dim, c.kv_lora_rank, stream);
+    if (err != hipSuccess) {
+        (void)hipFree(L.absorbed);
+        L.absorbed = nullptr;
+        return fail(LM_EHIP, std::string("absorbed weights: ") + hipGetErrorString(err));
+    }
     return LM_OK;
 }
 
@@ -682,8 +687,9 @@ int check_paged(lm_context* ctx, const lm_paged_step* step, AttnState** out) {
     const lm_mla_config& c = st->cfg;
     const int64_t widest = std::max({static_cast<int64_t>(c.hidden_size), static_cast<int64_t>(c.q_lora_rank),
                                      static_cast<int64_t>(c.num_heads) * c.v_head_dim});
-    if (step->tokens * widest > INT32_MAX / 2 || step->tokens * c.num_heads > INT32_MAX) {
-        return fail(LM_EINVAL, "too many tokens in one step");
+    // 32-bit offsets of the projections, 2^32 threads of the launches
+    if (step->tokens * widest > INT32_MAX / 2 || step->tokens * c.num_heads > 1 << 24) {
+        return fail(LM_EINVAL, "too many tokens in one step: tokens * heads at most 2^24, times the widest row 2^30");
     }
     if (step->tokens == 0) {
         return LM_OK;

@@ -180,8 +180,9 @@ int lm_paged_attention(lm_context* ctx, const lm_paged_step* step, const void* q
         if (s.tokens == 0) {
             return ctx != nullptr ? LM_OK : fail(LM_EINVAL, "null context");
         }
-        if (s.tokens * heads > INT32_MAX) {
-            return fail(LM_EINVAL, "tokens * heads must stay under 2^31");
+        if (s.tokens * heads > INT32_MAX / 2 ||
+            !lm::paged_shares_out(s.tokens, heads, static_cast<int64_t>(s.table_width) * s.page_size)) {
+            return fail(LM_EINVAL, "tokens * heads must stay under 2^30, and with the keys of a table row under 2^62");
         }
         if (s.table == nullptr || s.lengths == nullptr || s.starts == nullptr || !aligned(s.table, 4) ||
             !aligned(s.lengths, 4) || !aligned(s.starts, 4)) {

@@ -62,6 +62,8 @@ struct PagedAttention {
 // paged_workspace_bytes(), whatever the step.
 bool paged_tiled(int32_t rank, int32_t rope);
 int paged_block_rows(int32_t max_added, int32_t heads);
+// Whether the costs of a step's blocks fit in 64 bits (room: tokens that a table row covers).
+bool paged_shares_out(int64_t tokens, int32_t heads, int64_t room);
 int64_t paged_workspace_bytes(int rows);
 hipError_t launch_paged_attention(const PagedAttention& a, void* workspace, hipStream_t s);
 

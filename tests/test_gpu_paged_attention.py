@@ -271,3 +271,24 @@ def test_lengths_beyond_the_arrays(ctx):
     assert e.value.status == -5
     got = b.dev["out"].download()
     b.check(got, [0])
+
+
+@pytest.mark.parametrize("requests,heads,rank,rope", [(70000, 1, 512, 64), (131072, 9, 8, 0)])
+def test_very_many_requests(ctx, requests, heads, rank, rope):
+    """Single tokens of requests that share one page: each row is the one latent that it sees, to its bits."""
+    announce(f"paged attention: {requests} requests, {heads} heads, rank {rank}")
+    rng = np.random.default_rng(20)
+    width = rank + rope
+    pool = encode(rng.normal(size=(1, 16, width)), lm.DT_F16)
+    dev = {"table": ctx.to_device(np.zeros((requests, 1), np.int32)), "lengths": ctx.to_device(np.ones(requests, np.int32)),
+           "starts": ctx.to_device(np.arange(requests + 1, dtype=np.int32)),
+           "q": ctx.empty((requests, heads, width), np.uint16).zero(), "pool": ctx.to_device(pool),
+           "out": ctx.empty((requests, heads, rank), np.uint16).zero()}
+    step = lm.PagedStep(requests=requests, tokens=requests, pages=1, page_size=16, table_width=1, max_added=1)
+    for k in ("table", "lengths", "starts"):
+        setattr(step, k, dev[k].ptr)
+    ctx.paged_attention(step, dev["q"], dev["pool"], heads, SCALE, dev["out"], rank=rank, rope=rope)
+    out = dev["out"].download()
+    for b in dev.values():
+        b.free()
+    assert (out == pool[0, 0, :rank]).all()

@@ -163,3 +163,18 @@ def test_steps_in_turn(ctx):
         live = [table[r, :ref.pages_of(c, page)].tolist() for r, c in enumerate(cached)]
         held = [x for row in live for x in row] + [ring[(queue[0] + k) % pages] for k in range(queue[1])]
         assert sorted(held) == list(range(pages))  # every page in one place
+
+
+def test_rings_that_cannot_be(ctx):
+    """A negative count, and requests that give back more pages than the pool has room for: refused, nothing changed."""
+    announce("page plan: rings that cannot be")
+    table, ring = np.arange(12, dtype=np.int32).reshape(3, 4) % 9, np.arange(9, dtype=np.int32)
+    for cached, added, queue in (([1, 2, 3], [0, 0, 0], [0, -1]), ([64, 64, 64], [-1, -1, -1], [4, 0]),
+                                 ([64, 64, 1], [-1, -1, 1], [4, 2]), ([1, 2, 3], [0, 0, 0], [0, 10])):
+        plan = Plan(ctx, cached, added, table, ring, queue, 16, 4, 4)
+        ctx.page_plan(plan.step)
+        got = plan.read()
+        assert got["info"].tolist() == [lm.STEP_RING, 0, 0, 0]
+        assert got["queue_out"].tolist() == [queue[0], queue[1]] and got["starts"].tolist() == [0] * 4
+        assert np.array_equal(got["table"], table) and np.array_equal(got["ring"], ring)
+        assert got["lengths"].tolist() == cached and (got["slots"] == -1).all() and (got["positions"] == 0).all()

@@ -184,3 +184,55 @@ def test_greedy_is_the_heads_choice(ctx):
     x = rows_of(rng, 33, 5003, True)
     t, p = run(ctx, x, settings([(0.0, 0, 1.0, 0.0)] * 33), rng.random(33).astype(np.float32))
     assert np.array_equal(t, x.argmax(1)) and (p == 1).all()
+
+
+@pytest.mark.parametrize("vocab", [1000, 6007, 20011])
+def test_ranges(ctx, vocab):
+    """Logits over the whole range of the type or in its smallest steps, far outliers on either side, masked and not,
+    under temperatures as far apart: the stretches that the kernel divides a row into have nothing to hold on to."""
+    announce(f"sample: ranges, vocabulary {vocab}")
+    rng = np.random.default_rng(vocab)
+    big, tiny = np.finfo(np.float32).max, np.float32(1e-45)
+
+    def normal(k=1.0):
+        return rng.normal(size=vocab).astype(np.float32) * np.float32(k)
+
+    def masked(x):
+        y = x.copy()
+        y[rng.random(vocab) < 0.5] = -np.inf
+        return y
+
+    def put(x, v):
+        y = x.copy()
+        y[rng.integers(0, vocab)] = v
+        return y
+
+    rows = [(rng.uniform(-1, 1, vocab).astype(np.float32) * big, 1e38), (rng.uniform(-1, 1, vocab).astype(np.float32) * big, 1.0),
+            (rng.integers(0, 90, vocab).astype(np.float32) * tiny, 1.0), (rng.integers(0, 90, vocab).astype(np.float32) * tiny, 2e-44),
+            (put(normal(), big), 1.0), (put(normal(), -big), 1.0), (put(normal(), big), 1e38), (normal() + np.float32(1e6), 1.0),
+            (normal(200.0), 0.01), (normal(), 40.0), (normal(), 1e-3), (masked(normal()), 0.9), (masked(normal(1e-3)), 1.0),
+            (normal() - np.float32(2e38), 1e37), (masked(put(normal(), np.inf)), 1.0), (normal(), np.inf),
+            (np.full(vocab, -big, np.float32), 1.0), (put(normal(), np.inf), 1e38)]
+    for top_k, top_p, min_p in ((0, 1.0, 0.0), (50, 1.0, 0.0), (0, 0.9, 0.0), (3000, 0.8, 0.0), (0, 1.0, 0.3), (700, 0.6, 0.01)):
+        x = np.ascontiguousarray([r[0] for r in rows])
+        sets = settings([(r[1], top_k, top_p, min_p) for r in rows])
+        u = rng.random(len(rows)).astype(np.float32)
+        t, p = run(ctx, x, sets, u)
+        for i in range(len(rows)):
+            want, chance, near = ref.sample(x[i], *sets[i], u[i])
+            if near < vocab * 2.0 ** -45:
+                continue
+            assert t[i] == want, f"row {i}: {t[i]}, not {want} ({sets[i]}, u {u[i]})"
+            assert abs(p[i] - chance) <= 2.0 ** -24 * chance + 2.0 ** -38
+
+
+def test_more_rows_than_a_launch_takes(ctx):
+    announce("sample: two million rows")
+    rows = 2 ** 21 + 3
+    x = np.zeros((rows, 2), np.float32)
+    x[1::2, 1] = 1.0
+    token = ctx.to_device(np.full(rows + 1, -9, np.int32))
+    sets = np.zeros(rows, lm.SAMPLING)
+    ctx.sample(ctx.to_device(x), rows, 2, ctx.to_device(sets), ctx.to_device(np.zeros(rows, np.float32)), token)
+    t = token.download()
+    assert t[-1] == -9 and (t[:-1] == np.arange(rows) % 2).all()

@@ -65,7 +65,8 @@ def test_good_arguments_reach_the_context():
     dict(dtype=lm.DT_F32), dict(dtype=0), dict(heads=0), dict(heads=2 ** 30), dict(rank=0), dict(rank=12),
     dict(rank=1032), dict(rope=-8), dict(rope=4), dict(rope=264), dict(scale=float("nan")), dict(scale=float("inf")),
     dict(out=SOME), dict(out=SOME * 16),
-    dict(step=dict(table=None)), dict(step=dict(lengths=None)), dict(step=dict(starts=SOME + 1))], ids=str)
+    dict(step=dict(table=None)), dict(step=dict(lengths=None)), dict(step=dict(starts=SOME + 1)),
+    dict(step=dict(tokens=2 ** 20, page_size=16, pages=1, table_width=2 ** 26), heads=1023)], ids=str)
 def test_attention_arguments(bad):
     lib = lm.load_library()
     a = dict(q=SOME, pool=SOME * 16, dtype=lm.DT_F16, heads=16, rank=512, rope=64, scale=0.1, out=SOME * 65536)
@@ -129,3 +130,21 @@ def test_attention_bound_is_tight_and_catches_a_dropped_key():
     assert bound.max() < 0.01
     less, _ = ref.attention(q, rows[1:], 37, 0.2, 16, 2.0 ** -11)
     assert (np.abs(less - out) > bound).mean() > 0.5
+
+
+@pytest.mark.parametrize("pages,page_size", [(0, 64), (-1, 64), (2 ** 31, 64), (2 ** 25, 64), (4, 0), (4, 8), (4, 24), (4, 4112)])
+def test_pool_arguments(pages, page_size):
+    assert "null context" not in refused(lm.load_library().lm_paged_configure(None, pages, page_size))
+
+
+def test_layers_need_a_context():
+    lib, s, out = lm.load_library(), step(), C.c_void_p()
+    assert "null output" in refused(lib.lm_paged_pool(None, 0, None))
+    for f, *args in ((lib.lm_paged_configure, None, 4, 64), (lib.lm_paged_pool, None, 0, C.byref(out)),
+                 (lib.lm_paged_forward, None, 0, C.byref(s), SOME, SOME * 16, 0),
+                 (lib.lm_paged_decoder_forward, None, 0, 0, C.byref(s), SOME, 0)):
+        assert "null context" in refused(f(*args))
+    s.page_size = 17
+    for f, *args in ((lib.lm_paged_forward, None, 0, C.byref(s), SOME, SOME * 16, 0),
+                 (lib.lm_paged_decoder_forward, None, 0, 0, C.byref(s), SOME, 0), (lib.lm_paged_forward, None, 0, None, SOME, SOME * 16, 0)):
+        assert "null context" not in refused(f(*args))
