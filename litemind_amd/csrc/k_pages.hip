@@ -49,8 +49,9 @@ __device__ inline Request load_request(const lm_paged_step& s, int64_t r) {
     q.bad_length = q.cached < 0 || length > static_cast<int64_t>(s.table_width) * s.page_size;
     q.bad_added = q.added > s.max_added;
     if (!q.bad_length) {
-        q.had = (q.cached + s.page_size - 1) / s.page_size;
-        q.taken = static_cast<int32_t>((length + s.page_size - 1) / s.page_size) - q.had;
+        const uint32_t size = static_cast<uint32_t>(s.page_size);
+        q.had = static_cast<int32_t>((static_cast<uint32_t>(q.cached) + size - 1) / size);
+        q.taken = static_cast<int32_t>((static_cast<uint32_t>(length) + size - 1) / size) - q.had;
     }
     return q;
 }
@@ -75,12 +76,13 @@ __global__ __launch_bounds__(kThreads) void page_plan_kernel(const lm_paged_step
     __shared__ int64_t wave_tokens[kWaves], wave_taken[kWaves], wave_back[kWaves];
     __shared__ int32_t flags[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t pages = s.pages;
-    const int64_t head = ((s.queue_in[0] % pages) + pages) % pages;
-    const int32_t count = s.queue_in[1];
     // places in the ring in 32 bits: a division of 64 takes 150 instructions
-    const uint32_t ring = static_cast<uint32_t>(pages), front = static_cast<uint32_t>(head),
-                   behind = static_cast<uint32_t>((head + max(count, 0)) % pages);
+    const int32_t count = s.queue_in[1];
+    const uint32_t ring = static_cast<uint32_t>(s.pages);
+    const int32_t head = s.queue_in[0] % static_cast<int32_t>(ring);
+    const uint32_t front = static_cast<uint32_t>(head) + (head < 0 ? ring : 0);
+    const uint32_t behind = (front + static_cast<uint32_t>(max(count, 0))) % ring;
+    const Request mine = load_request(s, tid);  // of the first chunk
     // can the step be served: totals in 64 bits
     if (tid < 2) {
         flags[tid] = 0;
@@ -88,7 +90,7 @@ __global__ __launch_bounds__(kThreads) void page_plan_kernel(const lm_paged_step
     __syncthreads();
     int64_t tokens = 0, taken = 0, back = 0;
     for (int64_t r = tid; r < s.requests; r += kThreads) {
-        const Request q = load_request(s, r);
+        const Request q = r < kThreads ? mine : load_request(s, r);
         if (q.bad_length) {
             flags[0] = 1;
         }
@@ -119,14 +121,14 @@ __global__ __launch_bounds__(kThreads) void page_plan_kernel(const lm_paged_step
     const int32_t status = flags[0] != 0                             ? LM_STEP_LENGTH
                            : flags[1] != 0 || tokens > s.tokens      ? LM_STEP_TOKENS
                            : taken > max(static_cast<int64_t>(count), int64_t{0}) ? LM_STEP_PAGES
-                           : count < 0 || count - taken + back > pages ? LM_STEP_RING
+                           : count < 0 || count - taken + back > s.pages ? LM_STEP_RING
                                                                        : LM_STEP_OK;
     Sums before{};  // of the requests in earlier chunks
     if (status == LM_STEP_OK) {
         for (int64_t r0 = 0; r0 < s.requests; r0 += kThreads) {
             const int64_t r = r0 + tid;
             const int n = static_cast<int>(min(s.requests - r0, static_cast<int64_t>(kThreads)));
-            const Request q = load_request(s, r);
+            const Request q = r0 == 0 ? mine : load_request(s, r);
             const Sums own{q.added, q.over ? 0 : q.taken, q.over ? q.had : 0};
             Sums sum = own;
             for (int o = 1; o < 64; o <<= 1) {
@@ -205,7 +207,7 @@ __global__ __launch_bounds__(kThreads) void page_plan_kernel(const lm_paged_step
     }
     if (tid == 0) {
         s.starts[s.requests] = before.tokens;
-        s.queue_out[0] = static_cast<int32_t>((head + before.taken) % pages);
+        s.queue_out[0] = static_cast<int32_t>((front + static_cast<uint32_t>(before.taken)) % ring);
         s.queue_out[1] = status == LM_STEP_OK ? count - before.taken + before.back : count;
         s.info[0] = status;
         s.info[1] = before.tokens;
