@@ -7,7 +7,9 @@
 //
 // Three sums over the requests; per four tokens, and per taken and returned page,
 // one search in them.  Latency bound: a decode step of 48 requests reads and
-// writes 2 KB.  One workgroup; requests in chunks of one per thread.
+// writes 2 KB and takes 10 us by itself, 3.9 among others' calls; 509 requests of
+// up to 64 new tokens take 15.6 and 5.2.  One workgroup; requests in chunks of one
+// per thread.
 #include "serve_internal.h"
 
 namespace lm {
