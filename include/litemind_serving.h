@@ -114,9 +114,9 @@ int lm_paged_pool(lm_context* ctx, int32_t layer, void** out_dev);
  * step's slots of the layer's pool, attention over each request's pages, and
  * out_dev [tokens, hidden] = o_proj . context, or added to it (accumulate = 1).
  * The step's pages and page_size are those of lm_paged_configure; max_added,
- * positions and slots are read too.  Rows past the last new token are computed
- * from what x_dev holds there, without a store or attention: they neither reach
- * other rows nor mean anything.  Positions at or past context_length are not
+ * positions and slots are read too.  Rows past the last new token may hold
+ * anything in x_dev and reach no other row; in out_dev they become 0, or stay as
+ * they were (accumulate = 1).  Positions at or past context_length are not
  * rotated, as lm_attention_forward's.  kv_b_proj is absorbed into the query and
  * the output; queries, latents and weights round to fp16, within the MFMA
  * path's tolerance.  out_dev must not overlap x_dev.  tokens * heads at most

@@ -87,6 +87,7 @@ def test_forward_against_the_oracle(d, page):
             y = dout.download()
             ctx.paged_forward(1, s.step, dx, dsum, accumulate=True)  # the same latents into the same slots
             added_to = dsum.download()
+            assert (y[starts[-1]:] == 0).all() and np.array_equal(added_to[starts[-1]:], base[starts[-1]:])
             for r in range(5):
                 lo, hi = starts[r], starts[r + 1]
                 if hi == lo:
