@@ -1,4 +1,5 @@
 """lm_paged_attention on the GPU against the 64-bit restatement, within what its roundings allow element by element."""
+import ctypes as C
 import random
 
 import numpy as np
@@ -292,3 +293,59 @@ def test_very_many_requests(ctx, requests, heads, rank, rope):
     for b in dev.values():
         b.free()
     assert (out == pool[0, 0, :rank]).all()
+
+
+def put(ctx, ptr, host):
+    host = np.ascontiguousarray(host)
+    ctx._check(ctx.lib.lm_copy_h2d(ctx.handle, C.c_void_p(ptr), host.ctypes.data, host.nbytes))
+
+
+def get(ctx, ptr, like):
+    out = np.empty_like(like)
+    ctx._check(ctx.lib.lm_copy_d2h(ctx.handle, out.ctypes.data, C.c_void_p(ptr), out.nbytes))
+    return out
+
+
+@pytest.mark.parametrize("rank,rope,added", [(512, 64, [1, 1, 1]), (512, 64, [1, 70, 3]), (64, 16, [1, 2, 1])])
+def test_pages_past_four_gigabytes(ctx, rank, rope, added):
+    announce(f"paged attention: pages past 4 GiB, rank {rank}, {added}")
+    b = Batch([5000, 77, 300], added, 16, page=4096, rank=rank, rope=rope, seed=21)
+    page_bytes = 2 * b.page * (rank + rope)
+    base = (5 << 30) // page_bytes
+    pool = ctx.empty((base + b.pages) * page_bytes // 2, np.uint16)
+    b.table = np.where(b.table >= 0, b.table + base, -1).astype(np.int32)
+    b.upload(ctx)
+    put(ctx, pool.ptr + base * page_bytes, b.pool)
+    b.step.pages = base + b.pages
+    b.dev["pool"] = pool
+    b.call(ctx)
+    got = b.dev["out"].download()
+    pool.free()
+    b.check(got)
+
+
+def test_rows_past_four_gigabytes(ctx):
+    """Queries and outputs of 3.84 million rows: the last requests' rows are theirs."""
+    announce("paged attention: query rows past 4 GiB")
+    requests, heads, width = 30000, 128, 576
+    rng = np.random.default_rng(22)
+    pool, words = encode(rng.normal(size=(2, 16, width)), lm.DT_F16), heads * width
+    table, lengths = np.zeros((requests, 1), np.int32), np.ones(requests, np.int32)
+    table[-2:], lengths[-2:] = 1, 16
+    dev = {"table": ctx.to_device(table), "lengths": ctx.to_device(lengths),
+           "starts": ctx.to_device(np.arange(requests + 1, dtype=np.int32)),
+           "q": ctx.empty((requests, heads, width), np.uint16).zero(), "pool": ctx.to_device(pool),
+           "out": ctx.empty((requests, heads, 512), np.uint16).zero()}
+    q = encode(rng.normal(size=(2, heads, width)) * 0.7, lm.DT_F16)
+    put(ctx, dev["q"].ptr + 2 * (requests - 2) * words, q)
+    step = lm.PagedStep(requests=requests, tokens=requests, pages=2, page_size=16, table_width=1, max_added=1)
+    for k in ("table", "lengths", "starts"):
+        setattr(step, k, dev[k].ptr)
+    ctx.paged_attention(step, dev["q"], dev["pool"], heads, SCALE, dev["out"])
+    tail = get(ctx, dev["out"].ptr + 2 * (requests - 40) * heads * 512, np.empty((40, heads, 512), np.uint16))
+    for b in dev.values():
+        b.free()
+    assert (tail[:38] == pool[0, 0, :512]).all()
+    for i in range(2):
+        want, bound = ref.attention(decode(q[i:i + 1], lm.DT_F16), decode(pool[1], lm.DT_F16), 15, SCALE, 512, UNIT[lm.DT_F16])
+        assert (np.abs(decode(tail[38 + i:39 + i], lm.DT_F16) - want) <= bound).all()

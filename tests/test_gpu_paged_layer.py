@@ -153,6 +153,32 @@ def test_pool_rows():
         assert (np.abs(got - want) <= bound + (2.0 ** -11 + 2.0 ** -20) * (np.abs(want) + bound) + 2.0 ** -25).all()
 
 
+def test_pages_past_four_gigabytes():
+    """A layer's pool of 5 GB: latents stored to its last pages, and read there."""
+    announce("paged layer: pages past 4 GiB")
+    d = dataclasses.replace(SMALL, max_positions=64)
+    L, pages, page = wl.mla_layer(33, 0, d), 8000, 4096
+    with lm.Context(moe_dims(d.hidden).moe_config(num_layers=1)) as ctx:
+        ctx.attention_configure(wl.mla_config(d))
+        wl.upload_mla_layer(ctx, 0, L)
+        s = Service(ctx, 2, pages, page, 1, 40, 30)
+        s.put("ring", np.arange(pages)[::-1])
+        caches, seen = oracle_caches(d, 2), [0, 0]
+        for added in ([9, 30], [1, 1]):
+            starts = s.plan(added)
+            assert int(s.dev["slots"].download()[:starts[-1]].min()) * (d.kv_lora_rank + d.qk_rope) * 2 > 2 ** 32
+            x = wl.tokens(7 + added[0], s.tokens, d.hidden)
+            dout = ctx.to_device(np.zeros_like(x))
+            ctx.paged_forward(0, s.step, ctx.to_device(x), dout)
+            y = dout.download()
+            for r in range(2):
+                lo, hi = starts[r], starts[r + 1]
+                want, _ = ol.oracle_mla(L, x[lo:hi], seen[r], caches[r])
+                seen[r] += hi - lo
+                mx, rel = layer_error(y[lo:hi], want)
+                assert mx <= MAX_ABS and rel <= MEAN_REL
+
+
 def run_decoder(d, path, layers, prompts, follow):
     """The same tokens through pages, all requests together, and alone through the single-sequence caches."""
     dims = moe_dims(d.hidden, layers)

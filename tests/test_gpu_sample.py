@@ -1,4 +1,6 @@
 """lm_sample on the GPU against the 64-bit restatement: the same tokens, and probabilities to single precision."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -236,3 +238,20 @@ def test_more_rows_than_a_launch_takes(ctx):
     ctx.sample(ctx.to_device(x), rows, 2, ctx.to_device(sets), ctx.to_device(np.zeros(rows, np.float32)), token)
     t = token.download()
     assert t[-1] == -9 and (t[:-1] == np.arange(rows) % 2).all()
+
+
+def test_rows_far_apart(ctx):
+    """Rows 4 GiB apart."""
+    announce("sample: rows 4 GiB apart")
+    rng = np.random.default_rng(11)
+    rows, vocab, stride = 3, 5003, 2 ** 30 + 1
+    x, sets, u = rows_of(rng, rows, vocab), any_settings(rng, rows), rng.random(rows).astype(np.float32)
+    wide, token = ctx.empty((rows - 1) * stride + vocab), ctx.empty(rows, np.int32)
+    for r in range(rows):
+        ctx._check(ctx.lib.lm_copy_h2d(ctx.handle, C.c_void_p(wide.ptr + 4 * r * stride), x[r].ctypes.data, x[r].nbytes))
+    ctx.sample(wide, rows, vocab, ctx.to_device(sets), ctx.to_device(u), token, row_stride=stride)
+    t = token.download()
+    wide.free()
+    for r in range(rows):
+        want, _, near = ref.sample(x[r], *sets[r], u[r])
+        assert near < vocab * 2.0 ** -45 or t[r] == want
