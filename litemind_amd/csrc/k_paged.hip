@@ -82,7 +82,9 @@ struct Half<bf16> {
 // by itself: 64 keys 241 us, 128 176, 256 137, 384 136; 300 requests of 200 keys:
 // 48, 42, 41, 42; few long ones: all within 3 %).
 constexpr int kExtra = 256;
-// Keys per workgroup below which fewer take part.
+// Keys per workgroup below which fewer take part (one token after 4000 by itself,
+// with the join: 64 keys 18.5 us, 128 18.8, 256 21.9, 512 29.6; after 500 19.3,
+// 19.4, 21.4, 28.2).
 constexpr int kLeast = 128;
 
 struct Shares {
@@ -106,6 +108,9 @@ struct Piece {
     int32_t parts;
     int32_t request;  // that `begin` lies in
     int64_t base;     // cost of the requests before it
+    int32_t blocks;   // of all requests; more than kGrid: that many at least
+    int32_t first;    // of request `thread`, where there are as many threads
+    int32_t after;    // of a block cut by itself: its pieces after the first; -1: the line's
 };
 // Begin of piece g. (In doubles, as the cuts of blocks below: a 64-bit division
 // is 150 instructions. Neighbours form a border from the same numbers, so they
@@ -119,33 +124,44 @@ __device__ inline int32_t cut(int64_t x, int64_t cost, int32_t tiles) {
 }
 
 // Every thread of the workgroup calls it. Threads take stretches of requests;
-// `scratch` (kWaves + 2 words of 64 bits) passes the sums.
+// `scratch` (2 kWaves + 2 words of 64 bits) passes the sums.
 __device__ inline Piece find_piece(const PagedView& v, const Shares& sh, int32_t g, int64_t* scratch) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int32_t per = (v.requests + kThreads - 1) / kThreads;
     const int32_t r0 = min(tid * per, v.requests), r1 = min(r0 + per, v.requests);
     int64_t own = 0;
+    int32_t mine = 0;  // blocks; more than kGrid of a thread count as one more than kGrid
 #pragma unroll 1
     for (int32_t r = r0; r < r1; ++r) {
         const PagedRequest q = paged_request(v, r);
         own += sh.cost(q, sh.blocks(q));
+        mine = min(mine + min(sh.blocks(q), kGrid + 1), kGrid + 1);
     }
     int64_t sum = own;
+    int32_t many = mine;
 #pragma unroll 1
     for (int o = 1; o < 64; o <<= 1) {
         const int64_t up = __shfl_up(sum, o);
+        const int32_t up_many = __shfl_up(many, o);
         sum += lane >= o ? up : 0;
+        many += lane >= o ? up_many : 0;
     }
     if (lane == 63) {
         scratch[wave] = sum;
+        scratch[kWaves + 2 + wave] = many;
     }
     __syncthreads();
     int64_t before = sum - own, total = 0;
+    Piece p;
+    p.first = many - mine;
+    p.blocks = 0;
+    p.after = -1;
     for (int w = 0; w < kWaves; ++w) {
         before += w < wave ? scratch[w] : 0;
         total += scratch[w];
+        p.first += w < wave ? static_cast<int32_t>(scratch[kWaves + 2 + w]) : 0;
+        p.blocks += static_cast<int32_t>(scratch[kWaves + 2 + w]);
     }
-    Piece p;
     p.total = total;
     p.parts = static_cast<int32_t>(max(int64_t{1}, min(static_cast<int64_t>(kGrid), static_cast<int64_t>(static_cast<double>(total) / (kLeast * static_cast<double>(sh.heads))))));
     p.begin = g < p.parts ? border(total, p.parts, g) : total;
@@ -167,6 +183,119 @@ __device__ inline Piece find_piece(const PagedView& v, const Shares& sh, int32_t
     p.request = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(scratch[kWaves]));
     p.base = scratch[kWaves + 1];
     return p;
+}
+
+// Where the step has at most kGrid blocks, they are cut into equal pieces each by
+// itself if that leaves no piece much longer than the even share, so that no
+// workgroup has pieces of two: blocks of `tiles` tiles into ceil(tiles / T), T the
+// least, from the even share on, that needs no more than kGrid pieces, and at most
+// kSecond tiles past it, which is what a second piece costs. (By itself, with and
+// without: one token of 32 requests after up to 4000 28.3 and 33.0 us, of 16 with
+// 128 heads after up to 2500 29.8 and 36.8; 512 tokens after 3001 88.0 and 93.6. To
+// look for it costs 0.5 to 1.5 us where it is not taken.)
+constexpr int kSecond = 8;
+
+// Replaces p by the workgroup's piece of that kind, or leaves it. Every thread of
+// the workgroup calls it; `words` holds kThreads + kGrid + kWaves + 8.
+__device__ inline void own_piece(const PagedView& v, const Shares& sh, int32_t g, Piece& p, int32_t* words) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (v.requests > kThreads || p.blocks < 2 || p.blocks > kGrid) {
+        return;
+    }
+    int32_t* const firsts = words;  // of each request's blocks
+    int32_t* const tiles = words + kThreads;
+    int32_t* const part = tiles + kGrid;
+    int32_t* const found = part + kWaves;
+    firsts[tid] = p.first;
+    if (tid == 0) {
+        found[0] = 0x7fffffff;
+        found[4] = 0;
+    }
+    __syncthreads();
+    int32_t r = 0, mine = 0;
+    if (tid < p.blocks) {
+        // the last request whose blocks begin at or before this one
+        int32_t hi = v.requests;
+#pragma unroll 1
+        while (hi - r > 1) {
+            const int32_t mid = (r + hi) / 2;
+            if (firsts[mid] <= tid) {
+                r = mid;
+            } else {
+                hi = mid;
+            }
+        }
+        mine = min(sh.tiles(paged_request(v, r), tid - firsts[r]), 0x7fffffff / kGrid);  // (no longer ones fit the rest)
+        tiles[tid] = mine;
+    }
+    int32_t sum = mine;
+    for (int o = 32; o >= 1; o >>= 1) {
+        sum += __shfl_xor(sum, o);
+    }
+    if (lane == 0) {
+        part[wave] = sum;
+    }
+    __syncthreads();
+    sum = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        sum += part[w];
+    }
+    const uint32_t even = static_cast<uint32_t>(max((sum + kGrid - 1) / kGrid, kLeast / kTile));
+    // a wave for each T that is tried
+    static_assert(kWaves == 8 && kSecond == 8);
+    const uint32_t size = even + static_cast<uint32_t>(wave < 6 ? wave : 2 * wave - 6);
+    int32_t pieces = 0;
+#pragma unroll 1
+    for (int i = lane; i < p.blocks; i += 64) {
+        pieces += static_cast<int32_t>((static_cast<uint32_t>(tiles[i]) + size - 1) / size);
+    }
+    for (int o = 32; o >= 1; o >>= 1) {
+        pieces += __shfl_xor(pieces, o);
+    }
+    if (lane == 0 && pieces <= kGrid) {
+        atomicMin(&found[0], static_cast<int32_t>(size));
+    }
+    __syncthreads();
+    const int32_t T = found[0];
+    if (T == 0x7fffffff) {
+        return;
+    }
+    const int32_t parts = (mine + T - 1) / T;
+    int32_t first = parts;
+#pragma unroll 1
+    for (int o = 1; o < 64; o <<= 1) {
+        const int32_t up = __shfl_up(first, o);
+        first += lane >= o ? up : 0;
+    }
+    if (lane == 63) {
+        part[wave] = first;
+    }
+    __syncthreads();
+    first -= parts;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        first += w < wave ? part[w] : 0;
+    }
+    if (g >= first && g < first + parts) {
+        found[1] = r;
+        found[2] = tid - firsts[r];
+        found[3] = g - first;
+        found[4] = parts;
+    }
+    __syncthreads();
+    // the piece on its request's own line
+    p.request = __builtin_amdgcn_readfirstlane(found[1]);
+    const int32_t block = __builtin_amdgcn_readfirstlane(found[2]), at = __builtin_amdgcn_readfirstlane(found[3]);
+    p.after = __builtin_amdgcn_readfirstlane(found[4]) - 1;
+    p.base = p.begin = p.end = 0;
+    if (p.after >= 0) {
+        const PagedRequest q = paged_request(v, p.request);
+        const int64_t from = sh.cost(q, block), cost = sh.cost(q, block + 1) - from;
+        p.begin = from + border(cost, p.after + 1, at);
+        p.end = from + border(cost, p.after + 1, at + 1);
+    }
+    __syncthreads();
 }
 
 // A stretch of one block's tiles.
@@ -223,7 +352,9 @@ struct Walk {
         s.tile0 = s.begins ? 0 : cut(p.begin - at, cost, tiles);
         s.tile1 = s.ends ? tiles : cut(p.end - at, cost, tiles);
         s.parts_after = 0;
-        if (s.begins && !s.ends) {
+        if (p.after >= 0) {
+            s.parts_after = p.after;
+        } else if (s.begins && !s.ends) {
             // the last piece that begins before the block's end, from its share of the line
             const int32_t own = static_cast<int32_t>(blockIdx.x);
             int32_t g = static_cast<int32_t>(static_cast<double>(at + cost) * p.parts / static_cast<double>(p.total));
@@ -377,7 +508,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_rows_kernel(const TileArgs 
     __shared__ __align__(16) char weights[2][M * kTile * 2];
     __shared__ float tops[2][M];
     __shared__ int late_flags[4];
-    __shared__ int64_t scratch[kWaves + 2];
+    __shared__ int64_t scratch[2 * kWaves + 2];
     char* const ring[4] = {s0, s1, s2, s3};
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -386,6 +517,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_rows_kernel(const TileArgs 
     Walk walk;
     walk.sh = Shares{a.heads, M};
     walk.p = find_piece(a.view, walk.sh, blockIdx.x, scratch);
+    own_piece(a.view, walk.sh, blockIdx.x, walk.p, reinterpret_cast<int32_t*>(s0));
     if (tid == 0) {
         a.parts.heads[blockIdx.x].rows = 0;
     }
@@ -1107,6 +1239,9 @@ bool paged_shares_out(int64_t tokens, int32_t heads, int64_t room) {
     return (rows / 16 + static_cast<double>(tokens)) * ((static_cast<double>(room) + kExtra) * heads + rows + 64) < 0x1p62;
 }
 
+// 16 rows where no request has more (one token of 32 requests, 16 heads, three
+// contexts in turn: 22.8 us, in blocks of 64 24.9), or else 64 (32 heads, by itself:
+// 36 us, in blocks of 16 44).
 int paged_block_rows(int32_t max_added, int32_t heads) {
     return static_cast<int64_t>(max_added) * heads <= 16 ? 16 : 64;
 }
