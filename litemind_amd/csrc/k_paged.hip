@@ -110,6 +110,7 @@ struct Piece {
     int64_t base;     // cost of the requests before it
     int32_t blocks;   // of all requests; more than kGrid: that many at least
     int32_t first;    // of request `thread`, where there are as many threads
+    PagedRequest req; // `request`, where blocks are cut by themselves
     int32_t after;    // of a block cut by itself: its pieces after the first; -1: the line's
 };
 // Begin of piece g. (In doubles, as the cuts of blocks below: a 64-bit division
@@ -124,16 +125,20 @@ __device__ inline int32_t cut(int64_t x, int64_t cost, int32_t tiles) {
 }
 
 // Every thread of the workgroup calls it. Threads take stretches of requests;
-// `scratch` (2 kWaves + 2 words of 64 bits) passes the sums.
-__device__ inline Piece find_piece(const PagedView& v, const Shares& sh, int32_t g, int64_t* scratch) {
+// `scratch` (2 kWaves + 2 words of 64 bits) passes the sums; `last` is the thread's
+// last request.
+__device__ inline Piece find_piece(const PagedView& v, const Shares& sh, int32_t g, int64_t* scratch, PagedRequest& last) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int32_t per = (v.requests + kThreads - 1) / kThreads;
     const int32_t r0 = min(tid * per, v.requests), r1 = min(r0 + per, v.requests);
     int64_t own = 0;
     int32_t mine = 0;  // blocks; more than kGrid of a thread count as one more than kGrid
+    Piece p;
+    p.req = PagedRequest{};
 #pragma unroll 1
     for (int32_t r = r0; r < r1; ++r) {
         const PagedRequest q = paged_request(v, r);
+        last = q;
         own += sh.cost(q, sh.blocks(q));
         mine = min(mine + min(sh.blocks(q), kGrid + 1), kGrid + 1);
     }
@@ -152,7 +157,6 @@ __device__ inline Piece find_piece(const PagedView& v, const Shares& sh, int32_t
     }
     __syncthreads();
     int64_t before = sum - own, total = 0;
-    Piece p;
     p.first = many - mine;
     p.blocks = 0;
     p.after = -1;
@@ -196,17 +200,23 @@ __device__ inline Piece find_piece(const PagedView& v, const Shares& sh, int32_t
 constexpr int kSecond = 8;
 
 // Replaces p by the workgroup's piece of that kind, or leaves it. Every thread of
-// the workgroup calls it; `words` holds kThreads + kGrid + kWaves + 8.
-__device__ inline void own_piece(const PagedView& v, const Shares& sh, int32_t g, Piece& p, int32_t* words) {
+// the workgroup calls it; `words` holds 4 kThreads + kGrid + kWaves + 8.
+__device__ inline void own_piece(const PagedView& v, const Shares& sh, int32_t g, const PagedRequest& request_of, Piece& p,
+                                 int32_t* words) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     if (v.requests > kThreads || p.blocks < 2 || p.blocks > kGrid) {
         return;
     }
     int32_t* const firsts = words;  // of each request's blocks
-    int32_t* const tiles = words + kThreads;
+    int32_t* const request = words + kThreads;  // what they are
+    int32_t* const tiles = request + 3 * kThreads;
     int32_t* const part = tiles + kGrid;
     int32_t* const found = part + kWaves;
+    auto listed = [&](int32_t i) { return PagedRequest{request[3 * i], request[3 * i + 1], request[3 * i + 2]}; };
     firsts[tid] = p.first;
+    request[3 * tid] = request_of.first;
+    request[3 * tid + 1] = request_of.added;
+    request[3 * tid + 2] = request_of.cached;
     if (tid == 0) {
         found[0] = 0x7fffffff;
         found[4] = 0;
@@ -225,7 +235,7 @@ __device__ inline void own_piece(const PagedView& v, const Shares& sh, int32_t g
                 hi = mid;
             }
         }
-        mine = min(sh.tiles(paged_request(v, r), tid - firsts[r]), 0x7fffffff / kGrid);  // (no longer ones fit the rest)
+        mine = min(sh.tiles(listed(r), tid - firsts[r]), 0x7fffffff / kGrid);  // (no longer ones fit the rest)
         tiles[tid] = mine;
     }
     int32_t sum = mine;
@@ -290,8 +300,11 @@ __device__ inline void own_piece(const PagedView& v, const Shares& sh, int32_t g
     p.after = __builtin_amdgcn_readfirstlane(found[4]) - 1;
     p.base = p.begin = p.end = 0;
     if (p.after >= 0) {
-        const PagedRequest q = paged_request(v, p.request);
-        const int64_t from = sh.cost(q, block), cost = sh.cost(q, block + 1) - from;
+        // (the same for all threads: kept where that is known)
+        p.req.first = __builtin_amdgcn_readfirstlane(request[3 * p.request]);
+        p.req.added = __builtin_amdgcn_readfirstlane(request[3 * p.request + 1]);
+        p.req.cached = __builtin_amdgcn_readfirstlane(request[3 * p.request + 2]);
+        const int64_t from = sh.cost(p.req, block), cost = sh.cost(p.req, block + 1) - from;
         p.begin = from + border(cost, p.after + 1, at);
         p.end = from + border(cost, p.after + 1, at + 1);
     }
@@ -316,7 +329,7 @@ struct Walk {
     int64_t at;  // cost at the block's begin
     __device__ void start(const PagedView& v) {
         request = p.request;
-        req = paged_request(v, request);
+        req = p.after >= 0 ? p.req : paged_request(v, request);
         blocks = sh.blocks(req);
         // the block that `begin` lies in: the last whose cost line starts at or before it
         int32_t lo = 0, hi = blocks;
@@ -516,8 +529,11 @@ __global__ __launch_bounds__(kThreads, 2) void paged_rows_kernel(const TileArgs 
     const int col = lane & 15, grp = lane >> 4;
     Walk walk;
     walk.sh = Shares{a.heads, M};
-    walk.p = find_piece(a.view, walk.sh, blockIdx.x, scratch);
-    own_piece(a.view, walk.sh, blockIdx.x, walk.p, reinterpret_cast<int32_t*>(s0));
+    {
+        PagedRequest mine{};
+        walk.p = find_piece(a.view, walk.sh, blockIdx.x, scratch, mine);
+        own_piece(a.view, walk.sh, blockIdx.x, mine, walk.p, reinterpret_cast<int32_t*>(s0));
+    }
     if (tid == 0) {
         a.parts.heads[blockIdx.x].rows = 0;
     }
