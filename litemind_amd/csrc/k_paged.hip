@@ -77,11 +77,14 @@ struct Half<bf16> {
 // ---- sharing out the tiles ----
 // Block b of a request (rows b M .. of its added heads rows) costs the keys that
 // its last token sees, as a line in b and times heads, which keeps it whole:
-// (cached + kExtra) heads + (b + 1) M. kExtra stands for what a block costs
-// besides its tiles, 8 of 32 keys' 1.3 us (a prompt of 2048 tokens with 16 heads
-// by itself: 64 keys 241 us, 128 176, 256 137, 384 136; 300 requests of 200 keys:
-// 48, 42, 41, 42; few long ones: all within 3 %).
-constexpr int kExtra = 256;
+// (cached + kExtra) heads + (b + 1) M. kExtra, ten tiles, stands for what a block
+// costs besides its tiles and comes first, so that a workgroup which begins a
+// second block has so many tiles fewer. (By itself, with 64, 128, 192, 256, 320,
+// 384 keys: a prompt of 2048 tokens, 16 heads 235, 168, 137, 127, 122, 122 us; one
+// token of 32 requests after up to 4000 31.1, 30.0, 28.0, 25.9, 25.4, 25.6; of 128
+// requests after 1000 31.6, 30.6, 29.6, 28.2, 29.4, 29.9. Spread over the block's
+// tiles 256 keys made these 132, 33.4 and 32.3.)
+constexpr int kExtra = 320;
 // Keys per workgroup below which fewer take part (one token after 4000 by itself,
 // with the join: 64 keys 18.5 us, 128 18.8, 256 21.9, 512 29.6; after 500 19.3,
 // 19.4, 21.4, 28.2).
@@ -108,10 +111,6 @@ struct Piece {
     int32_t parts;
     int32_t request;  // that `begin` lies in
     int64_t base;     // cost of the requests before it
-    int32_t blocks;   // of all requests; more than kGrid: that many at least
-    int32_t first;    // of request `thread`, where there are as many threads
-    PagedRequest req; // `request`, where blocks are cut by themselves
-    int32_t after;    // of a block cut by itself: its pieces after the first; -1: the line's
 };
 // Begin of piece g. (In doubles, as the cuts of blocks below: a 64-bit division
 // is 150 instructions. Neighbours form a border from the same numbers, so they
@@ -119,53 +118,43 @@ struct Piece {
 __device__ inline int64_t border(int64_t total, int32_t parts, int32_t g) {
     return g >= parts ? total : static_cast<int64_t>(static_cast<double>(total) * g / parts);
 }
-// Tile of a block at which a border `x` past the block's begin cuts it.
-__device__ inline int32_t cut(int64_t x, int64_t cost, int32_t tiles) {
-    return min(tiles, static_cast<int32_t>(static_cast<double>(x) * tiles / static_cast<double>(cost)));
+// Tile of a block at which a border `x` past the block's begin cuts it: what the
+// block costs besides its tiles comes first, and a border in that does not cut.
+__device__ inline int32_t cut(int64_t x, int64_t cost, int32_t tiles, int32_t heads) {
+    const int64_t extra = static_cast<int64_t>(kExtra) * heads;
+    return x <= extra ? 0
+                      : min(tiles, static_cast<int32_t>(static_cast<double>(x - extra) * tiles /
+                                                        static_cast<double>(cost - extra)));
 }
 
 // Every thread of the workgroup calls it. Threads take stretches of requests;
-// `scratch` (2 kWaves + 2 words of 64 bits) passes the sums; `last` is the thread's
-// last request.
-__device__ inline Piece find_piece(const PagedView& v, const Shares& sh, int32_t g, int64_t* scratch, PagedRequest& last) {
+// `scratch` (kWaves + 2 words of 64 bits) passes the sums.
+__device__ inline Piece find_piece(const PagedView& v, const Shares& sh, int32_t g, int64_t* scratch) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int32_t per = (v.requests + kThreads - 1) / kThreads;
     const int32_t r0 = min(tid * per, v.requests), r1 = min(r0 + per, v.requests);
     int64_t own = 0;
-    int32_t mine = 0;  // blocks; more than kGrid of a thread count as one more than kGrid
-    Piece p;
-    p.req = PagedRequest{};
 #pragma unroll 1
     for (int32_t r = r0; r < r1; ++r) {
         const PagedRequest q = paged_request(v, r);
-        last = q;
         own += sh.cost(q, sh.blocks(q));
-        mine = min(mine + min(sh.blocks(q), kGrid + 1), kGrid + 1);
     }
     int64_t sum = own;
-    int32_t many = mine;
 #pragma unroll 1
     for (int o = 1; o < 64; o <<= 1) {
         const int64_t up = __shfl_up(sum, o);
-        const int32_t up_many = __shfl_up(many, o);
         sum += lane >= o ? up : 0;
-        many += lane >= o ? up_many : 0;
     }
     if (lane == 63) {
         scratch[wave] = sum;
-        scratch[kWaves + 2 + wave] = many;
     }
     __syncthreads();
     int64_t before = sum - own, total = 0;
-    p.first = many - mine;
-    p.blocks = 0;
-    p.after = -1;
     for (int w = 0; w < kWaves; ++w) {
         before += w < wave ? scratch[w] : 0;
         total += scratch[w];
-        p.first += w < wave ? static_cast<int32_t>(scratch[kWaves + 2 + w]) : 0;
-        p.blocks += static_cast<int32_t>(scratch[kWaves + 2 + w]);
     }
+    Piece p;
     p.total = total;
     p.parts = static_cast<int32_t>(max(int64_t{1}, min(static_cast<int64_t>(kGrid), static_cast<int64_t>(static_cast<double>(total) / (kLeast * static_cast<double>(sh.heads))))));
     p.begin = g < p.parts ? border(total, p.parts, g) : total;
@@ -189,128 +178,6 @@ __device__ inline Piece find_piece(const PagedView& v, const Shares& sh, int32_t
     return p;
 }
 
-// Where the step has at most kGrid blocks, they are cut into equal pieces each by
-// itself if that leaves no piece much longer than the even share, so that no
-// workgroup has pieces of two: blocks of `tiles` tiles into ceil(tiles / T), T the
-// least, from the even share on, that needs no more than kGrid pieces, and at most
-// kSecond tiles past it, which is what a second piece costs. (By itself, with and
-// without: one token of 32 requests after up to 4000 28.3 and 33.0 us, of 16 with
-// 128 heads after up to 2500 29.8 and 36.8; 512 tokens after 3001 88.0 and 93.6. To
-// look for it costs 0.5 to 1.5 us where it is not taken.)
-constexpr int kSecond = 8;
-
-// Replaces p by the workgroup's piece of that kind, or leaves it. Every thread of
-// the workgroup calls it; `words` holds 4 kThreads + kGrid + kWaves + 8.
-__device__ inline void own_piece(const PagedView& v, const Shares& sh, int32_t g, const PagedRequest& request_of, Piece& p,
-                                 int32_t* words) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    if (v.requests > kThreads || p.blocks < 2 || p.blocks > kGrid) {
-        return;
-    }
-    int32_t* const firsts = words;  // of each request's blocks
-    int32_t* const request = words + kThreads;  // what they are
-    int32_t* const tiles = request + 3 * kThreads;
-    int32_t* const part = tiles + kGrid;
-    int32_t* const found = part + kWaves;
-    auto listed = [&](int32_t i) { return PagedRequest{request[3 * i], request[3 * i + 1], request[3 * i + 2]}; };
-    firsts[tid] = p.first;
-    request[3 * tid] = request_of.first;
-    request[3 * tid + 1] = request_of.added;
-    request[3 * tid + 2] = request_of.cached;
-    if (tid == 0) {
-        found[0] = 0x7fffffff;
-        found[4] = 0;
-    }
-    __syncthreads();
-    int32_t r = 0, mine = 0;
-    if (tid < p.blocks) {
-        // the last request whose blocks begin at or before this one
-        int32_t hi = v.requests;
-#pragma unroll 1
-        while (hi - r > 1) {
-            const int32_t mid = (r + hi) / 2;
-            if (firsts[mid] <= tid) {
-                r = mid;
-            } else {
-                hi = mid;
-            }
-        }
-        mine = min(sh.tiles(listed(r), tid - firsts[r]), 0x7fffffff / kGrid);  // (no longer ones fit the rest)
-        tiles[tid] = mine;
-    }
-    int32_t sum = mine;
-    for (int o = 32; o >= 1; o >>= 1) {
-        sum += __shfl_xor(sum, o);
-    }
-    if (lane == 0) {
-        part[wave] = sum;
-    }
-    __syncthreads();
-    sum = 0;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-        sum += part[w];
-    }
-    const uint32_t even = static_cast<uint32_t>(max((sum + kGrid - 1) / kGrid, kLeast / kTile));
-    // a wave for each T that is tried
-    static_assert(kWaves == 8 && kSecond == 8);
-    const uint32_t size = even + static_cast<uint32_t>(wave < 6 ? wave : 2 * wave - 6);
-    int32_t pieces = 0;
-#pragma unroll 1
-    for (int i = lane; i < p.blocks; i += 64) {
-        pieces += static_cast<int32_t>((static_cast<uint32_t>(tiles[i]) + size - 1) / size);
-    }
-    for (int o = 32; o >= 1; o >>= 1) {
-        pieces += __shfl_xor(pieces, o);
-    }
-    if (lane == 0 && pieces <= kGrid) {
-        atomicMin(&found[0], static_cast<int32_t>(size));
-    }
-    __syncthreads();
-    const int32_t T = found[0];
-    if (T == 0x7fffffff) {
-        return;
-    }
-    const int32_t parts = (mine + T - 1) / T;
-    int32_t first = parts;
-#pragma unroll 1
-    for (int o = 1; o < 64; o <<= 1) {
-        const int32_t up = __shfl_up(first, o);
-        first += lane >= o ? up : 0;
-    }
-    if (lane == 63) {
-        part[wave] = first;
-    }
-    __syncthreads();
-    first -= parts;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-        first += w < wave ? part[w] : 0;
-    }
-    if (g >= first && g < first + parts) {
-        found[1] = r;
-        found[2] = tid - firsts[r];
-        found[3] = g - first;
-        found[4] = parts;
-    }
-    __syncthreads();
-    // the piece on its request's own line
-    p.request = __builtin_amdgcn_readfirstlane(found[1]);
-    const int32_t block = __builtin_amdgcn_readfirstlane(found[2]), at = __builtin_amdgcn_readfirstlane(found[3]);
-    p.after = __builtin_amdgcn_readfirstlane(found[4]) - 1;
-    p.base = p.begin = p.end = 0;
-    if (p.after >= 0) {
-        // (the same for all threads: kept where that is known)
-        p.req.first = __builtin_amdgcn_readfirstlane(request[3 * p.request]);
-        p.req.added = __builtin_amdgcn_readfirstlane(request[3 * p.request + 1]);
-        p.req.cached = __builtin_amdgcn_readfirstlane(request[3 * p.request + 2]);
-        const int64_t from = sh.cost(p.req, block), cost = sh.cost(p.req, block + 1) - from;
-        p.begin = from + border(cost, p.after + 1, at);
-        p.end = from + border(cost, p.after + 1, at + 1);
-    }
-    __syncthreads();
-}
-
 // A stretch of one block's tiles.
 struct Segment {
     PagedRequest req;
@@ -329,7 +196,7 @@ struct Walk {
     int64_t at;  // cost at the block's begin
     __device__ void start(const PagedView& v) {
         request = p.request;
-        req = p.after >= 0 ? p.req : paged_request(v, request);
+        req = paged_request(v, request);
         blocks = sh.blocks(req);
         // the block that `begin` lies in: the last whose cost line starts at or before it
         int32_t lo = 0, hi = blocks;
@@ -360,14 +227,15 @@ struct Walk {
         s.request = request;
         s.block = block;
         const int32_t tiles = sh.tiles(req, block);
-        s.begins = p.begin <= at;
         s.ends = p.end >= at + cost;
-        s.tile0 = s.begins ? 0 : cut(p.begin - at, cost, tiles);
-        s.tile1 = s.ends ? tiles : cut(p.end - at, cost, tiles);
+        s.tile0 = cut(p.begin - at, cost, tiles, sh.heads);
+        s.tile1 = s.ends ? tiles : cut(p.end - at, cost, tiles, sh.heads);
+        s.begins = s.tile0 == 0;
+        if (s.tile1 == 0) {
+            return false;  // the block begins in the next piece
+        }
         s.parts_after = 0;
-        if (p.after >= 0) {
-            s.parts_after = p.after;
-        } else if (s.begins && !s.ends) {
+        if (s.begins && !s.ends) {
             // the last piece that begins before the block's end, from its share of the line
             const int32_t own = static_cast<int32_t>(blockIdx.x);
             int32_t g = static_cast<int32_t>(static_cast<double>(at + cost) * p.parts / static_cast<double>(p.total));
@@ -521,7 +389,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_rows_kernel(const TileArgs 
     __shared__ __align__(16) char weights[2][M * kTile * 2];
     __shared__ float tops[2][M];
     __shared__ int late_flags[4];
-    __shared__ int64_t scratch[2 * kWaves + 2];
+    __shared__ int64_t scratch[kWaves + 2];
     char* const ring[4] = {s0, s1, s2, s3};
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -529,11 +397,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_rows_kernel(const TileArgs 
     const int col = lane & 15, grp = lane >> 4;
     Walk walk;
     walk.sh = Shares{a.heads, M};
-    {
-        PagedRequest mine{};
-        walk.p = find_piece(a.view, walk.sh, blockIdx.x, scratch, mine);
-        own_piece(a.view, walk.sh, blockIdx.x, mine, walk.p, reinterpret_cast<int32_t*>(s0));
-    }
+    walk.p = find_piece(a.view, walk.sh, blockIdx.x, scratch);
     if (tid == 0) {
         a.parts.heads[blockIdx.x].rows = 0;
     }
