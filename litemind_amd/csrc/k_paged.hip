@@ -22,8 +22,8 @@
 //
 // Measured, 16 heads, calls of three contexts in turn: one token over 131072 keys
 // 34 us, 4.4 TB/s (large reads reach 6.4); one each of 32 requests of up to 4000
-// keys 22.7 us; 512 tokens after 3001 83 us, 0.70 PFLOP/s, and 2048 after none 122
-// us, 0.60 (large library products reach 1.2). A call by itself takes 20 us at
+// keys 21.7 us; 512 tokens after 3001 84 us, 0.70 PFLOP/s, and 2048 after none 115
+// us, 0.64 (large library products reach 1.2). A call by itself takes 20 us at
 // least: the lengths, the tables, the first tiles and the sums each wait for the
 // one before.
 #include "serve_internal.h"
@@ -1120,7 +1120,7 @@ bool paged_shares_out(int64_t tokens, int32_t heads, int64_t room) {
 }
 
 // 16 rows where no request has more (one token of 32 requests, 16 heads, three
-// contexts in turn: 22.8 us, in blocks of 64 24.9), or else 64 (32 heads, by itself:
+// contexts in turn: 23.5 us, in blocks of 64 26.0), or else 64 (32 heads, by itself:
 // 36 us, in blocks of 16 44).
 int paged_block_rows(int32_t max_added, int32_t heads) {
     return static_cast<int64_t>(max_added) * heads <= 16 ? 16 : 64;
