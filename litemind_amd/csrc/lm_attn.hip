@@ -1513,7 +1513,7 @@ int lm_decoder_forward(lm_context* ctx, int32_t first_layer, int32_t last_layer,
     }
 }
 
-int lm_paged_configure(lm_context* ctx, int64_t pages, int32_t page_size) {
+int lm_paged_configure(lm_context* ctx, int64_t pages, int32_t page_size) try {
     if (page_size < 16 || page_size > 4096 || page_size % 16 != 0) {
         return fail(LM_EINVAL, "page_size must be a multiple of 16 up to 4096");
     }
@@ -1557,9 +1557,11 @@ int lm_paged_configure(lm_context* ctx, int64_t pages, int32_t page_size) {
     st->pages = pages;
     st->page_size = page_size;
     return LM_OK;
+} catch (const std::bad_alloc&) {
+    return fail(LM_ENOMEM, "host allocation failed");
 }
 
-int lm_paged_pool(lm_context* ctx, int32_t layer, void** out_dev) {
+int lm_paged_pool(lm_context* ctx, int32_t layer, void** out_dev) try {
     if (out_dev == nullptr) {
         return fail(LM_EINVAL, "null output");
     }
@@ -1577,6 +1579,8 @@ int lm_paged_pool(lm_context* ctx, int32_t layer, void** out_dev) {
     *out_dev = st->pools + static_cast<int64_t>(layer) * st->pages * st->page_size *
                                (st->cfg.kv_lora_rank + st->cfg.qk_rope_head_dim);
     return LM_OK;
+} catch (const std::bad_alloc&) {
+    return fail(LM_ENOMEM, "host allocation failed");
 }
 
 int lm_paged_forward(lm_context* ctx, int32_t layer, const lm_paged_step* step, const float* x_dev, float* out_dev,

@@ -132,7 +132,7 @@ int lm::check_step_sizes(const lm_paged_step* s) {
 
 extern "C" {
 
-int lm_page_plan(lm_context* ctx, const lm_paged_step* step) {
+int lm_page_plan(lm_context* ctx, const lm_paged_step* step) try {
     const int rc = lm::check_step_sizes(step);
     if (rc != LM_OK) {
         return rc;
@@ -158,6 +158,8 @@ int lm_page_plan(lm_context* ctx, const lm_paged_step* step) {
     LM_SERVE_HIP(hipSetDevice(info.device));
     LM_SERVE_HIP(lm::launch_page_plan(s, info.stream));
     return LM_OK;
+} catch (const std::bad_alloc&) {
+    return fail(LM_ENOMEM, "host allocation failed");
 }
 
 int lm_paged_attention(lm_context* ctx, const lm_paged_step* step, const void* q_dev, const void* pool_dev,
@@ -230,7 +232,7 @@ int lm_paged_attention(lm_context* ctx, const lm_paged_step* step, const void* q
 }
 
 int lm_sample(lm_context* ctx, const float* logits_dev, int64_t rows, int64_t vocab, int64_t row_stride,
-              const lm_sampling* settings_dev, const float* uniform_dev, int32_t* token_dev, float* probability_dev) {
+              const lm_sampling* settings_dev, const float* uniform_dev, int32_t* token_dev, float* probability_dev) try {
     if (rows < 0 || rows > INT32_MAX || vocab < 1 || vocab > (int64_t{1} << 24) || row_stride < vocab) {
         return fail(LM_EINVAL, "rows must be 0 .. 2^31 - 1, vocab 1 .. 2^24, row_stride at least vocab");
     }
@@ -262,6 +264,8 @@ int lm_sample(lm_context* ctx, const float* logits_dev, int64_t rows, int64_t vo
     a.probability = probability_dev;
     LM_SERVE_HIP(lm::launch_sample(a, info.stream));
     return LM_OK;
+} catch (const std::bad_alloc&) {
+    return fail(LM_ENOMEM, "host allocation failed");
 }
 
 }  // extern "C"
