@@ -89,7 +89,8 @@ int lm_page_plan(lm_context* ctx, const lm_paged_step* step);
  *   heads    tokens * heads under 2^30, and (tokens * heads / 16 + tokens) blocks
  *            of heads times the tokens of a table row under 2^62
  * Products have the inputs' 16 bits, sums 32; the softmax weights round to 16
- * bits before the second product, the output once at the end.  Rows past the
+ * bits before the second product (fp16 ones under 2^-19 of their row's largest to
+ * a multiple of 2^-29 of it), the output once at the end.  Rows past the
  * last request's are not written.  What lies in a page past a request's length,
  * or after a token's own position, does not reach its output, NaN and infinity
  * included.  Page ids outside the pool are not followed: the row reads page 0,

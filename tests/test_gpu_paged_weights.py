@@ -1,0 +1,84 @@
+"""The softmax weights of lm_paged_attention: what their 16 bits may cost, held to bounds that leave out what the
+arithmetic does exactly.
+
+Queries and keys lie on a grid on which their products add up exactly in 32 bits, so scores carry no rounding but those
+of their scale and of the exponent's one step: 8 roundings of 2^-24 of the largest score, 2^-22 with the exponential.
+Weights w_j round to 16 bits, relative `unit`, or in fp16 by half a step of 2^-24 where the row's largest is 2^5 at
+least: 2^-30 of it.  Sums of 32 bits take one rounding a key tile, 300 for the parts of a cut row and 64 within a tile.
+The output rounds once, by half of its own step."""
+import numpy as np
+import pytest
+
+import litemind_amd as lm
+from conftest import announce
+from litemind_amd import workload as wl
+from test_gpu_paged_attention import UNIT, Batch, decode, encode
+
+pytestmark = pytest.mark.gpu
+BITS = {lm.DT_F16: 10, lm.DT_BF16: 7}
+RANK, WIDTH = 512, 576
+DTYPES = [lm.DT_F16, lm.DT_BF16]
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = lm.Context(wl.V2_LITE.moe_config(num_layers=1))
+    yield c
+    c.close()
+
+
+def half_step(v, dtype):
+    """Half the distance between 16-bit numbers around |v|."""
+    v = np.abs(v)
+    low = -14 if dtype == lm.DT_F16 else -126
+    return 2.0 ** (np.floor(np.log2(np.maximum(v, 2.0 ** low))) - BITS[dtype] - 1)
+
+
+def lost(dtype):
+    return 2.0 ** -30 if dtype == lm.DT_F16 else 0.0
+
+
+def other(scores, keys):
+    return 8 * 2.0 ** -24 * np.abs(scores).max() + 2.0 ** -22 + (-(-keys // 32) + 364) * 2.0 ** -24
+
+
+def over_pages(pool, tables, lengths, starts, q, dtype, scale, pages):
+    """A Batch over pages that its requests may share."""
+    b = Batch.__new__(Batch)
+    b.pool, b.table, b.lengths, b.starts, b.q = pool, tables, lengths, starts, q
+    b.tokens, b.heads, b.rank, b.rope, b.dtype, b.scale = q.shape[0], q.shape[1], RANK, WIDTH - RANK, dtype, scale
+    b.R, b.pages, b.page, b.width, b.added = len(lengths), pages, pool.shape[1], tables.shape[1], list(np.diff(starts))
+    return b
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("requests,added", [(520, 1), (260, 9)])
+@pytest.mark.parametrize("depth", [4.0, 14.3, 18.7, 22.3, 24.6, 28.6])
+def test_a_first_key_above_a_long_tail(ctx, depth, requests, added, dtype):
+    """The first of 65536 keys outweighs each of the others by 2^depth and has a latent of zeros, in blocks that one
+    workgroup runs whole: what the others' weights lose shows in full."""
+    announce(f"paged attention: a first key 2^{depth} above 65535 others, {requests} x {added} tokens, dtype {dtype}")
+    keys, page, heads = 65536, 1024, 2
+    scale = float(np.float32(depth * np.log(2.0) / 32.0))
+    value = (np.arange(RANK) % 9 - 4) / 4.0
+    rows = np.zeros((2, page, WIDTH))
+    rows[:, :, :RANK] = value
+    rows[0, 0, :RANK], rows[0, 0, RANK] = 0.0, 4.0
+    table = np.ones((requests, keys // page), np.int32)
+    table[:, 0] = 0
+    q = np.zeros((requests * added, heads, WIDTH))
+    q[..., RANK] = 8.0
+    b = over_pages(encode(rows, dtype), table, np.full(requests, keys, np.int32),
+                   np.arange(requests + 1, dtype=np.int32) * added, encode(q, dtype), dtype, scale, 2).upload(ctx)
+    b.call(ctx)
+    got = decode(b.dev["out"].download()[:-1], dtype).reshape(requests, added, heads, RANK)
+    e = np.exp(-32.0 * scale)
+    for i in range(added):
+        tail = keys - added + i
+        total = 1.0 + tail * e
+        p = tail * e / total
+        want = p * value
+        bound = np.abs(value) * (tail * max(UNIT[dtype] * e, lost(dtype)) / total + 2 * other(np.array([32.0 * scale]), keys) * p)
+        bound = bound + half_step(np.abs(want) + bound, dtype)
+        off = np.abs(got[:, i] - want)
+        assert (off <= bound).all(), f"token {i}: {got[0, i, 0, 0]:.6g}, not {want[0]:.6g}"
