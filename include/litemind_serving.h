@@ -90,11 +90,12 @@ int lm_page_plan(lm_context* ctx, const lm_paged_step* step);
  *            of heads times the tokens of a table row under 2^62
  * Products have the inputs' 16 bits, sums 32; the softmax weights round to 16
  * bits before the second product (fp16 ones under 2^-19 of their row's largest to
- * a multiple of 2^-29 of it), the output once at the end.  Rows past the
- * last request's are not written.  What lies in a page past a request's length,
- * or after a token's own position, does not reach its output, NaN and infinity
- * included.  Page ids outside the pool are not followed: the row reads page 0,
- * and the next lm_synchronize or lm_copy_d2h returns LM_EKERNEL.  Asynchronous. */
+ * a multiple of 2^-29 of it) and are added up as rounded, the output once at the
+ * end.  Rows past the last request's are not written.  What lies in a page past a
+ * request's length, or after a token's own position, does not reach its output,
+ * NaN and infinity included.  Page ids outside the pool are not followed: the row
+ * reads page 0, and the next lm_synchronize or lm_copy_d2h returns LM_EKERNEL.
+ * Asynchronous. */
 int lm_paged_attention(lm_context* ctx, const lm_paged_step* step, const void* q_dev, const void* pool_dev,
                        int32_t dtype, int32_t heads, int32_t rank, int32_t rope, float scale, void* out_dev);
 

@@ -525,7 +525,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_rows_kernel(const TileArgs 
         float m = kNone;          // reference of row `lane`, the same in every wave
         float ref = kUnset;       // of this lane's row of the scores, times c, less kLift
         float l = 0.0f, sum = 0.0f;  // its total, and the newest tile's
-        // the newest tile's weights
+        // the newest tile's weights; their total is that of the rounded ones, so that what
+        // is rounded away of a key that outweighs the others goes from both
         float over = kNone;
         auto exps = [&](char* wt) {
             vec4 p;
@@ -535,8 +536,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_rows_kernel(const TileArgs 
             for (int e = 0; e < 4; ++e) {
                 const float x = __builtin_fmaf(sc[e], a.c, -ref);
                 over = fmaxf(over, x);
-                w[e] = __builtin_amdgcn_exp2f(x);
-                p[e] = static_cast<E>(w[e]);
+                p[e] = static_cast<E>(__builtin_amdgcn_exp2f(x));
+                w[e] = static_cast<float>(p[e]);
             }
             sum = (w[0] + w[1]) + (w[2] + w[3]);
             *reinterpret_cast<vec4*>(wt + weight_to) = p;

@@ -4,15 +4,16 @@ arithmetic does exactly.
 Queries and keys lie on a grid on which their products add up exactly in 32 bits, so scores carry no rounding but those
 of their scale and of the exponent's one step: 8 roundings of 2^-24 of the largest score, 2^-22 with the exponential.
 Weights w_j round to 16 bits, relative `unit`, or in fp16 by half a step of 2^-24 where the row's largest is 2^5 at
-least: 2^-30 of it.  Sums of 32 bits take one rounding a key tile, 300 for the parts of a cut row and 64 within a tile.
-The output rounds once, by half of its own step."""
+least: 2^-30 of it.  Their total is that of the rounded ones, so a weight's error moves an output by its distance from
+that output's value: sum_j |error_j| |c_j - out| / total.  Sums of 32 bits take one rounding a key tile, 300 for the
+parts of a cut row and 64 within a tile.  The output rounds once, by half of its own step."""
 import numpy as np
 import pytest
 
 import litemind_amd as lm
 from conftest import announce
 from litemind_amd import workload as wl
-from test_gpu_paged_attention import UNIT, Batch, decode, encode
+from test_gpu_paged_attention import SCALE, UNIT, Batch, decode, encode
 
 pytestmark = pytest.mark.gpu
 BITS = {lm.DT_F16: 10, lm.DT_BF16: 7}
@@ -82,3 +83,44 @@ def test_a_first_key_above_a_long_tail(ctx, depth, requests, added, dtype):
         bound = bound + half_step(np.abs(want) + bound, dtype)
         off = np.abs(got[:, i] - want)
         assert (off <= bound).all(), f"token {i}: {got[0, i, 0, 0]:.6g}, not {want[0]:.6g}"
+
+
+def grid(rng, shape, most):
+    return rng.integers(-most, most + 1, shape) * 0.25
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads,cached,added", [(16, [1, 33, 300, 1000, 64], [1, 1, 1, 1, 1]), (128, [500, 40], [1, 1]),
+                                                (16, [700, 0, 31], [40, 70, 9])])
+@pytest.mark.parametrize("most", [4, 24])
+def test_rows_of_few_keys_that_count(ctx, heads, cached, added, dtype, most):
+    """Scores so far apart that one or a few keys make up a row: their weights' rounding cancels against the total's."""
+    announce(f"paged attention: peaked rows, {heads} heads, {added} after {cached}, queries up to {most / 4}, dtype {dtype}")
+    rng = np.random.default_rng(heads + most + len(cached))
+    b = Batch(cached, added, heads, dtype=dtype, page=32, seed=5)
+    b.q = encode(grid(rng, b.q.shape, most), dtype)
+    for r, n in enumerate(b.lengths):
+        rows = grid(rng, (n, WIDTH), 4)
+        rows[:, :RANK] += (rows[:, :RANK] == 0)  # (values next to each other for the keys that count)
+        b.rows[r] = encode(rows, dtype)
+        for k in range(-(-int(n) // b.page)):
+            part = b.rows[r][k * b.page:(k + 1) * b.page]
+            b.pool[b.table[r, k], :len(part)] = part
+    got = decode(b.run(ctx), dtype)
+    unit = UNIT[dtype]
+    for r in range(b.R):
+        rows = decode(b.rows[r], dtype)
+        for t in range(b.starts[r], b.starts[r + 1]):
+            seen = rows[:cached[r] + t - b.starts[r] + 1]
+            s = (decode(b.q[t], dtype) @ seen.T) * np.float64(np.float32(SCALE))
+            e = np.exp(s - s.max(1, keepdims=True))
+            total = e.sum(1, keepdims=True)
+            want = (e / total) @ seen[:, :RANK]
+            error = np.maximum(unit * e, lost(dtype)) / total
+            bound = np.empty_like(want)
+            for h in range(heads):
+                bound[h] = error[h] @ np.abs(seen[:, :RANK] - want[h])
+            bound += 2 * other(s, len(seen)) * ((e / total) @ np.abs(seen[:, :RANK]))
+            bound += half_step(np.abs(want) + bound, dtype)
+            off = np.abs(got[t] - want)
+            assert (off <= bound).all(), f"request {r}, row {t}: {np.max(off / bound):.3g} of the bound"
