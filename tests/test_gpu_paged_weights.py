@@ -124,3 +124,41 @@ def test_rows_of_few_keys_that_count(ctx, heads, cached, added, dtype, most):
             bound += half_step(np.abs(want) + bound, dtype)
             off = np.abs(got[t] - want)
             assert (off <= bound).all(), f"request {r}, row {t}: {np.max(off / bound):.3g} of the bound"
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads,cached,added", [(16, [20001, 131071], [1, 1]), (128, [20001], [2]), (16, [8190, 30000], [11, 40]),
+                                                (3, [100000], [70]), (1, [50000, 77, 12345], [1, 1, 1])])
+def test_every_key_counts_once(ctx, heads, cached, added, dtype):
+    """Queries of zeros weigh all keys alike, and a channel of the latents counts the keys of every 256th tile or place: a
+    tile left out or taken twice changes a count by 1 in 16 at least, a key by 1 in 512, more than the output's rounding
+    but for bf16 past 60000 keys."""
+    announce(f"paged attention: counted keys, {heads} heads, {added} after {cached}, dtype {dtype}")
+    page, R = 64, len(cached)
+    lengths = np.array([c + a for c, a in zip(cached, added)], np.int32)
+    held = [-(-int(n) // page) for n in lengths]
+    starts = np.concatenate([[0], np.cumsum(added)]).astype(np.int32)
+    order = np.random.default_rng(7).permutation(sum(held)).astype(np.int32)
+    table, at = np.full((R, max(held)), -1, np.int32), 0
+    pool = np.zeros((sum(held), page, WIDTH), np.uint16)
+    one = encode(np.ones(1), dtype)[0]
+    for r, n in enumerate(lengths):
+        table[r, :held[r]] = order[at:at + held[r]]
+        at += held[r]
+        j = np.arange(held[r] * page)
+        rows = np.zeros((held[r] * page, WIDTH), np.uint16)
+        rows[j, j // 32 % 256] = one
+        rows[j, 256 + j % 256] = one
+        pool[table[r, :held[r]]] = rows.reshape(held[r], page, WIDTH)
+    q = np.zeros((int(starts[-1]), heads, WIDTH), np.uint16)
+    b = over_pages(pool, table, lengths, starts, q, dtype, SCALE, len(pool)).upload(ctx)
+    b.call(ctx)
+    got = decode(b.dev["out"].download()[:-1], dtype)
+    for r in range(R):
+        for t in range(starts[r], starts[r + 1]):
+            n = cached[r] + t - starts[r] + 1
+            j = np.arange(n)
+            want = np.concatenate([np.bincount(j // 32 % 256, minlength=256), np.bincount(j % 256, minlength=256)]) / n
+            # equal weights of a power of two: sums are whole numbers, the quotient takes two roundings to 32 bits
+            bound = want * 2.0 ** -22
+            assert (np.abs(got[t] - want) <= bound + half_step(want + bound, dtype)).all(), f"request {r}, row {t}"
