@@ -171,24 +171,26 @@ __global__ __launch_bounds__(kThreads) void page_plan_kernel(const lm_paged_step
                 const int k = find(backs, n, i);
                 s.ring[(behind + i) % ring] = s.table[(r0 + k) * s.table_width + i - backs[k]];
             }
-            for (int32_t t = from.tokens + 4 * tid; t < before.tokens; t += 4 * kThreads) {
-                int k = find(starts, n, t);
+            // (unsigned: rows past 2^31 - 1 are stepped to, not written)
+            const uint32_t end = static_cast<uint32_t>(before.tokens);
+            for (uint32_t t = static_cast<uint32_t>(from.tokens) + 4u * tid; t < end; t += 4u * kThreads) {
+                int k = find(starts, n, static_cast<int32_t>(t));
                 int32_t page[4], place[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (t + j < before.tokens) {
-                        while (k + 1 < n && starts[k + 1] <= t + j) {
+                for (uint32_t j = 0; j < 4; ++j) {
+                    if (t + j < end) {
+                        while (k + 1 < n && static_cast<uint32_t>(starts[k + 1]) <= t + j) {
                             ++k;
                         }
-                        place[j] = cached[k] + t + j - starts[k];
+                        place[j] = static_cast<int32_t>(cached[k] + t + j - starts[k]);
                         const int32_t column = place[j] / s.page_size;
                         page[j] = column < had[k] ? s.table[(r0 + k) * s.table_width + column]
                                                   : s.ring[(front + static_cast<uint32_t>(firsts[k] + column - had[k])) % ring];
                     }
                 }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (t + j < before.tokens) {
+                for (uint32_t j = 0; j < 4; ++j) {
+                    if (t + j < end) {
                         s.positions[t + j] = place[j];
                         s.slots[t + j] = static_cast<uint32_t>(page[j]) < ring
                                              ? page[j] * s.page_size + place[j] % s.page_size
@@ -203,7 +205,7 @@ __global__ __launch_bounds__(kThreads) void page_plan_kernel(const lm_paged_step
             s.starts[r] = 0;
         }
     }
-    for (int64_t t = before.tokens + tid; t < s.tokens; t += kThreads) {
+    for (int64_t t = static_cast<int64_t>(before.tokens) + tid; t < s.tokens; t += kThreads) {
         s.positions[t] = 0;
         s.slots[t] = -1;
     }

@@ -1,0 +1,64 @@
+"""lm_page_plan at the ends of the sizes and rings that it takes."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import litemind_amd as lm
+from conftest import announce
+from litemind_amd import workload as wl
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = lm.Context(wl.V2_LITE.moe_config(num_layers=1))
+    yield c
+    c.close()
+
+
+def words(ctx, buffer, first, count):
+    out = np.empty(count, np.int32)
+    ctx._check(ctx.lib.lm_copy_d2h(ctx.handle, out.ctypes.data, C.c_void_p(buffer.ptr + 4 * first), out.nbytes))
+    return out
+
+
+def test_as_many_tokens_as_a_step_takes(ctx):
+    """2^31 - 25 new tokens of two requests, a third without any between them, and five padded rows."""
+    announce("page plan: 2^31 - 25 new tokens")
+    page, pages = 16, 2 ** 27 - 1
+    first = 16 * 62500000 + 7
+    second = 16 * (pages - 62500001)
+    new, tokens = first + second, first + second + 5
+    assert new == 2 ** 31 - 25
+    width = second // 16
+    dev = {"cached": ctx.to_device(np.zeros(3, np.int32)), "added": ctx.to_device(np.array([first, 0, second], np.int32)),
+           "table": ctx.empty((3, width), np.int32), "ring": ctx.to_device(np.arange(pages, dtype=np.int32)),
+           "queue_in": ctx.to_device(np.array([0, pages], np.int32)), "queue_out": ctx.empty(2, np.int32),
+           "lengths": ctx.empty(3, np.int32), "starts": ctx.empty(4, np.int32),
+           "positions": ctx.empty(tokens + 64, np.int32), "slots": ctx.empty(tokens + 64, np.int32),
+           "info": ctx.empty(4, np.int32)}
+    step = lm.PagedStep(requests=3, tokens=tokens, pages=pages, page_size=page, table_width=width, max_added=second)
+    for k, b in dev.items():
+        setattr(step, k, b.ptr)
+    for k in ("positions", "slots"):
+        ctx._check(ctx.lib.lm_copy_h2d(ctx.handle, C.c_void_p(dev[k].ptr + 4 * (tokens - 100)),
+                                       np.full(164, 123, np.int32).ctypes.data, 4 * 164))
+    ctx.page_plan(step)
+    assert dev["info"].download().tolist() == [lm.STEP_OK, new, pages, 0]
+    assert dev["starts"].download().tolist() == [0, first, first, new]
+    assert dev["lengths"].download().tolist() == [first, 0, second]
+    assert dev["queue_out"].download().tolist() == [0, 0]
+    count = 1 << 20
+    for at in (0, first - count // 2, first, 2 ** 30 - 5000, 3 * 2 ** 29, new - 3 * count, new - count):
+        t = np.arange(at, at + count, dtype=np.int64)
+        position = np.where(t < first, t, t - first)
+        slot = position + np.where(t < first, 0, 62500001 * 16)
+        assert np.array_equal(words(ctx, dev["positions"], at, count), position), at
+        assert np.array_equal(words(ctx, dev["slots"], at, count), slot), at
+    assert words(ctx, dev["positions"], new, 5 + 64).tolist() == [0] * 5 + [123] * 64
+    assert words(ctx, dev["slots"], new, 5 + 64).tolist() == [-1] * 5 + [123] * 64
+    assert np.array_equal(words(ctx, dev["table"], 2 * width + width - 1000, 1000), np.arange(pages - 1000, pages))
+    for b in dev.values():
+        b.free()
