@@ -95,12 +95,12 @@ struct Shares {
     __device__ int32_t blocks(const PagedRequest& r) const { return (r.added * heads + rows - 1) / rows; }
     // Cost of the request's first b blocks.
     __device__ int64_t cost(const PagedRequest& r, int32_t b) const {
-        return static_cast<int64_t>(b) * (r.cached + kExtra) * heads + static_cast<int64_t>(b) * (b + 1) / 2 * rows;
+        return b * (static_cast<int64_t>(r.cached) + kExtra) * heads + static_cast<int64_t>(b) * (b + 1) / 2 * rows;
     }
     // Tiles of block b.
     __device__ int32_t tiles(const PagedRequest& r, int32_t b) const {
         const int32_t last = min((b + 1) * rows, r.added * heads) - 1;
-        return (r.cached + last / heads + kTile) / kTile;
+        return static_cast<int32_t>((static_cast<uint32_t>(r.cached + last / heads) + kTile) / kTile);
     }
 };
 
@@ -311,8 +311,8 @@ struct PageWalk {
     __device__ void start(const PagedView& v, int32_t request) {
         row = v.table + static_cast<int64_t>(request) * v.table_width;
     }
-    __device__ void look(const PagedView& v, uint32_t page_mul, int32_t key) {
-        const uint32_t d = static_cast<uint32_t>(v.page_size) / 16, n = static_cast<uint32_t>(key) / 16;
+    __device__ void look(const PagedView& v, uint32_t page_mul, uint32_t key) {
+        const uint32_t d = static_cast<uint32_t>(v.page_size) / 16, n = key / 16;
         uint32_t page = __umulhi(n, page_mul);
         if (d == 1) {
             page = n;
@@ -448,17 +448,18 @@ __global__ __launch_bounds__(kThreads, 2) void paged_rows_kernel(const TileArgs 
         int from, past;
     };
     auto prepare = [&](int32_t t, char* to) {
-        const int32_t key = t * kTile + 16 * (wave >> 2);
-        const int32_t first = min(key, last & ~15);
+        // (unsigned: tiles past a segment's end may begin past 2^31 - 1)
+        const uint32_t key = static_cast<uint32_t>(t) * kTile + 16 * (wave >> 2);
+        const uint32_t final16 = static_cast<uint32_t>(last) & ~15u, first = min(key, final16);
         // (tiles are prepared in order: the row looked up is this one's)
         const char* const base = static_cast<const char*>(a.pool) + pages.take(a.view) * kRowBytes;
-        pages.look(a.view, a.page_mul, min(key + kTile, last & ~15));
+        pages.look(a.view, a.page_mul, min(key + kTile, final16));
         Loads d;
         d.res = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, t < s.tile1 ? 16 * kRowBytes : 0, kBufferWord3);
         d.eight = to + (wave >> 1) * kEightBytes;
         // rows past the last key: the last key's once more
-        d.from = key - first + 4 * (wave & 3);
-        d.past = last - first;
+        d.from = static_cast<int32_t>(key - first) + 4 * (wave & 3);
+        d.past = static_cast<int32_t>(static_cast<uint32_t>(last) - first);
         return d;
     };
     auto load = [&](const Loads& d, int part) {
@@ -490,7 +491,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_rows_kernel(const TileArgs 
         rows = min(M, s.req.added * a.heads - in_request);
         last = s.req.cached + s.req.added - 1;
         pages.start(a.view, s.request);
-        pages.look(a.view, a.page_mul, min(s.tile0 * kTile + 16 * (wave >> 2), last & ~15));
+        pages.look(a.view, a.page_mul, min(static_cast<uint32_t>(s.tile0) * kTile + 16 * (wave >> 2), static_cast<uint32_t>(last) & ~15u));
         if (s.tile0 < s.tile1) {
             issue(s.tile0, ring[0]);
         }
@@ -1018,9 +1019,10 @@ __global__ __launch_bounds__(256) void paged_any_kernel(const PagedAttention a) 
         }
         float m = kNone, l = 0.0f;
         const int32_t keys = r.cached + t - r.first + 1;
-        for (int32_t j = wave; j < keys; j += 4) {
-            const int64_t page = checked_page(v, v.table[static_cast<int64_t>(lo) * v.table_width + j / v.page_size]);
-            const E* const key = static_cast<const E*>(a.pool) + (page * v.page_size + j % v.page_size) * width;
+        for (uint32_t j = wave; j < static_cast<uint32_t>(keys); j += 4) {
+            const uint32_t size = static_cast<uint32_t>(v.page_size);
+            const int64_t page = checked_page(v, v.table[static_cast<int64_t>(lo) * v.table_width + j / size]);
+            const E* const key = static_cast<const E*>(a.pool) + (page * v.page_size + j % size) * width;
             float c[kC], s = 0.0f;
 #pragma unroll
             for (int i = 0; i < kC; ++i) {

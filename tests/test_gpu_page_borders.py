@@ -1,4 +1,4 @@
-"""lm_page_plan at the ends of the sizes and rings that it takes."""
+"""lm_page_plan and lm_paged_attention at the ends of the sizes and rings that they take."""
 import ctypes as C
 
 import numpy as np
@@ -7,6 +7,7 @@ import pytest
 import litemind_amd as lm
 from conftest import announce
 from litemind_amd import workload as wl
+from test_gpu_paged_attention import SCALE, decode, encode
 
 pytestmark = pytest.mark.gpu
 
@@ -62,3 +63,35 @@ def test_as_many_tokens_as_a_step_takes(ctx):
     assert np.array_equal(words(ctx, dev["table"], 2 * width + width - 1000, 1000), np.arange(pages - 1000, pages))
     for b in dev.values():
         b.free()
+
+
+@pytest.mark.parametrize("heads,added", [(1, 1), (8, 3)])
+@pytest.mark.parametrize("dtype", [lm.DT_F16, lm.DT_BF16])
+def test_attention_over_the_longest_row(ctx, heads, added, dtype):
+    """2^31 - 16 keys: one page of zeros and ones named again and again, and another at the end.  Queries of zeros weigh
+    all alike, so the outputs are counts of keys over their number: sums of whole numbers in 32 bits, 300 parts and 16
+    tiles' roundings of 2^-24 at most where they pass 2^24, and the output's own."""
+    announce(f"paged attention: {added} tokens at the end of 2^31 - 16 keys, {heads} heads, dtype {dtype}")
+    page, columns, big = 16, 2 ** 27 - 1, 32768.0
+    rows = np.zeros((2, page, 576))
+    rows[0, :, 0], rows[0, ::2, 1], rows[1, :, 2] = 1.0, 1.0, big
+    table = np.zeros((1, columns), np.int32)
+    table[0, -1] = 1
+    dev = {"table": ctx.to_device(table), "lengths": ctx.to_device(np.array([page * columns], np.int32)),
+           "starts": ctx.to_device(np.array([0, added], np.int32)),
+           "q": ctx.to_device(np.zeros((added, heads, 576), np.uint16)), "pool": ctx.to_device(encode(rows, dtype)),
+           "out": ctx.to_device(np.full((added, heads, 512), 0x1234, np.uint16))}
+    step = lm.PagedStep(requests=1, tokens=added, pages=2, page_size=page, table_width=columns, max_added=added)
+    for k in ("table", "lengths", "starts"):
+        setattr(step, k, dev[k].ptr)
+    ctx.paged_attention(step, dev["q"], dev["pool"], heads, SCALE, dev["out"], dtype=dtype)
+    got = decode(dev["out"].download(), dtype)
+    for b in dev.values():
+        b.free()
+    unit = 2.0 ** -11 if dtype == lm.DT_F16 else 2.0 ** -8
+    for i in range(added):
+        last = page - added + i + 1
+        n = page * (columns - 1) + last
+        want = np.zeros(512)
+        want[:3] = page * (columns - 1) / n, page // 2 * (columns - 1) / n, big * last / n
+        assert (np.abs(got[i] - want) <= want * (unit + 316 * 2.0 ** -24)).all(), got[i, 0, :4]
