@@ -56,7 +56,7 @@ typedef struct lm_paged_step {
 #define LM_STEP_LENGTH 1  /* a negative cached length, or a request longer than its table row */
 #define LM_STEP_TOKENS 2  /* the new tokens exceed `tokens`, or a request's exceed max_added */
 #define LM_STEP_PAGES 3   /* the ring holds fewer pages than the step needs */
-#define LM_STEP_RING 4    /* a negative count, or more free pages after the step than the pool has */
+#define LM_STEP_RING 4    /* a negative count, or more pages free and given back together than the pool has */
 
 /* Plans a step from cached and added: writes lengths, starts, positions, slots,
  * queue_out and info.  A request takes the pages that its new tokens start from

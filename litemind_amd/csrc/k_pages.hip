@@ -120,10 +120,12 @@ __global__ __launch_bounds__(kThreads) void page_plan_kernel(const lm_paged_step
         taken += wave_taken[w];
         back += wave_back[w];
     }
+    // (returned pages go behind the free ones while taken ones are read: both have to
+    // have their own places in the ring)
     const int32_t status = flags[0] != 0                             ? LM_STEP_LENGTH
                            : flags[1] != 0 || tokens > s.tokens      ? LM_STEP_TOKENS
                            : taken > max(static_cast<int64_t>(count), int64_t{0}) ? LM_STEP_PAGES
-                           : count < 0 || count - taken + back > s.pages ? LM_STEP_RING
+                           : count < 0 || count + back > s.pages ? LM_STEP_RING
                                                                        : LM_STEP_OK;
     Sums before{};  // of the requests in earlier chunks
     if (status == LM_STEP_OK) {

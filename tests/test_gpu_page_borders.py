@@ -5,8 +5,10 @@ import numpy as np
 import pytest
 
 import litemind_amd as lm
+import serving_ref as ref
 from conftest import announce
 from litemind_amd import workload as wl
+from test_gpu_pages import Plan, check
 from test_gpu_paged_attention import SCALE, decode, encode
 
 pytestmark = pytest.mark.gpu
@@ -95,3 +97,40 @@ def test_attention_over_the_longest_row(ctx, heads, added, dtype):
         want = np.zeros(512)
         want[:3] = page * (columns - 1) / n, page // 2 * (columns - 1) / n, big * last / n
         assert (np.abs(got[i] - want) <= want * (unit + 316 * 2.0 ** -24)).all(), got[i, 0, :4]
+
+
+@pytest.mark.parametrize("pages,count,taken,back", [(10, 4, 4, 10), (9, 4, 4, 8), (9, 4, 4, 6), (9, 4, 1, 6), (9, 11, 3, 0),
+                                                    (9, 11, 11, 1), (9, 0, 0, 10), (1, 1, 1, 1)])
+def test_rings_without_room(ctx, pages, count, taken, back):
+    """Free and returned pages that need more places than the ring has, in steps that take pages too: refused, whatever
+    is left after the step, and nothing changed."""
+    announce(f"page plan: {count} free pages of {pages}, {taken} taken, {back} given back")
+    assert count + back > pages and taken <= count
+    width = max(taken, back, 1)
+    table, ring = np.arange(2 * width, dtype=np.int32).reshape(2, width) % pages, np.arange(pages, dtype=np.int32)
+    cached, added = [0, 16 * back], [16 * taken, -1]
+    plan = Plan(ctx, cached, added, table, ring, [3, count], 16, 16 * taken + 2, 16 * taken)
+    ctx.page_plan(plan.step)
+    got = plan.read()
+    assert got["info"].tolist() == [lm.STEP_RING, 0, 0, 0]
+    assert got["queue_out"].tolist() == [3 % pages, count] and got["starts"].tolist() == [0] * 3
+    assert np.array_equal(got["table"], table) and np.array_equal(got["ring"], ring)
+    assert got["lengths"].tolist() == cached and (got["slots"] == -1).all() and (got["positions"] == 0).all()
+
+
+@pytest.mark.parametrize("pages,count,taken,back", [(10, 4, 4, 6), (9, 4, 1, 5), (9, 9, 9, 0), (9, 0, 0, 9), (2, 1, 1, 1)])
+def test_rings_just_full(ctx, pages, count, taken, back):
+    """Free and returned pages that fill the ring: served, and the same when planned again."""
+    announce(f"page plan: {count} free pages of {pages}, {taken} taken, {back} given back, the ring full")
+    width = max(taken, back, 1)
+    ids = np.random.default_rng(pages).permutation(pages).astype(np.int32)
+    ring, table = np.full(pages, -5, np.int32), np.full((2, width), -7, np.int32)
+    ring[(3 + np.arange(count)) % pages] = ids[:count]
+    table[1, :back] = ids[count:count + back]
+    args = ([0, 16 * back], [16 * taken, -1], table, ring, [3 % pages, count], 16, 16 * taken, 16 * taken)
+    plan = Plan(ctx, *args)
+    want = ref.plan(*args)
+    assert want["info"].tolist() == [0, 16 * taken, taken, back]
+    for _ in range(2):
+        ctx.page_plan(plan.step)
+        check(plan, want)
