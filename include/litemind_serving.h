@@ -128,7 +128,9 @@ int lm_paged_forward(lm_context* ctx, int32_t layer, const lm_paged_step* step, 
                      int32_t accumulate);
 /* lm_decoder_forward's layer loop with lm_paged_forward as the attention:
  * hidden_dev [tokens, H] in place.  Rows past the last new token are taken as
- * zeros; what they come out as means nothing.  `path` as there. */
+ * zeros; what they come out as means nothing.  `path` as there.  A call that is
+ * refused, for a layer whose weights are not there or do not fit fp16 too, leaves
+ * hidden_dev and the pools as they were. */
 int lm_paged_decoder_forward(lm_context* ctx, int32_t first_layer, int32_t last_layer, const lm_paged_step* step,
                              float* hidden_dev, int32_t path);
 

@@ -711,6 +711,44 @@ int check_paged(lm_context* ctx, const lm_paged_step* step, AttnState** out) {
     return LM_OK;
 }
 
+// Where a step's rows lie in the scratch, in floats.
+struct PagedScratch {
+    size_t x16, q, ql, ql16, lat, q16, ctx16, v16;
+    size_t floats = 0;
+    PagedScratch(const lm_mla_config& c, int64_t T) {
+        const int64_t heads = c.num_heads, rank = c.kv_lora_rank, rope = c.qk_rope_head_dim;
+        auto region = [&](int64_t n) {
+            const size_t at = floats;
+            floats += static_cast<size_t>((n + 63) / 64 * 64);
+            return at;
+        };
+        auto halves = [](int64_t n) { return (n + 1) / 2; };
+        x16 = region(halves(T * c.hidden_size));
+        q = region(T * heads * (c.qk_nope_head_dim + rope));
+        ql = region(T * c.q_lora_rank);
+        ql16 = region(halves(T * c.q_lora_rank));
+        lat = region(T * (rank + rope));
+        q16 = region(halves(T * heads * (rank + rope)));
+        ctx16 = region(halves(T * heads * rank));
+        v16 = region(halves(T * heads * c.v_head_dim));
+    }
+};
+
+// What a layer's call needs besides its launches: weights in the pages' form and
+// scratch. Once it is there, attention_paged fails by the runtime alone.
+int paged_ready(lm_context* ctx, AttnState* st, int32_t layer, const lm_paged_step& step) {
+    const lm_mla_config& c = st->cfg;
+    const hipStream_t stream = lm::context_info(ctx).stream;
+    int rc = absorb(st, st->layers[static_cast<size_t>(layer)], layer, stream);
+    if (rc == LM_OK) {
+        rc = ensure_buffer(&st->ws, &st->ws_floats, stream, PagedScratch(c, step.tokens).floats);
+    }
+    if (rc == LM_OK) {
+        rc = lm::paged_attention_ready(ctx, step, c.num_heads, c.kv_lora_rank, c.qk_rope_head_dim);
+    }
+    return rc;
+}
+
 // A layer's attention for a step's tokens over its pages; as attention_tokens, x
 // may be `out` with in_norm.
 int attention_paged(lm_context* ctx, AttnState* st, int32_t layer, const lm_paged_step& step, const float* x,
@@ -719,35 +757,17 @@ int attention_paged(lm_context* ctx, AttnState* st, int32_t layer, const lm_page
     const hipStream_t stream = info.stream;
     const lm_mla_config& c = st->cfg;
     const lm::AttnShape& a = st->shape;
-    AttnLayer& L = st->layers[static_cast<size_t>(layer)];
-    int rc = absorb(st, L, layer, stream);
+    const AttnLayer& L = st->layers[static_cast<size_t>(layer)];
+    int rc = paged_ready(ctx, st, layer, step);
     if (rc != LM_OK) {
         return rc;
     }
     const int64_t T = step.tokens, H = c.hidden_size, heads = c.num_heads, nope = c.qk_nope_head_dim,
                   rope = c.qk_rope_head_dim, qk = nope + rope, rank = c.kv_lora_rank, vh = c.v_head_dim,
                   ql = c.q_lora_rank;
-    size_t total_f = 0;
-    auto region = [&](int64_t floats) {
-        const size_t at = total_f;
-        total_f += static_cast<size_t>((floats + 63) / 64 * 64);
-        return at;
-    };
-    auto halves = [](int64_t n) { return (n + 1) / 2; };
-    const size_t x16_at = region(halves(T * H));
-    const size_t q_at = region(T * heads * qk);
-    const size_t ql_at = region(T * ql);
-    const size_t ql16_at = region(halves(T * ql));
-    const size_t lat_at = region(T * (rank + rope));
-    const size_t q16_at = region(halves(T * heads * (rank + rope)));
-    const size_t ctx16_at = region(halves(T * heads * rank));
-    const size_t v16_at = region(halves(T * heads * vh));
-    rc = ensure_buffer(&st->ws, &st->ws_floats, stream, total_f);
-    if (rc != LM_OK) {
-        return rc;
-    }
+    const PagedScratch at(c, T);
     float* const ws = st->ws;
-    auto h16 = [&](size_t at) { return reinterpret_cast<_Float16*>(ws + at); };
+    auto h16 = [&](size_t from) { return reinterpret_cast<_Float16*>(ws + from); };
     lm::ProjArgs p;
     p.tokens = T;
     p.heads = a.heads;
@@ -761,24 +781,24 @@ int attention_paged(lm_context* ctx, AttnState* st, int32_t layer, const lm_page
         return seg;
     };
     if (in_norm != nullptr) {
-        LM_ATT_HIP(lm::launch_norm16(x, in_norm, h16(x16_at), T, static_cast<int32_t>(H), c.rms_norm_eps, stream));
+        LM_ATT_HIP(lm::launch_norm16(x, in_norm, h16(at.x16), T, static_cast<int32_t>(H), c.rms_norm_eps, stream));
     } else {
-        LM_ATT_HIP(lm::launch_to_f16_rows(x, h16(x16_at), T, static_cast<int32_t>(H), static_cast<int32_t>(H),
+        LM_ATT_HIP(lm::launch_to_f16_rows(x, h16(at.x16), T, static_cast<int32_t>(H), static_cast<int32_t>(H),
                                           stream));
     }
     // queries (src/Attention.cpp:33-48) and the compressed keys and values (:50-56)
-    p.x16 = h16(x16_at);
+    p.x16 = h16(at.x16);
     p.width = static_cast<int32_t>(H);
-    p.seg[0] = ql == 0 ? segment(lm::kProjQ, heads * qk, ws + q_at, 0) : segment(lm::kProjQa, ql, ws + ql_at, 0);
-    p.seg[1] = segment(lm::kProjKva, rank + rope, ws + lat_at, 0);
+    p.seg[0] = ql == 0 ? segment(lm::kProjQ, heads * qk, ws + at.q, 0) : segment(lm::kProjQa, ql, ws + at.ql, 0);
+    p.seg[1] = segment(lm::kProjKva, rank + rope, ws + at.lat, 0);
     LM_ATT_HIP(lm::launch_proj(p, stream));
     p.seg[1] = lm::ProjSegment{};
     if (ql != 0) {
-        LM_ATT_HIP(lm::launch_norm16(ws + ql_at, L.q_a_norm, h16(ql16_at), T, static_cast<int32_t>(ql),
+        LM_ATT_HIP(lm::launch_norm16(ws + at.ql, L.q_a_norm, h16(at.ql16), T, static_cast<int32_t>(ql),
                                      c.rms_norm_eps, stream));
-        p.x16 = h16(ql16_at);
+        p.x16 = h16(at.ql16);
         p.width = static_cast<int32_t>(ql);
-        p.seg[0] = segment(lm::kProjQb, heads * qk, ws + q_at, 0);
+        p.seg[0] = segment(lm::kProjQb, heads * qk, ws + at.q, 0);
         LM_ATT_HIP(lm::launch_proj(p, stream));
     }
     // the latents into their slots (:57-75), the queries' rotary part, and the rest
@@ -791,8 +811,8 @@ int attention_paged(lm_context* ctx, AttnState* st, int32_t layer, const lm_page
     r.nope = a.nope;
     r.rope = a.rope;
     r.rank = static_cast<int32_t>(rank);
-    r.q = ws + q_at;
-    r.lat = ws + lat_at;
+    r.q = ws + at.q;
+    r.lat = ws + at.lat;
     r.norm = L.kv_a_norm;
     r.eps = c.rms_norm_eps;
     r.positions = step.positions;
@@ -803,14 +823,14 @@ int attention_paged(lm_context* ctx, AttnState* st, int32_t layer, const lm_page
     r.sin_t = a.sin_t;
     r.pool = pool;
     r.pool_rows = st->pages * st->page_size;
-    r.q16 = h16(q16_at);
+    r.q16 = h16(at.q16);
     LM_ATT_HIP(lm::launch_latent_rows(r, stream));
     lm::HeadsArgs g;
     g.tokens = T;
     g.heads = a.heads;
     g.K = a.nope;
     g.N = static_cast<int32_t>(rank);
-    g.x = ws + q_at;
+    g.x = ws + at.q;
     g.x_f32 = 1;
     g.x_token = heads * qk;
     g.x_head = qk;
@@ -818,21 +838,21 @@ int attention_paged(lm_context* ctx, AttnState* st, int32_t layer, const lm_page
     g.w_rows = heads * rank;
     g.w_head = static_cast<int32_t>(rank);
     g.w_first = 0;
-    g.out = h16(q16_at);
+    g.out = h16(at.q16);
     g.out_panels = 0;
     g.out_token = heads * (rank + rope);
     g.out_head = rank + rope;
     g.live = nullptr;
     LM_ATT_HIP(lm::launch_heads(g, stream));
     // causal attention over the pages (:77-98), kv_b's value halves
-    rc = lm_paged_attention(ctx, &step, h16(q16_at), pool, LM_DT_F16, a.heads, static_cast<int32_t>(rank), a.rope,
-                            st->scale, h16(ctx16_at));
+    rc = lm_paged_attention(ctx, &step, h16(at.q16), pool, LM_DT_F16, a.heads, static_cast<int32_t>(rank), a.rope,
+                            st->scale, h16(at.ctx16));
     if (rc != LM_OK) {
         return rc;
     }
     g.K = static_cast<int32_t>(rank);
     g.N = a.vh;
-    g.x = h16(ctx16_at);
+    g.x = h16(at.ctx16);
     g.x_f32 = 0;
     g.x_token = heads * rank;
     g.x_head = rank;
@@ -840,12 +860,12 @@ int attention_paged(lm_context* ctx, AttnState* st, int32_t layer, const lm_page
     g.w_rows = heads * (nope + vh);
     g.w_head = static_cast<int32_t>(nope + vh);
     g.w_first = a.nope;
-    g.out = h16(v16_at);
+    g.out = h16(at.v16);
     g.out_panels = 1;
     g.live = live;
     LM_ATT_HIP(lm::launch_heads(g, stream));
     // output projection (:100-101)
-    p.x16 = h16(v16_at);
+    p.x16 = h16(at.v16);
     p.width = static_cast<int32_t>(heads * vh);
     p.seg[0] = segment(lm::kProjO, H, out, accumulate);
     LM_ATT_HIP(lm::launch_proj(p, stream));
@@ -1636,6 +1656,16 @@ int lm_paged_decoder_forward(lm_context* ctx, int32_t first_layer, int32_t last_
             const AttnLayer& L = st->layers[static_cast<size_t>(l)];
             if (L.input_norm == nullptr || L.kv_a == nullptr) {
                 return fail(LM_ENOTRES, "layer " + std::to_string(l) + " has no attention weights or input norm");
+            }
+        }
+        // a layer that cannot be run is found before anything is written
+        for (int32_t l = first_layer; l <= last_layer; ++l) {
+            rc = paged_ready(ctx, st, l, *step);
+            if (rc == LM_OK) {
+                rc = lm::ffn_ready(ctx, l, step->tokens, path);
+            }
+            if (rc != LM_OK) {
+                return rc;
             }
         }
         // what the caller left in rows past the last new token must not steer the experts

@@ -1037,6 +1037,25 @@ int lm::ffn_sublayer(lm_context* ctx, int32_t l, float* hidden, int64_t T, int32
     return ffn_sublayer_fused(ctx, l, hidden, T, path, nullptr, false);
 }
 
+int lm::ffn_ready(lm_context* ctx, int32_t l, int64_t T, int32_t path) {
+    const Layer& L = ctx->layers[static_cast<size_t>(l)];
+    if (L.norm == nullptr) {
+        return fail(LM_ENOTRES, "layer " + std::to_string(l) + " has no norm weight");
+    }
+    if (!L.allocated || (!L.dense && L.router_t == nullptr)) {
+        return fail(LM_ENOTRES, "layer " + std::to_string(l) + " has no resident FFN weights");
+    }
+    if (!L.finalized) {
+        return fail(LM_ENOTRES, "layer " + std::to_string(l) + " is not finalized (lm_finalize_layer)");
+    }
+    const int rc = ensure_workspace(ctx, T);
+    if (rc != LM_OK || L.dense || !takes_decode_path(ctx, L, T, path)) {
+        return rc;
+    }
+    DecodeScratch sc{};
+    return context_decode_scratch(ctx, &sc);
+}
+
 extern "C" {
 
 const char* lm_last_error(void) { return g_error.c_str(); }

@@ -637,6 +637,8 @@ AttnState*& context_attention(lm_context* ctx);
 // h += FFN_l(rms_norm(h, post_attention_layernorm_l)) for T rows of hidden
 // (src/DeepSeekRunner.cpp:264-290), as one layer of lm_stack_forward.
 int ffn_sublayer(lm_context* ctx, int32_t layer, float* hidden, int64_t T, int32_t path);
+// Whether ffn_sublayer can run layer l: its weights resident, its scratch made.
+int ffn_ready(lm_context* ctx, int32_t layer, int64_t T, int32_t path);
 // Frees what lm_attention_configure allocated (lm_attn.hip); null is a no-op.
 void attention_release(AttnState* st);
 

@@ -106,7 +106,23 @@ int serve_state(lm_context* ctx, int rows, lm::ServeState** out, void** parts) {
     return LM_OK;
 }
 
+int check_work(const lm_paged_step& s, int32_t heads) {
+    if (s.tokens * heads > INT32_MAX / 2 ||
+        !lm::paged_shares_out(s.tokens, heads, static_cast<int64_t>(s.table_width) * s.page_size)) {
+        return fail(LM_EINVAL, "tokens * heads must stay under 2^30, and with the keys of a table row under 2^62");
+    }
+    return LM_OK;
+}
+
 }  // namespace
+
+int lm::paged_attention_ready(lm_context* ctx, const lm_paged_step& step, int32_t heads, int32_t rank, int32_t rope) {
+    ServeState* st = nullptr;
+    void* parts = nullptr;
+    const int rc = check_work(step, heads);
+    return rc != LM_OK ? rc
+                       : serve_state(ctx, paged_tiled(rank, rope) ? paged_block_rows(step.max_added, heads) : 0, &st, &parts);
+}
 
 int lm::check_step_sizes(const lm_paged_step* s) {
     if (s == nullptr) {
@@ -182,9 +198,9 @@ int lm_paged_attention(lm_context* ctx, const lm_paged_step* step, const void* q
         if (s.tokens == 0) {
             return ctx != nullptr ? LM_OK : fail(LM_EINVAL, "null context");
         }
-        if (s.tokens * heads > INT32_MAX / 2 ||
-            !lm::paged_shares_out(s.tokens, heads, static_cast<int64_t>(s.table_width) * s.page_size)) {
-            return fail(LM_EINVAL, "tokens * heads must stay under 2^30, and with the keys of a table row under 2^62");
+        rc = check_work(s, heads);
+        if (rc != LM_OK) {
+            return rc;
         }
         if (s.table == nullptr || s.lengths == nullptr || s.starts == nullptr || !aligned(s.table, 4) ||
             !aligned(s.lengths, 4) || !aligned(s.starts, 4)) {

@@ -120,6 +120,9 @@ hipError_t launch_heads(const HeadsArgs& a, hipStream_t s);
 // ---- services of lm_serve.hip ----
 // LM_OK where a step's sizes can be relied on.
 int check_step_sizes(const lm_paged_step* step);
+// Whether lm_paged_attention can run a step of good sizes: its work fits in 64 bits,
+// its workspace is made.
+int paged_attention_ready(lm_context* ctx, const lm_paged_step& step, int32_t heads, int32_t rank, int32_t rope);
 struct ServeState;
 ServeState*& context_serve(lm_context* ctx);
 void serve_release(ServeState* st);
