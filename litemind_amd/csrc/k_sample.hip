@@ -425,6 +425,10 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a, in
     r.scale = static_cast<float>(48 * 0.6931471805599453 * temperature);
     r.scale = (kBins - 2) / (least > -__builtin_inff() ? fminf(r.scale, top - least) : r.scale);
     r.scale = fminf(r.scale, 1e30f / fmaxf(fabsf(r.top_inf ? 0.0f : top), 1.0f));
+    if (r.top_inf) {
+        // (temperatures past 1e37 leave no scale, and infinity times 0 is in no stretch)
+        r.scale = fmaxf(r.scale, 1e-30f);
+    }
     r.offset = static_cast<float>(kBins) - 0.5f - (r.top_inf ? 0.0f : top) * r.scale;
 
     Cut cut{kKeyMinusInf + 1, 0x7fffffff};
