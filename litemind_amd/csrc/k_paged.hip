@@ -276,7 +276,7 @@ struct TileArgs {
     const void* pool;
     void* out;
     int32_t heads;
-    int32_t negative;  // the scale is negative: the queries change sign
+    int32_t sign;      // of the scale, or 0: the queries are multiplied by it
     uint32_t page_mul; // 2^32 / (page_size / 16), rounded up
     float c;           // |scale| log2(e)
     Parts parts;
@@ -515,10 +515,10 @@ __global__ __launch_bounds__(kThreads, 2) void paged_rows_kernel(const TileArgs 
         late_flags[tid] = 0;
     }
     while (more) {
-        if (a.negative) {
+        if (a.sign != 1) {
 #pragma unroll
             for (int ks = 0; ks < 18; ++ks) {
-                q[ks] = -q[ks];
+                q[ks] = q[ks] * static_cast<E>(static_cast<float>(a.sign));
             }
         }
         f32x4 o[RB][4] = {};
@@ -1091,10 +1091,10 @@ hipError_t launch(const PagedAttention& a, void* workspace, hipStream_t s) {
     t.pool = a.pool;
     t.out = a.out;
     t.heads = a.heads;
-    t.negative = a.scale < 0.0f ? 1 : 0;
+    t.sign = a.scale < 0.0f ? -1 : a.scale > 0.0f ? 1 : 0;
     t.page_mul = static_cast<uint32_t>(((uint64_t{1} << 32) + a.view.page_size / 16 - 1) / (a.view.page_size / 16));
-    // a scale of 0 weighs all keys alike, as one this small does, and leaves -infinity what it is
-    t.c = std::max(std::fabs(a.scale) * 1.4426950408889634f, 1e-30f);
+    // (above 0 for any scale: scores of keys that a row may not see are -infinity times it)
+    t.c = t.sign == 0 ? 1.0f : std::fabs(a.scale) * 1.4426950408889634f;
     char* w = static_cast<char*>(workspace);
     const int m = paged_block_rows(a.max_added, a.heads);
     t.parts.heads = reinterpret_cast<PartHead*>(w);

@@ -162,3 +162,19 @@ def test_every_key_counts_once(ctx, heads, cached, added, dtype):
             # equal weights of a power of two: sums are whole numbers, the quotient takes two roundings to 32 bits
             bound = want * 2.0 ** -22
             assert (np.abs(got[t] - want) <= bound + half_step(want + bound, dtype)).all(), f"request {r}, row {t}"
+
+
+@pytest.mark.parametrize("rank,rope", [(512, 64), (64, 16)])
+@pytest.mark.parametrize("size,scale", [(1e17, 0.0), (1e17, 1e-35), (1e17, -1e-35), (1e18, 5e-39), (1.0, 1e-45)])
+def test_scales_of_any_size(ctx, size, scale, rank, rope):
+    """Scores of large numbers and small scales: it is their product that counts, and a scale of 0 weighs all alike."""
+    announce(f"paged attention: queries and keys of {size}, scale {scale}, rank {rank}")
+    rng = np.random.default_rng(3)
+    b = Batch([300, 0, 70], [1, 40, 3], 16, dtype=lm.DT_BF16, page=32, rank=rank, rope=rope, seed=4, scale=float(np.float32(scale)))
+    b.q = encode(rng.normal(size=b.q.shape) * size, b.dtype)
+    for r in range(b.R):
+        b.rows[r] = encode(decode(b.rows[r], b.dtype) * size, b.dtype)
+        for k in range(-(-int(b.lengths[r]) // b.page)):
+            part = b.rows[r][k * b.page:(k + 1) * b.page]
+            b.pool[b.table[r, k], :len(part)] = part
+    b.check(b.run(ctx))
