@@ -178,3 +178,35 @@ def test_scales_of_any_size(ctx, size, scale, rank, rope):
             part = b.rows[r][k * b.page:(k + 1) * b.page]
             b.pool[b.table[r, k], :len(part)] = part
     b.check(b.run(ctx))
+
+
+@pytest.mark.parametrize("heads,cached,added", [(16, [300, 40000], [1, 1]), (16, [100, 0], [40, 9])])
+@pytest.mark.parametrize("power", [20, 44, 58])
+def test_scores_of_any_size(ctx, power, heads, cached, added):
+    """Scores up to 2^60, one step of which outweighs everything: a row is the mean of the keys of its largest score."""
+    announce(f"paged attention: scores of 2^{power}, {heads} heads, {added} after {cached}")
+    rng = np.random.default_rng(power)
+    b = Batch(cached, added, heads, dtype=lm.DT_BF16, page=32, seed=6, scale=0.3)
+    b.q = encode(grid(rng, b.q.shape, 12) * 2.0 ** (power // 2), b.dtype)
+    for r, n in enumerate(b.lengths):
+        rows = grid(rng, (n, WIDTH), 4)
+        rows[:, RANK:] *= 2.0 ** (power - power // 2)  # (the rotary part alone is large, and alone counts)
+        b.rows[r] = encode(rows, b.dtype)
+        for k in range(-(-int(n) // b.page)):
+            part = b.rows[r][k * b.page:(k + 1) * b.page]
+            b.pool[b.table[r, k], :len(part)] = part
+    q = decode(b.q, b.dtype)
+    q[..., :RANK] = 0.0
+    b.q = encode(q, b.dtype)
+    got = decode(b.run(ctx), b.dtype)
+    for r in range(b.R):
+        rows = decode(b.rows[r], b.dtype)
+        for t in range(b.starts[r], b.starts[r + 1]):
+            seen = rows[:cached[r] + t - b.starts[r] + 1]
+            s = q[t] @ seen.T
+            first = (s == s.max(1, keepdims=True)).astype(np.float64)
+            want = (first / first.sum(1, keepdims=True)) @ seen[:, :RANK]
+            # equal weights: sums of a few values in 32 bits, and the quotient
+            bound = 2.0 ** -20 * ((first / first.sum(1, keepdims=True)) @ np.abs(seen[:, :RANK]))
+            off = np.abs(got[t] - want)
+            assert (off <= bound + half_step(np.abs(want) + bound, b.dtype)).all(), f"request {r}, row {t}"
