@@ -29,7 +29,8 @@ __device__ inline PagedRequest paged_request(const PagedView& v, int32_t r) {
     const int64_t room = static_cast<int64_t>(v.table_width) * v.page_size;
     const int32_t length = static_cast<int32_t>(min(static_cast<int64_t>(v.lengths[r]), room));
     q.first = min(max(v.starts[r], 0), v.tokens);
-    q.added = max(0, min(min(v.starts[r + 1], v.tokens) - q.first, length));
+    const int32_t end = min(max(v.starts[r + 1], q.first), v.tokens);
+    q.added = max(0, min(end - q.first, length));
     q.cached = length - q.added;
     return q;
 }

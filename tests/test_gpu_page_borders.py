@@ -9,7 +9,7 @@ import serving_ref as ref
 from conftest import announce
 from litemind_amd import workload as wl
 from test_gpu_pages import Plan, check
-from test_gpu_paged_attention import SCALE, decode, encode
+from test_gpu_paged_attention import SCALE, Batch, decode, encode
 
 pytestmark = pytest.mark.gpu
 
@@ -134,3 +134,17 @@ def test_rings_just_full(ctx, pages, count, taken, back):
     for _ in range(2):
         ctx.page_plan(plan.step)
         check(plan, want)
+
+
+@pytest.mark.parametrize("rank,rope", [(512, 64), (64, 16)])
+@pytest.mark.parametrize("starts", [[0, 2 ** 31 - 1, -2 ** 31, -2 ** 31], [-2 ** 31, 2 ** 31 - 1, -1, -2 ** 31],
+                                    [-5, 3, -2 ** 31, -2 ** 31 + 2]])
+def test_starts_that_run_backwards(ctx, starts, rank, rope):
+    """Starts as far apart as 32 bits allow, in either direction: each is cut to the token rows, and a request that ends
+    before it begins has none."""
+    announce(f"paged attention: starts {starts}, rank {rank}")
+    b = Batch([31, 40, 70], [3, 0, 0], 16, page=16, rank=rank, rope=rope, seed=19).upload(ctx)
+    b.dev["starts"].upload(np.array(starts, np.int32))
+    b.call(ctx)
+    ctx.synchronize()
+    b.check(b.dev["out"].download(), [0])
