@@ -131,8 +131,8 @@ __device__ inline int32_t cut(int64_t x, int64_t cost, int32_t tiles, int32_t he
 // `scratch` (kWaves + 2 words of 64 bits) passes the sums.
 __device__ inline Piece find_piece(const PagedView& v, const Shares& sh, int32_t g, int64_t* scratch) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int32_t per = (v.requests + kThreads - 1) / kThreads;
-    const int32_t r0 = min(tid * per, v.requests), r1 = min(r0 + per, v.requests);
+    const uint32_t requests = static_cast<uint32_t>(v.requests), per = (requests + kThreads - 1) / kThreads;
+    const int32_t r0 = static_cast<int32_t>(min(tid * per, requests)), r1 = static_cast<int32_t>(min(r0 + per, requests));
     int64_t own = 0;
 #pragma unroll 1
     for (int32_t r = r0; r < r1; ++r) {

@@ -148,3 +148,27 @@ def test_starts_that_run_backwards(ctx, starts, rank, rope):
     b.call(ctx)
     ctx.synchronize()
     b.check(b.dev["out"].download(), [0])
+
+
+def test_as_many_requests_as_a_step_takes(ctx):
+    """2^31 - 2 requests, the last with one token: its output is the one latent that it sees, to its bits."""
+    announce("paged attention: 2^31 - 2 requests")
+    requests, heads = 2 ** 31 - 2, 2
+    dev = {"table": ctx.empty(requests, np.int32), "lengths": ctx.empty(requests, np.int32),
+           "starts": ctx.empty(requests + 1, np.int32)}
+    for b in dev.values():
+        b.zero()
+    for at in (dev["lengths"].ptr + 4 * (requests - 1), dev["starts"].ptr + 4 * requests):
+        one = np.ones(1, np.int32)
+        ctx._check(ctx.lib.lm_copy_h2d(ctx.handle, C.c_void_p(at), one.ctypes.data, 4))
+    pool = encode(np.random.default_rng(23).normal(size=(1, 16, 576)), lm.DT_F16)
+    dev |= {"q": ctx.to_device(np.zeros((1, heads, 576), np.uint16)), "pool": ctx.to_device(pool),
+            "out": ctx.to_device(np.full((2, heads, 512), 0x1234, np.uint16))}
+    step = lm.PagedStep(requests=requests, tokens=1, pages=1, page_size=16, table_width=1, max_added=1)
+    for k in ("table", "lengths", "starts"):
+        setattr(step, k, dev[k].ptr)
+    ctx.paged_attention(step, dev["q"], dev["pool"], heads, SCALE, dev["out"])
+    got = dev["out"].download()
+    for b in dev.values():
+        b.free()
+    assert (got[0] == pool[0, 0, :512]).all() and (got[1] == 0x1234).all()
