@@ -121,9 +121,9 @@ int lm_paged_pool(lm_context* ctx, int32_t layer, void** out_dev);
  * they were (accumulate = 1).  Positions at or past context_length are not
  * rotated, as lm_attention_forward's.  kv_b_proj is absorbed into the query and
  * the output; queries, latents and weights round to fp16, within the MFMA
- * path's tolerance.  out_dev must not overlap x_dev.  tokens * heads at most
- * 2^24, and tokens times the widest of hidden_size, q_lora_rank and heads *
- * v_head_dim 2^30.  Asynchronous. */
+ * path's tolerance.  out_dev must not overlap x_dev.  tokens under 2^24, tokens *
+ * heads at most 2^24, and tokens times the widest of hidden_size, q_lora_rank and
+ * heads * v_head_dim under 2^30.  Asynchronous. */
 int lm_paged_forward(lm_context* ctx, int32_t layer, const lm_paged_step* step, const float* x_dev, float* out_dev,
                      int32_t accumulate);
 /* lm_decoder_forward's layer loop with lm_paged_forward as the attention:

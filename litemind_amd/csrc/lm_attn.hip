@@ -688,8 +688,9 @@ int check_paged(lm_context* ctx, const lm_paged_step* step, AttnState** out) {
     const int64_t widest = std::max({static_cast<int64_t>(c.hidden_size), static_cast<int64_t>(c.q_lora_rank),
                                      static_cast<int64_t>(c.num_heads) * c.v_head_dim});
     // 32-bit offsets of the projections, 2^32 threads of the launches
-    if (step->tokens * widest > INT32_MAX / 2 || step->tokens * c.num_heads > 1 << 24) {
-        return fail(LM_EINVAL, "too many tokens in one step: tokens * heads at most 2^24, times the widest row 2^30");
+    if (step->tokens * widest > INT32_MAX / 2 || step->tokens * c.num_heads > 1 << 24 || step->tokens >= 1 << 24) {
+        return fail(LM_EINVAL, "too many tokens in one step: under 2^24, times heads at most 2^24, times the widest row "
+                               "under 2^30");
     }
     if (step->tokens == 0) {
         return LM_OK;

@@ -1,4 +1,4 @@
-"""lm_paged_decoder_forward: what a refused call leaves."""
+"""lm_paged_forward and lm_paged_decoder_forward: refused sizes, and what a refused call leaves."""
 import ctypes as C
 import dataclasses
 
@@ -62,3 +62,21 @@ def test_a_layer_that_cannot_run_is_found_first(what):
         ctx.synchronize()
         y = dh.download()[:starts[-1]]
         assert np.isfinite(y).all() and (y != h[:starts[-1]]).any(axis=1).all()
+
+
+@pytest.mark.parametrize("hidden,heads,tokens", [(32, 1, 2 ** 24), (64, 1, 2 ** 24), (32, 1, 2 ** 25), (32, 2, 2 ** 23 + 1),
+                                                 (2048, 1, 2 ** 19)])
+def test_more_tokens_than_a_launch_takes(hidden, heads, tokens):
+    """Refused by its numbers, before an array is read or a kernel launched."""
+    announce(f"paged layers: {tokens} tokens of {hidden} channels, {heads} heads")
+    d = dataclasses.replace(SMALL, hidden=hidden, heads=heads, kv_lora_rank=32, qk_rope=8, max_positions=64)
+    with lm.Context(moe_dims(hidden, 1).moe_config(num_layers=1)) as ctx:
+        ctx.attention_configure(wl.mla_config(d))
+        ctx.paged_configure(4, 16)
+        step = lm.PagedStep(requests=1, tokens=tokens, pages=4, page_size=16, table_width=2, max_added=1)
+        words = ctx.to_device(np.zeros(8, np.int32))
+        for name in ("table", "lengths", "starts", "positions", "slots"):
+            setattr(step, name, words.ptr)
+        for call in (lambda: ctx.paged_forward(0, step, words, words), lambda: ctx.paged_decoder_forward(0, 0, step, words)):
+            with pytest.raises(lm.LmError, match="too many tokens"):
+                call()
