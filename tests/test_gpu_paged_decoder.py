@@ -1,4 +1,5 @@
-"""lm_paged_forward and lm_paged_decoder_forward: refused sizes, and what a refused call leaves."""
+"""lm_paged_forward and lm_paged_decoder_forward: the models' own latent widths, refused sizes, and what a
+refused call leaves."""
 import ctypes as C
 import dataclasses
 
@@ -8,7 +9,8 @@ import pytest
 import litemind_amd as lm
 from conftest import announce
 from litemind_amd import workload as wl
-from test_gpu_paged_layer import SMALL, Service, moe_dims
+from test_gpu_paged_layer import MEAN_REL, SMALL, Service, moe_dims, run_decoder
+from test_gpu_paged_layer import test_forward_against_the_oracle as forward_against_the_oracle
 
 pytestmark = pytest.mark.gpu
 
@@ -80,3 +82,25 @@ def test_more_tokens_than_a_launch_takes(hidden, heads, tokens):
         for call in (lambda: ctx.paged_forward(0, step, words, words), lambda: ctx.paged_decoder_forward(0, 0, step, words)):
             with pytest.raises(lm.LmError, match="too many tokens"):
                 call()
+
+
+@pytest.mark.parametrize("heads,page", [(128, 64), (20, 16)])
+def test_forward_with_many_heads(heads, page):
+    """DeepSeek-V2's 128 heads, and a number that no block of rows divides, against the oracle."""
+    forward_against_the_oracle(dataclasses.replace(wl.V2_LITE_MLA, hidden=256, heads=heads), page)
+
+
+@pytest.mark.parametrize("heads,path", [(16, lm.PATH_AUTO), (16, lm.PATH_MFMA), (128, lm.PATH_AUTO)])
+def test_decoder_over_latents_of_512(heads, path):
+    """The layer loop through the matrix-core attention, requests together and alone."""
+    announce(f"paged decoder: rank 512, {heads} heads, path {path}")
+    d = dataclasses.replace(wl.V2_LITE_MLA, hidden=256, heads=heads, max_positions=256)
+    together, alone, states = run_decoder(d, path, 2, [37, 1, 64, 18], [1, 1, 3])
+    for n, rows in enumerate(together):
+        for r, y in enumerate(rows):
+            want = alone[r][n]
+            change = np.abs(want - states[n][r])
+            rel = np.abs(y - want).sum() / change.sum()
+            print(f"step {n} request {r}: mean_rel={rel:.3e} of the change")
+            # two layers: their attention within its bar on both sides, and experts of 1e-3
+            assert np.isfinite(y).all() and rel <= 2 * (2 * MEAN_REL + 1e-3)
