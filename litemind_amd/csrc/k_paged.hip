@@ -369,7 +369,7 @@ __device__ inline int lds_address(const char* p) {
 // with 8 and 7, 120.5 with 6 and 9, 132.8 with 4 and 11.)
 constexpr float kSlack = 10.0f;
 constexpr float kLift = 5.0f;
-constexpr float kUnset = 1e30f;  // lift of a row without a score yet: any finite one passes its reference
+constexpr float kUnset = 3e38f;  // lift of a row without a score yet: any finite one passes its reference
 
 // Non-finite values as 0: keys that some row must not see weigh 0 there, and 0
 // times NaN or infinity is not 0. (Rows that see such a key have a NaN weight.)

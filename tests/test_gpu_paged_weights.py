@@ -210,3 +210,27 @@ def test_scores_of_any_size(ctx, power, heads, cached, added):
             bound = 2.0 ** -20 * ((first / first.sum(1, keepdims=True)) @ np.abs(seen[:, :RANK]))
             off = np.abs(got[t] - want)
             assert (off <= bound + half_step(np.abs(want) + bound, b.dtype)).all(), f"request {r}, row {t}"
+
+
+@pytest.mark.parametrize("heads", [16, 40])
+@pytest.mark.parametrize("size", [1e3, 1e15, 1e17, 1e18])
+def test_far_negative_scores_after_infinite_ones(ctx, size, heads):
+    """Two tiles of scores of -infinity, then equal ones down to -2e36: those alone have weight."""
+    announce(f"paged attention: 64 scores of -infinity, then -2 {size}^2, {heads} heads")
+    rng = np.random.default_rng(9)
+    b = Batch([140], [2], heads, dtype=lm.DT_BF16, page=16, seed=9, scale=1.0)
+    rows = grid(rng, (142, WIDTH), 4)
+    rows[:, RANK:] = 0.0
+    rows[:64, RANK] = -np.inf
+    rows[64:, RANK + 1] = -2.0 * size
+    q = np.zeros(b.q.shape)
+    q[..., RANK], q[..., RANK + 1] = 1.0, size
+    b.q, b.rows[0] = encode(q, b.dtype), encode(rows, b.dtype)
+    for k in range(9):
+        part = b.rows[0][k * 16:(k + 1) * 16]
+        b.pool[b.table[0, k], :len(part)] = part
+    got = decode(b.run(ctx), b.dtype)[:2]
+    for i in range(2):
+        want = rows[64:141 + i, :RANK].mean(0)
+        bound = 2.0 ** -20 * np.abs(rows[64:141 + i, :RANK]).mean(0)
+        assert (np.abs(got[i] - want) <= bound + half_step(np.abs(want) + bound, b.dtype)).all()
