@@ -369,7 +369,9 @@ __device__ inline int lds_address(const char* p) {
 // with 8 and 7, 120.5 with 6 and 9, 132.8 with 4 and 11.)
 constexpr float kSlack = 10.0f;
 constexpr float kLift = 5.0f;
-constexpr float kUnset = 3e38f;  // lift of a row without a score yet: any finite one passes its reference
+// Reference of a row without a score yet: finite ones pass it, or weigh against it as
+// against any other where the scale is that small; -infinity weighs 0.
+constexpr float kLowest = -0x1.fffffep127f;
 
 // Non-finite values as 0: keys that some row must not see weigh 0 there, and 0
 // times NaN or infinity is not 0. (Rows that see such a key have a NaN weight.)
@@ -523,8 +525,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_rows_kernel(const TileArgs 
         }
         f32x4 o[RB][4] = {};
         f32x4 sc;                 // scores of the newest tile
-        float m = kNone;          // reference of row `lane`, the same in every wave
-        float ref = 0.0f, lift = kUnset;  // of this lane's row of the scores
+        float m = kLowest;        // reference of row `lane`, the same in every wave
+        float ref = kLowest;      // of this lane's row of the scores
         float l = 0.0f, sum = 0.0f;  // its total, and the newest tile's
         // the newest tile's weights; their total is that of the rounded ones, so that what
         // is rounded away of a key that outweighs the others goes from both
@@ -536,8 +538,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_rows_kernel(const TileArgs 
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 // (the difference first: c times a reference of 2^28 and more is off by more
-                // than the range of the weights; a prompt of 2048 0.7 us)
-                const float x = __builtin_fmaf(sc[e] - ref, a.c, lift);
+                // than the range of the weights)
+                const float x = __builtin_fmaf(sc[e] - ref, a.c, kLift);
                 over = fmaxf(over, x);
                 p[e] = static_cast<E>(__builtin_amdgcn_exp2f(x));
                 w[e] = static_cast<float>(p[e]);
@@ -654,11 +656,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_rows_kernel(const TileArgs 
             meet();
             const int row = min(lane, rows - 1);  // (rows past the last are the last once more)
             const float up = fmaxf(m, fmaxf(tops[0][row], tops[1][row]));
-            const float alpha = up == kNone ? 1.0f : __builtin_amdgcn_exp2f((m - up) * a.c);
+            const float alpha = __builtin_amdgcn_exp2f((m - up) * a.c);
             m = up;
-            const float mine = __shfl(up, score_row);
-            ref = mine == kNone ? 0.0f : mine;
-            lift = mine == kNone ? kUnset : kLift;
+            ref = __shfl(up, score_row);
             return alpha;
         };
         // tile t's weights and tile t + 1 are in: all but tile t + 2's loads have come
@@ -839,7 +839,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_rows_kernel(const TileArgs 
             }
             if (tid < out_rows) {
                 float* const to = a.parts.stats + (slot * M + tid) * 2;
-                to[0] = m == kNone ? kNone : m * a.c;
+                to[0] = m * a.c;
                 to[1] = tops[0][tid] + tops[1][tid];
             }
             if (parts_after >= 0 && tid == 0) {
