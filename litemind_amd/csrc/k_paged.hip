@@ -21,9 +21,9 @@
 // border leaves unnormalised sums, which paged_join_kernel adds in order.
 //
 // Measured, 16 heads, calls of three contexts in turn: one token over 131072 keys
-// 34 us, 4.4 TB/s (large reads reach 6.4); one each of 32 requests of up to 4000
-// keys 21.7 us; 512 tokens after 3001 84 us, 0.70 PFLOP/s, and 2048 after none 115
-// us, 0.64 (large library products reach 1.2). A call by itself takes 20 us at
+// 35 us, 4.3 TB/s (large reads reach 6.4); one each of 32 requests of up to 4000
+// keys 21.8 us; 512 tokens after 3001 84 us, 0.70 PFLOP/s, and 2048 after none 117
+// us, 0.63 (large library products reach 1.2). A call by itself takes 20 us at
 // least: the lengths, the tables, the first tiles and the sums each wait for the
 // one before.
 #include "serve_internal.h"
@@ -365,8 +365,8 @@ __device__ inline int lds_address(const char* p) {
 // 2^-(14 + kLift) of a row's largest and are rounded to steps of 2^-(24 + kLift) of it
 // below: of n keys far under a first one, n 2^-30 of the row at most is lost, less than
 // its output's rounding for up to 2^18 keys to a workgroup. (More lift needs less slack,
-// and references move more often: a prompt of 2048 takes 115.9 us with these, 116.6
-// with 8 and 7, 120.5 with 6 and 9, 132.8 with 4 and 11.)
+// and references move more often: a prompt of 2048 takes 1 % longer with 8 and 7, 4 %
+// with 6 and 9, 15 % with 4 and 11.)
 constexpr float kSlack = 10.0f;
 constexpr float kLift = 5.0f;
 // Reference of a row without a score yet: finite ones pass it, or weigh against it as
@@ -1132,8 +1132,8 @@ bool paged_shares_out(int64_t tokens, int32_t heads, int64_t room) {
 }
 
 // 16 rows where no request has more (one token of 32 requests, 16 heads, three
-// contexts in turn: 23.5 us, in blocks of 64 26.0), or else 64 (32 heads, by itself:
-// 36 us, in blocks of 16 44).
+// contexts in turn: 22 us, in blocks of 64 25), or else 64 (32 heads: 28 us, in
+// blocks of 16 34).
 int paged_block_rows(int32_t max_added, int32_t heads) {
     return static_cast<int64_t>(max_added) * heads <= 16 ? 16 : 64;
 }

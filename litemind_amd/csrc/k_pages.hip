@@ -7,8 +7,8 @@
 //
 // Three sums over the requests; per four tokens, and per taken and returned page,
 // one search in them.  Latency bound: a decode step of 48 requests reads and
-// writes 2 KB and takes 10 us by itself, 3.9 among others' calls; 509 requests of
-// up to 64 new tokens take 15.6 and 5.2.  One workgroup; requests in chunks of one
+// writes 2 KB and takes 10 us by itself, 4.0 among others' calls; 509 requests of
+// up to 64 new tokens take 15.9 and 5.3.  One workgroup; requests in chunks of one
 // per thread.
 #include "serve_internal.h"
 

@@ -17,9 +17,9 @@
 // A row is a workgroup's; its sweeps after the first come from the caches. What
 // they cost is the e: 11 steps of 64-bit arithmetic and as many others, 22 us for
 // 102400 on one CU. By temperature alone a row has one such sweep (35 us by
-// itself, 256 rows 50 us), by top-k none (28 us), by top-p two (100 us). Sharing a
-// row among workgroups, a kernel for each sweep, was no faster: 40 us for top-k
-// and 76 for 32 rows of any settings, where this takes 72.
+// itself, 256 rows 49 us), by top-k none (29 us), by top-p two (78 us); a greedy row
+// takes 12. Sharing a row among workgroups, a kernel for each sweep, was no faster:
+// 40 us for top-k and 76 for 32 rows of any settings, where this takes 70.
 #include "serve_internal.h"
 
 #include <algorithm>
@@ -468,7 +468,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a, in
     // The list holds all that the cut keeps. For a short row that is any cut; for
     // top-k of fewer than there are threads, each thread's largest logit bounds the
     // k-th largest from below (a row of 102400 by itself, with the token drawn from the
-    // list: 28 us, and 68 by counts over the whole row).
+    // list: 29 us, and 68 by counts over the whole row).
     bool whole = r.n <= kList && (set.top_k > 0 || set.top_p < 1.0f);
     if (whole) {
         gather(0, true);
