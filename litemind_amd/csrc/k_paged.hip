@@ -360,15 +360,17 @@ __device__ inline int lds_address(const char* p) {
 // The weights' reference m, one per row, has to be the same for all waves: it is
 // moved only where a row's scores pass it by more than kSlack (in powers of
 // two), which a wave tells the others at the next barrier; the tile's weights
-// are then made anew. A score at the reference weighs 2^kLift: fp32 sums do not mind
-// the factor, and fp16 weights, which end at 2^16, keep their 11 bits down to
+// are then made anew. A score at the reference weighs 2^kLift. In bf16, whose latents
+// may lie near the end of the range of their fp32 sums, that is 2^-kSlack, so that no
+// weight passes 1. In fp16 the weights, which end at 2^16, keep 11 bits down to
 // 2^-(14 + kLift) of a row's largest and are rounded to steps of 2^-(24 + kLift) of it
 // below: of n keys far under a first one, n 2^-30 of the row at most is lost, less than
 // its output's rounding for up to 2^18 keys to a workgroup. (More lift needs less slack,
 // and references move more often: a prompt of 2048 takes 1 % longer with 8 and 7, 4 %
 // with 6 and 9, 15 % with 4 and 11.)
 constexpr float kSlack = 10.0f;
-constexpr float kLift = 5.0f;
+template <class E>
+constexpr float kLift = std::is_same_v<E, bf16> ? -kSlack : 5.0f;
 // Reference of a row without a score yet: finite ones pass it, or weigh against it as
 // against any other where the scale is that small; -infinity weighs 0.
 constexpr float kLowest = -0x1.fffffep127f;
@@ -539,7 +541,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_rows_kernel(const TileArgs 
             for (int e = 0; e < 4; ++e) {
                 // (the difference first: c times a reference of 2^28 and more is off by more
                 // than the range of the weights)
-                const float x = __builtin_fmaf(sc[e] - ref, a.c, kLift);
+                const float x = __builtin_fmaf(sc[e] - ref, a.c, kLift<E>);
                 over = fmaxf(over, x);
                 p[e] = static_cast<E>(__builtin_amdgcn_exp2f(x));
                 w[e] = static_cast<float>(p[e]);
@@ -549,7 +551,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_rows_kernel(const TileArgs 
         };
         // tells the others where a score passed the reference
         auto tell = [&](int u) {
-            if (__builtin_expect(__any(over > kSlack + kLift), 0)) {
+            if (__builtin_expect(__any(over > kSlack + kLift<E>), 0)) {
                 if (lane == 0) {
                     late_flags[u] = 1;
                 }

@@ -234,3 +234,20 @@ def test_far_negative_scores_after_infinite_ones(ctx, size, heads):
         want = rows[64:141 + i, :RANK].mean(0)
         bound = 2.0 ** -20 * np.abs(rows[64:141 + i, :RANK]).mean(0)
         assert (np.abs(got[i] - want) <= bound + half_step(np.abs(want) + bound, b.dtype)).all()
+
+
+@pytest.mark.parametrize("heads", [16, 40])
+@pytest.mark.parametrize("cached,at", [(0, 0), (3, 1), (6, 6), (40, 35), (100, 99)])
+def test_latents_near_the_end_of_the_range(ctx, cached, at, heads):
+    """BF16 latents of up to 3e37, one of which outweighs the others by 2^9.5: sums of weights up to 1 stay in 32 bits."""
+    announce(f"paged attention: latents of 3e37, {heads} heads, one token after {cached}")
+    rng = np.random.default_rng(cached)
+    b = Batch([cached], [1], heads, dtype=lm.DT_BF16, page=128, seed=10, scale=float(np.float32(9.5 * np.log(2.0))))
+    rows = grid(rng, (cached + 1, WIDTH), 4)
+    rows[:, :RANK] *= 3e37
+    rows[:, RANK] = np.arange(cached + 1) == at
+    q = np.zeros(b.q.shape)
+    q[..., RANK] = 1.0
+    b.q, b.rows[0] = encode(q, b.dtype), encode(rows, b.dtype)
+    b.pool[b.table[0, 0], :cached + 1] = b.rows[0]
+    b.check(b.run(ctx))
