@@ -1,0 +1,103 @@
+/*
+ * litemind_fp8.h -- C ABI of the 8-bit floating point (FP8) products of the
+ * feed-forward path on one MI355X (gfx950): rows and weights in blocks that
+ * share a scale, their matrix products, the products grouped by expert, and
+ * the layers' path through them at one byte a weight.
+ *
+ * LiteMind computes in BF16 and fp32; nothing here has a counterpart in it.
+ * Conventions are those of include/litemind_moe.h: int status, lm_last_error,
+ * *_dev device pointers, work on the context stream, one host thread at a time
+ * per context.
+ *
+ * Format.  Codes are OCP e4m3 (1 sign, 4 exponent, 3 mantissa bits, largest
+ * 448, no infinity; uint8_t here, row-major, rows of `features` bytes).  A
+ * block is 128 codes of a row, or 128 rows of 128; the last block of a row or
+ * column may be smaller.  With the largest magnitude m of a block's finite
+ * values its scale is s = max(m / 448, 2^-126) and the code of x is
+ * x * (1 / s) rounded to the nearest e4m3, ties to even, in fp32 arithmetic; x
+ * stands for code * s.  NaN and infinity become the NaN code 0x7f, and so reach
+ * every product of theirs.  Scales are fp32, [row blocks][ceil(features / 128)].
+ *
+ * lm_fp8_quantize, lm_fp8_gemm, lm_fp8_grouped_gemm and lm_fp8_grouped_swiglu
+ * may be captured into a HIP graph on the context's stream; the grouped ones
+ * after their first call on the context (before it LM_EINVAL).  Replays share
+ * the context's scratch: they run on the context's stream, or on another one
+ * that waits for it and that it waits for.
+ */
+#ifndef LITEMIND_FP8_H
+#define LITEMIND_FP8_H
+
+#include "litemind_moe.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define LM_FP8_BLOCK 128
+
+/* x [rows][width] of `dtype` (LM_DT_F32, LM_DT_F16 or LM_DT_BF16), rows
+ * row_stride elements apart (at least width), into q_dev [rows][width] codes and
+ * scale_dev [ceil(rows / block_rows)][ceil(width / 128)].  block_rows is 1 (a
+ * product's rows) or 128 (its weights).  rows under 2^31, width at most 2^24;
+ * q_dev 16-byte aligned; the outputs overlap nothing.  Asynchronous. */
+int lm_fp8_quantize(lm_context* ctx, const void* x_dev, int32_t dtype, int64_t rows, int64_t width, int64_t row_stride,
+                    int32_t block_rows, uint8_t* q_dev, float* scale_dev);
+
+/* out[r][n] = sum over blocks b of a_scale[r][b] * w_scale[n / 128][b] *
+ *             sum over k in b of a[r][k] * w[n][k]
+ *   a_dev [rows][in_features], a_scale_dev [rows][ceil(in_features / 128)]
+ *   w_dev [out_features][in_features],
+ *   w_scale_dev [ceil(out_features / 128)][ceil(in_features / 128)]
+ *   out_dev [rows][out_features] of out_dtype (LM_DT_F32, LM_DT_F16, LM_DT_BF16)
+ * Products are exact.  An fp32 output's sums are fp32; fp16 and BF16 outputs' are
+ * those of the FP8 matrix cores, off by 1.4e-5 to 4e-5 of their norm and at most
+ * 2^-10 of the sum of magnitudes, rounded once at the end.  in_features a multiple
+ * of 16 up to 2^20, out_features at most 2^24; rows, rows * in_features and
+ * out_features * in_features under 2^31, 2^32 and 2^32.  a_dev, w_dev and out_dev
+ * 16-byte aligned; out_dev overlaps no input.  Asynchronous. */
+int lm_fp8_gemm(lm_context* ctx, const uint8_t* a_dev, const float* a_scale_dev, int64_t rows, const uint8_t* w_dev,
+                const float* w_scale_dev, int64_t out_features, int64_t in_features, void* out_dev, int32_t out_dtype);
+
+/* The rows of each expert, as lm_permute leaves them: group g has rows
+ * offsets[g] .. offsets[g + 1] - 1, none of them where the two are equal.  All
+ * arrays are device memory of the caller. */
+typedef struct lm_fp8_groups {
+    int32_t groups;         /* 1 .. 512 */
+    int32_t divisor;        /* with source: at least 1; without: 0 */
+    int64_t rows;           /* rows that the arrays hold: at least offsets[groups] */
+    const int32_t* offsets; /* [groups + 1], 0 at first, rising */
+    const int32_t* source;  /* NULL: row i reads row i of a.  Or [rows]: row source[i] / divisor
+                               (lm_permute's perm and top_k: the token of each assignment) */
+    const int32_t* target;  /* NULL: row i of the output.  Or [rows]: row target[i], each at most
+                               once (lm_permute's perm: assignment order) */
+} lm_fp8_groups;
+
+/* lm_fp8_gemm with a matrix for each group: w_dev [groups][out_features]
+ * [in_features] and w_scale_dev [groups][ceil(out_features / 128)]
+ * [ceil(in_features / 128)].  a_dev has a_rows rows, out_dev out_rows; the sizes'
+ * limits hold for a_rows and for each group's matrix.  Output rows that no row is
+ * written to stay as they were.  Rows past `rows` and indexes outside a or out are
+ * not followed: what they would read is taken as row 0, what they would write is
+ * left out, and the next lm_synchronize or lm_copy_d2h returns LM_EKERNEL; so it
+ * does for offsets that fall.  Asynchronous. */
+int lm_fp8_grouped_gemm(lm_context* ctx, const lm_fp8_groups* groups, const uint8_t* a_dev, const float* a_scale_dev,
+                        int64_t a_rows, const uint8_t* w_dev, const float* w_scale_dev, int64_t out_features,
+                        int64_t in_features, void* out_dev, int64_t out_rows, int32_t out_dtype);
+
+/* The gate and up products of each group's expert, SwiGLU, and the down
+ * product's input blocks: w_dev [groups][2][inter][in_features] (gate, then up)
+ * and w_scale_dev [groups][2][ceil(inter / 128)][ceil(in_features / 128)]; with
+ * gate_i, up_i the two products of row i, both fp32,
+ *     act_i = gate_i / (1 + exp(-gate_i)) * up_i
+ * goes to row i of q_dev [rows][inter] and scale_dev [rows][ceil(inter / 128)] in
+ * blocks of 1 x 128.  target must be NULL.  inter a multiple of 16 up to 2^20,
+ * rows * inter and 2 * inter * in_features under 2^32; the rest as above.
+ * Asynchronous. */
+int lm_fp8_grouped_swiglu(lm_context* ctx, const lm_fp8_groups* groups, const uint8_t* a_dev, const float* a_scale_dev,
+                          int64_t a_rows, const uint8_t* w_dev, const float* w_scale_dev, int64_t inter,
+                          int64_t in_features, uint8_t* q_dev, float* scale_dev);
+
+#ifdef __cplusplus
+}
+#endif
+#endif

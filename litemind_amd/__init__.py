@@ -108,6 +108,22 @@ STEP_OK, STEP_LENGTH, STEP_TOKENS, STEP_PAGES, STEP_RING = range(5)  # LM_STEP_*
 # lm_sampling: one row's settings, as a numpy structured type
 SAMPLING = np.dtype([("temperature", np.float32), ("top_k", np.int32), ("top_p", np.float32), ("min_p", np.float32)])
 
+
+class Fp8Groups(C.Structure):
+    """lm_fp8_groups: the rows of each expert; the arrays are device addresses (include/litemind_fp8.h)."""
+
+    _fields_ = [
+        ("groups", C.c_int32),
+        ("divisor", C.c_int32),
+        ("rows", C.c_int64),
+        ("offsets", C.c_void_p),
+        ("source", C.c_void_p),
+        ("target", C.c_void_p),
+    ]
+
+
+FP8_BLOCK = 128  # LM_FP8_BLOCK: codes that share a scale, along a row
+
 _P = C.c_void_p
 _I32 = C.c_int32
 _I64 = C.c_int64
@@ -198,6 +214,10 @@ PROTOTYPES = {
     "lm_paged_forward": [_P, _I32, _P, _P, _P, _I32],
     "lm_paged_decoder_forward": [_P, _I32, _I32, _P, _P, _I32],
     "lm_sample": [_P, _P, _I64, _I64, _I64, _P, _P, _P, _P],
+    "lm_fp8_quantize": [_P, _P, _I32, _I64, _I64, _I64, _I32, _P, _P],
+    "lm_fp8_gemm": [_P, _P, _P, _I64, _P, _P, _I64, _I64, _P, _I32],
+    "lm_fp8_grouped_gemm": [_P, _P, _P, _P, _I64, _P, _P, _I64, _I64, _P, _I64, _I32],
+    "lm_fp8_grouped_swiglu": [_P, _P, _P, _P, _I64, _P, _P, _I64, _I64, _P, _P],
 }
 _RESTYPE = {"lm_last_error": C.c_char_p}
 
@@ -577,6 +597,31 @@ class Context:
         """The next token of each row of logits from its settings (SAMPLING) and a random number (lm_sample)."""
         self._check(self.lib.lm_sample(self.handle, _ptr(logits), rows, vocab, row_stride or vocab, _ptr(settings),
                                        _ptr(uniform), _ptr(token), _ptr(probability)))
+
+    # ---- products in 8-bit floating point (include/litemind_fp8.h) ----
+    def fp8_quantize(self, x, rows: int, width: int, q, scale, dtype: int = DT_F32, row_stride: int = 0,
+                     block_rows: int = 1) -> None:
+        """Rows (block_rows 1) or a matrix (128) as e4m3 codes and a scale per block (lm_fp8_quantize)."""
+        self._check(self.lib.lm_fp8_quantize(self.handle, _ptr(x), dtype, rows, width, row_stride or width, block_rows,
+                                             _ptr(q), _ptr(scale)))
+
+    def fp8_gemm(self, a, a_scale, rows: int, w, w_scale, out_features: int, in_features: int, out,
+                 dtype: int = DT_F32) -> None:
+        """out = a . w^T of FP8 rows and weights (lm_fp8_gemm)."""
+        self._check(self.lib.lm_fp8_gemm(self.handle, _ptr(a), _ptr(a_scale), rows, _ptr(w), _ptr(w_scale),
+                                         out_features, in_features, _ptr(out), dtype))
+
+    def fp8_grouped_gemm(self, groups: Fp8Groups, a, a_scale, a_rows: int, w, w_scale, out_features: int,
+                         in_features: int, out, out_rows: int, dtype: int = DT_F32) -> None:
+        """The same with a matrix for each expert's rows (lm_fp8_grouped_gemm)."""
+        self._check(self.lib.lm_fp8_grouped_gemm(self.handle, C.byref(groups), _ptr(a), _ptr(a_scale), a_rows, _ptr(w),
+                                                 _ptr(w_scale), out_features, in_features, _ptr(out), out_rows, dtype))
+
+    def fp8_grouped_swiglu(self, groups: Fp8Groups, a, a_scale, a_rows: int, w, w_scale, inter: int, in_features: int,
+                           q, scale) -> None:
+        """Gate and up products and SwiGLU of each expert's rows, in FP8 blocks again (lm_fp8_grouped_swiglu)."""
+        self._check(self.lib.lm_fp8_grouped_swiglu(self.handle, C.byref(groups), _ptr(a), _ptr(a_scale), a_rows,
+                                                   _ptr(w), _ptr(w_scale), inter, in_features, _ptr(q), _ptr(scale)))
 
     def moe_forward_noalloc(self, layer, x, tokens, y, bias=None, idx=None, w=None, logits=None) -> None:
         """lm_moe_forward_noalloc: the single-token kernel per token, scratch in a fixed device array."""

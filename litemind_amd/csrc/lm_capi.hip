@@ -7,6 +7,7 @@
 // enqueued asynchronously on the context stream.  No exception crosses the ABI;
 // every entry point returns a status and records a thread-local message.
 #include "litemind_moe.h"
+#include "fp8_internal.h"
 #include "lm_error.h"
 #include "lm_internal.h"
 #include "serve_internal.h"
@@ -208,6 +209,7 @@ struct lm_context {
     lm::HeadBest* head_partial = nullptr;  // per-block candidates of the greedy choice
     lm::AttnState* attention = nullptr;  // lm_attention_configure: MLA weights, rotary tables, KV caches
     lm::ServeState* serve = nullptr;     // the operators of litemind_serving.h, at their first call
+    lm::Fp8State* fp8 = nullptr;         // the grouped products of litemind_fp8.h, at their first call
     int32_t graphs = 0;  // live lm_stack_graph captures (they hold the workspace's pointers)
     // lm_clock_probe_*: its own stream (default priority) and sample buffer
     hipStream_t probe_stream = nullptr;
@@ -994,7 +996,18 @@ lm::AttnState*& lm::context_attention(lm_context* ctx) { return ctx->attention; 
 
 lm::ServeState*& lm::context_serve(lm_context* ctx) { return ctx->serve; }
 
+lm::Fp8State*& lm::context_fp8(lm_context* ctx) { return ctx->fp8; }
+
 namespace {
+
+// After the context's stream has drained: what its kernels reported, each once.
+int check_kernel_errors(lm_context* ctx) {
+    int rc = check_decode_error(ctx);
+    if (rc == LM_OK) {
+        rc = lm::serve_check_error(ctx);
+    }
+    return rc != LM_OK ? rc : lm::fp8_check_error(ctx);
+}
 
 // h += FFN(rms_norm(h)) (src/DeepSeekRunner.cpp:265-290) for one layer.  The
 // MoE block normalises the hidden state itself (inside the single-token
@@ -1181,6 +1194,7 @@ int lm_context_destroy(lm_context* ctx) {
     lm::attention_release(ctx->attention);
     ctx->attention = nullptr;
     lm::serve_release(ctx->serve);
+    lm::fp8_release(ctx->fp8);
     if (ctx->staging != nullptr) {
         (void)hipHostFree(ctx->staging);
     }
@@ -1207,8 +1221,7 @@ int lm_synchronize(lm_context* ctx) {
         return fail(LM_EINVAL, "null context");
     }
     LM_HIP(hipStreamSynchronize(ctx->stream));
-    const int rc = check_decode_error(ctx);
-    return rc != LM_OK ? rc : lm::serve_check_error(ctx);
+    return check_kernel_errors(ctx);
 }
 
 int lm_alloc(lm_context* ctx, size_t bytes, void** out_dev) {
@@ -1246,9 +1259,8 @@ int lm_copy_d2h(lm_context* ctx, void* dst_host, const void* src_dev, size_t byt
     }
     LM_HIP(hipMemcpyAsync(dst_host, src_dev, bytes, hipMemcpyDeviceToHost, ctx->stream));
     LM_HIP(hipStreamSynchronize(ctx->stream));
-    // the copied data may come from a decode whose wait gave up, or from pages outside a pool
-    const int rc = check_decode_error(ctx);
-    return rc != LM_OK ? rc : lm::serve_check_error(ctx);
+    // the copied data may come from a decode whose wait gave up, or from pages or rows out of range
+    return check_kernel_errors(ctx);
 }
 
 int lm_memset(lm_context* ctx, void* dst_dev, int32_t value, size_t bytes) {
