@@ -19,8 +19,8 @@
  * every product of theirs.  Scales are fp32, [row blocks][ceil(features / 128)].
  *
  * lm_fp8_quantize, lm_fp8_gemm, lm_fp8_grouped_gemm and lm_fp8_grouped_swiglu
- * may be captured into a HIP graph on the context's stream; the grouped ones
- * after their first call on the context (before it LM_EINVAL).  Replays share
+ * may be captured into a HIP graph on the context's stream; the products after
+ * the context's first call of one of them (before it LM_EINVAL).  Replays share
  * the context's scratch: they run on the context's stream, or on another one
  * that waits for it and that it waits for.
  */

@@ -45,7 +45,9 @@ struct Fp8Product {
     float* q_scale;          // SwiGLU: [rows][nb]
     uint32_t* error;         // set to 1 (host memory) by an index outside its range; null without offsets
 };
-hipError_t launch_fp8_gemm(const Fp8Product& p, hipStream_t s);
+// Sums of products whose reduced axis several workgroups share.
+constexpr int64_t kFp8WorkspaceBytes = 32 << 20;
+hipError_t launch_fp8_gemm(const Fp8Product& p, void* workspace, hipStream_t s);
 hipError_t launch_fp8_swiglu(const Fp8Product& p, hipStream_t s);
 
 #if defined(__HIPCC__)

@@ -92,6 +92,13 @@ __device__ inline void report(const Fp8Product& p) {
     __hip_atomic_store(p.error, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
 }
 
+__device__ inline void take(floatx4& acc, floatx4 d, float scale) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        acc[u] = __builtin_fmaf(d[u], scale, acc[u]);
+    }
+}
+
 // ---- which rows and features a workgroup computes ----
 
 struct Tile {
@@ -236,71 +243,159 @@ __device__ inline float swiglu(float gate, float up) {
 
 // ---- the kernel of large tiles ----
 //
-// WM x WN waves, each MI x NJ blocks of 16 rows x 16 features, so a tile has
-// 16 WM MI rows and 16 WN NJ weight rows (SwiGLU: half of each wave's are gate
-// rows and half the up rows of the same channels). A stage is one scale block,
-// 128 bytes of every row, loaded straight to LDS STAGES - 1 stages ahead, with
-// the rows' and the weights' scales of the block.
+// A tile has BM rows and BN weight rows (SwiGLU: blocks of 16 gate rows and the
+// 16 up rows of the same channels in turn). A stage is one scale block, 128
+// bytes of every row, loaded straight to LDS STAGES - 1 stages ahead, with the
+// rows' and the weights' scales of the block.
 //
-// LDS rows are 128 bytes: chunk c of row r lies at chunk position c ^ f(r),
-// f(r) = (r & 7) ^ (r >> 3 & 1), which puts any eight rows at eight positions
-// (32 banks) and any sixteen at sixteen places of two rows (64 banks).
-__device__ inline int chunk_swizzle(int r) { return (r & 7) ^ ((r >> 3) & 1); }
+// LDS rows are 128 bytes: chunk c of row r lies at chunk position c ^ (r / 2).
+// A 16-byte read takes sixteen lanes a clock over 64 banks (256 bytes, two
+// rows); whether those are lanes 0 .. 15 or, as it seems, 0 .. 3, 12 .. 15 and
+// 20 .. 27, they hold sixteen different rows, and land on different banks.
+// (c ^ (r & 7) ^ (r >> 3 & 1), free of conflicts in the first order alone, had one
+// a read: 1680 clocks of LDS a stage of 256 x 256 where this has 912.)
+__device__ inline int chunk_swizzle(int r) { return (r >> 1) & 7; }
 
-template <bool SWIGLU, int WM, int WN, int MI, int NJ, int STAGES>
+template <bool SWIGLU_, int BM_, int BN_, int WAVES_, int STAGES_>
 struct Shape {
-    static constexpr int WAVES = WM * WN;
-    static constexpr int BM = 16 * WM * MI, BN = 16 * WN * NJ;
+    static constexpr bool SWIGLU = SWIGLU_;
+    static constexpr int BM = BM_, BN = BN_, WAVES = WAVES_, STAGES = STAGES_;
     static constexpr int CN = SWIGLU ? BN / 2 : BN;  // output features of a tile
     static constexpr int kABytes = BM * 128, kBBytes = BN * 128;
     static constexpr int kScales = (BM + 63) / 64;  // 64-lane loads of row scales
     static constexpr int kBlocks = (BN + kFp8Block - 1) / kFp8Block;  // weight scales
     static constexpr int kRowScales = kABytes + kBBytes, kWeightScales = kRowScales + kScales * 256;
     static constexpr int kStageBytes = kWeightScales + 256;
-    static constexpr int AL = BM / 8 / WAVES, BL = BN / 8 / WAVES;
-    static constexpr int L = AL + BL + 2;
-    static_assert(AL * 8 * WAVES == BM && BL * 8 * WAVES == BN, "whole 1 KB loads per wave");
-    static_assert(kScales <= WAVES && (STAGES - 1) * L < 64, "a scale load per wave, vmcnt");
+    static_assert(STAGES >= 2 && STAGES <= 4 && kScales < WAVES, "a scale load per wave");
     static_assert(!SWIGLU || CN == kFp8Block, "a SwiGLU tile is one output block wide");
-    static_assert(16 * NJ <= (SWIGLU ? 2 : 1) * kFp8Block && CN % (SWIGLU ? 1 : 16 * NJ) == 0, "one weight scale per wave and part");
+    static_assert(kFp8Block % CN == 0 || CN % kFp8Block == 0, "tiles end where scale blocks do");
 };
 
-template <bool SWIGLU, bool EXACT, int WM, int WN, int MI, int NJ, int STAGES>
-struct Pipeline {
-    using Z = Shape<SWIGLU, WM, WN, MI, NJ, STAGES>;
-    __amdgpu_buffer_rsrc_t ra, rs, rb, rw;  // rows, their scales, weights, their scales
-    unsigned va[Z::AL], vb[Z::BL], vs, vw;  // this lane's byte offsets in stage 0
-    unsigned ta[Z::AL], tb[Z::BL];      // the same in the last stage
-    int lane, wave, wm, wn, nk;
-    int live;                           // this wave's 16-row blocks that hold rows
-    int last_chunks;                    // chunks of the last stage that hold channels
-    int fa, fb, fs, ws;                 // this lane's row chunk, weight chunk, row scale and weight scale in a stage
+// What every wave of a tile needs.
+template <class Z>
+struct Stage {
+    char* const (&bufs)[4];
+    Tile t;
+    int m0, n0;  // the tile's first row in its group, its first feature
+    int lane, wave;
+    int first, stages;  // the tile's share of the reduced axis, in scale blocks
+};
+
+// The products of a tile's first 16 WM MI rows: WM x WN waves of MI x NJ blocks
+// of 16 rows x 16 weight rows.
+template <class Z, bool EXACT, int WM, int WN, int MI, int NJ>
+struct Work {
+    static constexpr bool SWIGLU = Z::SWIGLU;
+    static constexpr int STAGES = Z::STAGES, BM = 16 * WM * MI;
+    // 1 KB loads of a wave and stage; where the rows have fewer than there are
+    // waves, two waves load the same
+    static constexpr int AL = BM / 8 > Z::WAVES ? BM / 8 / Z::WAVES : 1, BL = Z::BN / 8 / Z::WAVES;
+    static constexpr int L = AL + BL + 1;
+    static_assert(WM * WN == Z::WAVES && BM <= Z::BM && 16 * WN * NJ == Z::BN);
+    static_assert((AL * 8 * Z::WAVES == BM || Z::WAVES * 8 % BM == 0) && BL * 8 * Z::WAVES == Z::BN,
+                  "whole loads per wave");
+    static_assert((STAGES - 1) * L < 64, "vmcnt");
+    static_assert(SWIGLU ? NJ % 2 == 0 : (16 * NJ <= kFp8Block && kFp8Block % (16 * NJ) == 0),
+                  "gate and up in one wave, one weight scale otherwise");
+
+    __amdgpu_buffer_rsrc_t ra, rb, rs;  // rows, weights, the scales that this wave loads
+    unsigned va[AL], vb[BL], vs;        // this lane's byte offsets in stage 0
+    unsigned ta[AL], tb[BL];            // the same in the last block's stage
+    int scales_at;                      // where the scales go in a stage
+    int lane, wave, wm, wn;
+    int blocks;          // scale blocks of the reduced axis
+    int last_chunks;     // chunks of the last one that hold channels
+    bool idle;           // none of this wave's rows is the group's: it loads for the others
+    int fa, fb, fs, ws;  // this lane's row chunk, weight chunk, row scale and weight scale in a stage
     floatx4 acc[MI][NJ];
 
-    __device__ void load(int ks, char* buf, bool last) {
+    __device__ __forceinline__ Work(const Fp8Product& p, const Stage<Z>& st) {
+        const Tile& t = st.t;
+        lane = st.lane;
+        wave = st.wave;
+        wm = wave / WN;
+        wn = wave % WN;
+        blocks = p.kb;
+        last_chunks = (p.k - (p.kb - 1) * kFp8Block) / 16;
+        idle = st.m0 + 16 * MI * wm >= t.rows;
+        const int chunk = (lane & 15) * 128 + (((lane >> 4) ^ chunk_swizzle(lane & 15)) << 4);
+        fa = 2048 * MI * wm + chunk;
+        fb = Z::kABytes + 2048 * NJ * wn + chunk;
+        fs = Z::kRowScales + 64 * MI * wm + 4 * (lane & 15);
+        ws = Z::kWeightScales + (SWIGLU ? 0 : wn * 16 * NJ / kFp8Block * 4);
+        constexpr int kParts = SWIGLU ? 2 : 1;
+        const int64_t matrix = static_cast<int64_t>(p.n) * p.k, scales = static_cast<int64_t>(kParts) * p.nb * p.kb;
+        ra = __builtin_amdgcn_make_buffer_rsrc((void*)p.a, 0, static_cast<int>(p.a_rows * p.k), kBufferWord3);
+        rb = __builtin_amdgcn_make_buffer_rsrc((void*)(p.w + t.g * kParts * matrix), 0,
+                                               static_cast<int>(kParts * matrix), kBufferWord3);
+        // rows past the group's last repeat it, and are not stored
+        const auto row_of = [&](int r) { return source_row(p, t.first + min(st.m0 + r, t.rows - 1)); };
 #pragma unroll
-        for (int q = 0; q < Z::AL; ++q) {
-            buffer_lds16(ra, buf + (Z::WAVES * q + wave) * 1024, last ? ta[q] : va[q], static_cast<unsigned>(ks) * 128u);
+        for (int q = 0; q < AL; ++q) {
+            const int r = load_row(q);
+            const int c = (lane & 7) ^ chunk_swizzle(r);
+            const unsigned row = row_of(r) * static_cast<unsigned>(p.k);
+            va[q] = row + 16 * c;
+            ta[q] = c < last_chunks ? va[q] : row;
         }
 #pragma unroll
-        for (int q = 0; q < Z::BL; ++q) {
-            buffer_lds16(rb, buf + Z::kABytes + (Z::WAVES * q + wave) * 1024, last ? tb[q] : vb[q],
-                         static_cast<unsigned>(ks) * 128u);
+        for (int q = 0; q < BL; ++q) {
+            const int r = 8 * (Z::WAVES * q + wave) + (lane >> 3);
+            const int c = (lane & 7) ^ chunk_swizzle(r);
+            const int n = SWIGLU ? st.n0 + (r >> 5) * 16 + (r & 15) : st.n0 + r;
+            const unsigned part = SWIGLU ? (r >> 4) & 1 : 0;
+            const unsigned row = (part * static_cast<unsigned>(p.n) + min(n, p.n - 1)) * static_cast<unsigned>(p.k);
+            vb[q] = row + 16 * c;
+            tb[q] = c < last_chunks ? vb[q] : row;
         }
-        buffer_lds4(rs, buf + Z::kRowScales + (wave % Z::kScales) * 256, vs, static_cast<unsigned>(ks) * 4u);
-        buffer_lds4(rw, buf + Z::kWeightScales, vw, static_cast<unsigned>(ks) * 4u);
+        // The first waves load 64 rows' scales each, a line of memory for every
+        // row; the others the weights', one or two lines, all of them the same.
+        if (wave < Z::kScales) {
+            rs = __builtin_amdgcn_make_buffer_rsrc((void*)p.a_scale, 0, static_cast<int>(p.a_rows * p.kb * 4),
+                                                   kBufferWord3);
+            vs = row_of(min(64 * wave + lane, BM - 1)) * static_cast<unsigned>(p.kb) * 4u;
+            scales_at = Z::kRowScales + wave * 256;
+        } else {
+            rs = __builtin_amdgcn_make_buffer_rsrc((void*)(p.w_scale + t.g * scales), 0, static_cast<int>(4 * scales),
+                                                   kBufferWord3);
+            const int block = SWIGLU ? (lane & 1) * p.nb + t.nt : min(st.n0 / kFp8Block + lane % Z::kBlocks, p.nb - 1);
+            vs = static_cast<unsigned>(block) * static_cast<unsigned>(p.kb) * 4u;
+            scales_at = Z::kWeightScales;
+        }
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+        }
+    }
+
+    // The row of which load q of the rows has this lane's chunk.
+    __device__ __forceinline__ int load_row(int q) const { return 8 * ((Z::WAVES * q + wave) % (BM / 8)) + (lane >> 3); }
+    // Load q of this wave's stage loads: rows, weights, then the scales.
+    __device__ __forceinline__ void load1(int ks, char* buf, bool last, int q) {
+        const unsigned at = static_cast<unsigned>(ks) * 128u;
+        if (q < AL) {
+            buffer_lds16(ra, buf + (Z::WAVES * q + wave) % (BM / 8) * 1024, last ? ta[q] : va[q], at);
+        } else if (q < AL + BL) {
+            const int w = q - AL;
+            buffer_lds16(rb, buf + Z::kABytes + (Z::WAVES * w + wave) * 1024, last ? tb[w] : vb[w], at);
+        } else {
+            buffer_lds4(rs, buf + scales_at, vs, at / 32);
+        }
     }
     // Sixteen rows' fragment: `at` is this lane's first chunk in the stage (one
     // addition from the array's start, so that the compiler sees which it is).
-    __device__ void read(const char* cur, int at, Operand<EXACT>& to) const {
+    __device__ __forceinline__ void read(const char* cur, int at, Operand<EXACT>& to) const {
         to.set(*reinterpret_cast<const uint4*>(cur + at), *reinterpret_cast<const uint4*>(cur + (at ^ 64)));
     }
     // Zeros past the reduced axis in the last stage, each lane into the chunks
     // that it loaded.
-    __device__ void clear_past(char* buf) {
+    __device__ __forceinline__ void clear_past(char* buf) {
 #pragma unroll
-        for (int q = 0; q < Z::AL; ++q) {
-            const int r = 8 * (Z::WAVES * q + wave) + (lane >> 3);
+        for (int q = 0; q < AL; ++q) {
+            const int r = load_row(q);
             if (((lane & 7) ^ chunk_swizzle(r)) >= last_chunks) {
                 *reinterpret_cast<uint4*>(buf + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
             }
@@ -308,60 +403,89 @@ struct Pipeline {
         __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
     }
     // No read of one stage's buffer may cross it, in either direction.
-    __device__ void barrier() {
+    __device__ __forceinline__ void barrier() {
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     }
-    // The products of a stage. FULL: all of the wave's row blocks hold rows.
-    template <bool FULL>
-    __device__ void multiply(const char* cur) {
+    // The products of a stage: row block i's on the matrix cores beside block
+    // i - 1's FMAs and the reads of block i + 1. between(i) issues a part of the
+    // next loads: a wave's run of them would wait for each to be accepted (256 x
+    // 256 x 16384: 209 -> 201 us, 128 x 256 of three stages 265 -> 223).
+    template <class Between>
+    __device__ __forceinline__ void multiply(const char* cur, Between between) {
         const float w0 = *reinterpret_cast<const float*>(cur + ws);
         const float w1 = SWIGLU ? *reinterpret_cast<const float*>(cur + (ws + 4)) : w0;
-        Operand<EXACT> b[NJ];
+        Operand<EXACT> b[NJ], a[2];
+        floatx4 d[2][NJ];
+        float scale[2], s0[2], s1[2];
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             read(cur, fb + 2048 * j, b[j]);
         }
+        read(cur, fa, a[0]);
+        scale[0] = *reinterpret_cast<const float*>(cur + fs);
 #pragma unroll
-        for (int i = 0; i < MI; ++i) {
-            if (FULL || i < live) {
-                Operand<EXACT> a;
-                read(cur, fa + 2048 * i, a);
-                const float scale = *reinterpret_cast<const float*>(cur + (fs + 64 * i));
-                const float s0 = scale * w0, s1 = SWIGLU ? scale * w1 : s0;
+        for (int i = 0; i <= MI; ++i) {
+            const int now = i & 1, before = now ^ 1;
+            if (i < MI) {
+                if (i + 1 < MI) {
+                    read(cur, fa + 2048 * (i + 1), a[before]);
+                    scale[before] = *reinterpret_cast<const float*>(cur + (fs + 64 * (i + 1)));
+                }
+                s0[now] = scale[now] * w0;
+                s1[now] = SWIGLU ? scale[now] * w1 : s0[now];
+            }
 #pragma unroll
-                for (int j = 0; j < NJ; ++j) {
-                    const floatx4 d = block_sum(b[j], a);
-                    const float s = SWIGLU && j >= NJ / 2 ? s1 : s0;
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        acc[i][j][u] = __builtin_fmaf(d[u], s, acc[i][j][u]);
-                    }
+            for (int j = 0; j < NJ; ++j) {
+                if (i < MI) {
+                    d[now][j] = block_sum(b[j], a[now]);
+                }
+                if (i > 0) {
+                    take(acc[i - 1][j], d[before][j], SWIGLU && j % 2 == 1 ? s1[before] : s0[before]);
                 }
             }
+            if (i < MI) {
+                between(i);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
-    // All nk stages: stage ks lives in buffer ks % STAGES; its loads are issued
+    // The nk stages from `first` on: stage ks lives in buffer ks % STAGES; its loads are issued
     // STAGES - 1 stages before, into the buffer that every wave has read when it
     // passes the barrier of stage ks - STAGES + 1. The first loop's stages have
-    // later ones behind them that are not the last.
-    template <bool FULL>
-    __device__ void run(char* const (&bufs)[4]) {
+    // later ones behind them that are not the last block's.
+    __device__ __forceinline__ void run(char* const (&bufs)[4], int first, int nk) {
+        const auto spread = [&](int ks, char* buf, bool last, int i) {
+#pragma unroll
+            for (int q = i * L / MI; q < (i + 1) * L / MI; ++q) {
+                load1(first + ks, buf, last, q);
+            }
+        };
 #pragma unroll
         for (int d = 0; d < STAGES - 1; ++d) {
             if (d < nk) {
-                load(d, bufs[d], d == nk - 1);
+#pragma unroll
+                for (int i = 0; i < MI; ++i) {
+                    spread(d, bufs[d], first + d == blocks - 1, i);
+                }
             }
         }
         int ks = 0;
         for (; ks + 2 * STAGES - 1 < nk; ks += STAGES) {
 #pragma unroll
             for (int j = 0; j < STAGES; ++j) {
-                LM_WAIT_VM((STAGES - 2) * Z::L);
+                LM_WAIT_VM((STAGES - 2) * L);
                 barrier();
-                load(ks + j + STAGES - 1, bufs[(j + STAGES - 1) % STAGES], false);
-                multiply<FULL>(bufs[j]);
+                const auto next = [&](int i) { spread(ks + j + STAGES - 1, bufs[(j + STAGES - 1) % STAGES], false, i); };
+                if (idle) {
+#pragma unroll
+                    for (int i = 0; i < MI; ++i) {
+                        next(i);
+                    }
+                } else {
+                    multiply(bufs[j], next);
+                }
             }
         }
         for (; ks < nk; ks += STAGES) {
@@ -370,181 +494,143 @@ struct Pipeline {
                 const int k = ks + j;
                 if (k < nk) {
                     if (STAGES > 2 && k + STAGES - 2 < nk) {
-                        LM_WAIT_VM((STAGES - 2) * Z::L);
+                        LM_WAIT_VM((STAGES - 2) * L);
                     } else {
                         LM_WAIT_VM(0);
                     }
-                    if (k == nk - 1 && last_chunks < 8) {
+                    if (first + k == blocks - 1 && last_chunks < 8) {
                         clear_past(bufs[j]);
                     }
                     barrier();
                     if (k + STAGES - 1 < nk) {
-                        load(k + STAGES - 1, bufs[(j + STAGES - 1) % STAGES], k + STAGES == nk);
+#pragma unroll
+                        for (int i = 0; i < MI; ++i) {
+                            spread(k + STAGES - 1, bufs[(j + STAGES - 1) % STAGES], first + k + STAGES == blocks, i);
+                        }
                     }
-                    multiply<FULL>(bufs[j]);
+                    if (!idle) {
+                        multiply(bufs[j], [](int) {});
+                    }
                 }
             }
         }
     }
-};
-
-template <bool SWIGLU, bool EXACT, int WM, int WN, int MI, int NJ, int STAGES, int PER_EU>
-__global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(PER_EU, PER_EU))) void fp8_tile_kernel(
-    Fp8Product p) {
-    using Z = Shape<SWIGLU, WM, WN, MI, NJ, STAGES>;
-    static_assert(STAGES >= 2 && STAGES <= 4);
-    // one LDS array per stage: the compiler tracks the asynchronous writes by array
-    __shared__ __attribute__((aligned(1024))) char s0[Z::kStageBytes], s1[Z::kStageBytes],
-        s2[STAGES > 2 ? Z::kStageBytes : 16], s3[STAGES > 3 ? Z::kStageBytes : 16];
-    char* const bufs[4] = {s0, s1, s2, s3};
-    Tile t;
-    if (!find_tile(p, Z::BM, (p.n + Z::CN - 1) / Z::CN, t)) {
-        return;
-    }
-    Pipeline<SWIGLU, EXACT, WM, WN, MI, NJ, STAGES> pipe;
-    const int lane = pipe.lane = threadIdx.x & 63;
-    const int wave = pipe.wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-    const int wm = pipe.wm = wave / WN;
-    const int wn = pipe.wn = wave % WN;
-    pipe.nk = p.kb;
-    pipe.last_chunks = (p.k - (p.kb - 1) * kFp8Block) / 16;
-    const int m0 = t.mt * Z::BM, n0 = t.nt * Z::CN;
-    const int chunk = (lane & 15) * 128 + (((lane >> 4) ^ chunk_swizzle(lane & 15)) << 4);
-    pipe.fa = 2048 * MI * wm + chunk;
-    pipe.fb = Z::kABytes + 2048 * NJ * wn + chunk;
-    pipe.fs = Z::kRowScales + 64 * MI * wm + 4 * (lane & 15);
-    pipe.ws = Z::kWeightScales + (SWIGLU ? 0 : wn * 16 * NJ / kFp8Block * 4);
-    pipe.live = (t.rows - m0 - 16 * MI * wm + 15) / 16;
-    constexpr int kParts = SWIGLU ? 2 : 1;
-    const int64_t matrix = static_cast<int64_t>(p.n) * p.k;
-    pipe.ra = __builtin_amdgcn_make_buffer_rsrc((void*)p.a, 0, static_cast<int>(p.a_rows * p.k), kBufferWord3);
-    pipe.rs = __builtin_amdgcn_make_buffer_rsrc((void*)p.a_scale, 0, static_cast<int>(p.a_rows * p.kb * 4), kBufferWord3);
-    pipe.rb = __builtin_amdgcn_make_buffer_rsrc((void*)(p.w + t.g * kParts * matrix), 0,
-                                                static_cast<int>(kParts * matrix), kBufferWord3);
-    const int64_t blocks = static_cast<int64_t>(kParts) * p.nb * p.kb;
-    pipe.rw = __builtin_amdgcn_make_buffer_rsrc((void*)(p.w_scale + t.g * blocks), 0, static_cast<int>(4 * blocks),
-                                                kBufferWord3);
-    // rows past the group's last repeat it, and are not stored
-    const auto row_of = [&](int r) { return source_row(p, t.first + min(m0 + r, t.rows - 1)); };
-#pragma unroll
-    for (int q = 0; q < Z::AL; ++q) {
-        const int r = 8 * (Z::WAVES * q + wave) + (lane >> 3);
-        const int c = (lane & 7) ^ chunk_swizzle(r);
-        const unsigned row = row_of(r) * static_cast<unsigned>(p.k);
-        pipe.va[q] = row + 16 * c;
-        pipe.ta[q] = c < pipe.last_chunks ? pipe.va[q] : row;
-    }
-    pipe.vs = row_of(min(64 * (wave % Z::kScales) + lane, Z::BM - 1)) * static_cast<unsigned>(p.kb) * 4u;
-#pragma unroll
-    for (int q = 0; q < Z::BL; ++q) {
-        const int r = 8 * (Z::WAVES * q + wave) + (lane >> 3);
-        const int c = (lane & 7) ^ chunk_swizzle(r);
-        int n = n0 + r;
-        unsigned part = 0;
-        if (SWIGLU) {  // wave r / (16 NJ): its gate rows, then the up rows of the same channels
-            const int in = r % (16 * NJ);
-            part = in >= 8 * NJ ? 1u : 0u;
-            n = n0 + r / (16 * NJ) * 8 * NJ + in % (8 * NJ);
-        }
-        const unsigned row = (part * static_cast<unsigned>(p.n) + min(n, p.n - 1)) * static_cast<unsigned>(p.k);
-        pipe.vb[q] = row + 16 * c;
-        pipe.tb[q] = c < pipe.last_chunks ? pipe.vb[q] : row;
-    }
-    const int block = SWIGLU ? (lane & 1) * p.nb + t.nt : min(n0 / kFp8Block + lane % Z::kBlocks, p.nb - 1);
-    pipe.vw = static_cast<unsigned>(block) * static_cast<unsigned>(p.kb) * 4u;
-#pragma unroll
-    for (int i = 0; i < MI; ++i) {
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            pipe.acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-        }
-    }
-    if (pipe.live >= MI) {
-        pipe.template run<true>(bufs);
-    } else {
-        pipe.template run<false>(bufs);
-    }
-
-    const int quad = 4 * (lane >> 4);
-    if constexpr (!SWIGLU) {
+    __device__ __forceinline__ void store(const Fp8Product& p, const Stage<Z>& st) {
+        const int quad = 4 * (lane >> 4);
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
-            const int m = m0 + 16 * (wm * MI + i) + (lane & 15);
-            const int64_t row = m < t.rows ? target_row(p, t.first + m) : -1;
+            const int m = st.m0 + 16 * (wm * MI + i) + (lane & 15);
+            const int64_t row = m < st.t.rows ? target_row(p, st.t.first + m) : -1;
             if (row >= 0) {
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
-                    const int n = n0 + 16 * (wn * NJ + j) + quad;
+                    const int n = st.n0 + 16 * (wn * NJ + j) + quad;
                     if (n < p.n) {
-                        store4(p, row, n, pipe.acc[i][j]);
+                        store4(p, row, n, acc[i][j]);
                     }
                 }
             }
         }
-    } else {
-        // Each row's largest magnitude over the tile's 128 channels, from the
-        // waves that share the row, then the codes through LDS to 16-byte stores.
+    }
+    // SwiGLU, each row's largest magnitude over the tile's 128 channels from the
+    // waves that share the row, and the codes through LDS to 16-byte stores.
+    __device__ __forceinline__ void store_swiglu(const Fp8Product& p, const Stage<Z>& st, char* codes, float* most_of) {
         constexpr int kPitch = kFp8Block + 16;  // a row's 16 lanes write to 16 different banks
-        static_assert(Z::BM * kPitch <= Z::kStageBytes);
-        __shared__ float most_of[WN][Z::BM];
-        char* const codes = s0;  // written once every wave has passed a barrier after its products
+        static_assert(BM * kPitch <= Z::kStageBytes);
+        const int quad = 4 * (lane >> 4);
+        const int rows = st.t.rows - st.m0;
+        const int64_t first = st.t.first + st.m0;
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
             float most = 0.0f;
 #pragma unroll
-            for (int j = 0; j < NJ / 2; ++j) {
-                const bool in = n0 + 8 * NJ * wn + 16 * j + quad < p.n;  // p.n is a multiple of 16
+            for (int j = 0; j < NJ; j += 2) {
+                const bool in = st.n0 + 8 * (wn * NJ + j) + quad < p.n;  // p.n is a multiple of 16
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    const float v = in ? swiglu(pipe.acc[i][j][u], pipe.acc[i][j + NJ / 2][u]) : 0.0f;
-                    pipe.acc[i][j][u] = v;
+                    const float v = in ? swiglu(acc[i][j][u], acc[i][j + 1][u]) : 0.0f;
+                    acc[i][j][u] = v;
                     most = __builtin_fmaxf(most, fp8_magnitude(v));
                 }
             }
             most = __builtin_fmaxf(most, __shfl_xor(most, 16));
             most = __builtin_fmaxf(most, __shfl_xor(most, 32));
             if (lane < 16) {
-                most_of[wn][16 * (wm * MI + i) + lane] = most;
+                most_of[wn * BM + 16 * (wm * MI + i) + lane] = most;
             }
         }
-        __syncthreads();
+        __syncthreads();  // `codes` is a stage's buffer: every wave's products are done
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
             const int r = 16 * (wm * MI + i) + (lane & 15);
-            float most = most_of[0][r];
+            float most = most_of[r];
 #pragma unroll
             for (int w = 1; w < WN; ++w) {
-                most = __builtin_fmaxf(most, most_of[w][r]);
+                most = __builtin_fmaxf(most, most_of[w * BM + r]);
             }
             const float scale = fp8_scale(most), inverse = 1.0f / scale;
 #pragma unroll
-            for (int j = 0; j < NJ / 2; ++j) {
+            for (int j = 0; j < NJ; j += 2) {
                 float v[4];
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    v[u] = fp8_finite_or_nan(pipe.acc[i][j][u]) * inverse;
+                    v[u] = fp8_finite_or_nan(acc[i][j][u]) * inverse;
                 }
-                *reinterpret_cast<uint32_t*>(codes + r * kPitch + 8 * NJ * wn + 16 * j + quad) =
+                *reinterpret_cast<uint32_t*>(codes + r * kPitch + 8 * (wn * NJ + j) + quad) =
                     fp8_pack4(v[0], v[1], v[2], v[3]);
             }
-            if (wn == 0 && lane < 16 && m0 + r < t.rows) {
-                p.q_scale[static_cast<int64_t>(t.first + m0 + r) * p.nb + t.nt] = scale;
+            if (wn == 0 && lane < 16 && r < rows) {
+                p.q_scale[(first + r) * p.nb + st.t.nt] = scale;
             }
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < Z::BM * 8; i += 64 * Z::WAVES) {
-            const int r = i / 8, n = n0 + 16 * (i % 8);
-            if (m0 + r < t.rows && n < p.n) {
-                *reinterpret_cast<uint4*>(p.q + static_cast<int64_t>(t.first + m0 + r) * p.n + n) =
+        for (int i = threadIdx.x; i < BM * 8; i += 64 * Z::WAVES) {
+            const int r = i / 8, n = st.n0 + 16 * (i % 8);
+            if (r < rows && n < p.n) {
+                *reinterpret_cast<uint4*>(p.q + (first + r) * p.n + n) =
                     *reinterpret_cast<const uint4*>(codes + r * kPitch + 16 * (i % 8));
             }
         }
     }
+};
+
+template <class Z, bool EXACT, int WM, int WN, int MI, int NJ>
+__device__ __forceinline__ void run_tile(const Fp8Product& p, const Stage<Z>& st, char* codes, float* most_of) {
+    Work<Z, EXACT, WM, WN, MI, NJ> work(p, st);
+    work.run(st.bufs, st.first, st.stages);
+    if constexpr (Z::SWIGLU) {
+        work.store_swiglu(p, st, codes, most_of);
+    } else {
+        work.store(p, st);
+    }
 }
 
-template <bool SWIGLU, bool EXACT, int WM, int WN, int MI, int NJ, int STAGES, int PER_EU>
-hipError_t launch_tiles(const Fp8Product& p, hipStream_t s) {
-    using Z = Shape<SWIGLU, WM, WN, MI, NJ, STAGES>;
+template <class Z, bool EXACT, int WM, int WN, int MI, int NJ>
+__global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2, 2))) void fp8_tile_kernel(Fp8Product p) {
+    // one LDS array per stage: the compiler tracks the asynchronous writes by array
+    __shared__ __attribute__((aligned(1024))) char s0[Z::kStageBytes], s1[Z::kStageBytes],
+        s2[Z::STAGES > 2 ? Z::kStageBytes : 16], s3[Z::STAGES > 3 ? Z::kStageBytes : 16];
+    __shared__ float most_of[Z::SWIGLU ? WN * Z::BM : 1];
+    char* const bufs[4] = {s0, s1, s2, s3};
+    Tile t;
+    if (!find_tile(p, Z::BM, (p.n + Z::CN - 1) / Z::CN, t)) {
+        return;
+    }
+    int first = 0, stages = p.kb;
+    if (gridDim.y > 1) {  // a share of the reduced axis, into a plane of fp32 sums of its own
+        const int per = (p.kb + gridDim.y - 1) / gridDim.y;
+        first = blockIdx.y * per;
+        stages = min(per, p.kb - first);
+        p.out = static_cast<float*>(p.out) + blockIdx.y * p.rows * p.n;
+    }
+    const Stage<Z> st{bufs, t, t.mt * Z::BM, t.nt * Z::CN, static_cast<int>(threadIdx.x & 63),
+                      __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)), first, stages};
+    run_tile<Z, EXACT, WM, WN, MI, NJ>(p, st, s0, most_of);
+}
+
+template <bool SWIGLU, bool EXACT, int WM, int WN, int MI, int NJ, int STAGES>
+hipError_t launch_tiles(const Fp8Product& p, hipStream_t s, int shares = 1) {
+    using Z = Shape<SWIGLU, 16 * WM * MI, 16 * WN * NJ, WM * WN, STAGES>;
     // a group of n rows takes ceil(n / BM) row tiles: at most one more than
     // n / BM for each group that has any
     const int64_t mts = p.offsets == nullptr ? (p.rows + Z::BM - 1) / Z::BM
@@ -553,20 +639,295 @@ hipError_t launch_tiles(const Fp8Product& p, hipStream_t s) {
     if (tiles > (1 << 22)) {
         return hipErrorInvalidValue;
     }
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(fp8_tile_kernel<SWIGLU, EXACT, WM, WN, MI, NJ, STAGES, PER_EU>),
-                       dim3(static_cast<unsigned>(round_up(tiles, kXcds))), dim3(64 * Z::WAVES), 0, s, p);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(fp8_tile_kernel<Z, EXACT, WM, WN, MI, NJ>),
+                       dim3(static_cast<unsigned>(round_up(tiles, kXcds)), static_cast<unsigned>(shares)), dim3(64 * Z::WAVES),
+                       0, s, p);
     return hipGetLastError();
+}
+
+// ---- the kernel of few rows ----
+//
+// Tiles of 16 rows at most: the weights are read once, straight to registers,
+// and the waves of a workgroup take turns at the scale blocks of the reduced
+// axis; their sums are added up in LDS, wave by wave. What counts is the bytes
+// in flight: U blocks of NT times 2 KB a wave.
+//
+// Scale blocks b0, b0 + step, ... (U of them, as far as there are any) of NT
+// times 16 weight rows and the rows of a.
+template <int NT, int U>
+__device__ __forceinline__ void stream_blocks(const Fp8Product& p, int b0, int step, const uint8_t* a, const float* a_scale,
+                                              bool live, const uint8_t* const (&w)[NT],
+                                              const float* const (&w_scale)[NT], floatx4 (&acc)[NT]) {
+    const int lane = threadIdx.x & 63, chunks = p.k / 16;
+    uint4 wv[U][NT][2], av[U][2];
+    float sa[U], sw[U][NT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int b = min(b0 + u * step, p.kb - 1);  // past the last block: it again, which counts for nothing
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int c = 8 * b + 4 * h + (lane >> 4);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                wv[u][j][h] = load_stream16(w[j] + (c < chunks ? 16 * c : 0));
+            }
+            av[u][h] = make_uint4(0, 0, 0, 0);
+            if (live && c < chunks) {
+                av[u][h] = *reinterpret_cast<const uint4*>(a + 16 * c);
+            }
+        }
+        sa[u] = live && b0 + u * step < p.kb ? a_scale[b] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            sw[u][j] = w_scale[j][b];
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        Operand<true> rows;
+        rows.set(av[u][0], av[u][1]);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            Operand<true> weights;
+            weights.set(wv[u][j][0], wv[u][j][1]);
+            take(acc[j], block_sum(weights, rows), sa[u] * sw[u][j]);
+        }
+    }
+}
+
+template <int NT, int WAVES, int U>
+__global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(Fp8Product p) {
+    constexpr int CN = 16 * NT;
+    __shared__ floatx4 sums[WAVES][NT][64];
+    Tile t;
+    if (!find_tile(p, 16, (p.n + CN - 1) / CN, t)) {
+        return;
+    }
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+    const int m = t.mt * 16 + (lane & 15), n0 = t.nt * CN;
+    const bool live = m < t.rows;
+    const int64_t row = live ? source_row(p, t.first + m) : 0;
+    const uint8_t* w[NT];
+    const float* w_scale[NT];
+    floatx4 acc[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const int n = n0 + 16 * j;
+        w[j] = p.w + (static_cast<int64_t>(t.g) * p.n + min(n + (lane & 15), p.n - 1)) * p.k;
+        w_scale[j] = p.w_scale + (static_cast<int64_t>(t.g) * p.nb + min(n, p.n - 1) / kFp8Block) * p.kb;
+        acc[j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    for (int b0 = wave; b0 < p.kb; b0 += WAVES * U) {
+        stream_blocks<NT, U>(p, b0, WAVES, p.a + row * p.k, p.a_scale + row * p.kb, live, w, w_scale, acc);
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        sums[wave][j][lane] = acc[j];
+    }
+    __syncthreads();
+    const int n = n0 + 16 * wave + 4 * (lane >> 4);
+    if (wave < NT && live && n < p.n) {
+        floatx4 v = sums[0][wave][lane];
+#pragma unroll
+        for (int i = 1; i < WAVES; ++i) {
+            v += sums[i][wave][lane];
+        }
+        const int64_t to = target_row(p, t.first + m);
+        if (to >= 0) {
+            store4(p, to, n, v);
+        }
+    }
+}
+
+// Row tiles of 16 and workgroups of the kernels of few rows.
+int64_t stream_tiles(const Fp8Product& p, int64_t feature_tiles) {
+    return (p.offsets == nullptr ? (p.rows + 15) / 16 : p.rows / 16 + std::min<int64_t>(p.groups, p.rows)) * feature_tiles;
+}
+
+template <int NT, int WAVES, int U>
+hipError_t launch_stream(const Fp8Product& p, hipStream_t s) {
+    const int64_t tiles = stream_tiles(p, (p.n + 16 * NT - 1) / (16 * NT));
+    if (tiles > (1 << 20)) {
+        return hipErrorInvalidValue;
+    }
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(fp8_stream_kernel<NT, WAVES, U>),
+                       dim3(static_cast<unsigned>(round_up(tiles, kXcds))), dim3(64 * WAVES), 0, s, p);
+    return hipGetLastError();
+}
+
+// out = the shares' sums, added up in order.
+__global__ __launch_bounds__(256) void fp8_join_kernel(Fp8Product p, const float* __restrict__ sums, int64_t count,
+                                                       int32_t shares) {
+    const int64_t at = 4 * (blockIdx.x * int64_t{256} + threadIdx.x);
+    if (at >= count) {
+        return;
+    }
+    // rows follow each other without a gap: a row of all values, cut in fours
+    p.n = static_cast<int32_t>(min(count - at, int64_t{4}));
+    floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < shares; ++i) {
+        const float* const from = sums + i * count + at;
+        if (p.n == 4 && count % 4 == 0) {
+            v += *reinterpret_cast<const floatx4*>(from);
+        } else {
+            for (int u = 0; u < p.n; ++u) {
+                v[u] += from[u];
+            }
+        }
+    }
+    p.out = static_cast<char*>(p.out) + at * (p.out_dtype == LM_DT_F32 ? 4 : 2);
+    store4(p, 0, 0, v);
+}
+
+// ---- which kernel ----
+
+// What a tile costs, in microseconds (measured with operands that lie in the
+// L2s, 2048 and 8192 reduced channels): a stage where at most half the places of
+// workgroups are taken and where all are, and what is no stage's (finding the
+// tile, its first loads, its outputs). Up to 128 x 128 two workgroups share a CU.
+struct TileCost {
+    int bm, bn, places;
+    float solo, full, fixed;
+};
+constexpr TileCost kFp8Tiles[] = {{32, 128, 512, 0.29f, 0.49f, 1.5f},
+                                  {64, 128, 512, 0.38f, 0.72f, 3.0f},
+                                  {128, 128, 512, 0.85f, 1.13f, 4.0f},
+                                  {128, 256, 256, 0.80f, 1.04f, 6.0f},
+                                  {256, 256, 256, 1.54f, 1.88f, 8.0f}};
+constexpr TileCost kExactTiles[] = {{32, 128, 512, 0.41f, 0.69f, 1.5f},
+                                    {64, 128, 512, 0.59f, 1.15f, 3.0f},
+                                    {128, 128, 512, 1.13f, 1.90f, 4.0f},
+                                    {128, 256, 256, 1.43f, 1.80f, 6.0f}};
+constexpr TileCost kSwigluTiles[] = {{32, 128, 256, 0.62f, 0.69f, 3.0f},
+                                     {32, 128, 512, 0.87f, 1.22f, 3.0f},
+                                     {64, 128, 256, 0.94f, 1.11f, 4.0f},
+                                     {128, 128, 256, 1.45f, 1.80f, 6.0f}};
+
+// Groups that have rows, at most.
+int64_t active_groups(const Fp8Product& p) { return p.offsets == nullptr ? 1 : std::min<int64_t>(p.groups, p.rows); }
+
+// About how many row tiles there are: the host does not know the groups' sizes,
+// and takes the last tile of each for half full.
+double row_tiles(const Fp8Product& p, int bm) {
+    if (p.offsets == nullptr) {
+        return static_cast<double>((p.rows + bm - 1) / bm);
+    }
+    const double groups = static_cast<double>(active_groups(p));
+    return std::max(groups, static_cast<double>(p.rows) / bm + 0.5 * groups);
+}
+
+double tile_time(const TileCost& c, double tiles, int64_t stages) {
+    const double per = static_cast<double>(stages) * (2.0 * tiles <= c.places ? c.solo : c.full) + c.fixed;
+    return tiles <= c.places ? per : per * (tiles / c.places + 0.5);
+}
+
+// Where tiles leave places empty and the reduced axis is long, several
+// workgroups share a tile's reduced axis, and a second launch joins their sums:
+// that costs 4 us and their way through memory. One row by 16384 x 5120: 25 us in
+// one share, 17 in four; 100 rows by 10944 x 2048: 28 and 15.
+struct TileChoice {
+    int tile = 0;
+    int shares = 1;
+};
+template <size_t N>
+TileChoice choose_tile(const Fp8Product& p, const TileCost (&tiles)[N], bool split) {
+    constexpr int kShares[] = {1, 2, 3, 4, 6, 8, 12};
+    TileChoice best;
+    double least = 1e30;
+    for (size_t i = 0; i < N; ++i) {
+        const TileCost& c = tiles[i];
+        const double count = row_tiles(p, c.bm) * static_cast<double>((p.n + c.bn - 1) / c.bn);
+        for (const int shares : kShares) {
+            const int64_t stages = (p.kb + shares - 1) / shares;
+            double t = tile_time(c, count * shares, stages);
+            if (shares > 1) {
+                const int64_t sums = p.rows * p.n * shares;
+                if (!split || stages < 4 || count * shares > c.places || 4 * sums > kFp8WorkspaceBytes) {
+                    break;
+                }
+                t += 4.0 + 4.0 * static_cast<double>(2 * sums + p.rows * p.n) / 4e6;
+            }
+            if (t < least) {
+                least = t;
+                best = TileChoice{static_cast<int>(i), shares};
+            }
+        }
+    }
+    // every share has a part of the reduced axis
+    const int per = (p.kb + best.shares - 1) / best.shares;
+    best.shares = (p.kb + per - 1) / per;
+    return best;
+}
+
+template <bool EXACT>
+hipError_t launch_gemm_tile(const Fp8Product& p, const TileChoice& c, hipStream_t s) {
+    switch (c.tile) {
+        case 0:
+            return launch_tiles<false, EXACT, 1, 4, 2, 2, 3>(p, s, c.shares);
+        case 1:
+            return launch_tiles<false, EXACT, 1, 4, 4, 2, 3>(p, s, c.shares);
+        case 2:
+            return launch_tiles<false, EXACT, 2, 2, 4, 4, 2>(p, s, c.shares);
+        case 3:
+            return launch_tiles<false, EXACT, 2, 4, 4, 4, 3>(p, s, c.shares);
+        default:
+            if constexpr (!EXACT) {
+                return launch_tiles<false, false, 2, 4, 8, 4, 2>(p, s, c.shares);
+            }
+            return hipErrorInvalidValue;
+    }
+}
+
+// Whether the kernel of few rows is the faster: what its workgroups read, each
+// the weights of its 16 features and its rows, stays under 24 MB. One row by 2048
+// channels and 10944 features (23 MB) 6.1 us, 9.9 in tiles; 8 rows (34 MB) 8.3 and
+// 7.6; six experts of 2048 features (18 MB) 5.8 and 8.7, of 5120 (50 MB) 16 and 12.
+bool streams(const Fp8Product& p) {
+    const int64_t groups = active_groups(p), rows = std::min<int64_t>(16, (p.rows + groups - 1) / groups);
+    const int64_t tiles = stream_tiles(p, (p.n + 15) / 16);
+    return tiles <= 4096 && tiles * p.kb * (16 + rows) * kFp8Block <= (24 << 20);
 }
 
 }  // namespace
 
-hipError_t launch_fp8_gemm(const Fp8Product& p, hipStream_t s) {
-    return p.out_dtype == LM_DT_F32 ? launch_tiles<false, true, 1, 8, 4, 2, 2, 2>(p, s)
-                                    : launch_tiles<false, false, 1, 8, 4, 2, 2, 2>(p, s);
+hipError_t launch_fp8_gemm(const Fp8Product& p, void* workspace, hipStream_t s) {
+    if (streams(p)) {
+        // all of a wave's loads in flight at once where the axis is short, many
+        // waves where it is long (10944 channels: 9.5 us, 11 with four waves)
+        return p.kb <= 12   ? launch_stream<1, 4, 3>(p, s)
+               : p.kb <= 16 ? launch_stream<1, 4, 4>(p, s)
+               : p.kb <= 40 ? launch_stream<1, 8, 2>(p, s)
+                            : launch_stream<1, 16, 2>(p, s);
+    }
+    const bool exact = p.out_dtype == LM_DT_F32, split = p.offsets == nullptr;
+    const TileChoice c = exact ? choose_tile(p, kExactTiles, split) : choose_tile(p, kFp8Tiles, split);
+    Fp8Product q = p;
+    if (c.shares > 1) {
+        q.out = workspace;
+        q.out_dtype = LM_DT_F32;
+    }
+    const hipError_t e = exact ? launch_gemm_tile<true>(q, c, s) : launch_gemm_tile<false>(q, c, s);
+    if (e != hipSuccess || c.shares == 1) {
+        return e;
+    }
+    const int64_t count = p.rows * p.n;
+    hipLaunchKernelGGL(fp8_join_kernel, dim3(static_cast<unsigned>((count + 1023) / 1024)), dim3(256), 0, s, p,
+                       static_cast<const float*>(workspace), count, c.shares);
+    return hipGetLastError();
 }
 
 hipError_t launch_fp8_swiglu(const Fp8Product& p, hipStream_t s) {
-    return launch_tiles<true, true, 1, 8, 4, 2, 2, 2>(p, s);
+    switch (choose_tile(p, kSwigluTiles, false).tile) {
+        case 0:
+            return launch_tiles<true, true, 1, 8, 2, 2, 3>(p, s);
+        case 1:
+            return launch_tiles<true, true, 1, 4, 2, 4, 2>(p, s);
+        case 2:
+            return launch_tiles<true, true, 1, 8, 4, 2, 3>(p, s);
+        default:
+            return launch_tiles<true, true, 2, 4, 4, 4, 3>(p, s);
+    }
 }
 
 }  // namespace lm

@@ -20,6 +20,9 @@ struct Fp8State {
     // Host memory that the grouped kernels write when an index lies outside its
     // range: read without a copy once the stream has drained.
     uint32_t* error = nullptr;
+    // Sums of products whose reduced axis several workgroups share: of a fixed
+    // size, so captured graphs keep its pointer. Calls on the stream take turns.
+    void* workspace = nullptr;
 };
 
 void fp8_release(Fp8State* st) {
@@ -27,6 +30,7 @@ void fp8_release(Fp8State* st) {
         return;
     }
     (void)hipHostFree(st->error);
+    (void)hipFree(st->workspace);
     delete st;
 }
 
@@ -72,15 +76,21 @@ int fp8_state(lm_context* ctx, lm::Fp8State** out) {
         hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
         LM_FP8_HIP(hipStreamIsCapturing(info.stream, &capture));
         if (capture != hipStreamCaptureStatusNone) {
-            return fail(LM_EINVAL, "the context's first FP8 product by groups cannot be captured: call it once before");
+            return fail(LM_EINVAL, "the context's first FP8 product cannot be captured: call one before");
         }
         auto* made = new lm::Fp8State();
-        const hipError_t err = hipHostMalloc(reinterpret_cast<void**>(&made->error), sizeof(uint32_t),
-                                             hipHostMallocMapped | hipHostMallocCoherent);
+        hipError_t err = hipHostMalloc(reinterpret_cast<void**>(&made->error), sizeof(uint32_t),
+                                       hipHostMallocMapped | hipHostMallocCoherent);
+        if (err == hipSuccess) {
+            err = hipMalloc(&made->workspace, lm::kFp8WorkspaceBytes);
+            made->workspace = err == hipSuccess ? made->workspace : nullptr;
+        } else {
+            made->error = nullptr;
+        }
         if (err != hipSuccess) {
             (void)hipGetLastError();  // or the next launch would report it
-            delete made;
-            return fail(LM_ENOMEM, std::string("FP8 products' error word: ") + hipGetErrorString(err));
+            lm::fp8_release(made);
+            return fail(LM_ENOMEM, std::string("FP8 products' error word and workspace: ") + hipGetErrorString(err));
         }
         *made->error = 0;
         st = made;
@@ -243,7 +253,12 @@ int lm_fp8_gemm(lm_context* ctx, const uint8_t* a_dev, const float* a_scale_dev,
     }
     const lm::ContextInfo info = lm::context_info(ctx);
     LM_FP8_HIP(hipSetDevice(info.device));
-    LM_FP8_HIP(lm::launch_fp8_gemm(p, info.stream));
+    lm::Fp8State* st = nullptr;
+    rc = fp8_state(ctx, &st);
+    if (rc != LM_OK) {
+        return rc;
+    }
+    LM_FP8_HIP(lm::launch_fp8_gemm(p, st->workspace, info.stream));
     return LM_OK;
 } catch (const std::bad_alloc&) {
     return fail(LM_ENOMEM, "host allocation failed");
@@ -300,7 +315,7 @@ int lm_fp8_grouped_gemm(lm_context* ctx, const lm_fp8_groups* groups, const uint
         p.out_rows = out_rows;
         p.out_dtype = out_dtype;
         p.error = st->error;
-        LM_FP8_HIP(lm::launch_fp8_gemm(p, info.stream));
+        LM_FP8_HIP(lm::launch_fp8_gemm(p, st->workspace, info.stream));
         return LM_OK;
     } catch (const std::bad_alloc&) {
         return fail(LM_ENOMEM, "host allocation failed");
