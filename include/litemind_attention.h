@@ -175,7 +175,8 @@ int lm_kv_cache_truncate(lm_context* ctx, int32_t layer, int64_t tokens);
  * then h += FFN(rms_norm(h, post_attention_layernorm)) as lm_stack_forward.
  * Every layer needs its attention weights, input norm, norm and FFN resident.
  * `path` selects the FFN's expert path (as lm_moe_forward) and the attention's
- * projection path (as lm_attention_set_path) of every layer.
+ * projection path (as lm_attention_set_path; LM_PATH_FP8 leaves it to LM_PATH_AUTO)
+ * of every layer.
  * LM_EFULL as lm_attention_forward (hidden_dev is then partly updated). */
 int lm_decoder_forward(lm_context* ctx, int32_t first_layer, int32_t last_layer, float* hidden_dev, int64_t tokens,
                        int64_t position0, int32_t path);

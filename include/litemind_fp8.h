@@ -97,6 +97,22 @@ int lm_fp8_grouped_swiglu(lm_context* ctx, const lm_fp8_groups* groups, const ui
                           int64_t a_rows, const uint8_t* w_dev, const float* w_scale_dev, int64_t inter,
                           int64_t in_features, uint8_t* q_dev, float* scale_dev);
 
+/* ---- the layers' FFNs at one byte a weight ----
+ * After lm_finalize_layer: the layer's experts and shared experts, or its dense
+ * FFN, in FP8 blocks of 128 x 128, from the BF16 weights. LM_PATH_FP8 then runs
+ * the layer in lm_moe_forward, lm_grouped_swiglu, lm_dense_forward,
+ * lm_stack_forward and its graphs, lm_decoder_forward and
+ * lm_paged_decoder_forward: router and weights of the experts as on the other
+ * paths, the FFN's input and activations in blocks of 1 x 128, outputs fp32.
+ * The quantization is what results differ by: a layer's outputs are off by some
+ * 4e-2 of their norm. only = 1 frees the layer's BF16 and fp16 weights (4 bytes a
+ * weight beside FP8's 1: DeepSeek-V2's 236 GB fit one MI355X); the other paths
+ * are LM_ENOTRES then. An upload into the layer ends its FP8 weights until the
+ * next lm_fp8_layer; after only = 1 all its FFN weights are uploaded again. H and
+ * the FFNs' widths in multiples of 16. LM_EINVAL with only = 1 while stack graphs
+ * are alive. */
+int lm_fp8_layer(lm_context* ctx, int32_t layer, int32_t only);
+
 #ifdef __cplusplus
 }
 #endif

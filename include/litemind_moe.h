@@ -61,6 +61,7 @@ typedef struct lm_moe_config {
                             MFMA above */
 #define LM_PATH_GEMV 1  /* fp32-activation weight-streaming kernels */
 #define LM_PATH_MFMA 2  /* fp16-operand MFMA grouped GEMM, fp32 accumulate */
+#define LM_PATH_FP8 3   /* FP8 weights and activations (lm_fp8_layer, litemind_fp8.h) */
 #define LM_MFMA_CROSSOVER 2  /* LM_PATH_AUTO: token counts above this take the MFMA path */
 #define LM_DECODE_TOKENS 3   /* LM_PATH_AUTO: token counts up to this take the single-token kernel per token */
 

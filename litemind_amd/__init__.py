@@ -16,7 +16,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "liblitemind_moe.so")
 
 LM_OK = 0
-PATH_AUTO, PATH_GEMV, PATH_MFMA = 0, 1, 2
+PATH_AUTO, PATH_GEMV, PATH_MFMA, PATH_FP8 = 0, 1, 2, 3
 MFMA_CROSSOVER = 2  # LM_MFMA_CROSSOVER: PATH_AUTO takes the MFMA path above this many tokens
 DECODE_TOKENS = 3  # LM_DECODE_TOKENS: LM_PATH_AUTO runs up to this many tokens one at a time on the single-token kernel
 OP_DOT, OP_AXPY, OP_SOFTMAX, OP_SILU_MUL, OP_RMS_NORM, OP_WIDEN = range(6)
@@ -214,6 +214,7 @@ PROTOTYPES = {
     "lm_paged_forward": [_P, _I32, _P, _P, _P, _I32],
     "lm_paged_decoder_forward": [_P, _I32, _I32, _P, _P, _I32],
     "lm_sample": [_P, _P, _I64, _I64, _I64, _P, _P, _P, _P],
+    "lm_fp8_layer": [_P, _I32, _I32],
     "lm_fp8_quantize": [_P, _P, _I32, _I64, _I64, _I64, _I32, _P, _P],
     "lm_fp8_gemm": [_P, _P, _P, _I64, _P, _P, _I64, _I64, _P, _I32],
     "lm_fp8_grouped_gemm": [_P, _P, _P, _P, _I64, _P, _P, _I64, _I64, _P, _I64, _I32],
@@ -599,6 +600,10 @@ class Context:
                                        _ptr(uniform), _ptr(token), _ptr(probability)))
 
     # ---- products in 8-bit floating point (include/litemind_fp8.h) ----
+    def fp8_layer(self, layer: int, only: bool = False) -> None:
+        """A finalized layer's FFN in FP8 for PATH_FP8; `only` frees its other weights (lm_fp8_layer)."""
+        self._check(self.lib.lm_fp8_layer(self.handle, layer, int(only)))
+
     def fp8_quantize(self, x, rows: int, width: int, q, scale, dtype: int = DT_F32, row_stride: int = 0,
                      block_rows: int = 1) -> None:
         """Rows (block_rows 1) or a matrix (128) as e4m3 codes and a scale per block (lm_fp8_quantize)."""

@@ -19,6 +19,7 @@ struct Fp8Rows {
     int32_t dtype;  // LM_DT_F32, LM_DT_F16 or LM_DT_BF16
     int64_t rows, width, stride;
     int32_t block_rows;  // 1 or 128
+    int32_t group;       // of a matrix: 0, or its rows lie in groups of so many, with as many others between
     uint8_t* q;
     float* scale;
 };
@@ -75,6 +76,13 @@ __device__ inline float fp8_magnitude(float x) { return x - x == 0.0f ? __builti
 struct Fp8State;
 Fp8State*& context_fp8(lm_context* ctx);
 void fp8_release(Fp8State* st);
+// What products need of the context, made at its first call (not while the stream
+// is being captured).
+struct Fp8Scratch {
+    uint32_t* error;
+    void* workspace;
+};
+int fp8_scratch(lm_context* ctx, Fp8Scratch* out);
 // LM_EKERNEL, once, where a kernel met an index outside its range.
 int fp8_check_error(lm_context* ctx);
 

@@ -108,8 +108,9 @@ __global__ __launch_bounds__(256) void fp8_matrix_kernel(Fp8Rows a, bool vec, in
     float most = 0.0f;
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
-        const int64_t r = r0 + 16 * p;
-        load8(static_cast<const T*>(a.x) + (r < a.rows ? r : a.rows - 1) * a.stride, c0, a.width, vec, v[p]);
+        const int64_t r = min(r0 + 16 * p, a.rows - 1);
+        const int64_t at = a.group == 0 ? r : r / a.group * (2 * a.group) + r % a.group;
+        load8(static_cast<const T*>(a.x) + at * a.stride, c0, a.width, vec, v[p]);
     }
 #pragma unroll
     for (int p = 0; p < 8; ++p) {

@@ -1515,8 +1515,8 @@ int lm_decoder_forward(lm_context* ctx, int32_t first_layer, int32_t last_layer,
             }
             float* xn = st->xn;
             for (int32_t l = first_layer; l <= last_layer && rc == LM_OK; ++l) {
-                rc = attention_tokens(st, info.stream, l, hidden_dev, F, position0, hidden_dev, 1, path,
-                                      st->layers[l].input_norm, xn);
+                rc = attention_tokens(st, info.stream, l, hidden_dev, F, position0, hidden_dev, 1,
+                                      path == LM_PATH_FP8 ? LM_PATH_AUTO : path, st->layers[l].input_norm, xn);
                 if (rc == LM_OK) {
                     rc = lm::ffn_sublayer(ctx, l, hidden_dev, F, path);
                 }

@@ -68,6 +68,22 @@ constexpr int64_t kMfmaCrossover = LM_MFMA_CROSSOVER;
 // 3 x 33.8 against 129.8 us on the MFMA path at T = 3 (about even at T = 4).
 constexpr int64_t kDecodeTokens = LM_DECODE_TOKENS;
 
+// One FFN, or all routed experts of a layer, in FP8 blocks (lm_fp8_layer).
+struct Fp8Ffn {
+    uint8_t* gate_up = nullptr;   // [experts][2][inter][H]
+    float* gate_up_scale = nullptr;
+    uint8_t* down = nullptr;      // [experts][H][inter]
+    float* down_scale = nullptr;
+};
+
+struct Fp8Layer {
+    void* slab = nullptr;
+    size_t bytes = 0;
+    Fp8Ffn routed;
+    Fp8Ffn other;        // the shared experts, or the dense FFN
+    bool ready = false;  // holds the weights uploaded last
+};
+
 struct Layer {
     bool allocated = false;
     bool dense = false;
@@ -83,6 +99,7 @@ struct Layer {
     std::vector<unsigned char> expert_present;
     bool shared_present = false;
     void** table = nullptr;            // device: gu[E+1], down[E+1], gu_h[E+1], down_h[E+1]
+    Fp8Layer fp8;                      // LM_PATH_FP8's weights
 };
 
 struct Workspace {
@@ -108,6 +125,13 @@ struct Workspace {
     uint32_t* spec_sync = nullptr;   // speculative router + gate/up launches: counters, tags, partial logits (zeroed once)
     uint32_t* ticket = nullptr;      // single-token router arrival counter (kept at 0 between launches)
     int32_t* permute_scratch = nullptr;  // segment counts and arrival ticket of the permutation
+    // LM_PATH_FP8: the tokens' codes and scales, and the activations'
+    void* fp8_slab = nullptr;
+    int64_t fp8_tokens = 0;
+    uint8_t* fp8_x = nullptr;
+    float* fp8_x_scale = nullptr;
+    uint8_t* fp8_act = nullptr;
+    float* fp8_act_scale = nullptr;
 };
 
 struct EventSet {
@@ -529,18 +553,140 @@ int launch_expert_kernels(lm_context* ctx, const Layer& L, const lm::ExpertArgs&
     return LM_OK;
 }
 
+// The FP8 path's buffers for `tokens` tokens.
+int ensure_fp8_workspace(lm_context* ctx, int64_t tokens) {
+    Workspace& w = ctx->ws;
+    if (w.fp8_tokens >= tokens) {
+        return LM_OK;
+    }
+    if (ctx->graphs > 0) {
+        return fail(LM_EINVAL, "a captured stack graph holds the workspace (FP8: sized for " + std::to_string(w.fp8_tokens) +
+                                   " tokens); destroy it before a call with " + std::to_string(tokens));
+    }
+    LM_HIP(hipStreamSynchronize(ctx->stream));
+    const int64_t T = tokens, TK = T * ctx->K, other = std::max(ctx->S, ctx->D);
+    const int64_t x = T * ctx->H, x_scale = 4 * T * lm::fp8_blocks(ctx->H);
+    const int64_t act = TK * ctx->I + T * other;
+    const int64_t act_scale = 4 * (TK * lm::fp8_blocks(ctx->I) + T * lm::fp8_blocks(other));
+    auto padded = [](int64_t bytes) { return (bytes + 255) / 256 * 256; };
+    LM_HIP(hipFree(w.fp8_slab));
+    w.fp8_slab = nullptr;
+    w.fp8_tokens = 0;
+    if (const hipError_t err = hipMalloc(&w.fp8_slab, static_cast<size_t>(padded(x) + padded(x_scale) + padded(act) + act_scale));
+        err != hipSuccess) {
+        w.fp8_slab = nullptr;
+        (void)hipGetLastError();  // or the next launch would report it
+        return fail(LM_ENOMEM, std::string("FP8 workspace: ") + hipGetErrorString(err));
+    }
+    char* next = static_cast<char*>(w.fp8_slab);
+    w.fp8_x = reinterpret_cast<uint8_t*>(next);
+    w.fp8_x_scale = reinterpret_cast<float*>(next += padded(x));
+    w.fp8_act = reinterpret_cast<uint8_t*>(next += padded(x_scale));
+    w.fp8_act_scale = reinterpret_cast<float*>(next += padded(act));
+    w.fp8_tokens = tokens;
+    return LM_OK;
+}
+
+// Both products of one FFN in FP8: `first` and `count` the rows of its
+// activations and outputs (slots of routed experts in permuted order, then the
+// shared experts' rows or the dense FFN's).
+int fp8_ffn(lm_context* ctx, const Fp8Ffn& f, int64_t inter, int64_t T, const lm::RouteBufs* rb, uint8_t* act,
+            float* act_scale, float* down_out, const lm::Fp8Scratch& sc, bool down) {
+    const Workspace& w = ctx->ws;
+    lm::Fp8Product p{};
+    p.groups = rb != nullptr ? ctx->E : 1;
+    p.rows = rb != nullptr ? T * ctx->K : T;
+    p.offsets = rb != nullptr ? rb->offsets : nullptr;
+    p.error = sc.error;
+    if (!down) {
+        p.a = w.fp8_x;
+        p.a_scale = w.fp8_x_scale;
+        p.a_rows = T;
+        p.w = f.gate_up;
+        p.w_scale = f.gate_up_scale;
+        p.n = static_cast<int32_t>(inter);
+        p.k = ctx->H;
+        p.source = rb != nullptr ? rb->perm : nullptr;
+        p.divisor = rb != nullptr ? ctx->K : 0;
+        p.q = act;
+        p.q_scale = act_scale;
+    } else {
+        p.a = act;
+        p.a_scale = act_scale;
+        p.a_rows = p.rows;
+        p.w = f.down;
+        p.w_scale = f.down_scale;
+        p.n = ctx->H;
+        p.k = static_cast<int32_t>(inter);
+        p.out = down_out;
+        p.out_rows = p.rows;
+        p.out_dtype = LM_DT_F32;
+    }
+    p.nb = static_cast<int32_t>(lm::fp8_blocks(p.n));
+    p.kb = static_cast<int32_t>(lm::fp8_blocks(p.k));
+    LM_HIP(down ? lm::launch_fp8_gemm(p, sc.workspace, ctx->stream) : lm::launch_fp8_swiglu(p, ctx->stream));
+    return LM_OK;
+}
+
+// launch_expert_kernels in FP8: the tokens' blocks, gate/up and down of the
+// routed experts and of the shared (or dense) FFN into ws.down_out.
+int launch_expert_kernels_fp8(lm_context* ctx, const Layer& L, const float* x, int64_t T, const lm::RouteBufs& rb) {
+    lm::Fp8Scratch sc{};
+    int rc = lm::fp8_scratch(ctx, &sc);
+    if (rc != LM_OK) {
+        return rc;
+    }
+    const Workspace& w = ctx->ws;
+    const int64_t TK = L.dense ? 0 : T * ctx->K, inter = L.dense ? ctx->D : ctx->S;
+    uint8_t* const other_act = w.fp8_act + TK * ctx->I;
+    float* const other_scale = w.fp8_act_scale + TK * lm::fp8_blocks(ctx->I);
+    stage_mark(ctx, 2);
+    LM_HIP(lm::launch_fp8_quantize(
+        lm::Fp8Rows{x, LM_DT_F32, T, ctx->H, ctx->H, 1, 0, w.fp8_x, w.fp8_x_scale}, ctx->stream));
+    for (const bool down : {false, true}) {
+        if (down) {
+            stage_mark(ctx, 3);
+        }
+        if (!L.dense) {
+            rc = fp8_ffn(ctx, L.fp8.routed, ctx->I, T, &rb, w.fp8_act, w.fp8_act_scale, w.down_out, sc, down);
+        }
+        if (rc == LM_OK && L.fp8.other.gate_up != nullptr) {
+            rc = fp8_ffn(ctx, L.fp8.other, inter, T, nullptr, other_act, other_scale, w.down_out + TK * ctx->H, sc, down);
+        }
+        if (rc != LM_OK) {
+            return rc;
+        }
+    }
+    return LM_OK;
+}
+
+// Whether a layer can run `path`.
+int check_path(const lm_context* ctx, int32_t layer, int32_t path) {
+    const Layer& L = ctx->layers[static_cast<size_t>(layer)];
+    if (path == LM_PATH_FP8 && !L.fp8.ready) {
+        return fail(LM_ENOTRES, "layer " + std::to_string(layer) + " has no FP8 weights (lm_fp8_layer)");
+    }
+    if (path != LM_PATH_FP8 && !L.finalized && L.fp8.ready && !L.allocated) {
+        return fail(LM_ENOTRES, "layer " + std::to_string(layer) + " holds FP8 weights alone (LM_PATH_FP8)");
+    }
+    return LM_OK;
+}
+
 // Expert kernels + combine for a layer whose routing is in rb (or a dense FFN).
 // next_norm: the next stack layer's RMSNorm weight; the combine then also
 // writes that layer's input (ws.xnorm, and ws.x16 when the MFMA path follows).
 int run_experts(lm_context* ctx, Layer& L, const float* x, const _Float16* x16, int64_t T, const lm::RouteBufs& rb,
-                float* y, const float* residual, bool mfma, const float* next_norm = nullptr,
+                float* y, const float* residual, bool mfma, bool fp8, const float* next_norm = nullptr,
                 bool gateup_done = false) {
     lm::ExpertArgs ea = expert_args(ctx, L, x, x16, T, rb);
+    if (fp8) {
+        ea.has_shared = L.fp8.other.gate_up != nullptr ? 1 : 0;
+    }
     ea.ksplit = mfma ? lm::mfma_shared_chunks(ea) : 1;
     if (T * (ea.top_k + (ea.has_shared ? ea.ksplit : 0)) > ctx->ws.down_rows) {
         return fail(LM_EINVAL, "the down projection's rows exceed the workspace");
     }
-    const int rc = launch_expert_kernels(ctx, L, ea, T, mfma, gateup_done);
+    const int rc = fp8 ? launch_expert_kernels_fp8(ctx, L, x, T, rb) : launch_expert_kernels(ctx, L, ea, T, mfma, gateup_done);
     if (rc != LM_OK) {
         return rc;
     }
@@ -577,7 +723,7 @@ bool decode_eligible(const lm_context* ctx, const Layer& L) {
 // True when lm_moe_forward runs T tokens of this MoE layer through the
 // single-token kernel (one launch per token) rather than the batched path.
 bool takes_decode_path(const lm_context* ctx, const Layer& L, int64_t T, int32_t path) {
-    return (T == 1 && !want_mfma(path, T) && decode_eligible(ctx, L)) ||
+    return (T == 1 && !want_mfma(path, T) && path != LM_PATH_FP8 && decode_eligible(ctx, L)) ||
            (path == LM_PATH_AUTO && T <= kDecodeTokens && decode_eligible(ctx, L));
 }
 
@@ -718,14 +864,22 @@ int moe_layer(lm_context* ctx, int32_t layer, const float* x, int64_t T, float* 
               const float* bias, int32_t* idx_out, float* w_out, float* logits_out, int32_t path,
               const float* norm = nullptr, const float* next_norm = nullptr, bool prenormed = false) {
     Layer& L = ctx->layers[static_cast<size_t>(layer)];
-    if (!L.allocated || L.dense || L.router_t == nullptr) {
+    const bool fp8 = path == LM_PATH_FP8;
+    int rc = check_path(ctx, layer, path);
+    if (rc != LM_OK) {
+        return rc;
+    }
+    if ((!fp8 && !L.allocated) || L.dense || L.router_t == nullptr) {
         return fail(LM_ENOTRES, "layer " + std::to_string(layer) + " has no resident MoE weights");
     }
-    if (!L.finalized) {
+    if (!fp8 && !L.finalized) {
         return fail(LM_ENOTRES, "layer " + std::to_string(layer) + " is not finalized (lm_finalize_layer)");
     }
     const bool mfma = want_mfma(path, T);
-    int rc = ensure_workspace(ctx, T);
+    rc = ensure_workspace(ctx, T);
+    if (rc == LM_OK && fp8) {
+        rc = ensure_fp8_workspace(ctx, T);
+    }
     if (rc != LM_OK) {
         return rc;
     }
@@ -785,7 +939,7 @@ int moe_layer(lm_context* ctx, int32_t layer, const float* x, int64_t T, float* 
     stage_mark(ctx, 0);
     bool permuted = false;
     bool speculated = false;
-    rc = spec_router_gateup(ctx, L, ra, T, mfma, &speculated);
+    rc = fp8 ? LM_OK : spec_router_gateup(ctx, L, ra, T, mfma, &speculated);
     if (rc != LM_OK) {
         return rc;
     }
@@ -807,7 +961,7 @@ int moe_layer(lm_context* ctx, int32_t layer, const float* x, int64_t T, float* 
         LM_HIP(lm::launch_permute(pa, ctx->stream));
     }
 
-    rc = run_experts(ctx, L, x, ctx->ws.x16, T, pa.rb, y, residual, mfma, next_norm, speculated);
+    rc = run_experts(ctx, L, x, ctx->ws.x16, T, pa.rb, y, residual, mfma, fp8, next_norm, speculated);
     if (rc != LM_OK) {
         return rc;
     }
@@ -817,11 +971,19 @@ int moe_layer(lm_context* ctx, int32_t layer, const float* x, int64_t T, float* 
 int dense_layer(lm_context* ctx, int32_t layer, const float* x, int64_t T, float* y, const float* residual,
                 int32_t path, const float* next_norm = nullptr, bool prenormed = false) {
     Layer& L = ctx->layers[static_cast<size_t>(layer)];
-    if (!L.allocated || !L.dense || !L.finalized) {
+    const bool fp8 = path == LM_PATH_FP8;
+    int rc = check_path(ctx, layer, path);
+    if (rc != LM_OK) {
+        return rc;
+    }
+    if (!L.dense || (!fp8 && (!L.allocated || !L.finalized))) {
         return fail(LM_ENOTRES, "layer " + std::to_string(layer) + " has no finalized dense FFN");
     }
     const bool mfma = want_mfma(path, T);
-    int rc = ensure_workspace(ctx, T);
+    rc = ensure_workspace(ctx, T);
+    if (rc == LM_OK && fp8) {
+        rc = ensure_fp8_workspace(ctx, T);
+    }
     if (rc != LM_OK) {
         return rc;
     }
@@ -838,7 +1000,7 @@ int dense_layer(lm_context* ctx, int32_t layer, const float* x, int64_t T, float
     rb.wt = ctx->ws.wts;
     stage_mark(ctx, 0);
     stage_mark(ctx, 1);
-    rc = run_experts(ctx, L, x, ctx->ws.x16, T, rb, y, residual, mfma, next_norm);
+    rc = run_experts(ctx, L, x, ctx->ws.x16, T, rb, y, residual, mfma, fp8, next_norm);
     if (rc != LM_OK) {
         return rc;
     }
@@ -1038,7 +1200,7 @@ int ffn_sublayer_fused(lm_context* ctx, int32_t l, float* hidden, int64_t T, int
 // combine can hand the next layer its normalised input).
 bool batched_layer(const lm_context* ctx, int32_t l, int64_t T, int32_t path) {
     const Layer& L = ctx->layers[static_cast<size_t>(l)];
-    if (!L.allocated || !L.finalized || L.norm == nullptr) {
+    if (!(path == LM_PATH_FP8 ? L.fp8.ready : L.allocated && L.finalized) || L.norm == nullptr) {
         return false;  // the layer reports its own error
     }
     return L.dense || (L.router_t != nullptr && !takes_decode_path(ctx, L, T, path));
@@ -1055,13 +1217,21 @@ int lm::ffn_ready(lm_context* ctx, int32_t l, int64_t T, int32_t path) {
     if (L.norm == nullptr) {
         return fail(LM_ENOTRES, "layer " + std::to_string(l) + " has no norm weight");
     }
-    if (!L.allocated || (!L.dense && L.router_t == nullptr)) {
+    const bool fp8 = path == LM_PATH_FP8;
+    int rc = check_path(ctx, l, path);
+    if (rc != LM_OK) {
+        return rc;
+    }
+    if ((!fp8 && !L.allocated) || (!L.dense && L.router_t == nullptr)) {
         return fail(LM_ENOTRES, "layer " + std::to_string(l) + " has no resident FFN weights");
     }
-    if (!L.finalized) {
+    if (!fp8 && !L.finalized) {
         return fail(LM_ENOTRES, "layer " + std::to_string(l) + " is not finalized (lm_finalize_layer)");
     }
-    const int rc = ensure_workspace(ctx, T);
+    rc = ensure_workspace(ctx, T);
+    if (rc == LM_OK && fp8) {
+        rc = ensure_fp8_workspace(ctx, T);
+    }
     if (rc != LM_OK || L.dense || !takes_decode_path(ctx, L, T, path)) {
         return rc;
     }
@@ -1172,9 +1342,11 @@ int lm_context_destroy(lm_context* ctx) {
         (void)hipFree(L.norm);
         (void)hipFree(L.slab);
         (void)hipFree(L.table);
+        (void)hipFree(L.fp8.slab);
     }
     Workspace& w = ctx->ws;
     (void)hipFree(w.slab);
+    (void)hipFree(w.fp8_slab);
     for (auto& kv : ctx->resident_ptrs) {
         (void)hipFree(kv.second.dev);
     }
@@ -1330,6 +1502,7 @@ int lm_upload_expert(lm_context* ctx, int32_t layer, int32_t expert, const uint1
     if (rc == LM_OK) {
         L.expert_present[static_cast<size_t>(expert)] = 1;
         L.finalized = false;
+        L.fp8.ready = false;
     }
     return rc;
     LM_GUARD_END
@@ -1360,6 +1533,7 @@ int lm_upload_shared(lm_context* ctx, int32_t layer, const uint16_t* gate_host, 
     if (rc == LM_OK) {
         L.shared_present = true;
         L.finalized = false;
+        L.fp8.ready = false;
     }
     return rc;
     LM_GUARD_END
@@ -1389,6 +1563,7 @@ int lm_upload_dense(lm_context* ctx, int32_t layer, const uint16_t* gate_host, c
     rc = upload_ffn(ctx, L.dense_ffn, gate_host, up_host, down_host);
     if (rc == LM_OK) {
         L.finalized = false;
+        L.fp8.ready = false;
     }
     return rc;
     LM_GUARD_END
@@ -1558,6 +1733,115 @@ int lm_finalize_layer(lm_context* ctx, int32_t layer) {
     LM_GUARD_END
 }
 
+int lm_fp8_layer(lm_context* ctx, int32_t layer, int32_t only) {
+    LM_GUARD_BEGIN
+    int rc = check_layer(ctx, layer);
+    if (rc != LM_OK) {
+        return rc;
+    }
+    Layer& L = ctx->layers[static_cast<size_t>(layer)];
+    if (only != 0 && only != 1) {
+        return fail(LM_EINVAL, "only must be 0 or 1");
+    }
+    if (!L.allocated || !L.finalized) {
+        return fail(LM_ENOTRES, "layer " + std::to_string(layer) + " is not finalized (lm_finalize_layer)");
+    }
+    if (only == 1 && ctx->graphs > 0) {
+        return fail(LM_EINVAL, "a captured stack graph may hold the layer's weights; destroy it before they are freed");
+    }
+    const bool shared = !L.dense && L.shared_present;
+    const int64_t H = ctx->H, E = L.dense ? 0 : ctx->E, I = ctx->I, O = L.dense ? ctx->D : shared ? ctx->S : 0;
+    if (H % 16 != 0 || (E > 0 && I % 16 != 0) || O % 16 != 0) {
+        return fail(LM_EINVAL, "FP8 weights need widths in multiples of 16");
+    }
+    rc = set_device(ctx);
+    lm::Fp8Scratch sc{};
+    if (rc == LM_OK) {
+        rc = lm::fp8_scratch(ctx, &sc);
+    }
+    if (rc != LM_OK) {
+        return rc;
+    }
+    const int64_t hb = lm::fp8_blocks(H), ib = lm::fp8_blocks(I), ob = lm::fp8_blocks(O);
+    auto padded = [](int64_t bytes) { return (bytes + 255) / 256 * 256; };
+    const int64_t sizes[8] = {padded(E * 2 * I * H), padded(4 * E * 2 * ib * hb), padded(E * H * I), padded(4 * E * hb * ib),
+                              padded(2 * O * H),     padded(4 * 2 * ob * hb),     padded(H * O),     padded(4 * hb * ob)};
+    int64_t total = 0;
+    for (const int64_t bytes : sizes) {
+        total += bytes;
+    }
+    Fp8Layer& f = L.fp8;
+    f.ready = false;
+    if (f.slab == nullptr || f.bytes != static_cast<size_t>(total)) {
+        if (f.slab != nullptr && ctx->graphs > 0) {
+            return fail(LM_EINVAL, "a captured stack graph holds the layer's FP8 weights of another size");
+        }
+        LM_HIP(hipStreamSynchronize(ctx->stream));
+        LM_HIP(hipFree(f.slab));
+        ctx->resident -= f.bytes;
+        f = Fp8Layer{};
+        if (const hipError_t err = hipMalloc(&f.slab, static_cast<size_t>(total)); err != hipSuccess) {
+            f.slab = nullptr;
+            (void)hipGetLastError();  // or the next launch would report it
+            return fail(LM_ENOMEM, "FP8 weights of " + std::to_string(total) + " bytes: " + hipGetErrorString(err));
+        }
+        f.bytes = static_cast<size_t>(total);
+        ctx->resident += f.bytes;
+    }
+    char* next = static_cast<char*>(f.slab);
+    char* at[8];
+    for (int i = 0; i < 8; ++i) {
+        at[i] = next;
+        next += sizes[i];
+    }
+    auto ffn = [&](int i, int64_t inter) {
+        return inter == 0 ? Fp8Ffn{}
+                          : Fp8Ffn{reinterpret_cast<uint8_t*>(at[i]), reinterpret_cast<float*>(at[i + 1]),
+                                   reinterpret_cast<uint8_t*>(at[i + 2]), reinterpret_cast<float*>(at[i + 3])};
+    };
+    f.routed = ffn(0, E * I);
+    f.other = ffn(4, O);
+    // gate and up rows are interleaved in groups of kGroupRows in the resident layout
+    auto quantize = [&](const lm::FfnDev& from, const Fp8Ffn& to, int64_t e, int64_t inter) {
+        const int64_t nb = lm::fp8_blocks(inter);
+        for (int64_t part = 0; part < 2; ++part) {
+            const hipError_t err = lm::launch_fp8_quantize(
+                lm::Fp8Rows{from.gu + part * lm::kGroupRows * ctx->Hp, LM_DT_BF16, inter, H, ctx->Hp, lm::kFp8Block,
+                            lm::kGroupRows, to.gate_up + (2 * e + part) * inter * H, to.gate_up_scale + (2 * e + part) * nb * hb},
+                ctx->stream);
+            if (err != hipSuccess) {
+                return err;
+            }
+        }
+        return lm::launch_fp8_quantize(lm::Fp8Rows{from.down, LM_DT_BF16, H, inter, from.inter_p, lm::kFp8Block, 0,
+                                                   to.down + e * H * inter, to.down_scale + e * hb * nb},
+                                       ctx->stream);
+    };
+    for (int64_t e = 0; e < E; ++e) {
+        LM_HIP(quantize(L.experts[static_cast<size_t>(e)], f.routed, e, I));
+    }
+    if (O > 0) {
+        LM_HIP(quantize(L.dense ? L.dense_ffn : L.shared, f.other, 0, O));
+    }
+    if (only == 1) {
+        LM_HIP(hipStreamSynchronize(ctx->stream));
+        LM_HIP(hipFree(L.slab));
+        ctx->resident -= L.slab_bytes;
+        L.slab = nullptr;
+        L.slab_bytes = 0;
+        L.allocated = false;
+        L.finalized = false;
+        L.shared_present = false;
+        L.experts.clear();
+        L.expert_present.clear();
+        L.shared = lm::FfnDev{};
+        L.dense_ffn = lm::FfnDev{};
+    }
+    f.ready = true;
+    return LM_OK;
+    LM_GUARD_END
+}
+
 int lm_layer_fp16_inexact(lm_context* ctx, int32_t layer, int64_t* out_count) {
     LM_GUARD_BEGIN
     int rc = check_layer(ctx, layer);
@@ -1595,7 +1879,7 @@ int lm_moe_forward(lm_context* ctx, int32_t layer, const float* x_dev, int64_t t
     if (tokens < 0 || (tokens > 0 && (x_dev == nullptr || y_dev == nullptr))) {
         return fail(LM_EINVAL, "bad token count or null x / y");
     }
-    if (path < LM_PATH_AUTO || path > LM_PATH_MFMA) {
+    if (path < LM_PATH_AUTO || path > LM_PATH_FP8) {
         return fail(LM_EINVAL, "unknown path");
     }
     if (tokens == 0) {
@@ -1787,11 +2071,16 @@ int lm_grouped_swiglu(lm_context* ctx, int32_t layer, const float* x_dev, int64_
     if (tokens < 0 || (tokens > 0 && (x_dev == nullptr || topk_index_dev == nullptr || out_dev == nullptr))) {
         return fail(LM_EINVAL, "bad token count or null x / topk_index / out");
     }
-    if (path < LM_PATH_AUTO || path > LM_PATH_MFMA) {
+    if (path < LM_PATH_AUTO || path > LM_PATH_FP8) {
         return fail(LM_EINVAL, "unknown path");
     }
     Layer& L = ctx->layers[static_cast<size_t>(layer)];
-    if (!L.allocated || L.dense || L.router_t == nullptr || !L.finalized) {
+    const bool fp8 = path == LM_PATH_FP8;
+    rc = check_path(ctx, layer, path);
+    if (rc != LM_OK) {
+        return rc;
+    }
+    if (L.dense || L.router_t == nullptr || (!fp8 && (!L.allocated || !L.finalized))) {
         return fail(LM_ENOTRES, "layer " + std::to_string(layer) + " has no finalized MoE weights");
     }
     if (tokens == 0) {
@@ -1800,6 +2089,9 @@ int lm_grouped_swiglu(lm_context* ctx, int32_t layer, const float* x_dev, int64_
     rc = set_device(ctx);
     if (rc == LM_OK) {
         rc = ensure_workspace(ctx, tokens);
+    }
+    if (rc == LM_OK && fp8) {
+        rc = ensure_fp8_workspace(ctx, tokens);
     }
     if (rc != LM_OK) {
         return rc;
@@ -1838,12 +2130,13 @@ int lm_grouped_swiglu(lm_context* ctx, int32_t layer, const float* x_dev, int64_
         LM_HIP(lm::launch_to_f16_rows(x_dev, ctx->ws.x16, tokens, ctx->H, ctx->Hp, ctx->stream));
     }
     const lm::ExpertArgs ea = expert_args(ctx, L, x_dev, ctx->ws.x16, tokens, rb);
-    rc = launch_expert_kernels(ctx, L, ea, tokens, mfma);
+    rc = fp8 ? launch_expert_kernels_fp8(ctx, L, x_dev, tokens, rb) : launch_expert_kernels(ctx, L, ea, tokens, mfma);
     if (rc != LM_OK) {
         return rc;
     }
+    const int32_t has_shared = fp8 ? (L.fp8.other.gate_up != nullptr ? 1 : 0) : ea.has_shared;
     stage_mark(ctx, 4);
-    LM_HIP(lm::launch_gather_slots(ctx->ws.down_out, rb.slot_of, out_dev, TK, tokens, ctx->H, ea.has_shared,
+    LM_HIP(lm::launch_gather_slots(ctx->ws.down_out, rb.slot_of, out_dev, TK, tokens, ctx->H, has_shared,
                                    ctx->stream));
     stage_mark(ctx, 5);
     return stage_finish(ctx);
@@ -1935,6 +2228,7 @@ struct lm_stack_graph {
     hipGraph_t graph = nullptr;
     hipGraphExec_t exec = nullptr;
     int32_t first = 0, last = -1;
+    int32_t path = LM_PATH_AUTO;
 };
 
 int lm_stack_graph_create(lm_context* ctx, int32_t first_layer, int32_t last_layer, float* hidden_dev,
@@ -1965,6 +2259,9 @@ int lm_stack_graph_create(lm_context* ctx, int32_t first_layer, int32_t last_lay
         }
     }
     rc = ensure_workspace(ctx, tokens);
+    if (rc == LM_OK && path == LM_PATH_FP8) {
+        rc = ensure_fp8_workspace(ctx, tokens);
+    }
     if (rc != LM_OK) {
         return rc;
     }
@@ -1984,7 +2281,7 @@ int lm_stack_graph_create(lm_context* ctx, int32_t first_layer, int32_t last_lay
         (void)hipGraphDestroy(g);
         return fail(LM_EHIP, std::string("stack graph instantiate: ") + hipGetErrorString(inst));
     }
-    *graph = new lm_stack_graph{ctx, g, exec, first_layer, last_layer};
+    *graph = new lm_stack_graph{ctx, g, exec, first_layer, last_layer, path};
     ++ctx->graphs;
     return LM_OK;
     LM_GUARD_END
@@ -1999,9 +2296,11 @@ int lm_stack_graph_launch(lm_stack_graph* graph) {
     // upload into a layer since then (without lm_finalize_layer) leaves its fp16
     // copy stale, which the eager path refuses too.
     for (int32_t l = graph->first; l <= graph->last; ++l) {
-        if (!graph->ctx->layers[static_cast<size_t>(l)].finalized) {
+        const Layer& L = graph->ctx->layers[static_cast<size_t>(l)];
+        if (!(graph->path == LM_PATH_FP8 ? L.fp8.ready : L.finalized)) {
             return fail(LM_ENOTRES, "lm_stack_graph_launch: layer " + std::to_string(l) +
-                                        " was uploaded since the capture and is not finalized (lm_finalize_layer)");
+                                        " was uploaded since the capture and is not finalized (lm_finalize_layer" +
+                                        (graph->path == LM_PATH_FP8 ? ", lm_fp8_layer)" : ")"));
         }
     }
     LM_HIP(hipGraphLaunch(graph->exec, graph->ctx->stream));

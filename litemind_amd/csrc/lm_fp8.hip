@@ -67,38 +67,6 @@ int64_t element_bytes(int32_t dtype) {
     return dtype == LM_DT_F32 ? 4 : dtype == LM_DT_F16 || dtype == LM_DT_BF16 ? 2 : 0;
 }
 
-// The context's FP8 state, made at the first call that needs it (not while the
-// stream is being captured: an allocation would end the capture).
-int fp8_state(lm_context* ctx, lm::Fp8State** out) {
-    lm::Fp8State*& st = lm::context_fp8(ctx);
-    if (st == nullptr) {
-        const lm::ContextInfo info = lm::context_info(ctx);
-        hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
-        LM_FP8_HIP(hipStreamIsCapturing(info.stream, &capture));
-        if (capture != hipStreamCaptureStatusNone) {
-            return fail(LM_EINVAL, "the context's first FP8 product cannot be captured: call one before");
-        }
-        auto* made = new lm::Fp8State();
-        hipError_t err = hipHostMalloc(reinterpret_cast<void**>(&made->error), sizeof(uint32_t),
-                                       hipHostMallocMapped | hipHostMallocCoherent);
-        if (err == hipSuccess) {
-            err = hipMalloc(&made->workspace, lm::kFp8WorkspaceBytes);
-            made->workspace = err == hipSuccess ? made->workspace : nullptr;
-        } else {
-            made->error = nullptr;
-        }
-        if (err != hipSuccess) {
-            (void)hipGetLastError();  // or the next launch would report it
-            lm::fp8_release(made);
-            return fail(LM_ENOMEM, std::string("FP8 products' error word and workspace: ") + hipGetErrorString(err));
-        }
-        *made->error = 0;
-        st = made;
-    }
-    *out = st;
-    return LM_OK;
-}
-
 constexpr int64_t kMost32 = int64_t{1} << 32;
 
 // The sizes of a product: p's n, k, nb, kb, a_rows and rows on success.
@@ -177,6 +145,36 @@ int product_overlap(const lm::Fp8Product& p, int64_t parts, const Range& out, co
 
 }  // namespace
 
+int lm::fp8_scratch(lm_context* ctx, Fp8Scratch* out) {
+    Fp8State*& st = context_fp8(ctx);
+    if (st == nullptr) {
+        const lm::ContextInfo info = context_info(ctx);
+        hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+        LM_FP8_HIP(hipStreamIsCapturing(info.stream, &capture));
+        if (capture != hipStreamCaptureStatusNone) {  // an allocation would end the capture
+            return fail(LM_EINVAL, "the context's first FP8 product cannot be captured: call one before");
+        }
+        auto* made = new Fp8State();
+        hipError_t err = hipHostMalloc(reinterpret_cast<void**>(&made->error), sizeof(uint32_t),
+                                       hipHostMallocMapped | hipHostMallocCoherent);
+        if (err == hipSuccess) {
+            err = hipMalloc(&made->workspace, kFp8WorkspaceBytes);
+            made->workspace = err == hipSuccess ? made->workspace : nullptr;
+        } else {
+            made->error = nullptr;
+        }
+        if (err != hipSuccess) {
+            (void)hipGetLastError();  // or the next launch would report it
+            fp8_release(made);
+            return fail(LM_ENOMEM, std::string("FP8 products' error word and workspace: ") + hipGetErrorString(err));
+        }
+        *made->error = 0;
+        st = made;
+    }
+    *out = Fp8Scratch{st->error, st->workspace};
+    return LM_OK;
+}
+
 extern "C" {
 
 int lm_fp8_quantize(lm_context* ctx, const void* x_dev, int32_t dtype, int64_t rows, int64_t width, int64_t row_stride,
@@ -211,7 +209,7 @@ int lm_fp8_quantize(lm_context* ctx, const void* x_dev, int32_t dtype, int64_t r
     const lm::ContextInfo info = lm::context_info(ctx);
     LM_FP8_HIP(hipSetDevice(info.device));
     LM_FP8_HIP(lm::launch_fp8_quantize(
-        lm::Fp8Rows{x_dev, dtype, rows, width, row_stride, block_rows, q_dev, scale_dev}, info.stream));
+        lm::Fp8Rows{x_dev, dtype, rows, width, row_stride, block_rows, 0, q_dev, scale_dev}, info.stream));
     return LM_OK;
 } catch (const std::bad_alloc&) {
     return fail(LM_ENOMEM, "host allocation failed");
@@ -253,12 +251,12 @@ int lm_fp8_gemm(lm_context* ctx, const uint8_t* a_dev, const float* a_scale_dev,
     }
     const lm::ContextInfo info = lm::context_info(ctx);
     LM_FP8_HIP(hipSetDevice(info.device));
-    lm::Fp8State* st = nullptr;
-    rc = fp8_state(ctx, &st);
+    lm::Fp8Scratch sc{};
+    rc = lm::fp8_scratch(ctx, &sc);
     if (rc != LM_OK) {
         return rc;
     }
-    LM_FP8_HIP(lm::launch_fp8_gemm(p, st->workspace, info.stream));
+    LM_FP8_HIP(lm::launch_fp8_gemm(p, sc.workspace, info.stream));
     return LM_OK;
 } catch (const std::bad_alloc&) {
     return fail(LM_ENOMEM, "host allocation failed");
@@ -306,16 +304,16 @@ int lm_fp8_grouped_gemm(lm_context* ctx, const lm_fp8_groups* groups, const uint
         }
         const lm::ContextInfo info = lm::context_info(ctx);
         LM_FP8_HIP(hipSetDevice(info.device));
-        lm::Fp8State* st = nullptr;
-        rc = fp8_state(ctx, &st);
+        lm::Fp8Scratch sc{};
+        rc = lm::fp8_scratch(ctx, &sc);
         if (rc != LM_OK) {
             return rc;
         }
         p.out = out_dev;
         p.out_rows = out_rows;
         p.out_dtype = out_dtype;
-        p.error = st->error;
-        LM_FP8_HIP(lm::launch_fp8_gemm(p, st->workspace, info.stream));
+        p.error = sc.error;
+        LM_FP8_HIP(lm::launch_fp8_gemm(p, sc.workspace, info.stream));
         return LM_OK;
     } catch (const std::bad_alloc&) {
         return fail(LM_ENOMEM, "host allocation failed");
@@ -363,14 +361,14 @@ int lm_fp8_grouped_swiglu(lm_context* ctx, const lm_fp8_groups* groups, const ui
         }
         const lm::ContextInfo info = lm::context_info(ctx);
         LM_FP8_HIP(hipSetDevice(info.device));
-        lm::Fp8State* st = nullptr;
-        rc = fp8_state(ctx, &st);
+        lm::Fp8Scratch sc{};
+        rc = lm::fp8_scratch(ctx, &sc);
         if (rc != LM_OK) {
             return rc;
         }
         p.q = q_dev;
         p.q_scale = scale_dev;
-        p.error = st->error;
+        p.error = sc.error;
         LM_FP8_HIP(lm::launch_fp8_swiglu(p, info.stream));
         return LM_OK;
     } catch (const std::bad_alloc&) {
