@@ -103,9 +103,9 @@ int lm_fp8_grouped_swiglu(lm_context* ctx, const lm_fp8_groups* groups, const ui
  * the layer in lm_moe_forward, lm_grouped_swiglu, lm_dense_forward,
  * lm_stack_forward and its graphs, lm_decoder_forward and
  * lm_paged_decoder_forward: router and weights of the experts as on the other
- * paths, the FFN's input and activations in blocks of 1 x 128, outputs fp32.
- * The quantization is what results differ by: a layer's outputs are off by some
- * 4e-2 of their norm. only = 1 frees the layer's BF16 and fp16 weights (4 bytes a
+ * paths, the FFN's input and activations in blocks of 1 x 128, outputs fp32, the
+ * sums of large batches those of the FP8 matrix cores.  The quantization is what
+ * results differ by: a layer's outputs are off by 6.4e-2 of their norm. only = 1 frees the layer's BF16 and fp16 weights (4 bytes a
  * weight beside FP8's 1: DeepSeek-V2's 236 GB fit one MI355X); the other paths
  * are LM_ENOTRES then. An upload into the layer ends its FP8 weights until the
  * next lm_fp8_layer; after only = 1 all its FFN weights are uploaded again. H and

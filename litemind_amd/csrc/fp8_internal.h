@@ -44,6 +44,7 @@ struct Fp8Product {
     int32_t out_dtype;
     uint8_t* q;              // SwiGLU: [rows][n] codes
     float* q_scale;          // SwiGLU: [rows][nb]
+    int32_t exact;           // 1: fp32 sums; 0: large tiles on the FP8 matrix cores
     uint32_t* error;         // set to 1 (host memory) by an index outside its range; null without offsets
 };
 // Sums of products whose reduced axis several workgroups share.

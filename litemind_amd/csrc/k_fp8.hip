@@ -457,8 +457,11 @@ struct Work {
     // later ones behind them that are not the last block's.
     __device__ __forceinline__ void run(char* const (&bufs)[4], int first, int nk) {
         const auto spread = [&](int ks, char* buf, bool last, int i) {
+            // two stages: the next one's loads go out in the first half of this one, or
+            // they are still on their way at its end (256 x 256: 1.55 -> 1.32 us a stage)
+            constexpr int kSteps = STAGES == 2 ? (MI + 1) / 2 : MI;
 #pragma unroll
-            for (int q = i * L / MI; q < (i + 1) * L / MI; ++q) {
+            for (int q = i * L / kSteps; q < (i + 1) * L / kSteps && q < L; ++q) {
                 load1(first + ks, buf, last, q);
             }
         };
@@ -792,17 +795,24 @@ struct TileCost {
 };
 constexpr TileCost kFp8Tiles[] = {{32, 128, 512, 0.29f, 0.49f, 1.5f},
                                   {64, 128, 512, 0.38f, 0.72f, 3.0f},
-                                  {128, 128, 512, 0.85f, 1.13f, 4.0f},
-                                  {128, 256, 256, 0.80f, 1.04f, 6.0f},
-                                  {256, 256, 256, 1.54f, 1.88f, 8.0f}};
+                                  {128, 128, 512, 0.71f, 1.05f, 5.0f},
+                                  {128, 256, 256, 0.79f, 1.02f, 7.0f},
+                                  {256, 256, 256, 1.32f, 1.72f, 11.0f}};
 constexpr TileCost kExactTiles[] = {{32, 128, 512, 0.41f, 0.69f, 1.5f},
                                     {64, 128, 512, 0.59f, 1.15f, 3.0f},
-                                    {128, 128, 512, 1.13f, 1.90f, 4.0f},
-                                    {128, 256, 256, 1.43f, 1.80f, 6.0f}};
+                                    {128, 128, 512, 0.90f, 1.80f, 5.0f},
+                                    {128, 256, 256, 1.44f, 1.73f, 7.0f}};
 constexpr TileCost kSwigluTiles[] = {{32, 128, 256, 0.62f, 0.69f, 3.0f},
                                      {32, 128, 512, 0.87f, 1.22f, 3.0f},
                                      {64, 128, 256, 0.94f, 1.11f, 4.0f},
                                      {128, 128, 256, 1.45f, 1.80f, 6.0f}};
+// SwiGLU on the FP8 matrix cores: the small tiles wait for their weights, and
+// keep fp32 sums.
+constexpr TileCost kSwigluFp8Tiles[] = {{32, 128, 256, 0.62f, 0.69f, 3.0f},
+                                        {32, 128, 512, 0.87f, 1.22f, 3.0f},
+                                        {64, 128, 256, 0.94f, 1.11f, 4.0f},
+                                        {128, 128, 256, 0.80f, 1.05f, 7.0f},
+                                        {256, 128, 256, 1.35f, 1.75f, 9.0f}};
 
 // Groups that have rows, at most.
 int64_t active_groups(const Fp8Product& p) { return p.offsets == nullptr ? 1 : std::min<int64_t>(p.groups, p.rows); }
@@ -900,7 +910,7 @@ hipError_t launch_fp8_gemm(const Fp8Product& p, void* workspace, hipStream_t s) 
                : p.kb <= 40 ? launch_stream<1, 8, 2>(p, s)
                             : launch_stream<1, 16, 2>(p, s);
     }
-    const bool exact = p.out_dtype == LM_DT_F32, split = p.offsets == nullptr;
+    const bool exact = p.exact != 0, split = p.offsets == nullptr;
     const TileChoice c = exact ? choose_tile(p, kExactTiles, split) : choose_tile(p, kFp8Tiles, split);
     Fp8Product q = p;
     if (c.shares > 1) {
@@ -918,15 +928,18 @@ hipError_t launch_fp8_gemm(const Fp8Product& p, void* workspace, hipStream_t s) 
 }
 
 hipError_t launch_fp8_swiglu(const Fp8Product& p, hipStream_t s) {
-    switch (choose_tile(p, kSwigluTiles, false).tile) {
+    const bool exact = p.exact != 0;
+    switch ((exact ? choose_tile(p, kSwigluTiles, false) : choose_tile(p, kSwigluFp8Tiles, false)).tile) {
         case 0:
             return launch_tiles<true, true, 1, 8, 2, 2, 3>(p, s);
         case 1:
             return launch_tiles<true, true, 1, 4, 2, 4, 2>(p, s);
         case 2:
             return launch_tiles<true, true, 1, 8, 4, 2, 3>(p, s);
+        case 3:
+            return exact ? launch_tiles<true, true, 2, 4, 4, 4, 3>(p, s) : launch_tiles<true, false, 2, 4, 4, 4, 3>(p, s);
         default:
-            return launch_tiles<true, true, 2, 4, 4, 4, 3>(p, s);
+            return launch_tiles<true, false, 2, 4, 8, 4, 2>(p, s);
     }
 }
 

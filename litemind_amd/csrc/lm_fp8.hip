@@ -232,6 +232,7 @@ int lm_fp8_gemm(lm_context* ctx, const uint8_t* a_dev, const float* a_scale_dev,
     p.out_rows = rows;
     p.out = out_dev;
     p.out_dtype = out_dtype;
+    p.exact = out_dtype == LM_DT_F32 ? 1 : 0;
     if (rows == 0) {
         return ctx != nullptr ? LM_OK : fail(LM_EINVAL, "null context");
     }
@@ -312,6 +313,7 @@ int lm_fp8_grouped_gemm(lm_context* ctx, const lm_fp8_groups* groups, const uint
         p.out = out_dev;
         p.out_rows = out_rows;
         p.out_dtype = out_dtype;
+        p.exact = out_dtype == LM_DT_F32 ? 1 : 0;
         p.error = sc.error;
         LM_FP8_HIP(lm::launch_fp8_gemm(p, sc.workspace, info.stream));
         return LM_OK;
@@ -368,6 +370,7 @@ int lm_fp8_grouped_swiglu(lm_context* ctx, const lm_fp8_groups* groups, const ui
         }
         p.q = q_dev;
         p.q_scale = scale_dev;
+        p.exact = 1;
         p.error = sc.error;
         LM_FP8_HIP(lm::launch_fp8_swiglu(p, info.stream));
         return LM_OK;

@@ -73,14 +73,18 @@ def model(request):
     m.ctx.close()
 
 
-def near(got, want, parts):
+def near(got, want, parts, exact):
     """Sums of the same fp32 numbers in another order: each of at most 20 additions and products is off by a step of
-    what has been added up."""
+    what has been added up. Not `exact`: the layers' large tiles take the FP8 matrix cores' sums, off by 4e-5 of their
+    norm, which puts 6e-4 of the activations' codes on the other side of a border, a step of 2^-3.5 away: 2e-3 of an
+    output's norm."""
     assert np.isfinite(got).all()
-    assert (np.abs(got - want) <= 20 * 2.0 ** -23 * parts + 2.0 ** -126).all()
+    if exact:
+        assert (np.abs(got - want) <= 20 * 2.0 ** -23 * parts + 2.0 ** -126).all()
+    assert (np.linalg.norm(got - want, axis=-1) <= 1e-2 * np.linalg.norm(parts + np.zeros_like(want), axis=-1)).all()
 
 
-TOKENS = [1, 2, 3, 17, 100, 300]
+TOKENS = [1, 2, 3, 17, 100, 300, 1500]
 
 
 @pytest.mark.parametrize("T", TOKENS)
@@ -98,7 +102,7 @@ def test_moe_layer(model, T):
     routed, shared = model.assignments(x, gi)
     terms = [gw[:, r, None].astype(np.float64) * routed[:, r] for r in range(d.top_k)]
     terms += [] if shared is None else [shared.astype(np.float64)]
-    near(y.download(), sum(terms), sum(np.abs(t) for t in terms))
+    near(y.download(), sum(terms), sum(np.abs(t) for t in terms), T <= 17)
     # Rounding to e4m3 is off by 2.6e-2 of the norm (half a step of 2^-3 .. 2^-4, evenly spread): products of two such
     # operands by 3.7e-2, an activation by 5.2e-2 and its own rounding, an output by 6.4e-2. Twice that is far from
     # what a wrong weight or row gives.
@@ -117,11 +121,12 @@ def test_grouped_swiglu(model, T):
     ctx.grouped_swiglu(1, ctx.to_device(x), T, ctx.to_device(idx), out, path=lm.PATH_FP8)
     routed, shared = model.assignments(x, idx)
     got = out.download()
-    near(got[:T * d.top_k], routed.reshape(T * d.top_k, -1), np.abs(routed).reshape(T * d.top_k, -1))
-    near(got[T * d.top_k:], np.zeros_like(got[T * d.top_k:]) if shared is None else shared, 0 if shared is None else np.abs(shared))
+    near(got[:T * d.top_k], routed.reshape(T * d.top_k, -1), np.abs(routed).reshape(T * d.top_k, -1), T <= 17)
+    near(got[T * d.top_k:], np.zeros_like(got[T * d.top_k:]) if shared is None else shared, np.zeros_like(got[T * d.top_k:]) if shared is None else np.abs(shared),
+         T <= 17)
 
 
-@pytest.mark.parametrize("T", [1, 5, 40, 200])
+@pytest.mark.parametrize("T", [1, 5, 40, 200, 2000])
 def test_dense_layer(model, T):
     announce(f"fp8 dense layer, {T} tokens")
     d, ctx = model.dims, model.ctx
@@ -132,7 +137,7 @@ def test_dense_layer(model, T):
     want = model.operators([(gate, up)], [down], x)
     # The down product's sums may be in another order; 1040 terms of either sign add up to a thirtieth of their
     # magnitudes, the row's largest output to more than that.
-    near(y.download(), want, 40 * np.abs(want).max(1, keepdims=True))
+    near(y.download(), want, 40 * np.abs(want).max(1, keepdims=True), T <= 17)
 
 
 @pytest.mark.parametrize("T", [1, 3, 40])
@@ -168,7 +173,7 @@ def test_stack_and_graph(model, T):
             ctx.moe_forward(1, other, 1, ctx.empty((1, d.hidden)), path=lm.PATH_FP8)
             assert (h.download() == expected).all()
         with pytest.raises(lm.LmError) as e:  # the graph holds the workspace
-            ctx.stack_forward(0, 1, ctx.to_device(wl.tokens(10, 700, d.hidden)), 700, path=lm.PATH_FP8)
+            ctx.stack_forward(0, 1, ctx.to_device(wl.tokens(10, 2500, d.hidden)), 2500, path=lm.PATH_FP8)
         assert e.value.status == -1
         with pytest.raises(lm.LmError):
             ctx.fp8_layer(1, only=True)
