@@ -785,34 +785,40 @@ __global__ __launch_bounds__(256) void fp8_join_kernel(Fp8Product p, const float
 
 // ---- which kernel ----
 
-// What a tile costs, in microseconds (measured with operands that lie in the
-// L2s, 2048 and 8192 reduced channels): a stage where at most half the places of
-// workgroups are taken and where all are, and what is no stage's (finding the
-// tile, its first loads, its outputs). Up to 128 x 128 two workgroups share a CU.
+// What a tile costs, in microseconds: a stage where at most half the places of
+// workgroups are taken and where all are (measured with operands that lie in the
+// L2s, 2048 and 8192 reduced channels), a stage with weights for each group, and
+// what is no stage's (finding the tile, its first loads, its outputs). A group's
+// few row tiles wait together for weights from memory that no tile has read
+// before, so that the larger tile gains there: fitted to the experts of layers
+// with 64 x 1408 x 2048 and 160 x 1536 x 5120 at 32 to 4096 tokens (gate and up
+// of 1024 tokens by the latter: 648 us by two 32 x 256 tiles a CU, which the
+// other figures take, 548 by 128 x 256; at 256 tokens 483 and 519). Up to 128 x
+// 128 two workgroups share a CU.
 struct TileCost {
     int bm, bn, places;
-    float solo, full, fixed;
+    float solo, full, grouped, fixed;
 };
-constexpr TileCost kFp8Tiles[] = {{32, 128, 512, 0.29f, 0.49f, 1.5f},
-                                  {64, 128, 512, 0.38f, 0.72f, 3.0f},
-                                  {128, 128, 512, 0.71f, 1.05f, 5.0f},
-                                  {128, 256, 256, 0.79f, 1.02f, 7.0f},
-                                  {256, 256, 256, 1.32f, 1.72f, 11.0f}};
-constexpr TileCost kExactTiles[] = {{32, 128, 512, 0.41f, 0.69f, 1.5f},
-                                    {64, 128, 512, 0.59f, 1.15f, 3.0f},
-                                    {128, 128, 512, 0.90f, 1.80f, 5.0f},
-                                    {128, 256, 256, 1.44f, 1.73f, 7.0f}};
-constexpr TileCost kSwigluTiles[] = {{32, 128, 256, 0.62f, 0.69f, 3.0f},
-                                     {32, 128, 512, 0.87f, 1.22f, 3.0f},
-                                     {64, 128, 256, 0.94f, 1.11f, 4.0f},
-                                     {128, 128, 256, 1.45f, 1.80f, 6.0f}};
+constexpr TileCost kFp8Tiles[] = {{32, 128, 512, 0.29f, 0.49f, 0.90f, 1.5f},
+                                  {64, 128, 512, 0.38f, 0.72f, 1.25f, 3.0f},
+                                  {128, 128, 512, 0.71f, 1.05f, 1.80f, 5.0f},
+                                  {128, 256, 256, 0.79f, 1.02f, 1.70f, 7.0f},
+                                  {256, 256, 256, 1.32f, 1.72f, 2.15f, 11.0f}};
+constexpr TileCost kExactTiles[] = {{32, 128, 512, 0.41f, 0.69f, 0.90f, 1.5f},
+                                    {64, 128, 512, 0.59f, 1.15f, 1.25f, 3.0f},
+                                    {128, 128, 512, 0.90f, 1.80f, 1.85f, 5.0f},
+                                    {128, 256, 256, 1.44f, 1.73f, 1.75f, 7.0f}};
+constexpr TileCost kSwigluTiles[] = {{32, 128, 256, 0.62f, 0.69f, 1.10f, 3.0f},
+                                     {32, 128, 512, 0.87f, 1.22f, 1.85f, 3.0f},
+                                     {64, 128, 256, 0.94f, 1.11f, 1.60f, 4.0f},
+                                     {128, 128, 256, 1.45f, 1.80f, 1.80f, 6.0f}};
 // SwiGLU on the FP8 matrix cores: the small tiles wait for their weights, and
 // keep fp32 sums.
-constexpr TileCost kSwigluFp8Tiles[] = {{32, 128, 256, 0.62f, 0.69f, 3.0f},
-                                        {32, 128, 512, 0.87f, 1.22f, 3.0f},
-                                        {64, 128, 256, 0.94f, 1.11f, 4.0f},
-                                        {128, 128, 256, 0.80f, 1.05f, 7.0f},
-                                        {256, 128, 256, 1.35f, 1.75f, 9.0f}};
+constexpr TileCost kSwigluFp8Tiles[] = {{32, 128, 256, 0.62f, 0.69f, 1.10f, 3.0f},
+                                        {32, 128, 512, 0.87f, 1.22f, 1.85f, 3.0f},
+                                        {64, 128, 256, 0.94f, 1.11f, 1.60f, 4.0f},
+                                        {128, 128, 256, 0.80f, 1.05f, 1.40f, 7.0f},
+                                        {256, 128, 256, 1.35f, 1.75f, 2.10f, 9.0f}};
 
 // Groups that have rows, at most.
 int64_t active_groups(const Fp8Product& p) { return p.offsets == nullptr ? 1 : std::min<int64_t>(p.groups, p.rows); }
@@ -827,8 +833,9 @@ double row_tiles(const Fp8Product& p, int bm) {
     return std::max(groups, static_cast<double>(p.rows) / bm + 0.5 * groups);
 }
 
-double tile_time(const TileCost& c, double tiles, int64_t stages) {
-    const double per = static_cast<double>(stages) * (2.0 * tiles <= c.places ? c.solo : c.full) + c.fixed;
+double tile_time(const TileCost& c, double tiles, int64_t stages, bool grouped) {
+    const double stage = 2.0 * tiles <= c.places ? c.solo : grouped ? c.grouped : c.full;
+    const double per = static_cast<double>(stages) * stage + c.fixed;
     return tiles <= c.places ? per : per * (tiles / c.places + 0.5);
 }
 
@@ -850,7 +857,7 @@ TileChoice choose_tile(const Fp8Product& p, const TileCost (&tiles)[N], bool spl
         const double count = row_tiles(p, c.bm) * static_cast<double>((p.n + c.bn - 1) / c.bn);
         for (const int shares : kShares) {
             const int64_t stages = (p.kb + shares - 1) / shares;
-            double t = tile_time(c, count * shares, stages);
+            double t = tile_time(c, count * shares, stages, p.offsets != nullptr);
             if (shares > 1) {
                 const int64_t sums = p.rows * p.n * shares;
                 if (!split || stages < 4 || count * shares > c.places || 4 * sums > kFp8WorkspaceBytes) {
