@@ -17,6 +17,9 @@
  * x * (1 / s) rounded to the nearest e4m3, ties to even, in fp32 arithmetic; x
  * stands for code * s.  NaN and infinity become the NaN code 0x7f, and so reach
  * every product of theirs.  Scales are fp32, [row blocks][ceil(features / 128)].
+ * Where two blocks meet in a product, their scales are multiplied in fp32 first:
+ * past its range (blocks of 1e20 times others of 1e20) the output is infinite or
+ * NaN, under it (1e-17 times 1e-17) bits are lost.
  *
  * lm_fp8_quantize, lm_fp8_gemm, lm_fp8_grouped_gemm and lm_fp8_grouped_swiglu
  * may be captured into a HIP graph on the context's stream; the products after
@@ -99,18 +102,23 @@ int lm_fp8_grouped_swiglu(lm_context* ctx, const lm_fp8_groups* groups, const ui
 
 /* ---- the layers' FFNs at one byte a weight ----
  * After lm_finalize_layer: the layer's experts and shared experts, or its dense
- * FFN, in FP8 blocks of 128 x 128, from the BF16 weights. LM_PATH_FP8 then runs
+ * FFN, in FP8 blocks of 128 x 128, from the BF16 weights.  LM_PATH_FP8 then runs
  * the layer in lm_moe_forward, lm_grouped_swiglu, lm_dense_forward,
  * lm_stack_forward and its graphs, lm_decoder_forward and
  * lm_paged_decoder_forward: router and weights of the experts as on the other
  * paths, the FFN's input and activations in blocks of 1 x 128, outputs fp32, the
  * sums of large batches those of the FP8 matrix cores.  The quantization is what
- * results differ by: a layer's outputs are off by 6.4e-2 of their norm. only = 1 frees the layer's BF16 and fp16 weights (4 bytes a
- * weight beside FP8's 1: DeepSeek-V2's 236 GB fit one MI355X); the other paths
- * are LM_ENOTRES then. An upload into the layer ends its FP8 weights until the
- * next lm_fp8_layer; after only = 1 all its FFN weights are uploaded again. H and
- * the FFNs' widths in multiples of 16. LM_EINVAL with only = 1 while stack graphs
- * are alive. */
+ * results differ by: a layer's outputs are off by 6.4e-2 of their norm.  A call
+ * takes fewer tokens than 2^32 over the widest of H, a token's routed activations
+ * (experts per token * moe_intermediate_size), the shared experts' and the dense
+ * FFN's.
+ *
+ * only = 1 frees the layer's BF16 and fp16 weights (4 bytes a weight beside FP8's
+ * 1: DeepSeek-V2's 236 GB fit one MI355X); the other paths are LM_ENOTRES then.
+ * An upload into the layer ends its FP8 weights until the next lm_fp8_layer;
+ * after only = 1 all its FFN weights are uploaded again.  H and the FFNs' widths
+ * in multiples of 16 up to 2^20, gate and up together under 2^32 weights.
+ * LM_EINVAL with only = 1 while stack graphs are alive. */
 int lm_fp8_layer(lm_context* ctx, int32_t layer, int32_t only);
 
 #ifdef __cplusplus

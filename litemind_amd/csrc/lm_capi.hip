@@ -661,11 +661,19 @@ int launch_expert_kernels_fp8(lm_context* ctx, const Layer& L, const float* x, i
     return LM_OK;
 }
 
-// Whether a layer can run `path`.
-int check_path(const lm_context* ctx, int32_t layer, int32_t path) {
+// The FP8 products address the codes of their rows, and of a matrix, with 32 bits.
+constexpr int64_t kFp8Codes = int64_t{1} << 32;
+
+// Whether a layer can run `path` for T tokens.
+int check_path(const lm_context* ctx, int32_t layer, int32_t path, int64_t T) {
     const Layer& L = ctx->layers[static_cast<size_t>(layer)];
     if (path == LM_PATH_FP8 && !L.fp8.ready) {
         return fail(LM_ENOTRES, "layer " + std::to_string(layer) + " has no FP8 weights (lm_fp8_layer)");
+    }
+    const int64_t widest = L.dense ? ctx->D : std::max<int64_t>(int64_t{ctx->K} * ctx->I, ctx->S);
+    if (path == LM_PATH_FP8 && T >= kFp8Codes / std::max<int64_t>(ctx->H, widest)) {
+        return fail(LM_EINVAL, "LM_PATH_FP8 takes under 2^32 / " + std::to_string(std::max<int64_t>(ctx->H, widest)) +
+                                   " tokens a call");
     }
     if (path != LM_PATH_FP8 && !L.finalized && L.fp8.ready && !L.allocated) {
         return fail(LM_ENOTRES, "layer " + std::to_string(layer) + " holds FP8 weights alone (LM_PATH_FP8)");
@@ -866,7 +874,7 @@ int moe_layer(lm_context* ctx, int32_t layer, const float* x, int64_t T, float* 
               const float* norm = nullptr, const float* next_norm = nullptr, bool prenormed = false) {
     Layer& L = ctx->layers[static_cast<size_t>(layer)];
     const bool fp8 = path == LM_PATH_FP8;
-    int rc = check_path(ctx, layer, path);
+    int rc = check_path(ctx, layer, path, T);
     if (rc != LM_OK) {
         return rc;
     }
@@ -973,7 +981,7 @@ int dense_layer(lm_context* ctx, int32_t layer, const float* x, int64_t T, float
                 int32_t path, const float* next_norm = nullptr, bool prenormed = false) {
     Layer& L = ctx->layers[static_cast<size_t>(layer)];
     const bool fp8 = path == LM_PATH_FP8;
-    int rc = check_path(ctx, layer, path);
+    int rc = check_path(ctx, layer, path, T);
     if (rc != LM_OK) {
         return rc;
     }
@@ -1219,7 +1227,7 @@ int lm::ffn_ready(lm_context* ctx, int32_t l, int64_t T, int32_t path) {
         return fail(LM_ENOTRES, "layer " + std::to_string(l) + " has no norm weight");
     }
     const bool fp8 = path == LM_PATH_FP8;
-    int rc = check_path(ctx, l, path);
+    int rc = check_path(ctx, l, path, T);
     if (rc != LM_OK) {
         return rc;
     }
@@ -1755,6 +1763,10 @@ int lm_fp8_layer(lm_context* ctx, int32_t layer, int32_t only) {
     if (H % 16 != 0 || (E > 0 && I % 16 != 0) || O % 16 != 0) {
         return fail(LM_EINVAL, "FP8 weights need widths in multiples of 16");
     }
+    const int64_t widest = std::max(E > 0 ? I : 0, O);
+    if (std::max(H, widest) > lm::kFp8MaxInner || 2 * widest * H >= kFp8Codes) {
+        return fail(LM_EINVAL, "FP8 weights take widths up to 2^20 and under 2^32 weights in gate and up together");
+    }
     rc = set_device(ctx);
     lm::Fp8Scratch sc{};
     if (rc == LM_OK) {
@@ -2077,7 +2089,7 @@ int lm_grouped_swiglu(lm_context* ctx, int32_t layer, const float* x_dev, int64_
     }
     Layer& L = ctx->layers[static_cast<size_t>(layer)];
     const bool fp8 = path == LM_PATH_FP8;
-    rc = check_path(ctx, layer, path);
+    rc = check_path(ctx, layer, path, tokens);
     if (rc != LM_OK) {
         return rc;
     }

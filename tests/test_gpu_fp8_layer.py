@@ -283,3 +283,19 @@ def test_decoder_loops():
         h = ctx.to_device(h0)
         ctx.paged_decoder_forward(0, 1, step, h, path=lm.PATH_FP8)
         assert np.linalg.norm(h.download() - runs[lm.PATH_FP8]) <= 0.13 * change
+
+
+def test_sizes_past_32_bits_are_refused():
+    announce("fp8 layers: sizes past 32 bits")
+    d = ALONE
+    T = 2 ** 32 // (d.top_k * d.inter)  # one token's activations are the widest rows
+    with lm.Context(d.moe_config(num_layers=2)) as ctx:
+        wl.upload_moe_layer(ctx, 1, wl.moe_layer(31, 1, d))
+        ctx.fp8_layer(1)
+        x, y = ctx.empty((T, d.hidden)), ctx.empty((T, d.hidden))
+        refused(-1, ctx.moe_forward, 1, x, T, y, path=lm.PATH_FP8)
+    d = dataclasses.replace(SMALL, hidden=16, dense_inter=2 ** 20 + 16)
+    with lm.Context(d.moe_config(num_layers=1)) as ctx:
+        ctx.upload_dense(0, *wl.dense_ffn(1, 0, d))
+        ctx.finalize_layer(0)
+        refused(-1, ctx.fp8_layer, 0)
