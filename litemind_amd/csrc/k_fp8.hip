@@ -281,17 +281,17 @@ struct Stage {
     int first, stages;  // the tile's share of the reduced axis, in scale blocks
 };
 
-// The products of a tile's first 16 WM MI rows: WM x WN waves of MI x NJ blocks
-// of 16 rows x 16 weight rows.
+// The products of a tile: WM x WN waves of MI x NJ blocks of 16 rows x 16 weight
+// rows.
 template <class Z, bool EXACT, int WM, int WN, int MI, int NJ>
 struct Work {
     static constexpr bool SWIGLU = Z::SWIGLU;
-    static constexpr int STAGES = Z::STAGES, BM = 16 * WM * MI;
+    static constexpr int STAGES = Z::STAGES, BM = Z::BM;
     // 1 KB loads of a wave and stage; where the rows have fewer than there are
     // waves, two waves load the same
     static constexpr int AL = BM / 8 > Z::WAVES ? BM / 8 / Z::WAVES : 1, BL = Z::BN / 8 / Z::WAVES;
     static constexpr int L = AL + BL + 1;
-    static_assert(WM * WN == Z::WAVES && BM <= Z::BM && 16 * WN * NJ == Z::BN);
+    static_assert(WM * WN == Z::WAVES && 16 * WM * MI == BM && 16 * WN * NJ == Z::BN);
     static_assert((AL * 8 * Z::WAVES == BM || Z::WAVES * 8 % BM == 0) && BL * 8 * Z::WAVES == Z::BN,
                   "whole loads per wave");
     static_assert((STAGES - 1) * L < 64, "vmcnt");
@@ -451,10 +451,10 @@ struct Work {
             __builtin_amdgcn_sched_barrier(0);
         }
     }
-    // The nk stages from `first` on: stage ks lives in buffer ks % STAGES; its loads are issued
-    // STAGES - 1 stages before, into the buffer that every wave has read when it
-    // passes the barrier of stage ks - STAGES + 1. The first loop's stages have
-    // later ones behind them that are not the last block's.
+    // The nk stages from `first` on: stage ks lives in buffer ks % STAGES; its loads
+    // are issued STAGES - 1 stages before, into the buffer that every wave has read
+    // when it passes the barrier of stage ks - STAGES + 1. The first loop's stages
+    // have later ones behind them that are not the last block's.
     __device__ __forceinline__ void run(char* const (&bufs)[4], int first, int nk) {
         const auto spread = [&](int ks, char* buf, bool last, int i) {
             // two stages: the next one's loads go out in the first half of this one, or
@@ -598,17 +598,6 @@ struct Work {
 };
 
 template <class Z, bool EXACT, int WM, int WN, int MI, int NJ>
-__device__ __forceinline__ void run_tile(const Fp8Product& p, const Stage<Z>& st, char* codes, float* most_of) {
-    Work<Z, EXACT, WM, WN, MI, NJ> work(p, st);
-    work.run(st.bufs, st.first, st.stages);
-    if constexpr (Z::SWIGLU) {
-        work.store_swiglu(p, st, codes, most_of);
-    } else {
-        work.store(p, st);
-    }
-}
-
-template <class Z, bool EXACT, int WM, int WN, int MI, int NJ>
 __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2, 2))) void fp8_tile_kernel(Fp8Product p) {
     // one LDS array per stage: the compiler tracks the asynchronous writes by array
     __shared__ __attribute__((aligned(1024))) char s0[Z::kStageBytes], s1[Z::kStageBytes],
@@ -628,7 +617,13 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2,
     }
     const Stage<Z> st{bufs, t, t.mt * Z::BM, t.nt * Z::CN, static_cast<int>(threadIdx.x & 63),
                       __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)), first, stages};
-    run_tile<Z, EXACT, WM, WN, MI, NJ>(p, st, s0, most_of);
+    Work<Z, EXACT, WM, WN, MI, NJ> work(p, st);
+    work.run(st.bufs, st.first, st.stages);
+    if constexpr (Z::SWIGLU) {
+        work.store_swiglu(p, st, s0, most_of);
+    } else {
+        work.store(p, st);
+    }
 }
 
 template <bool SWIGLU, bool EXACT, int WM, int WN, int MI, int NJ, int STAGES>
@@ -639,8 +634,8 @@ hipError_t launch_tiles(const Fp8Product& p, hipStream_t s, int shares = 1) {
     const int64_t mts = p.offsets == nullptr ? (p.rows + Z::BM - 1) / Z::BM
                                              : p.rows / Z::BM + std::min<int64_t>(p.groups, p.rows);
     const int64_t tiles = mts * ((p.n + Z::CN - 1) / Z::CN);
-    if (tiles > (1 << 22)) {
-        return hipErrorInvalidValue;
+    if (tiles > (1 << 22)) {  // 2^31 threads
+        return hipErrorInvalidConfiguration;
     }
     hipLaunchKernelGGL(HIP_KERNEL_NAME(fp8_tile_kernel<Z, EXACT, WM, WN, MI, NJ>),
                        dim3(static_cast<unsigned>(round_up(tiles, kXcds)), static_cast<unsigned>(shares)), dim3(64 * Z::WAVES),
@@ -650,112 +645,86 @@ hipError_t launch_tiles(const Fp8Product& p, hipStream_t s, int shares = 1) {
 
 // ---- the kernel of few rows ----
 //
-// Tiles of 16 rows at most: the weights are read once, straight to registers,
-// and the waves of a workgroup take turns at the scale blocks of the reduced
-// axis; their sums are added up in LDS, wave by wave. What counts is the bytes
-// in flight: U blocks of NT times 2 KB a wave.
+// Tiles of 16 rows at most by 16 features: the weights are read once, straight to
+// registers, and the waves of a workgroup take turns at the scale blocks of the
+// reduced axis; their sums are added up in LDS, wave by wave. What counts is the
+// bytes in flight: U blocks of 2 KB a wave.
 //
-// Scale blocks b0, b0 + step, ... (U of them, as far as there are any) of NT
-// times 16 weight rows and the rows of a.
-template <int NT, int U>
+// Scale blocks b0, b0 + step, ... (U of them, as far as there are any) of 16
+// weight rows and the rows of a.
+template <int U>
 __device__ __forceinline__ void stream_blocks(const Fp8Product& p, int b0, int step, const uint8_t* a, const float* a_scale,
-                                              bool live, const uint8_t* const (&w)[NT],
-                                              const float* const (&w_scale)[NT], floatx4 (&acc)[NT]) {
+                                              bool live, const uint8_t* w, const float* w_scale, floatx4& acc) {
     const int lane = threadIdx.x & 63, chunks = p.k / 16;
-    uint4 wv[U][NT][2], av[U][2];
-    float sa[U], sw[U][NT];
+    uint4 wv[U][2], av[U][2];
+    float sa[U], sw[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int b = min(b0 + u * step, p.kb - 1);  // past the last block: it again, which counts for nothing
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int c = 8 * b + 4 * h + (lane >> 4);
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                wv[u][j][h] = load_stream16(w[j] + (c < chunks ? 16 * c : 0));
-            }
+            wv[u][h] = load_stream16(w + (c < chunks ? 16 * c : 0));
             av[u][h] = make_uint4(0, 0, 0, 0);
             if (live && c < chunks) {
                 av[u][h] = *reinterpret_cast<const uint4*>(a + 16 * c);
             }
         }
         sa[u] = live && b0 + u * step < p.kb ? a_scale[b] : 0.0f;
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            sw[u][j] = w_scale[j][b];
-        }
+        sw[u] = w_scale[b];
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        Operand<true> rows;
+        Operand<true> rows, weights;
         rows.set(av[u][0], av[u][1]);
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            Operand<true> weights;
-            weights.set(wv[u][j][0], wv[u][j][1]);
-            take(acc[j], block_sum(weights, rows), sa[u] * sw[u][j]);
-        }
+        weights.set(wv[u][0], wv[u][1]);
+        take(acc, block_sum(weights, rows), sa[u] * sw[u]);
     }
 }
 
-template <int NT, int WAVES, int U>
+template <int WAVES, int U>
 __global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(Fp8Product p) {
-    constexpr int CN = 16 * NT;
-    __shared__ floatx4 sums[WAVES][NT][64];
+    __shared__ floatx4 sums[WAVES][64];
     Tile t;
-    if (!find_tile(p, 16, (p.n + CN - 1) / CN, t)) {
+    if (!find_tile(p, 16, (p.n + 15) / 16, t)) {
         return;
     }
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-    const int m = t.mt * 16 + (lane & 15), n0 = t.nt * CN;
+    const int m = t.mt * 16 + (lane & 15), n0 = t.nt * 16;
     const bool live = m < t.rows;
     const int64_t row = live ? source_row(p, t.first + m) : 0;
-    const uint8_t* w[NT];
-    const float* w_scale[NT];
-    floatx4 acc[NT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-        const int n = n0 + 16 * j;
-        w[j] = p.w + (static_cast<int64_t>(t.g) * p.n + min(n + (lane & 15), p.n - 1)) * p.k;
-        w_scale[j] = p.w_scale + (static_cast<int64_t>(t.g) * p.nb + min(n, p.n - 1) / kFp8Block) * p.kb;
-        acc[j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
+    const uint8_t* const w = p.w + (static_cast<int64_t>(t.g) * p.n + min(n0 + (lane & 15), p.n - 1)) * p.k;
+    const float* const w_scale = p.w_scale + (static_cast<int64_t>(t.g) * p.nb + n0 / kFp8Block) * p.kb;
+    floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int b0 = wave; b0 < p.kb; b0 += WAVES * U) {
-        stream_blocks<NT, U>(p, b0, WAVES, p.a + row * p.k, p.a_scale + row * p.kb, live, w, w_scale, acc);
+        stream_blocks<U>(p, b0, WAVES, p.a + row * p.k, p.a_scale + row * p.kb, live, w, w_scale, acc);
     }
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-        sums[wave][j][lane] = acc[j];
-    }
+    sums[wave][lane] = acc;
     __syncthreads();
-    const int n = n0 + 16 * wave + 4 * (lane >> 4);
-    if (wave < NT && live && n < p.n) {
-        floatx4 v = sums[0][wave][lane];
+    const int n = n0 + 4 * (lane >> 4);
+    if (wave == 0 && live && n < p.n) {
 #pragma unroll
         for (int i = 1; i < WAVES; ++i) {
-            v += sums[i][wave][lane];
+            acc += sums[i][lane];
         }
         const int64_t to = target_row(p, t.first + m);
         if (to >= 0) {
-            store4(p, to, n, v);
+            store4(p, to, n, acc);
         }
     }
 }
 
-// Row tiles of 16 and workgroups of the kernels of few rows.
-int64_t stream_tiles(const Fp8Product& p, int64_t feature_tiles) {
-    return (p.offsets == nullptr ? (p.rows + 15) / 16 : p.rows / 16 + std::min<int64_t>(p.groups, p.rows)) * feature_tiles;
+// Workgroups of the kernel of few rows.
+int64_t stream_tiles(const Fp8Product& p) {
+    const int64_t row_tiles = p.offsets == nullptr ? (p.rows + 15) / 16 : p.rows / 16 + std::min<int64_t>(p.groups, p.rows);
+    return row_tiles * ((p.n + 15) / 16);
 }
 
-template <int NT, int WAVES, int U>
+template <int WAVES, int U>
 hipError_t launch_stream(const Fp8Product& p, hipStream_t s) {
-    const int64_t tiles = stream_tiles(p, (p.n + 16 * NT - 1) / (16 * NT));
-    if (tiles > (1 << 20)) {
-        return hipErrorInvalidValue;
-    }
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(fp8_stream_kernel<NT, WAVES, U>),
-                       dim3(static_cast<unsigned>(round_up(tiles, kXcds))), dim3(64 * WAVES), 0, s, p);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(fp8_stream_kernel<WAVES, U>),
+                       dim3(static_cast<unsigned>(round_up(stream_tiles(p), kXcds))), dim3(64 * WAVES), 0, s, p);
     return hipGetLastError();
 }
 
@@ -886,13 +855,13 @@ hipError_t launch_gemm_tile(const Fp8Product& p, const TileChoice& c, hipStream_
             return launch_tiles<false, EXACT, 1, 4, 4, 2, 3>(p, s, c.shares);
         case 2:
             return launch_tiles<false, EXACT, 2, 2, 4, 4, 2>(p, s, c.shares);
-        case 3:
-            return launch_tiles<false, EXACT, 2, 4, 4, 4, 3>(p, s, c.shares);
-        default:
+        case 4:
             if constexpr (!EXACT) {
                 return launch_tiles<false, false, 2, 4, 8, 4, 2>(p, s, c.shares);
             }
-            return hipErrorInvalidValue;
+            [[fallthrough]];
+        default:
+            return launch_tiles<false, EXACT, 2, 4, 4, 4, 3>(p, s, c.shares);
     }
 }
 
@@ -902,7 +871,7 @@ hipError_t launch_gemm_tile(const Fp8Product& p, const TileChoice& c, hipStream_
 // 7.6; six experts of 2048 features (18 MB) 5.8 and 8.7, of 5120 (50 MB) 16 and 12.
 bool streams(const Fp8Product& p) {
     const int64_t groups = active_groups(p), rows = std::min<int64_t>(16, (p.rows + groups - 1) / groups);
-    const int64_t tiles = stream_tiles(p, (p.n + 15) / 16);
+    const int64_t tiles = stream_tiles(p);
     return tiles <= 4096 && tiles * p.kb * (16 + rows) * kFp8Block <= (24 << 20);
 }
 
@@ -912,10 +881,10 @@ hipError_t launch_fp8_gemm(const Fp8Product& p, void* workspace, hipStream_t s) 
     if (streams(p)) {
         // all of a wave's loads in flight at once where the axis is short, many
         // waves where it is long (10944 channels: 9.5 us, 11 with four waves)
-        return p.kb <= 12   ? launch_stream<1, 4, 3>(p, s)
-               : p.kb <= 16 ? launch_stream<1, 4, 4>(p, s)
-               : p.kb <= 40 ? launch_stream<1, 8, 2>(p, s)
-                            : launch_stream<1, 16, 2>(p, s);
+        return p.kb <= 12   ? launch_stream<4, 3>(p, s)
+               : p.kb <= 16 ? launch_stream<4, 4>(p, s)
+               : p.kb <= 40 ? launch_stream<8, 2>(p, s)
+                            : launch_stream<16, 2>(p, s);
     }
     const bool exact = p.exact != 0, split = p.offsets == nullptr;
     const TileChoice c = exact ? choose_tile(p, kExactTiles, split) : choose_tile(p, kFp8Tiles, split);

