@@ -13,9 +13,9 @@
  * 448, no infinity; uint8_t here, row-major, rows of `features` bytes).  A
  * block is 128 codes of a row, or 128 rows of 128; the last block of a row or
  * column may be smaller.  With the largest magnitude m of a block's finite
- * values its scale is s = max(m / 448, 2^-126) and the code of x is
- * x * (1 / s) rounded to the nearest e4m3, ties to even, in fp32 arithmetic; x
- * stands for code * s.  NaN and infinity become the NaN code 0x7f, and so reach
+ * values its scale is s = max(m / 448, 2^-126) and the code of x the e4m3 nearest
+ * to 448 x / m (to x 2^126 where s is 2^-126), ties to even, the quotient exact; a
+ * code stands for code * s.  NaN and infinity become the NaN code 0x7f, and so reach
  * every product of theirs.  Scales are fp32, [row blocks][ceil(features / 128)].
  * Where two blocks meet in a product, their scales are multiplied in fp32 first:
  * past its range (blocks of 1e20 times others of 1e20) the output is infinite or

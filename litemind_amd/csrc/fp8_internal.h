@@ -19,7 +19,7 @@ struct Fp8Rows {
     int32_t dtype;  // LM_DT_F32, LM_DT_F16 or LM_DT_BF16
     int64_t rows, width, stride;
     int32_t block_rows;  // 1 or 128
-    int32_t group;       // of a matrix: 0, or its rows lie in groups of so many, with as many others between
+    int32_t group;       // of a matrix: 0, or its rows lie in groups of so many (a power of two), as many others between
     uint8_t* q;
     float* scale;
 };
@@ -53,18 +53,19 @@ hipError_t launch_fp8_gemm(const Fp8Product& p, void* workspace, hipStream_t s);
 hipError_t launch_fp8_swiglu(const Fp8Product& p, hipStream_t s);
 
 #if defined(__HIPCC__)
-// The scale of a block whose finite values' largest magnitude is `most`, and
-// what its values are multiplied by: the reciprocal is one correctly rounded
-// division, so a code is off by at most 2^-23 of itself before its rounding.
+// The scale of a block whose finite values' largest magnitude is `most`.
 __device__ inline float fp8_scale(float most) { return __builtin_fmaxf(most / kFp8Largest, 0x1p-126f); }
 
 // The codes of four values already divided by their scale, the first in the
-// lowest byte.  |v| <= 448 (1 + 2^-22), which rounds to 448.  The conversion
-// makes NaN 0xff: bytes of magnitude 0x7f, the only ones that 1 carries into
-// their sign bit, lose their sign.
-__device__ inline uint32_t fp8_pack4(float a, float b, float c, float d) {
+// lowest byte.  |v| <= 448 (1 + 2^-21), which rounds to 448.
+__device__ inline uint32_t fp8_pack4_finite(float a, float b, float c, float d) {
     const int low = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-    const uint32_t v = static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, low, true));
+    return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, low, true));
+}
+// The same, NaN too.  The conversion makes it 0xff: bytes of magnitude 0x7f, the
+// only ones that 1 carries into their sign bit, lose their sign.
+__device__ inline uint32_t fp8_pack4(float a, float b, float c, float d) {
+    const uint32_t v = fp8_pack4_finite(a, b, c, d);
     return v & ~(((v & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u);
 }
 

@@ -536,7 +536,8 @@ struct Work {
         }
     }
     // SwiGLU, each row's largest magnitude over the tile's 128 channels from the
-    // waves that share the row, and the codes through LDS to 16-byte stores.
+    // waves that share the row, and the codes through LDS to 16-byte stores. The
+    // quotients are fp32's: the sums are off by more.
     __device__ __forceinline__ void store_swiglu(const Fp8Product& p, const Stage<Z>& st, char* codes, float* most_of) {
         constexpr int kPitch = kFp8Block + 16;  // a row's 16 lanes write to 16 different banks
         static_assert(BM * kPitch <= Z::kStageBytes);

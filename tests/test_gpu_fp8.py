@@ -99,6 +99,27 @@ def test_quantize_extremes(ctx, block_rows):
     assert (q == want_q).all()
 
 
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_quantize_next_to_middles(ctx, block_rows):
+    """Values a step of fp32 or two from where two codes meet, for largest magnitudes of all kinds."""
+    announce(f"fp8 quantize next to the middles, blocks of {block_rows}")
+    rng = np.random.default_rng(5)
+    most = (rng.uniform(1, 2, 300) * 2.0 ** rng.integers(-110, 100, 300)).astype(np.float32)
+    most[:3] = [448, 1, 448 * 2.0 ** -126]
+    middle = (ref.POSITIVE[:-1] + ref.POSITIVE[1:]) / 2
+    x = np.zeros((len(most), block_rows, 5, 128), np.float32)
+    x[:, 0, :, 1:127] = (middle * most[:, None].astype(np.float64) / 448).astype(np.float32)[:, None]
+    for b, steps in enumerate((-2, -1, 0, 1, 2)):
+        for _ in range(abs(steps)):
+            x[:, 0, b] = np.nextafter(x[:, 0, b], np.float32(np.sign(steps) * np.inf))
+    x[:, 0, :, 127] = -x[:, 0, :, 64]
+    x[:, 0, :, 0] = most[:, None]
+    x = x.reshape(-1, 640)
+    q, s = quantized(ctx, x, "f32", block_rows)
+    want_q, want_s = ref.quantize(x, block_rows)
+    assert (s == want_s).all() and (q == want_q).all()
+
+
 def test_quantize_nothing(ctx):
     announce("fp8 quantize without rows")
     q = Out(ctx, (4,), np.uint8)
