@@ -49,8 +49,10 @@ struct Fp8Product {
 };
 // Sums of products whose reduced axis several workgroups share.
 constexpr int64_t kFp8WorkspaceBytes = 32 << 20;
-hipError_t launch_fp8_gemm(const Fp8Product& p, void* workspace, hipStream_t s);
-hipError_t launch_fp8_swiglu(const Fp8Product& p, hipStream_t s);
+// `beside`: another product of the same kind without offsets, in the same launch
+// (p has offsets then, and neither exact sums but SwiGLU's).
+hipError_t launch_fp8_gemm(const Fp8Product& p, void* workspace, hipStream_t s, const Fp8Product* beside = nullptr);
+hipError_t launch_fp8_swiglu(const Fp8Product& p, hipStream_t s, const Fp8Product* beside = nullptr);
 
 #if defined(__HIPCC__)
 // The scale of a block whose finite values' largest magnitude is `most`.

@@ -122,13 +122,22 @@ __device__ inline void group_rows(const Fp8Product& p, int g, int32_t& first, in
 // The tile of workgroup blockIdx.x, the same in every wave (each looks for it
 // by itself: no barrier). Workgroup b runs on XCD b % 8; every XCD takes a
 // contiguous eighth of the tiles, in which the row tiles of one feature tile
-// follow each other, so that their weights are read from one L2.
-__device__ inline bool find_tile(const Fp8Product& p, int bm, int nts, Tile& t) {
+// follow each other, so that their weights are read from one L2. The first `beside`
+// tiles are another product's, whose group is -1 here, of rows_beside rows.
+__device__ inline bool find_tile(const Fp8Product& p, int bm, int nts, Tile& t, int32_t beside = 0,
+                                 int32_t rows_beside = 0) {
     const int lane = threadIdx.x & 63;
+    // the workgroup's place among all tiles, from which `beside` count back; none: INT32_MIN
     auto share = [&](int32_t total) {
+        total += beside;
         const int32_t xcd = blockIdx.x % kXcds, idx = blockIdx.x / kXcds;
         const int32_t per = total / kXcds, extra = total % kXcds;
-        return idx < per + (xcd < extra ? 1 : 0) ? xcd * per + min(xcd, extra) + idx : -1;
+        return idx < per + (xcd < extra ? 1 : 0) ? xcd * per + min(xcd, extra) + idx - beside : INT32_MIN;
+    };
+    auto take_beside = [&](int32_t tile) {
+        const int32_t mts = (rows_beside + bm - 1) / bm;
+        t = Tile{-1, (tile + beside) % mts, (tile + beside) / mts, 0, rows_beside};
+        return true;
     };
     if (p.offsets == nullptr) {
         const int32_t mts = static_cast<int32_t>((p.rows + bm - 1) / bm);
@@ -158,7 +167,7 @@ __device__ inline bool find_tile(const Fp8Product& p, int bm, int nts, Tile& t) 
     }
     const int32_t tile = share(total);
     if (tile < 0) {
-        return false;
+        return tile != INT32_MIN && take_beside(tile);
     }
     int32_t before = 0;
     for (int g0 = 0; g0 < p.groups; g0 += 64) {
@@ -182,6 +191,10 @@ __device__ inline bool find_tile(const Fp8Product& p, int bm, int nts, Tile& t) 
         before = min(before + __builtin_amdgcn_readlane(sum, 63), kMost);
     }
     return false;
+}
+
+__host__ __device__ inline int32_t tiles_beside(const Fp8Product& q, int bm, int bn) {
+    return static_cast<int32_t>((q.rows + bm - 1) / bm) * ((q.n + bn - 1) / bn);
 }
 
 // The row of a that row i of the groups reads.
@@ -598,16 +611,23 @@ struct Work {
     }
 };
 
-template <class Z, bool EXACT, int WM, int WN, int MI, int NJ>
-__global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2, 2))) void fp8_tile_kernel(Fp8Product p) {
+// BESIDE: the tiles of q, which has no offsets, are computed beside p's.
+template <class Z, bool EXACT, int WM, int WN, int MI, int NJ, bool BESIDE>
+__global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2, 2))) void fp8_tile_kernel(Fp8Product p,
+                                                                                                         Fp8Product q) {
     // one LDS array per stage: the compiler tracks the asynchronous writes by array
     __shared__ __attribute__((aligned(1024))) char s0[Z::kStageBytes], s1[Z::kStageBytes],
         s2[Z::STAGES > 2 ? Z::kStageBytes : 16], s3[Z::STAGES > 3 ? Z::kStageBytes : 16];
     __shared__ float most_of[Z::SWIGLU ? WN * Z::BM : 1];
     char* const bufs[4] = {s0, s1, s2, s3};
     Tile t;
-    if (!find_tile(p, Z::BM, (p.n + Z::CN - 1) / Z::CN, t)) {
+    if (!find_tile(p, Z::BM, (p.n + Z::CN - 1) / Z::CN, t, BESIDE ? tiles_beside(q, Z::BM, Z::CN) : 0,
+                   BESIDE ? static_cast<int32_t>(q.rows) : 0)) {
         return;
+    }
+    if (BESIDE && t.g < 0) {
+        p = q;
+        t.g = 0;
     }
     int first = 0, stages = p.kb;
     if (gridDim.y > 1) {  // a share of the reduced axis, into a plane of fp32 sums of its own
@@ -628,19 +648,24 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2,
 }
 
 template <bool SWIGLU, bool EXACT, int WM, int WN, int MI, int NJ, int STAGES>
-hipError_t launch_tiles(const Fp8Product& p, hipStream_t s, int shares = 1) {
+hipError_t launch_tiles(const Fp8Product& p, const Fp8Product* beside, hipStream_t s, int shares = 1) {
     using Z = Shape<SWIGLU, 16 * WM * MI, 16 * WN * NJ, WM * WN, STAGES>;
     // a group of n rows takes ceil(n / BM) row tiles: at most one more than
     // n / BM for each group that has any
     const int64_t mts = p.offsets == nullptr ? (p.rows + Z::BM - 1) / Z::BM
                                              : p.rows / Z::BM + std::min<int64_t>(p.groups, p.rows);
-    const int64_t tiles = mts * ((p.n + Z::CN - 1) / Z::CN);
+    const int64_t tiles = mts * ((p.n + Z::CN - 1) / Z::CN) + (beside != nullptr ? tiles_beside(*beside, Z::BM, Z::CN) : 0);
     if (tiles > (1 << 22)) {  // 2^31 threads
         return hipErrorInvalidConfiguration;
     }
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(fp8_tile_kernel<Z, EXACT, WM, WN, MI, NJ>),
-                       dim3(static_cast<unsigned>(round_up(tiles, kXcds)), static_cast<unsigned>(shares)), dim3(64 * Z::WAVES),
-                       0, s, p);
+    const dim3 grid(static_cast<unsigned>(round_up(tiles, kXcds)), static_cast<unsigned>(shares)), block(64 * Z::WAVES);
+    if constexpr (SWIGLU || !EXACT) {  // a layer's products
+        if (beside != nullptr) {
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(fp8_tile_kernel<Z, EXACT, WM, WN, MI, NJ, true>), grid, block, 0, s, p, *beside);
+            return hipGetLastError();
+        }
+    }
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(fp8_tile_kernel<Z, EXACT, WM, WN, MI, NJ, false>), grid, block, 0, s, p, p);
     return hipGetLastError();
 }
 
@@ -683,12 +708,17 @@ __device__ __forceinline__ void stream_blocks(const Fp8Product& p, int b0, int s
     }
 }
 
-template <int WAVES, int U>
-__global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(Fp8Product p) {
+template <int WAVES, int U, bool BESIDE>
+__global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(Fp8Product p, Fp8Product q) {
     __shared__ floatx4 sums[WAVES][64];
     Tile t;
-    if (!find_tile(p, 16, (p.n + 15) / 16, t)) {
+    if (!find_tile(p, 16, (p.n + 15) / 16, t, BESIDE ? tiles_beside(q, 16, 16) : 0,
+                   BESIDE ? static_cast<int32_t>(q.rows) : 0)) {
         return;
+    }
+    if (BESIDE && t.g < 0) {
+        p = q;
+        t.g = 0;
     }
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
@@ -723,9 +753,14 @@ int64_t stream_tiles(const Fp8Product& p) {
 }
 
 template <int WAVES, int U>
-hipError_t launch_stream(const Fp8Product& p, hipStream_t s) {
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(fp8_stream_kernel<WAVES, U>),
-                       dim3(static_cast<unsigned>(round_up(stream_tiles(p), kXcds))), dim3(64 * WAVES), 0, s, p);
+hipError_t launch_stream(const Fp8Product& p, const Fp8Product* beside, hipStream_t s) {
+    const int64_t tiles = stream_tiles(p) + (beside != nullptr ? stream_tiles(*beside) : 0);
+    const dim3 grid(static_cast<unsigned>(round_up(tiles, kXcds))), block(64 * WAVES);
+    if (beside != nullptr) {
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(fp8_stream_kernel<WAVES, U, true>), grid, block, 0, s, p, *beside);
+    } else {
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(fp8_stream_kernel<WAVES, U, false>), grid, block, 0, s, p, p);
+    }
     return hipGetLastError();
 }
 
@@ -818,13 +853,16 @@ struct TileChoice {
     int shares = 1;
 };
 template <size_t N>
-TileChoice choose_tile(const Fp8Product& p, const TileCost (&tiles)[N], bool split) {
+TileChoice choose_tile(const Fp8Product& p, const Fp8Product* beside, const TileCost (&tiles)[N], bool split) {
     constexpr int kShares[] = {1, 2, 3, 4, 6, 8, 12};
     TileChoice best;
     double least = 1e30;
     for (size_t i = 0; i < N; ++i) {
         const TileCost& c = tiles[i];
-        const double count = row_tiles(p, c.bm) * static_cast<double>((p.n + c.bn - 1) / c.bn);
+        double count = row_tiles(p, c.bm) * static_cast<double>((p.n + c.bn - 1) / c.bn);
+        if (beside != nullptr) {  // by their stages
+            count += static_cast<double>(tiles_beside(*beside, c.bm, c.bn)) * beside->kb / p.kb;
+        }
         for (const int shares : kShares) {
             const int64_t stages = (p.kb + shares - 1) / shares;
             double t = tile_time(c, count * shares, stages, p.offsets != nullptr);
@@ -848,21 +886,21 @@ TileChoice choose_tile(const Fp8Product& p, const TileCost (&tiles)[N], bool spl
 }
 
 template <bool EXACT>
-hipError_t launch_gemm_tile(const Fp8Product& p, const TileChoice& c, hipStream_t s) {
+hipError_t launch_gemm_tile(const Fp8Product& p, const Fp8Product* beside, const TileChoice& c, hipStream_t s) {
     switch (c.tile) {
         case 0:
-            return launch_tiles<false, EXACT, 1, 4, 2, 2, 3>(p, s, c.shares);
+            return launch_tiles<false, EXACT, 1, 4, 2, 2, 3>(p, beside, s, c.shares);
         case 1:
-            return launch_tiles<false, EXACT, 1, 4, 4, 2, 3>(p, s, c.shares);
+            return launch_tiles<false, EXACT, 1, 4, 4, 2, 3>(p, beside, s, c.shares);
         case 2:
-            return launch_tiles<false, EXACT, 2, 2, 4, 4, 2>(p, s, c.shares);
+            return launch_tiles<false, EXACT, 2, 2, 4, 4, 2>(p, beside, s, c.shares);
         case 4:
             if constexpr (!EXACT) {
-                return launch_tiles<false, false, 2, 4, 8, 4, 2>(p, s, c.shares);
+                return launch_tiles<false, false, 2, 4, 8, 4, 2>(p, beside, s, c.shares);
             }
             [[fallthrough]];
         default:
-            return launch_tiles<false, EXACT, 2, 4, 4, 4, 3>(p, s, c.shares);
+            return launch_tiles<false, EXACT, 2, 4, 4, 4, 3>(p, beside, s, c.shares);
     }
 }
 
@@ -870,31 +908,34 @@ hipError_t launch_gemm_tile(const Fp8Product& p, const TileChoice& c, hipStream_
 // the weights of its 16 features and its rows, stays under 24 MB. One row by 2048
 // channels and 10944 features (23 MB) 6.1 us, 9.9 in tiles; 8 rows (34 MB) 8.3 and
 // 7.6; six experts of 2048 features (18 MB) 5.8 and 8.7, of 5120 (50 MB) 16 and 12.
-bool streams(const Fp8Product& p) {
+int64_t stream_bytes(const Fp8Product& p) {
     const int64_t groups = active_groups(p), rows = std::min<int64_t>(16, (p.rows + groups - 1) / groups);
     const int64_t tiles = stream_tiles(p);
-    return tiles <= 4096 && tiles * p.kb * (16 + rows) * kFp8Block <= (24 << 20);
+    return tiles <= 4096 ? tiles * p.kb * (16 + rows) * kFp8Block : INT32_MAX;
+}
+bool streams(const Fp8Product& p, const Fp8Product* beside) {
+    return stream_bytes(p) + (beside != nullptr ? stream_bytes(*beside) : 0) <= (24 << 20);
 }
 
 }  // namespace
 
-hipError_t launch_fp8_gemm(const Fp8Product& p, void* workspace, hipStream_t s) {
-    if (streams(p)) {
+hipError_t launch_fp8_gemm(const Fp8Product& p, void* workspace, hipStream_t s, const Fp8Product* beside) {
+    if (streams(p, beside)) {
         // all of a wave's loads in flight at once where the axis is short, many
         // waves where it is long (10944 channels: 9.5 us, 11 with four waves)
-        return p.kb <= 12   ? launch_stream<4, 3>(p, s)
-               : p.kb <= 16 ? launch_stream<4, 4>(p, s)
-               : p.kb <= 40 ? launch_stream<8, 2>(p, s)
-                            : launch_stream<16, 2>(p, s);
+        return p.kb <= 12   ? launch_stream<4, 3>(p, beside, s)
+               : p.kb <= 16 ? launch_stream<4, 4>(p, beside, s)
+               : p.kb <= 40 ? launch_stream<8, 2>(p, beside, s)
+                            : launch_stream<16, 2>(p, beside, s);
     }
     const bool exact = p.exact != 0, split = p.offsets == nullptr;
-    const TileChoice c = exact ? choose_tile(p, kExactTiles, split) : choose_tile(p, kFp8Tiles, split);
+    const TileChoice c = exact ? choose_tile(p, beside, kExactTiles, split) : choose_tile(p, beside, kFp8Tiles, split);
     Fp8Product q = p;
     if (c.shares > 1) {
         q.out = workspace;
         q.out_dtype = LM_DT_F32;
     }
-    const hipError_t e = exact ? launch_gemm_tile<true>(q, c, s) : launch_gemm_tile<false>(q, c, s);
+    const hipError_t e = exact ? launch_gemm_tile<true>(q, beside, c, s) : launch_gemm_tile<false>(q, beside, c, s);
     if (e != hipSuccess || c.shares == 1) {
         return e;
     }
@@ -904,19 +945,19 @@ hipError_t launch_fp8_gemm(const Fp8Product& p, void* workspace, hipStream_t s) 
     return hipGetLastError();
 }
 
-hipError_t launch_fp8_swiglu(const Fp8Product& p, hipStream_t s) {
+hipError_t launch_fp8_swiglu(const Fp8Product& p, hipStream_t s, const Fp8Product* beside) {
     const bool exact = p.exact != 0;
-    switch ((exact ? choose_tile(p, kSwigluTiles, false) : choose_tile(p, kSwigluFp8Tiles, false)).tile) {
+    switch ((exact ? choose_tile(p, beside, kSwigluTiles, false) : choose_tile(p, beside, kSwigluFp8Tiles, false)).tile) {
         case 0:
-            return launch_tiles<true, true, 1, 8, 2, 2, 3>(p, s);
+            return launch_tiles<true, true, 1, 8, 2, 2, 3>(p, beside, s);
         case 1:
-            return launch_tiles<true, true, 1, 4, 2, 4, 2>(p, s);
+            return launch_tiles<true, true, 1, 4, 2, 4, 2>(p, beside, s);
         case 2:
-            return launch_tiles<true, true, 1, 8, 4, 2, 3>(p, s);
+            return launch_tiles<true, true, 1, 8, 4, 2, 3>(p, beside, s);
         case 3:
-            return exact ? launch_tiles<true, true, 2, 4, 4, 4, 3>(p, s) : launch_tiles<true, false, 2, 4, 4, 4, 3>(p, s);
+            return exact ? launch_tiles<true, true, 2, 4, 4, 4, 3>(p, beside, s) : launch_tiles<true, false, 2, 4, 4, 4, 3>(p, beside, s);
         default:
-            return launch_tiles<true, false, 2, 4, 8, 4, 2>(p, s);
+            return launch_tiles<true, false, 2, 4, 8, 4, 2>(p, beside, s);
     }
 }
 

@@ -587,11 +587,10 @@ int ensure_fp8_workspace(lm_context* ctx, int64_t tokens) {
     return LM_OK;
 }
 
-// Both products of one FFN in FP8: `first` and `count` the rows of its
-// activations and outputs (slots of routed experts in permuted order, then the
-// shared experts' rows or the dense FFN's).
-int fp8_ffn(lm_context* ctx, const Fp8Ffn& f, int64_t inter, int64_t T, const lm::RouteBufs* rb, uint8_t* act,
-            float* act_scale, float* down_out, const lm::Fp8Scratch& sc, bool down) {
+// A product of one FFN in FP8, of its gate and up matrices or of its down one; rb:
+// of the routed experts.
+lm::Fp8Product fp8_product(const lm_context* ctx, const Fp8Ffn& f, int64_t inter, int64_t T, const lm::RouteBufs* rb,
+                           uint8_t* act, float* act_scale, float* down_out, const lm::Fp8Scratch& sc, bool down) {
     const Workspace& w = ctx->ws;
     lm::Fp8Product p{};
     p.groups = rb != nullptr ? ctx->E : 1;
@@ -625,22 +624,29 @@ int fp8_ffn(lm_context* ctx, const Fp8Ffn& f, int64_t inter, int64_t T, const lm
     }
     p.nb = static_cast<int32_t>(lm::fp8_blocks(p.n));
     p.kb = static_cast<int32_t>(lm::fp8_blocks(p.k));
-    LM_HIP(down ? lm::launch_fp8_gemm(p, sc.workspace, ctx->stream) : lm::launch_fp8_swiglu(p, ctx->stream));
-    return LM_OK;
+    return p;
 }
 
+// Up to so many tokens the shared experts' products lie in the launches of the
+// routed experts', whose tiles leave CUs empty or wait for memory; more fill the
+// CUs with tiles of their own. A layer of 64 experts at 1, 128, 512 and 2048 tokens
+// takes 59, 153, 207 and 377 us in shared launches, 72, 174, 205 and 341 in
+// launches of their own; one of 160 89, 787, 1022 and 1305, and 121, 820, 1006 and
+// 1287.
+constexpr int64_t kFp8Beside = 128;
+
 // launch_expert_kernels in FP8: the tokens' blocks, gate/up and down of the
-// routed experts and of the shared (or dense) FFN into ws.down_out.
+// routed experts (slots in permuted order) and of the shared (or dense) FFN, whose
+// rows follow, into ws.down_out.
 int launch_expert_kernels_fp8(lm_context* ctx, const Layer& L, const float* x, int64_t T, const lm::RouteBufs& rb) {
     lm::Fp8Scratch sc{};
-    int rc = lm::fp8_scratch(ctx, &sc);
+    const int rc = lm::fp8_scratch(ctx, &sc);
     if (rc != LM_OK) {
         return rc;
     }
     const Workspace& w = ctx->ws;
     const int64_t TK = L.dense ? 0 : T * ctx->K, inter = L.dense ? ctx->D : ctx->S;
-    uint8_t* const other_act = w.fp8_act + TK * ctx->I;
-    float* const other_scale = w.fp8_act_scale + TK * lm::fp8_blocks(ctx->I);
+    const bool other = L.fp8.other.gate_up != nullptr;
     stage_mark(ctx, 2);
     LM_HIP(lm::launch_fp8_quantize(
         lm::Fp8Rows{x, LM_DT_F32, T, ctx->H, ctx->H, 1, 0, w.fp8_x, w.fp8_x_scale}, ctx->stream));
@@ -648,14 +654,24 @@ int launch_expert_kernels_fp8(lm_context* ctx, const Layer& L, const float* x, i
         if (down) {
             stage_mark(ctx, 3);
         }
+        lm::Fp8Product routed{}, rest{};
         if (!L.dense) {
-            rc = fp8_ffn(ctx, L.fp8.routed, ctx->I, T, &rb, w.fp8_act, w.fp8_act_scale, w.down_out, sc, down);
+            routed = fp8_product(ctx, L.fp8.routed, ctx->I, T, &rb, w.fp8_act, w.fp8_act_scale, w.down_out, sc, down);
         }
-        if (rc == LM_OK && L.fp8.other.gate_up != nullptr) {
-            rc = fp8_ffn(ctx, L.fp8.other, inter, T, nullptr, other_act, other_scale, w.down_out + TK * ctx->H, sc, down);
+        if (other) {
+            rest = fp8_product(ctx, L.fp8.other, inter, T, nullptr, w.fp8_act + TK * ctx->I,
+                               w.fp8_act_scale + TK * lm::fp8_blocks(ctx->I), w.down_out + TK * ctx->H, sc, down);
         }
-        if (rc != LM_OK) {
-            return rc;
+        const bool beside = !L.dense && other && T <= kFp8Beside;
+        const auto launch = [&](const lm::Fp8Product& p) {
+            const lm::Fp8Product* const q = beside ? &rest : nullptr;
+            return down ? lm::launch_fp8_gemm(p, sc.workspace, ctx->stream, q) : lm::launch_fp8_swiglu(p, ctx->stream, q);
+        };
+        if (!L.dense) {
+            LM_HIP(launch(routed));
+        }
+        if (other && !beside) {
+            LM_HIP(launch(rest));
         }
     }
     return LM_OK;

@@ -84,7 +84,7 @@ def near(got, want, parts, exact):
     assert (np.linalg.norm(got - want, axis=-1) <= 1e-2 * np.linalg.norm(parts + np.zeros_like(want), axis=-1)).all()
 
 
-TOKENS = [1, 2, 3, 17, 100, 300, 1500]
+TOKENS = [1, 2, 3, 17, 100, 128, 129, 300, 1500]
 
 
 @pytest.mark.parametrize("T", TOKENS)
