@@ -905,16 +905,19 @@ hipError_t launch_gemm_tile(const Fp8Product& p, const Fp8Product* beside, const
 }
 
 // Whether the kernel of few rows is the faster: what its workgroups read, each
-// the weights of its 16 features and its rows, stays under 24 MB. One row by 2048
-// channels and 10944 features (23 MB) 6.1 us, 9.9 in tiles; 8 rows (34 MB) 8.3 and
-// 7.6; six experts of 2048 features (18 MB) 5.8 and 8.7, of 5120 (50 MB) 16 and 12.
+// the weights of its 16 features and its rows, stays under 28 MB. A call in turn
+// with others' and by itself, and the same in tiles: four rows by 10944 channels
+// and 2048 features (27 MB) 5.7 and 10.6 us, 9.1 and 11.3; by 2048 and 10944 5.3
+// and 6.9, 5.4 and 7.8; twelve (37 MB) 6.1 and 8.6, 5.3 and 7.8; six experts of
+// 2048 features (18 MB) 5.6 and 5.9, 5.5 and 7.3, of 5120 (48 MB) 13 and 17, 6.3
+// and 12.
 int64_t stream_bytes(const Fp8Product& p) {
     const int64_t groups = active_groups(p), rows = std::min<int64_t>(16, (p.rows + groups - 1) / groups);
     const int64_t tiles = stream_tiles(p);
     return tiles <= 4096 ? tiles * p.kb * (16 + rows) * kFp8Block : INT32_MAX;
 }
 bool streams(const Fp8Product& p, const Fp8Product* beside) {
-    return stream_bytes(p) + (beside != nullptr ? stream_bytes(*beside) : 0) <= (24 << 20);
+    return stream_bytes(p) + (beside != nullptr ? stream_bytes(*beside) : 0) <= (28 << 20);
 }
 
 }  // namespace
