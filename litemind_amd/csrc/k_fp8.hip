@@ -261,6 +261,13 @@ __device__ inline float swiglu(float gate, float up) {
 // bytes of every row, loaded straight to LDS STAGES - 1 stages ahead, with the
 // rows' and the weights' scales of the block.
 //
+// What bounds it: many rows the matrix cores and the FMAs or conversions beside them,
+// under whose load the clock falls (2048 x 5120 x 16384 160 us in turn with others,
+// 2.14 PFLOP/s; fp32 sums, experts of 12288 rows, 104 and 189 us, 0.7 PFLOP/s of rows
+// that count); few rows of many experts their weights (187 MB 31 us, 1731 MB 278 us:
+// 6.0 and 6.2 TB/s). Larger tiles read less and wait longer: which is taken is decided
+// by their costs below.
+//
 // LDS rows are 128 bytes: chunk c of row r lies at chunk position c ^ (r / 2).
 // A 16-byte read takes sixteen lanes a clock over 64 banks (256 bytes, two
 // rows); whether those are lanes 0 .. 15 or, as it seems, 0 .. 3, 12 .. 15 and
@@ -424,7 +431,7 @@ struct Work {
     // The products of a stage: row block i's on the matrix cores beside block
     // i - 1's FMAs and the reads of block i + 1. between(i) issues a part of the
     // next loads: a wave's run of them would wait for each to be accepted (256 x
-    // 256 x 16384: 209 -> 201 us, 128 x 256 of three stages 265 -> 223).
+    // 256 in tiles, 2048 x 5120 x 16384: 209 -> 201 us, 128 x 256 265 -> 223).
     template <class Between>
     __device__ __forceinline__ void multiply(const char* cur, Between between) {
         const float w0 = *reinterpret_cast<const float*>(cur + ws);
@@ -674,7 +681,9 @@ hipError_t launch_tiles(const Fp8Product& p, const Fp8Product* beside, hipStream
 // Tiles of 16 rows at most by 16 features: the weights are read once, straight to
 // registers, and the waves of a workgroup take turns at the scale blocks of the
 // reduced axis; their sums are added up in LDS, wave by wave. What counts is the
-// bytes in flight: U blocks of 2 KB a wave.
+// bytes in flight: U blocks of 2 KB a wave. One row by 10944 x 2048 (22 MB) 8.8 us,
+// 5.4 in turn with others (4.2 TB/s), six experts of 2048 x 1408 (17 MB) 7.3 and 5.5;
+// by themselves a round trip to memory and its waiting make up half of it.
 //
 // Scale blocks b0, b0 + step, ... (U of them, as far as there are any) of 16
 // weight rows and the rows of a.

@@ -353,6 +353,7 @@ int allocate_layer(lm_context* ctx, int32_t layer, bool dense) {
     L.slab_bytes = 2 * total + t_bytes;
     L.allocated = true;
     L.dense = dense;
+    L.fp8.ready = false;  // of another kind, maybe, whatever comes of the upload
     ctx->resident += 2 * total + t_bytes;
     return LM_OK;
 }
