@@ -33,6 +33,7 @@
 #include "fp8_internal.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace lm {
 namespace {
@@ -192,6 +193,9 @@ __device__ inline bool find_tile(const Fp8Product& p, int bm, int nts, Tile& t, 
     }
     return false;
 }
+
+// Floats from one share's sums to the next one's: 16-byte aligned.
+__host__ __device__ inline int64_t plane(int64_t count) { return (count + 3) / 4 * 4; }
 
 __host__ __device__ inline int32_t tiles_beside(const Fp8Product& q, int bm, int bn) {
     return static_cast<int32_t>((q.rows + bm - 1) / bm) * ((q.n + bn - 1) / bn);
@@ -430,8 +434,8 @@ struct Work {
     }
     // The products of a stage: row block i's on the matrix cores beside block
     // i - 1's FMAs and the reads of block i + 1. between(i) issues a part of the
-    // next loads: a wave's run of them would wait for each to be accepted (256 x
-    // 256 in tiles, 2048 x 5120 x 16384: 209 -> 201 us, 128 x 256 265 -> 223).
+    // next loads: a wave's run of them would wait for each to be accepted (2048 x
+    // 5120 x 16384 in tiles of 256 x 256: 209 -> 201 us, of 128 x 256 265 -> 223).
     template <class Between>
     __device__ __forceinline__ void multiply(const char* cur, Between between) {
         const float w0 = *reinterpret_cast<const float*>(cur + ws);
@@ -641,7 +645,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2,
         const int per = (p.kb + gridDim.y - 1) / gridDim.y;
         first = blockIdx.y * per;
         stages = min(per, p.kb - first);
-        p.out = static_cast<float*>(p.out) + blockIdx.y * p.rows * p.n;
+        p.out = static_cast<float*>(p.out) + blockIdx.y * plane(p.rows * p.n);
     }
     const Stage<Z> st{bufs, t, t.mt * Z::BM, t.nt * Z::CN, static_cast<int>(threadIdx.x & 63),
                       __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)), first, stages};
@@ -782,15 +786,17 @@ __global__ __launch_bounds__(256) void fp8_join_kernel(Fp8Product p, const float
     }
     // rows follow each other without a gap: a row of all values, cut in fours
     p.n = static_cast<int32_t>(min(count - at, int64_t{4}));
+    constexpr int kAtOnce = 4;  // loads in flight
     floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int i = 0; i < shares; ++i) {
-        const float* const from = sums + i * count + at;
-        if (p.n == 4 && count % 4 == 0) {
-            v += *reinterpret_cast<const floatx4*>(from);
-        } else {
-            for (int u = 0; u < p.n; ++u) {
-                v[u] += from[u];
-            }
+    for (int i = 0; i < shares; i += kAtOnce) {
+        floatx4 part[kAtOnce];
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) {
+            part[j] = *reinterpret_cast<const floatx4*>(sums + min(i + j, shares - 1) * plane(count) + at);
+        }
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) {
+            v += i + j < shares ? part[j] : floatx4{0.0f, 0.0f, 0.0f, 0.0f};
         }
     }
     p.out = static_cast<char*>(p.out) + at * (p.out_dtype == LM_DT_F32 ? 4 : 2);
@@ -800,21 +806,20 @@ __global__ __launch_bounds__(256) void fp8_join_kernel(Fp8Product p, const float
 // ---- which kernel ----
 
 // What a tile costs, in microseconds: a stage where at most half the places of
-// workgroups are taken and where all are (measured with operands that lie in the
-// L2s, 2048 and 8192 reduced channels), a stage with weights for each group, and
-// what is no stage's (finding the tile, its first loads, its outputs). A group's
-// few row tiles wait together for weights from memory that no tile has read
-// before, so that the larger tile gains there: fitted to the experts of layers
-// with 64 x 1408 x 2048 and 160 x 1536 x 5120 at 32 to 4096 tokens (gate and up
-// of 1024 tokens by the latter: 648 us by two 32 x 256 tiles a CU, which the
-// other figures take, 548 by 128 x 256; at 256 tokens 483 and 519). Up to 128 x
-// 128 two workgroups share a CU.
+// workgroups are taken and where all are (measured with 1408 to 16384 reduced
+// channels), a stage with weights for each group, and what is no stage's (finding
+// the tile, its first loads, its outputs). A group's few row tiles wait together
+// for weights from memory that no tile has read before, so that the larger tile
+// gains there: fitted to the experts of layers with 64 x 1408 x 2048 and 160 x 1536
+// x 5120 at 32 to 4096 tokens (gate and up of 1024 tokens by the latter: 648 us by
+// two 32 x 256 tiles a CU, which the other figures take, 548 by 128 x 256; at 256
+// tokens 483 and 519). Up to 128 x 128 two workgroups share a CU.
 struct TileCost {
     int bm, bn, places;
     float solo, full, grouped, fixed;
 };
-constexpr TileCost kFp8Tiles[] = {{32, 128, 512, 0.29f, 0.49f, 0.90f, 1.5f},
-                                  {64, 128, 512, 0.38f, 0.72f, 1.25f, 3.0f},
+constexpr TileCost kFp8Tiles[] = {{32, 128, 512, 0.33f, 0.62f, 0.90f, 1.5f},
+                                  {64, 128, 512, 0.38f, 0.85f, 1.25f, 3.0f},
                                   {128, 128, 512, 0.71f, 1.05f, 1.80f, 5.0f},
                                   {128, 256, 256, 0.79f, 1.02f, 1.70f, 7.0f},
                                   {256, 256, 256, 1.32f, 1.72f, 2.15f, 11.0f}};
@@ -847,16 +852,31 @@ double row_tiles(const Fp8Product& p, int bm) {
     return std::max(groups, static_cast<double>(p.rows) / bm + 0.5 * groups);
 }
 
+// The time of all tiles: rounds in which all places are taken, and one of the rest.
+// Where two workgroups share a CU, one more tile than CUs makes some CUs run two (128
+// stages in 258 tiles of 64 x 128, fp32 sums, 120 us; 79 in 240); one to a CU, they
+// share the memory and the clock alone. (700 rows by 10944 x 16384 in 258 tiles of 128
+// x 256, a round and two tiles, 399 us; in 946 of 64 x 128 280.) Of groups the number
+// of tiles is a guess: half a round more.
 double tile_time(const TileCost& c, double tiles, int64_t stages, bool grouped) {
-    const double stage = 2.0 * tiles <= c.places ? c.solo : grouped ? c.grouped : c.full;
-    const double per = static_cast<double>(stages) * stage + c.fixed;
-    return tiles <= c.places ? per : per * (tiles / c.places + 0.5);
+    const double n = static_cast<double>(stages);
+    if (grouped) {
+        const double per = n * (2.0 * tiles <= c.places ? c.solo : c.grouped) + c.fixed;
+        return tiles <= c.places ? per : per * (tiles / c.places + 0.5);
+    }
+    const double rounds = std::floor(tiles / c.places), rest = tiles / c.places - rounds;
+    const double past = 2.0 * rest - 1.0;
+    const double stage = past <= 0.0       ? c.solo
+                         : c.places > 256 ? std::max<double>(c.solo, (0.8 + 0.2 * past) * c.full)
+                                          : c.solo + past * (c.full - c.solo);
+    return rounds * (n * c.full + c.fixed) + (rest > 0.0 ? n * stage + c.fixed : 0.0);
 }
 
 // Where tiles leave places empty and the reduced axis is long, several
 // workgroups share a tile's reduced axis, and a second launch joins their sums:
-// that costs 4 us and their way through memory. One row by 16384 x 5120: 25 us in
-// one share, 17 in four; 100 rows by 10944 x 2048: 28 and 15.
+// that costs 5 us and their way through memory (6 TB/s). 80 rows by 16384 channels
+// and 10944 features, fp32: 69 us in two shares, 60 in four; 40 by 10944 and 2048:
+// 13.4 in four, 10.7 in eight.
 struct TileChoice {
     int tile = 0;
     int shares = 1;
@@ -876,11 +896,11 @@ TileChoice choose_tile(const Fp8Product& p, const Fp8Product* beside, const Tile
             const int64_t stages = (p.kb + shares - 1) / shares;
             double t = tile_time(c, count * shares, stages, p.offsets != nullptr);
             if (shares > 1) {
-                const int64_t sums = p.rows * p.n * shares;
+                const int64_t sums = plane(p.rows * p.n) * shares;
                 if (!split || stages < 4 || count * shares > c.places || 4 * sums > kFp8WorkspaceBytes) {
                     break;
                 }
-                t += 4.0 + 4.0 * static_cast<double>(2 * sums + p.rows * p.n) / 4e6;
+                t += 5.0 + 4.0 * static_cast<double>(2 * sums + p.rows * p.n) / 6e6;
             }
             if (t < least) {
                 least = t;
