@@ -1866,6 +1866,9 @@ int lm_fp8_layer(lm_context* ctx, int32_t layer, int32_t only) {
         L.expert_present.clear();
         L.shared = lm::FfnDev{};
         L.dense_ffn = lm::FfnDev{};
+        // as long as this kind's groups, where the next upload may be of the other kind
+        LM_HIP(hipFree(L.table));
+        L.table = nullptr;
     }
     f.ready = true;
     return LM_OK;
