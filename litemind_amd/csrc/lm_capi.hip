@@ -235,6 +235,7 @@ struct lm_context {
     lm::ServeState* serve = nullptr;     // the operators of litemind_serving.h, at their first call
     lm::Fp8State* fp8 = nullptr;         // the grouped products of litemind_fp8.h, at their first call
     int32_t graphs = 0;  // live lm_stack_graph captures (they hold the workspace's pointers)
+    int32_t fp8_graphs = 0;  // those of LM_PATH_FP8 (they alone hold the FP8 weights' and workspace's)
     // lm_clock_probe_*: its own stream (default priority) and sample buffer
     hipStream_t probe_stream = nullptr;
     uint64_t* probe_buf = nullptr;
@@ -560,7 +561,7 @@ int ensure_fp8_workspace(lm_context* ctx, int64_t tokens) {
     if (w.fp8_tokens >= tokens) {
         return LM_OK;
     }
-    if (ctx->graphs > 0) {
+    if (ctx->fp8_graphs > 0) {
         return fail(LM_EINVAL, "a captured stack graph holds the workspace (FP8: sized for " + std::to_string(w.fp8_tokens) +
                                    " tokens); destroy it before a call with " + std::to_string(tokens));
     }
@@ -1803,7 +1804,7 @@ int lm_fp8_layer(lm_context* ctx, int32_t layer, int32_t only) {
     Fp8Layer& f = L.fp8;
     f.ready = false;
     if (f.slab == nullptr || f.bytes != static_cast<size_t>(total)) {
-        if (f.slab != nullptr && ctx->graphs > 0) {
+        if (f.slab != nullptr && ctx->fp8_graphs > 0) {
             return fail(LM_EINVAL, "a captured stack graph holds the layer's FP8 weights of another size");
         }
         LM_HIP(hipStreamSynchronize(ctx->stream));
@@ -2316,6 +2317,7 @@ int lm_stack_graph_create(lm_context* ctx, int32_t first_layer, int32_t last_lay
     }
     *graph = new lm_stack_graph{ctx, g, exec, first_layer, last_layer, path};
     ++ctx->graphs;
+    ctx->fp8_graphs += path == LM_PATH_FP8 ? 1 : 0;
     return LM_OK;
     LM_GUARD_END
 }
@@ -2350,6 +2352,7 @@ int lm_stack_graph_destroy(lm_stack_graph* graph) {
     (void)hipGraphExecDestroy(graph->exec);
     (void)hipGraphDestroy(graph->graph);
     --graph->ctx->graphs;
+    graph->ctx->fp8_graphs -= graph->path == LM_PATH_FP8 ? 1 : 0;
     delete graph;
     return LM_OK;
     LM_GUARD_END

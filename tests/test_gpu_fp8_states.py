@@ -49,3 +49,54 @@ def test_another_kind_after_only(kinds):
                 assert (a == b).all(), (kind, path)
             ctx.fp8_layer(0, only=True)
             assert (outputs(ctx, kind, SMALL, [lm.PATH_FP8])[0] == want[-1]).all()
+
+
+def test_beside_a_graph_of_another_path():
+    """A live graph of the MFMA path holds nothing of the FP8 path, whose calls grow their workspace beside it; a live
+    graph of the FP8 path holds it."""
+    announce("fp8 layers: calls beside a live graph of another path")
+    d = dataclasses.replace(SMALL, experts=12)
+    with lm.Context(d.moe_config(num_layers=1)) as ctx:
+        upload(ctx, "moe", d)
+        ctx.upload_norm(0, np.ones(d.hidden, np.float32))
+        want = {}
+        with lm.Context(d.moe_config(num_layers=1)) as fresh:
+            upload(fresh, "moe", d)
+            fresh.fp8_layer(0)
+            for n in (3, 17, T):
+                x, y = fresh.to_device(wl.tokens(5, n, d.hidden)), fresh.empty((n, d.hidden))
+                fresh.moe_forward(0, x, n, y, path=lm.PATH_FP8)
+                want[n] = y.download()
+        h0 = wl.tokens(6, T, d.hidden)
+        h = ctx.to_device(h0)
+        ctx.stack_forward(0, 0, h, T, path=lm.PATH_MFMA)
+        once = h.download()
+
+        def fp8(n):
+            x, y = ctx.to_device(wl.tokens(5, n, d.hidden)), ctx.empty((n, d.hidden))
+            ctx.moe_forward(0, x, n, y, path=lm.PATH_FP8)
+            assert (y.download() == want[n]).all(), n
+
+        graph = ctx.stack_graph_create(0, 0, h, T, path=lm.PATH_MFMA)
+        try:
+            ctx.fp8_layer(0)  # the layer's first FP8 weights, and the path's first workspace
+            for n in (3, 17, T):
+                h.upload(h0)
+                fp8(n)
+                ctx.stack_graph_launch(graph)
+                assert (h.download() == once).all(), n
+        finally:
+            ctx.stack_graph_destroy(graph)
+        more = T + 24  # once the FP8 graph holds them, more tokens than T are refused
+        h.upload(h0)
+        graph = ctx.stack_graph_create(0, 0, h, T, path=lm.PATH_FP8)
+        try:
+            x, y = ctx.empty((more, d.hidden)).zero(), ctx.empty((more, d.hidden))
+            with pytest.raises(lm.LmError) as e:
+                ctx.moe_forward(0, x, more, y, path=lm.PATH_FP8)
+            assert e.value.status == -1
+            fp8(T)
+        finally:
+            ctx.stack_graph_destroy(graph)
+        ctx.moe_forward(0, x, more, y, path=lm.PATH_FP8)
+        ctx.synchronize()
