@@ -13,6 +13,7 @@
 #include "serve_internal.h"
 
 #include <algorithm>
+#include <array>
 #include <cstdio>
 #include <cstring>
 #include <exception>
@@ -79,6 +80,7 @@ struct Fp8Ffn {
 struct Fp8Layer {
     void* slab = nullptr;
     size_t bytes = 0;
+    std::array<int64_t, 8> sizes{};  // bytes of each FFN's arrays in turn, the routed experts' first
     Fp8Ffn routed;
     Fp8Ffn other;        // the shared experts, or the dense FFN
     bool ready = false;  // holds the weights uploaded last
@@ -1795,17 +1797,18 @@ int lm_fp8_layer(lm_context* ctx, int32_t layer, int32_t only) {
     }
     const int64_t hb = lm::fp8_blocks(H), ib = lm::fp8_blocks(I), ob = lm::fp8_blocks(O);
     auto padded = [](int64_t bytes) { return (bytes + 255) / 256 * 256; };
-    const int64_t sizes[8] = {padded(E * 2 * I * H), padded(4 * E * 2 * ib * hb), padded(E * H * I), padded(4 * E * hb * ib),
-                              padded(2 * O * H),     padded(4 * 2 * ob * hb),     padded(H * O),     padded(4 * hb * ob)};
+    const std::array<int64_t, 8> sizes = {padded(E * 2 * I * H), padded(4 * E * 2 * ib * hb), padded(E * H * I),
+                                          padded(4 * E * hb * ib), padded(2 * O * H), padded(4 * 2 * ob * hb),
+                                          padded(H * O), padded(4 * hb * ob)};
     int64_t total = 0;
     for (const int64_t bytes : sizes) {
         total += bytes;
     }
     Fp8Layer& f = L.fp8;
     f.ready = false;
-    if (f.slab == nullptr || f.bytes != static_cast<size_t>(total)) {
+    if (f.slab == nullptr || f.sizes != sizes) {
         if (f.slab != nullptr && ctx->fp8_graphs > 0) {
-            return fail(LM_EINVAL, "a captured stack graph holds the layer's FP8 weights of another size");
+            return fail(LM_EINVAL, "a captured stack graph holds the layer's FP8 weights of another kind or size");
         }
         LM_HIP(hipStreamSynchronize(ctx->stream));
         LM_HIP(hipFree(f.slab));
@@ -1817,6 +1820,7 @@ int lm_fp8_layer(lm_context* ctx, int32_t layer, int32_t only) {
             return fail(LM_ENOMEM, "FP8 weights of " + std::to_string(total) + " bytes: " + hipGetErrorString(err));
         }
         f.bytes = static_cast<size_t>(total);
+        f.sizes = sizes;
         ctx->resident += f.bytes;
     }
     char* next = static_cast<char*>(f.slab);

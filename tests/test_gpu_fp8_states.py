@@ -100,3 +100,32 @@ def test_beside_a_graph_of_another_path():
             ctx.stack_graph_destroy(graph)
         ctx.moe_forward(0, x, more, y, path=lm.PATH_FP8)
         ctx.synchronize()
+
+
+def test_another_kind_under_a_graph():
+    """A graph of a MoE layer's FP8 weights, and then a dense FFN in that layer whose FP8 weights take as many bytes."""
+    announce("fp8 layers: another kind under a live graph")
+    d = dataclasses.replace(SMALL, hidden=128, inter=128, experts=8, top_k=2, n_shared=0, dense_inter=1024)
+    with lm.Context(d.moe_config(num_layers=1)) as ctx:
+        upload(ctx, "moe", d)
+        ctx.upload_norm(0, np.ones(d.hidden, np.float32))
+        ctx.fp8_layer(0, only=True)
+        as_moe = ctx.resident_bytes()
+        h = ctx.to_device(wl.tokens(6, T, d.hidden))
+        graph = ctx.stack_graph_create(0, 0, h, T, path=lm.PATH_FP8)
+        try:
+            upload(ctx, "dense", d)
+            for call in (lambda: ctx.fp8_layer(0), lambda: ctx.stack_graph_launch(graph)):
+                with pytest.raises(lm.LmError) as e:
+                    call()
+                assert e.value.status in (-1, -4)
+        finally:
+            ctx.stack_graph_destroy(graph)
+        ctx.fp8_layer(0)
+        got = outputs(ctx, "dense", d)
+        with lm.Context(d.moe_config(num_layers=1)) as fresh:
+            upload(fresh, "dense", d)
+            fresh.fp8_layer(0)
+            assert all((a == b).all() for a, b in zip(got, outputs(fresh, "dense", d)))
+        ctx.fp8_layer(0, only=True)
+        assert ctx.resident_bytes() == as_moe  # the sizes that this test is about
