@@ -118,7 +118,8 @@ int lm_fp8_grouped_swiglu(lm_context* ctx, const lm_fp8_groups* groups, const ui
  * An upload into the layer ends its FP8 weights until the next lm_fp8_layer;
  * after only = 1 all its FFN weights are uploaded again.  H and the FFNs' widths
  * in multiples of 16 up to 2^20, gate and up together under 2^32 weights.
- * LM_EINVAL with only = 1 while stack graphs are alive. */
+ * LM_EINVAL while the context's stream is being captured, and with only = 1 while
+ * stack graphs are alive. */
 int lm_fp8_layer(lm_context* ctx, int32_t layer, int32_t only);
 
 #ifdef __cplusplus

@@ -1788,10 +1788,16 @@ int lm_fp8_layer(lm_context* ctx, int32_t layer, int32_t only) {
         return fail(LM_EINVAL, "FP8 weights take widths up to 2^20 and under 2^32 weights in gate and up together");
     }
     rc = set_device(ctx);
-    lm::Fp8Scratch sc{};
-    if (rc == LM_OK) {
-        rc = lm::fp8_scratch(ctx, &sc);
+    if (rc != LM_OK) {
+        return rc;
     }
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    LM_HIP(hipStreamIsCapturing(ctx->stream, &capture));
+    if (capture != hipStreamCaptureStatusNone) {  // the layer would pass for ready with nothing computed
+        return fail(LM_EINVAL, "lm_fp8_layer cannot be captured");
+    }
+    lm::Fp8Scratch sc{};
+    rc = lm::fp8_scratch(ctx, &sc);
     if (rc != LM_OK) {
         return rc;
     }

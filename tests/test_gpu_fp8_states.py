@@ -4,9 +4,11 @@ import dataclasses
 import numpy as np
 import pytest
 
+import fp8_ref as ref
 import litemind_amd as lm
 from conftest import announce
 from litemind_amd import workload as wl
+from test_gpu_serving_run import Hip
 
 pytestmark = pytest.mark.gpu
 
@@ -129,3 +131,35 @@ def test_another_kind_under_a_graph():
             assert all((a == b).all() for a, b in zip(got, outputs(fresh, "dense", d)))
         ctx.fp8_layer(0, only=True)
         assert ctx.resident_bytes() == as_moe  # the sizes that this test is about
+
+
+def test_layers_are_not_captured():
+    """lm_fp8_layer under capture is refused and ends neither the capture nor the layer's FP8 weights."""
+    announce("fp8 layers: lm_fp8_layer under capture")
+    with lm.Context(SMALL.moe_config(num_layers=2)) as ctx:
+        hip = Hip(ctx)
+        for layer in (0, 1):
+            upload(ctx, "dense", SMALL, layer)
+        ctx.fp8_layer(0)
+        want = outputs(ctx, "dense", SMALL)
+        said = []
+        x = np.random.default_rng(1).standard_normal((4, 128)).astype(np.float32)
+        dx, q, s = ctx.to_device(x), ctx.empty((4, 128), np.uint8), ctx.empty((4, 1))
+
+        def work():
+            for layer in (0, 1):  # with FP8 weights, and without
+                try:
+                    ctx.fp8_layer(layer)
+                except lm.LmError as e:
+                    said.append(e.status)
+            ctx.fp8_quantize(dx, 4, 128, q, s)
+
+        graph = hip.capture(work)
+        hip.replay(graph[1])
+        ctx.synchronize()
+        hip.free(*graph)
+        assert said == [-1, -1]
+        assert (q.download() == ref.quantize(x)[0]).all()
+        assert all((a == b).all() for a, b in zip(outputs(ctx, "dense", SMALL), want))
+        ctx.fp8_layer(1)
+        assert all((a == b).all() for a, b in zip(outputs(ctx, "dense", SMALL, layer=1), want))
