@@ -56,7 +56,9 @@ int lm_fp8_quantize(lm_context* ctx, const void* x_dev, int32_t dtype, int64_t r
  * those of the FP8 matrix cores, off by 1.4e-5 to 4e-5 of their norm and at most
  * 2^-10 of the sum of magnitudes, rounded once at the end.  in_features a multiple
  * of 16 up to 2^20, out_features at most 2^24; rows, rows * in_features and
- * out_features * in_features under 2^31, 2^32 and 2^32.  a_dev, w_dev and out_dev
+ * out_features * in_features under 2^31, 2^32 and 2^32; and one launch has room for
+ * 2^22 tiles, of 128 rows by 256 features at most (16-bit outputs 256 by 256; of
+ * groups each has a row tile begun): LM_EINVAL past it.  a_dev, w_dev and out_dev
  * 16-byte aligned; out_dev overlaps no input.  Asynchronous. */
 int lm_fp8_gemm(lm_context* ctx, const uint8_t* a_dev, const float* a_scale_dev, int64_t rows, const uint8_t* w_dev,
                 const float* w_scale_dev, int64_t out_features, int64_t in_features, void* out_dev, int32_t out_dtype);
@@ -94,11 +96,28 @@ int lm_fp8_grouped_gemm(lm_context* ctx, const lm_fp8_groups* groups, const uint
  *     act_i = gate_i / (1 + exp(-gate_i)) * up_i
  * goes to row i of q_dev [rows][inter] and scale_dev [rows][ceil(inter / 128)] in
  * blocks of 1 x 128.  target must be NULL.  inter a multiple of 16 up to 2^20,
- * rows * inter and 2 * inter * in_features under 2^32; the rest as above.
- * Asynchronous. */
+ * rows * inter and 2 * inter * in_features under 2^32; tiles of 128 rows by 128
+ * channels at most; the rest as above.  Asynchronous. */
 int lm_fp8_grouped_swiglu(lm_context* ctx, const lm_fp8_groups* groups, const uint8_t* a_dev, const float* a_scale_dev,
                           int64_t a_rows, const uint8_t* w_dev, const float* w_scale_dev, int64_t inter,
                           int64_t in_features, uint8_t* q_dev, float* scale_dev);
+
+/* ---- which kernel ----
+ * What lm_fp8_gemm (groups = 0), lm_fp8_grouped_gemm and lm_fp8_grouped_swiglu
+ * launch for given sizes (rows: what the groups' arrays hold); host only, no context
+ * or GPU.  Sizes that they refuse are LM_EINVAL. */
+typedef struct lm_fp8_plan {
+    int32_t tile_rows;     /* of a workgroup's tile */
+    int32_t tile_features; /* 16 x 16: the kernel of few rows */
+    int32_t shares;        /* workgroups that share a tile's reduced axis; more than 1: a second launch adds them up */
+    int32_t fp32_sums;     /* 1: fp32 sums, 0: the FP8 matrix cores' */
+    int32_t kernel;        /* which of the kernels of its kind, -1: that of few rows */
+    int32_t reserved;
+    int64_t tiles;         /* that the launch has room for, at most 2^22 */
+} lm_fp8_plan;
+int lm_fp8_plan_gemm(int32_t groups, int64_t rows, int64_t out_features, int64_t in_features, int32_t out_dtype,
+                     lm_fp8_plan* out);
+int lm_fp8_plan_swiglu(int32_t groups, int64_t rows, int64_t inter, int64_t in_features, lm_fp8_plan* out);
 
 /* ---- the layers' FFNs at one byte a weight ----
  * After lm_finalize_layer: the layer's experts and shared experts, or its dense
@@ -121,6 +140,16 @@ int lm_fp8_grouped_swiglu(lm_context* ctx, const lm_fp8_groups* groups, const ui
  * LM_EINVAL while the context's stream is being captured, and with only = 1 while
  * stack graphs are alive. */
 int lm_fp8_layer(lm_context* ctx, int32_t layer, int32_t only);
+
+/* What LM_PATH_FP8 launches for `tokens` tokens of a MoE layer (dense = 0) or of
+ * a dense FFN; host only. */
+typedef struct lm_fp8_layer_plan {
+    lm_fp8_plan gate_up, down;             /* the routed experts' */
+    lm_fp8_plan other_gate_up, other_down; /* the shared experts' or the dense FFN's, where they have launches of their own */
+    int32_t beside;                        /* 1: the shared experts' tiles lie in the routed experts' launches */
+    int32_t reserved;
+} lm_fp8_layer_plan;
+int lm_fp8_plan_layer(const lm_moe_config* config, int32_t dense, int64_t tokens, lm_fp8_layer_plan* out);
 
 #ifdef __cplusplus
 }

@@ -122,6 +122,33 @@ class Fp8Groups(C.Structure):
     ]
 
 
+class Fp8Plan(C.Structure):
+    """lm_fp8_plan: the kernel that a product takes."""
+
+    _fields_ = [
+        ("tile_rows", C.c_int32),
+        ("tile_features", C.c_int32),
+        ("shares", C.c_int32),
+        ("fp32_sums", C.c_int32),
+        ("kernel", C.c_int32),
+        ("reserved", C.c_int32),
+        ("tiles", C.c_int64),
+    ]
+
+
+class Fp8LayerPlan(C.Structure):
+    """lm_fp8_layer_plan: the kernels that a layer's FFN takes on PATH_FP8."""
+
+    _fields_ = [
+        ("gate_up", Fp8Plan),
+        ("down", Fp8Plan),
+        ("other_gate_up", Fp8Plan),
+        ("other_down", Fp8Plan),
+        ("beside", C.c_int32),
+        ("reserved", C.c_int32),
+    ]
+
+
 FP8_BLOCK = 128  # LM_FP8_BLOCK: codes that share a scale, along a row
 
 _P = C.c_void_p
@@ -218,6 +245,9 @@ PROTOTYPES = {
     "lm_fp8_quantize": [_P, _P, _I32, _I64, _I64, _I64, _I32, _P, _P],
     "lm_fp8_gemm": [_P, _P, _P, _I64, _P, _P, _I64, _I64, _P, _I32],
     "lm_fp8_grouped_gemm": [_P, _P, _P, _P, _I64, _P, _P, _I64, _I64, _P, _I64, _I32],
+    "lm_fp8_plan_gemm": [_I32, _I64, _I64, _I64, _I32, _P],
+    "lm_fp8_plan_swiglu": [_I32, _I64, _I64, _I64, _P],
+    "lm_fp8_plan_layer": [_P, _I32, _I64, _P],
     "lm_fp8_grouped_swiglu": [_P, _P, _P, _P, _I64, _P, _P, _I64, _I64, _P, _P],
 }
 _RESTYPE = {"lm_last_error": C.c_char_p}
@@ -333,6 +363,30 @@ def attention_plan_core(config: MlaConfig, cached: int, tokens: int, path: int =
     out = AttentionCorePlan()
     _check_status(lib, lib.lm_attention_plan_core(C.byref(config), cached, tokens, path, budget_bytes,
                                                   C.byref(out)))
+    return out
+
+
+def fp8_plan_gemm(rows: int, out_features: int, in_features: int, dtype: int = DT_F32, groups: int = 0) -> Fp8Plan:
+    """The kernel of lm_fp8_gemm, or with groups of lm_fp8_grouped_gemm (lm_fp8_plan_gemm, host only)."""
+    lib = load_library()
+    out = Fp8Plan()
+    _check_status(lib, lib.lm_fp8_plan_gemm(groups, rows, out_features, in_features, dtype, C.byref(out)))
+    return out
+
+
+def fp8_plan_swiglu(groups: int, rows: int, inter: int, in_features: int) -> Fp8Plan:
+    """The kernel of lm_fp8_grouped_swiglu (lm_fp8_plan_swiglu, host only)."""
+    lib = load_library()
+    out = Fp8Plan()
+    _check_status(lib, lib.lm_fp8_plan_swiglu(groups, rows, inter, in_features, C.byref(out)))
+    return out
+
+
+def fp8_plan_layer(config: MoeConfig, tokens: int, dense: bool = False) -> Fp8LayerPlan:
+    """The kernels of a layer's FFN on PATH_FP8 (lm_fp8_plan_layer, host only)."""
+    lib = load_library()
+    out = Fp8LayerPlan()
+    _check_status(lib, lib.lm_fp8_plan_layer(C.byref(config), int(dense), tokens, C.byref(out)))
     return out
 
 

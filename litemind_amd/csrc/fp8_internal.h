@@ -49,6 +49,17 @@ struct Fp8Product {
 };
 // Sums of products whose reduced axis several workgroups share.
 constexpr int64_t kFp8WorkspaceBytes = 32 << 20;
+// The kernel that a product takes.
+constexpr int64_t kFp8MaxTiles = int64_t{1} << 22;  // of a launch: 2^31 threads
+struct Fp8Plan {
+    int32_t tile;            // which of the kernels of tiles, -1: the kernel of few rows
+    int32_t rows, features;  // of a tile (SwiGLU: features of gate and up each)
+    int32_t shares;          // workgroups that share a tile's reduced axis
+    bool exact;              // fp32 sums
+    int64_t tiles;           // that the launch has room for: refused past kFp8MaxTiles
+};
+Fp8Plan plan_fp8_gemm(const Fp8Product& p, const Fp8Product* beside = nullptr);
+Fp8Plan plan_fp8_swiglu(const Fp8Product& p, const Fp8Product* beside = nullptr);
 // `beside`: another product of the same kind without offsets, in the same launch
 // (p has offsets then, and neither exact sums but SwiGLU's).
 hipError_t launch_fp8_gemm(const Fp8Product& p, void* workspace, hipStream_t s, const Fp8Product* beside = nullptr);
@@ -87,6 +98,10 @@ struct Fp8Scratch {
     void* workspace;
 };
 int fp8_scratch(lm_context* ctx, Fp8Scratch* out);
+// The status of a product's launch.
+int fp8_launched(hipError_t e);
+// A plan as the ABI gives it, LM_EINVAL where the product would be.
+int fp8_plan_out(const Fp8Plan& plan, lm_fp8_plan* out);
 // LM_EKERNEL, once, where a kernel met an index outside its range.
 int fp8_check_error(lm_context* ctx);
 

@@ -658,15 +658,19 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2,
     }
 }
 
+// Tiles of bm rows and bn features that a launch has room for: a group of n rows
+// takes ceil(n / bm) row tiles, at most one more than n / bm for each group that
+// has any.
+int64_t most_tiles(const Fp8Product& p, const Fp8Product* beside, int bm, int bn) {
+    const int64_t mts = p.offsets == nullptr ? (p.rows + bm - 1) / bm : p.rows / bm + std::min<int64_t>(p.groups, p.rows);
+    return mts * ((p.n + bn - 1) / bn) + (beside != nullptr ? tiles_beside(*beside, bm, bn) : 0);
+}
+
 template <bool SWIGLU, bool EXACT, int WM, int WN, int MI, int NJ, int STAGES>
 hipError_t launch_tiles(const Fp8Product& p, const Fp8Product* beside, hipStream_t s, int shares = 1) {
     using Z = Shape<SWIGLU, 16 * WM * MI, 16 * WN * NJ, WM * WN, STAGES>;
-    // a group of n rows takes ceil(n / BM) row tiles: at most one more than
-    // n / BM for each group that has any
-    const int64_t mts = p.offsets == nullptr ? (p.rows + Z::BM - 1) / Z::BM
-                                             : p.rows / Z::BM + std::min<int64_t>(p.groups, p.rows);
-    const int64_t tiles = mts * ((p.n + Z::CN - 1) / Z::CN) + (beside != nullptr ? tiles_beside(*beside, Z::BM, Z::CN) : 0);
-    if (tiles > (1 << 22)) {  // 2^31 threads
+    const int64_t tiles = most_tiles(p, beside, Z::BM, Z::CN);
+    if (tiles > kFp8MaxTiles) {
         return hipErrorInvalidConfiguration;
     }
     const dim3 grid(static_cast<unsigned>(round_up(tiles, kXcds)), static_cast<unsigned>(shares)), block(64 * Z::WAVES);
@@ -759,15 +763,12 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(Fp8Product p, Fp
     }
 }
 
-// Workgroups of the kernel of few rows.
-int64_t stream_tiles(const Fp8Product& p) {
-    const int64_t row_tiles = p.offsets == nullptr ? (p.rows + 15) / 16 : p.rows / 16 + std::min<int64_t>(p.groups, p.rows);
-    return row_tiles * ((p.n + 15) / 16);
-}
+// Rows and features of a tile of the kernel of few rows.
+constexpr int kStreamTile = 16;
 
 template <int WAVES, int U>
 hipError_t launch_stream(const Fp8Product& p, const Fp8Product* beside, hipStream_t s) {
-    const int64_t tiles = stream_tiles(p) + (beside != nullptr ? stream_tiles(*beside) : 0);
+    const int64_t tiles = most_tiles(p, beside, kStreamTile, kStreamTile);
     const dim3 grid(static_cast<unsigned>(round_up(tiles, kXcds))), block(64 * WAVES);
     if (beside != nullptr) {
         hipLaunchKernelGGL(HIP_KERNEL_NAME(fp8_stream_kernel<WAVES, U, true>), grid, block, 0, s, p, *beside);
@@ -884,10 +885,13 @@ struct TileChoice {
 template <size_t N>
 TileChoice choose_tile(const Fp8Product& p, const Fp8Product* beside, const TileCost (&tiles)[N], bool split) {
     constexpr int kShares[] = {1, 2, 3, 4, 6, 8, 12};
-    TileChoice best;
+    TileChoice best{static_cast<int>(N) - 1, 1};
     double least = 1e30;
     for (size_t i = 0; i < N; ++i) {
         const TileCost& c = tiles[i];
+        if (most_tiles(p, beside, c.bm, c.bn) > kFp8MaxTiles) {
+            continue;  // a launch of larger ones may have room
+        }
         double count = row_tiles(p, c.bm) * static_cast<double>((p.n + c.bn - 1) / c.bn);
         if (beside != nullptr) {  // by their stages
             count += static_cast<double>(tiles_beside(*beside, c.bm, c.bn)) * beside->kb / p.kb;
@@ -915,7 +919,7 @@ TileChoice choose_tile(const Fp8Product& p, const Fp8Product* beside, const Tile
 }
 
 template <bool EXACT>
-hipError_t launch_gemm_tile(const Fp8Product& p, const Fp8Product* beside, const TileChoice& c, hipStream_t s) {
+hipError_t launch_gemm_tile(const Fp8Product& p, const Fp8Product* beside, const Fp8Plan& c, hipStream_t s) {
     switch (c.tile) {
         case 0:
             return launch_tiles<false, EXACT, 1, 4, 2, 2, 3>(p, beside, s, c.shares);
@@ -942,7 +946,7 @@ hipError_t launch_gemm_tile(const Fp8Product& p, const Fp8Product* beside, const
 // and 12.
 int64_t stream_bytes(const Fp8Product& p) {
     const int64_t groups = active_groups(p), rows = std::min<int64_t>(16, (p.rows + groups - 1) / groups);
-    const int64_t tiles = stream_tiles(p);
+    const int64_t tiles = most_tiles(p, nullptr, kStreamTile, kStreamTile);
     return tiles <= 4096 ? tiles * p.kb * (16 + rows) * kFp8Block : INT32_MAX;
 }
 bool streams(const Fp8Product& p, const Fp8Product* beside) {
@@ -951,8 +955,26 @@ bool streams(const Fp8Product& p, const Fp8Product* beside) {
 
 }  // namespace
 
-hipError_t launch_fp8_gemm(const Fp8Product& p, void* workspace, hipStream_t s, const Fp8Product* beside) {
+Fp8Plan plan_fp8_gemm(const Fp8Product& p, const Fp8Product* beside) {
     if (streams(p, beside)) {
+        return Fp8Plan{-1, kStreamTile, kStreamTile, 1, true, most_tiles(p, beside, kStreamTile, kStreamTile)};
+    }
+    const bool exact = p.exact != 0, split = p.offsets == nullptr;
+    const TileChoice c = exact ? choose_tile(p, beside, kExactTiles, split) : choose_tile(p, beside, kFp8Tiles, split);
+    const TileCost& t = exact ? kExactTiles[c.tile] : kFp8Tiles[c.tile];
+    return Fp8Plan{c.tile, t.bm, t.bn, c.shares, exact, most_tiles(p, beside, t.bm, t.bn)};
+}
+
+Fp8Plan plan_fp8_swiglu(const Fp8Product& p, const Fp8Product* beside) {
+    const bool exact = p.exact != 0;
+    const TileChoice c = exact ? choose_tile(p, beside, kSwigluTiles, false) : choose_tile(p, beside, kSwigluFp8Tiles, false);
+    const TileCost& t = exact ? kSwigluTiles[c.tile] : kSwigluFp8Tiles[c.tile];
+    return Fp8Plan{c.tile, t.bm, t.bn, 1, exact || c.tile < 3, most_tiles(p, beside, t.bm, t.bn)};
+}
+
+hipError_t launch_fp8_gemm(const Fp8Product& p, void* workspace, hipStream_t s, const Fp8Product* beside) {
+    const Fp8Plan plan = plan_fp8_gemm(p, beside);
+    if (plan.tile < 0) {
         // all of a wave's loads in flight at once where the axis is short, many
         // waves where it is long (10944 channels: 9.5 us, 11 with four waves)
         return p.kb <= 12   ? launch_stream<4, 3>(p, beside, s)
@@ -960,26 +982,24 @@ hipError_t launch_fp8_gemm(const Fp8Product& p, void* workspace, hipStream_t s, 
                : p.kb <= 40 ? launch_stream<8, 2>(p, beside, s)
                             : launch_stream<16, 2>(p, beside, s);
     }
-    const bool exact = p.exact != 0, split = p.offsets == nullptr;
-    const TileChoice c = exact ? choose_tile(p, beside, kExactTiles, split) : choose_tile(p, beside, kFp8Tiles, split);
     Fp8Product q = p;
-    if (c.shares > 1) {
+    if (plan.shares > 1) {
         q.out = workspace;
         q.out_dtype = LM_DT_F32;
     }
-    const hipError_t e = exact ? launch_gemm_tile<true>(q, beside, c, s) : launch_gemm_tile<false>(q, beside, c, s);
-    if (e != hipSuccess || c.shares == 1) {
+    const hipError_t e = plan.exact ? launch_gemm_tile<true>(q, beside, plan, s) : launch_gemm_tile<false>(q, beside, plan, s);
+    if (e != hipSuccess || plan.shares == 1) {
         return e;
     }
     const int64_t count = p.rows * p.n;
     hipLaunchKernelGGL(fp8_join_kernel, dim3(static_cast<unsigned>((count + 1023) / 1024)), dim3(256), 0, s, p,
-                       static_cast<const float*>(workspace), count, c.shares);
+                       static_cast<const float*>(workspace), count, plan.shares);
     return hipGetLastError();
 }
 
 hipError_t launch_fp8_swiglu(const Fp8Product& p, hipStream_t s, const Fp8Product* beside) {
-    const bool exact = p.exact != 0;
-    switch ((exact ? choose_tile(p, beside, kSwigluTiles, false) : choose_tile(p, beside, kSwigluFp8Tiles, false)).tile) {
+    const Fp8Plan plan = plan_fp8_swiglu(p, beside);
+    switch (plan.tile) {
         case 0:
             return launch_tiles<true, true, 1, 8, 2, 2, 3>(p, beside, s);
         case 1:
@@ -987,7 +1007,8 @@ hipError_t launch_fp8_swiglu(const Fp8Product& p, hipStream_t s, const Fp8Produc
         case 2:
             return launch_tiles<true, true, 1, 8, 4, 2, 3>(p, beside, s);
         case 3:
-            return exact ? launch_tiles<true, true, 2, 4, 4, 4, 3>(p, beside, s) : launch_tiles<true, false, 2, 4, 4, 4, 3>(p, beside, s);
+            return plan.exact ? launch_tiles<true, true, 2, 4, 4, 4, 3>(p, beside, s)
+                              : launch_tiles<true, false, 2, 4, 4, 4, 3>(p, beside, s);
         default:
             return launch_tiles<true, false, 2, 4, 8, 4, 2>(p, beside, s);
     }

@@ -591,43 +591,49 @@ int ensure_fp8_workspace(lm_context* ctx, int64_t tokens) {
     return LM_OK;
 }
 
-// A product of one FFN in FP8, of its gate and up matrices or of its down one; rb:
-// of the routed experts.
+// The sizes of a product of one FFN in FP8, of its gate and up matrices or of its
+// down one; routed: of the routed experts.
+lm::Fp8Product fp8_sizes(int64_t H, int64_t E, int64_t K, int64_t inter, int64_t T, bool routed, bool down) {
+    lm::Fp8Product p{};
+    p.groups = routed ? static_cast<int32_t>(E) : 1;
+    p.rows = routed ? T * K : T;
+    p.exact = 0;  // the FP8 cores' sums are off by 4e-5 of their norm, the codes by 4e-2
+    p.a_rows = down ? p.rows : T;
+    p.n = static_cast<int32_t>(down ? H : inter);
+    p.k = static_cast<int32_t>(down ? inter : H);
+    p.nb = static_cast<int32_t>(lm::fp8_blocks(p.n));
+    p.kb = static_cast<int32_t>(lm::fp8_blocks(p.k));
+    if (down) {
+        p.out_rows = p.rows;
+        p.out_dtype = LM_DT_F32;
+    } else {
+        p.divisor = routed ? static_cast<int32_t>(K) : 0;
+    }
+    return p;
+}
+
+// The product with its operands; rb: of the routed experts.
 lm::Fp8Product fp8_product(const lm_context* ctx, const Fp8Ffn& f, int64_t inter, int64_t T, const lm::RouteBufs* rb,
                            uint8_t* act, float* act_scale, float* down_out, const lm::Fp8Scratch& sc, bool down) {
     const Workspace& w = ctx->ws;
-    lm::Fp8Product p{};
-    p.groups = rb != nullptr ? ctx->E : 1;
-    p.rows = rb != nullptr ? T * ctx->K : T;
+    lm::Fp8Product p = fp8_sizes(ctx->H, ctx->E, ctx->K, inter, T, rb != nullptr, down);
     p.offsets = rb != nullptr ? rb->offsets : nullptr;
     p.error = sc.error;
-    p.exact = 0;  // the FP8 cores' sums are off by 4e-5 of their norm, the codes by 4e-2
     if (!down) {
         p.a = w.fp8_x;
         p.a_scale = w.fp8_x_scale;
-        p.a_rows = T;
         p.w = f.gate_up;
         p.w_scale = f.gate_up_scale;
-        p.n = static_cast<int32_t>(inter);
-        p.k = ctx->H;
         p.source = rb != nullptr ? rb->perm : nullptr;
-        p.divisor = rb != nullptr ? ctx->K : 0;
         p.q = act;
         p.q_scale = act_scale;
     } else {
         p.a = act;
         p.a_scale = act_scale;
-        p.a_rows = p.rows;
         p.w = f.down;
         p.w_scale = f.down_scale;
-        p.n = ctx->H;
-        p.k = static_cast<int32_t>(inter);
         p.out = down_out;
-        p.out_rows = p.rows;
-        p.out_dtype = LM_DT_F32;
     }
-    p.nb = static_cast<int32_t>(lm::fp8_blocks(p.n));
-    p.kb = static_cast<int32_t>(lm::fp8_blocks(p.k));
     return p;
 }
 
@@ -638,6 +644,7 @@ lm::Fp8Product fp8_product(const lm_context* ctx, const Fp8Ffn& f, int64_t inter
 // launches of their own; one of 160 89, 787, 1022 and 1305, and 121, 820, 1006 and
 // 1287.
 constexpr int64_t kFp8Beside = 128;
+bool fp8_beside(bool routed, bool shared, int64_t T) { return routed && shared && T <= kFp8Beside; }
 
 // launch_expert_kernels in FP8: the tokens' blocks, gate/up and down of the
 // routed experts (slots in permuted order) and of the shared (or dense) FFN, whose
@@ -666,16 +673,17 @@ int launch_expert_kernels_fp8(lm_context* ctx, const Layer& L, const float* x, i
             rest = fp8_product(ctx, L.fp8.other, inter, T, nullptr, w.fp8_act + TK * ctx->I,
                                w.fp8_act_scale + TK * lm::fp8_blocks(ctx->I), w.down_out + TK * ctx->H, sc, down);
         }
-        const bool beside = !L.dense && other && T <= kFp8Beside;
-        const auto launch = [&](const lm::Fp8Product& p) {
-            const lm::Fp8Product* const q = beside ? &rest : nullptr;
-            return down ? lm::launch_fp8_gemm(p, sc.workspace, ctx->stream, q) : lm::launch_fp8_swiglu(p, ctx->stream, q);
+        const bool beside = fp8_beside(!L.dense, other, T);
+        const auto launch = [&](const lm::Fp8Product& p, const lm::Fp8Product* q) {
+            return lm::fp8_launched(down ? lm::launch_fp8_gemm(p, sc.workspace, ctx->stream, q)
+                                         : lm::launch_fp8_swiglu(p, ctx->stream, q));
         };
-        if (!L.dense) {
-            LM_HIP(launch(routed));
+        int status = L.dense ? LM_OK : launch(routed, beside ? &rest : nullptr);
+        if (status == LM_OK && other && !beside) {
+            status = launch(rest, nullptr);
         }
-        if (other && !beside) {
-            LM_HIP(launch(rest));
+        if (status != LM_OK) {
+            return status;
         }
     }
     return LM_OK;
@@ -1882,6 +1890,47 @@ int lm_fp8_layer(lm_context* ctx, int32_t layer, int32_t only) {
         L.table = nullptr;
     }
     f.ready = true;
+    return LM_OK;
+    LM_GUARD_END
+}
+
+int lm_fp8_plan_layer(const lm_moe_config* config, int32_t dense, int64_t tokens, lm_fp8_layer_plan* out) {
+    LM_GUARD_BEGIN
+    if (config == nullptr || out == nullptr || tokens < 1 || (dense != 0 && dense != 1)) {
+        return fail(LM_EINVAL, "null config or output, no tokens, or dense not 0 or 1");
+    }
+    const lm_moe_config& c = *config;
+    const int64_t H = c.hidden_size, I = c.moe_intermediate_size, S = I * c.n_shared_experts, D = c.intermediate_size,
+                  E = c.n_routed_experts, K = c.num_experts_per_tok, other = dense != 0 ? D : S;
+    if (H < 16 || H % 16 != 0 || other < 0 || other % 16 != 0 ||
+        (dense != 0 ? D < 16 : I < 16 || I % 16 != 0 || E < 1 || E > lm::kFp8MaxGroups || K < 1 || K > lm::kMaxTopK)) {
+        return fail(LM_EINVAL, "FP8 layers have widths in multiples of 16, up to 512 experts and 16 of them a token");
+    }
+    const int64_t widest = dense != 0 ? D : std::max(I, S), row = dense != 0 ? D : std::max(K * I, S);
+    if (std::max(H, widest) > lm::kFp8MaxInner || 2 * widest * H >= kFp8Codes || tokens >= kFp8Codes / std::max(H, row)) {
+        return fail(LM_EINVAL, "widths or tokens past what LM_PATH_FP8 takes");
+    }
+    *out = lm_fp8_layer_plan{};
+    out->beside = fp8_beside(dense == 0, S > 0, tokens) ? 1 : 0;
+    const int32_t offsets = 0;  // that there are some; never followed
+    int rc = LM_OK;
+    for (const bool down : {false, true}) {
+        const auto plan = [&](const lm::Fp8Product& p, const lm::Fp8Product* q, lm_fp8_plan* to) {
+            return lm::fp8_plan_out(down ? lm::plan_fp8_gemm(p, q) : lm::plan_fp8_swiglu(p, q), to);
+        };
+        const lm::Fp8Product rest = fp8_sizes(H, E, K, other, tokens, false, down);
+        if (dense == 0) {
+            lm::Fp8Product routed = fp8_sizes(H, E, K, I, tokens, true, down);
+            routed.offsets = &offsets;
+            rc = plan(routed, out->beside != 0 ? &rest : nullptr, down ? &out->down : &out->gate_up);
+        }
+        if (rc == LM_OK && other > 0 && out->beside == 0) {
+            rc = plan(rest, nullptr, down ? &out->other_down : &out->other_gate_up);
+        }
+        if (rc != LM_OK) {
+            return rc;
+        }
+    }
     return LM_OK;
     LM_GUARD_END
 }

@@ -3,6 +3,7 @@
 #include "fp8_internal.h"
 #include "lm_error.h"
 
+#include <algorithm>
 #include <new>
 #include <string>
 
@@ -69,15 +70,6 @@ int64_t element_bytes(int32_t dtype) {
 
 constexpr int64_t kMost32 = int64_t{1} << 32;
 
-// A product's launch.
-int launched(hipError_t e) {
-    if (e == hipErrorInvalidConfiguration) {
-        return fail(LM_EINVAL, "more than 2^22 output tiles: call it for fewer rows, groups or features at a time");
-    }
-    LM_FP8_HIP(e);
-    return LM_OK;
-}
-
 // The sizes of a product: p's n, k, nb, kb, a_rows and rows on success.
 int product_sizes(lm::Fp8Product& p, int64_t a_rows, int64_t n, int64_t k, int64_t parts) {
     if (k < 16 || k > lm::kFp8MaxInner || k % 16 != 0) {
@@ -95,6 +87,14 @@ int product_sizes(lm::Fp8Product& p, int64_t a_rows, int64_t n, int64_t k, int64
     p.nb = static_cast<int32_t>(lm::fp8_blocks(n));
     p.kb = static_cast<int32_t>(lm::fp8_blocks(k));
     return LM_OK;
+}
+
+// The same for gate and up, whose outputs are the next product's rows.
+int swiglu_sizes(lm::Fp8Product& p, int64_t a_rows, int64_t inter, int64_t k) {
+    if (inter < 16 || inter > lm::kFp8MaxInner || inter % 16 != 0 || p.rows * inter >= kMost32) {
+        return fail(LM_EINVAL, "inter must be a multiple of 16 up to 2^20, with under 2^32 codes");
+    }
+    return product_sizes(p, a_rows, inter, k, 2);
 }
 
 // The operands' pointers.
@@ -184,6 +184,22 @@ int lm::fp8_scratch(lm_context* ctx, Fp8Scratch* out) {
     return LM_OK;
 }
 
+int lm::fp8_launched(hipError_t e) {
+    if (e == hipErrorInvalidConfiguration) {
+        return fail(LM_EINVAL, "more than 2^22 output tiles: call it for fewer rows, groups or features at a time");
+    }
+    LM_FP8_HIP(e);
+    return LM_OK;
+}
+
+int lm::fp8_plan_out(const Fp8Plan& plan, lm_fp8_plan* out) {
+    if (plan.tiles > kFp8MaxTiles) {
+        return fp8_launched(hipErrorInvalidConfiguration);
+    }
+    *out = lm_fp8_plan{plan.rows, plan.features, plan.shares, plan.exact ? 1 : 0, plan.tile, 0, plan.tiles};
+    return LM_OK;
+}
+
 extern "C" {
 
 int lm_fp8_quantize(lm_context* ctx, const void* x_dev, int32_t dtype, int64_t rows, int64_t width, int64_t row_stride,
@@ -266,7 +282,7 @@ int lm_fp8_gemm(lm_context* ctx, const uint8_t* a_dev, const float* a_scale_dev,
     if (rc != LM_OK) {
         return rc;
     }
-    return launched(lm::launch_fp8_gemm(p, sc.workspace, info.stream));
+    return lm::fp8_launched(lm::launch_fp8_gemm(p, sc.workspace, info.stream));
 } catch (const std::bad_alloc&) {
     return fail(LM_ENOMEM, "host allocation failed");
 }
@@ -323,7 +339,7 @@ int lm_fp8_grouped_gemm(lm_context* ctx, const lm_fp8_groups* groups, const uint
         p.out_dtype = out_dtype;
         p.exact = out_dtype == LM_DT_F32 ? 1 : 0;
         p.error = sc.error;
-        return launched(lm::launch_fp8_gemm(p, sc.workspace, info.stream));
+        return lm::fp8_launched(lm::launch_fp8_gemm(p, sc.workspace, info.stream));
     } catch (const std::bad_alloc&) {
         return fail(LM_ENOMEM, "host allocation failed");
     }
@@ -341,10 +357,7 @@ int lm_fp8_grouped_swiglu(lm_context* ctx, const lm_fp8_groups* groups, const ui
         if (p.target != nullptr) {
             return fail(LM_EINVAL, "target must be NULL: row i of the groups is row i of the codes");
         }
-        if (inter < 16 || inter > lm::kFp8MaxInner || inter % 16 != 0 || p.rows * inter >= kMost32) {
-            return fail(LM_EINVAL, "inter must be a multiple of 16 up to 2^20, with under 2^32 codes");
-        }
-        rc = product_sizes(p, a_rows, inter, in_features, 2);
+        rc = swiglu_sizes(p, a_rows, inter, in_features);
         if (rc != LM_OK) {
             return rc;
         }
@@ -379,10 +392,53 @@ int lm_fp8_grouped_swiglu(lm_context* ctx, const lm_fp8_groups* groups, const ui
         p.q_scale = scale_dev;
         p.exact = 1;
         p.error = sc.error;
-        return launched(lm::launch_fp8_swiglu(p, info.stream));
+        return lm::fp8_launched(lm::launch_fp8_swiglu(p, info.stream));
     } catch (const std::bad_alloc&) {
         return fail(LM_ENOMEM, "host allocation failed");
     }
+}
+
+int lm_fp8_plan_gemm(int32_t groups, int64_t rows, int64_t out_features, int64_t in_features, int32_t out_dtype,
+                     lm_fp8_plan* out) try {
+    lm::Fp8Product p{};
+    const int32_t none = 0;
+    const lm_fp8_groups g{groups, 0, rows, &none, nullptr, nullptr};
+    int rc = groups == 0 ? LM_OK : product_groups(p, &g);
+    if (rc == LM_OK) {
+        rc = product_sizes(p, groups == 0 ? rows : 1, out_features, in_features, 1);
+    }
+    if (rc != LM_OK) {
+        return rc;
+    }
+    if (out == nullptr || rows < 1 || element_bytes(out_dtype) == 0) {
+        return fail(LM_EINVAL, "null output, no rows, or not LM_DT_F32, LM_DT_F16 or LM_DT_BF16");
+    }
+    p.groups = std::max(groups, 1);
+    p.rows = rows;
+    p.exact = out_dtype == LM_DT_F32 ? 1 : 0;
+    return lm::fp8_plan_out(lm::plan_fp8_gemm(p), out);
+} catch (const std::bad_alloc&) {
+    return fail(LM_ENOMEM, "host allocation failed");
+}
+
+int lm_fp8_plan_swiglu(int32_t groups, int64_t rows, int64_t inter, int64_t in_features, lm_fp8_plan* out) try {
+    lm::Fp8Product p{};
+    const int32_t none = 0;
+    const lm_fp8_groups g{groups, 0, rows, &none, nullptr, nullptr};
+    int rc = product_groups(p, &g);
+    if (rc == LM_OK) {
+        rc = swiglu_sizes(p, 1, inter, in_features);
+    }
+    if (rc != LM_OK) {
+        return rc;
+    }
+    if (out == nullptr || rows < 1) {
+        return fail(LM_EINVAL, "null output or no rows");
+    }
+    p.exact = 1;
+    return lm::fp8_plan_out(lm::plan_fp8_swiglu(p), out);
+} catch (const std::bad_alloc&) {
+    return fail(LM_ENOMEM, "host allocation failed");
 }
 
 }  // extern "C"
