@@ -41,8 +41,9 @@ extern "C" {
 /* x [rows][width] of `dtype` (LM_DT_F32, LM_DT_F16 or LM_DT_BF16), rows
  * row_stride elements apart (at least width), into q_dev [rows][width] codes and
  * scale_dev [ceil(rows / block_rows)][ceil(width / 128)].  block_rows is 1 (a
- * product's rows) or 128 (its weights).  rows under 2^31, width at most 2^24;
- * q_dev 16-byte aligned; the outputs overlap nothing.  Asynchronous. */
+ * product's rows) or 128 (its weights).  rows under 2^31, of a matrix at most 2^23 -
+ * 128 (more in several calls, from a multiple of 128 on); width at most 2^24,
+ * row_stride 2^28; q_dev 16-byte aligned; the outputs overlap nothing.  Asynchronous. */
 int lm_fp8_quantize(lm_context* ctx, const void* x_dev, int32_t dtype, int64_t rows, int64_t width, int64_t row_stride,
                     int32_t block_rows, uint8_t* q_dev, float* scale_dev);
 
@@ -53,12 +54,14 @@ int lm_fp8_quantize(lm_context* ctx, const void* x_dev, int32_t dtype, int64_t r
  *   w_scale_dev [ceil(out_features / 128)][ceil(in_features / 128)]
  *   out_dev [rows][out_features] of out_dtype (LM_DT_F32, LM_DT_F16, LM_DT_BF16)
  * Products are exact.  An fp32 output's sums are fp32; fp16 and BF16 outputs' are
- * those of the FP8 matrix cores, off by 1.4e-5 to 4e-5 of their norm and at most
- * 2^-10 of the sum of magnitudes, rounded once at the end.  in_features a multiple
- * of 16 up to 2^20, out_features at most 2^24; rows, rows * in_features and
- * out_features * in_features under 2^31, 2^32 and 2^32; and one launch has room for
- * 2^22 tiles, of 128 rows by 256 features at most (16-bit outputs 256 by 256; of
- * groups each has a row tile begun): LM_EINVAL past it.  a_dev, w_dev and out_dev
+ * so for few rows, and else (lm_fp8_plan_gemm's fp32_sums) those of the FP8 matrix
+ * cores, off by 1.4e-5 to 4e-5 of their norm and at most 2^-10 of the sum of
+ * magnitudes, rounded once at the end: one that is far smaller than its products
+ * keeps less than its type's bits; where those count, the output is fp32.
+ * in_features a multiple of 16 up to 2^20, out_features at most 2^24; rows, rows *
+ * in_features and out_features * in_features under 2^31, 2^32 and 2^32.  A launch
+ * has room for 2^22 tiles, of 128 rows by 256 features at most (16-bit outputs 256
+ * by 256; every group begins one): LM_EINVAL past it.  a_dev, w_dev and out_dev
  * 16-byte aligned; out_dev overlaps no input.  Asynchronous. */
 int lm_fp8_gemm(lm_context* ctx, const uint8_t* a_dev, const float* a_scale_dev, int64_t rows, const uint8_t* w_dev,
                 const float* w_scale_dev, int64_t out_features, int64_t in_features, void* out_dev, int32_t out_dtype);
@@ -95,7 +98,9 @@ int lm_fp8_grouped_gemm(lm_context* ctx, const lm_fp8_groups* groups, const uint
  * gate_i, up_i the two products of row i, both fp32,
  *     act_i = gate_i / (1 + exp(-gate_i)) * up_i
  * goes to row i of q_dev [rows][inter] and scale_dev [rows][ceil(inter / 128)] in
- * blocks of 1 x 128.  target must be NULL.  inter a multiple of 16 up to 2^20,
+ * blocks of 1 x 128, by fp32's quotients: the code of a value within 2^-22 of the
+ * middle between two may be the other.  The exponential is off by 2^-23 (2 +
+ * |gate_i|) of itself, and 1 / (1 + exp(-gate_i)) under 2^-126 may be 0.  target must be NULL.  inter a multiple of 16 up to 2^20,
  * rows * inter and 2 * inter * in_features under 2^32; tiles of 128 rows by 128
  * channels at most; the rest as above.  Asynchronous. */
 int lm_fp8_grouped_swiglu(lm_context* ctx, const lm_fp8_groups* groups, const uint8_t* a_dev, const float* a_scale_dev,

@@ -252,8 +252,10 @@ __device__ inline void store4(const Fp8Product& p, int64_t row, int32_t n, float
     }
 }
 
-// gate / (1 + exp(-gate)) * up; the hardware's exponential and reciprocal are
-// off by a few 2^-24, far below the rounding to e4m3 (2^-4).
+// gate / (1 + exp(-gate)) * up.  The exponential is taken of gate / ln 2 in fp32 and
+// is off by 2^-23 (2 + |gate|) of itself; what of that reaches the quotient, its
+// share of 1 + exp(-gate), is at most 2^-16 (at -87, under which the quotient is
+// subnormal and taken as 0) and far below the rounding to e4m3 (2^-4).
 __device__ inline float swiglu(float gate, float up) {
     return gate * __builtin_amdgcn_rcpf(1.0f + __expf(-gate)) * up;
 }

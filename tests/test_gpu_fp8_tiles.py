@@ -55,3 +55,15 @@ def test_larger_tiles_where_small_ones_are_too_many(ctx):
         ref.check_product(got[:, 88:], *ref.product(a[e:e + 1], sa[e:e + 1], w, sw), "f32", e)
     for b in (dw, dsw, y):
         b.free()
+
+
+def test_matrix_in_several_calls(ctx):
+    """A matrix quantized from a multiple of 128 rows on: the same codes and scales as in one call."""
+    announce("fp8 quantize, a matrix in two calls")
+    rows, width, first = 700, 208, 384
+    x = np.random.default_rng(91).standard_normal((rows, width)).astype(np.float32)
+    dx, q, s = ctx.to_device(x), ctx.empty((rows, width), np.uint8), ctx.empty((6, 2))
+    for at, n in ((0, first), (first, rows - first)):
+        ctx.fp8_quantize(dx.ptr + 4 * at * width, n, width, q.ptr + at * width, s.ptr + 4 * at // 128 * 2, block_rows=128)
+    want_q, want_s = ref.quantize(x, 128)
+    assert (q.download() == want_q).all() and (s.download() == want_s).all()
