@@ -1,6 +1,8 @@
 """LM_PATH_FP8 at DeepSeek-V2-Lite's widths, where the layers' own launches run: the shared experts' tiles beside the
 routed experts', SwiGLU and fp32 outputs on the FP8 matrix cores, tiles of up to 256 rows, shared sums of the dense
 FFN.  Against the FP8 operators one after another, whose sums are fp32's."""
+import dataclasses
+
 import numpy as np
 import pytest
 
@@ -84,27 +86,21 @@ def near(got, want, gate_up_exact):
     assert (d <= 4e-2 * norm).all(), (d / norm).max()
 
 
-def moe(lite, T, skewed):
-    ctx, _, routed, shared = lite
-    x = wl.tokens(7, T, D.hidden)
-    dx, y, idx, w = ctx.to_device(x), ctx.empty((T, D.hidden)), ctx.empty((T, D.top_k), np.int32), ctx.empty((T, D.top_k))
-    bias = None
-    if skewed:  # most assignments to eight experts, and experts without any
-        b = np.zeros(D.experts, np.float32)
-        b[3::8] = 2.5
-        b[:3] = -1e4
-        bias = ctx.to_device(b)
-    ctx.moe_forward(1, dx, T, y, bias=bias, idx=idx, w=w, path=lm.PATH_FP8)
+def moe(ctx, layer, d, routed, shared, x, bias=None):
+    """The layer's outputs, those of the operators for its routing, and the assignments of each expert."""
+    T = len(x)
+    dx, y, idx, w = ctx.to_device(x), ctx.empty((T, d.hidden)), ctx.empty((T, d.top_k), np.int32), ctx.empty((T, d.top_k))
+    ctx.moe_forward(layer, dx, T, y, bias=bias, idx=idx, w=w, path=lm.PATH_FP8)
     got = y.download()
-    ctx.moe_forward(1, dx, T, y, bias=bias, idx=idx, w=w, path=lm.PATH_FP8)
+    ctx.moe_forward(layer, dx, T, y, bias=bias, idx=idx, w=w, path=lm.PATH_FP8)
     assert (y.download() == got).all()  # the same bits every time
     gi, gw = idx.download(), w.download().astype(np.float64)
-    counts = np.bincount(gi.reshape(-1), minlength=D.experts)
+    counts = np.bincount(gi.reshape(-1), minlength=d.experts)
     offsets = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
     perm = np.argsort(gi.reshape(-1), kind="stable").astype(np.int32)
-    rows = routed.run(x, offsets, perm, D.top_k).reshape(T, D.top_k, -1)
-    want = sum(gw[:, r, None] * rows[:, r] for r in range(D.top_k)) + shared.alone(x)
-    return x, got, want, counts
+    rows = routed.run(x, offsets, perm, d.top_k).reshape(T, d.top_k, -1)
+    want = sum(gw[:, r, None] * rows[:, r] for r in range(d.top_k)) + shared.alone(x)
+    return got, want, counts
 
 
 # V2-Lite's calls: the single row's launch, few rows beside the shared experts', up to the last of these, the first with
@@ -116,16 +112,41 @@ def test_moe_layer(lite, T, skewed):
     announce(f"fp8 V2-Lite MoE layer, {T} tokens{', skewed' if skewed else ''}: gate/up {plan.gate_up.kernel}, down "
              f"{plan.down.tile_rows} x {plan.down.tile_features}, beside {plan.beside}")
     assert plan.beside == (T <= 128)
-    x, got, want, counts = moe(lite, T, skewed)
+    ctx, _, routed, shared = lite
+    x, bias = wl.tokens(7, T, D.hidden), None
+    if skewed:  # most assignments to eight experts, and experts without any
+        b = np.zeros(D.experts, np.float32)
+        b[3::8] = 2.5
+        b[:3] = -1e4
+        bias = ctx.to_device(b)
+    got, want, counts = moe(ctx, 1, D, routed, shared, x, bias)
     if skewed:
         assert (counts[:3] == 0).all() and (T < 100 or counts.max() > 2 * T * D.top_k / D.experts)
     exact = plan.gate_up.fp32_sums and (plan.beside or plan.other_gate_up.fp32_sums)
     near(got, want, exact)
-    ctx = lite[0]
     y = ctx.empty(got.shape)
     if not skewed:
         ctx.moe_forward(1, ctx.to_device(x), T, y, path=lm.PATH_AUTO)
         assert np.linalg.norm(y.download() - got) <= 0.13 * np.linalg.norm(got)  # twice what rounding to e4m3 comes to
+
+
+# few experts: the larger tiles with the shared experts' beside them
+@pytest.mark.parametrize("experts,top_k,hidden,inter,n_shared,T,gate_up,down", [
+    (20, 6, 5120, 1536, 2, 1, 0, 0), (16, 16, 1040, 144, 1, 128, 1, 1), (2, 2, 1040, 4112, 1, 128, 2, 0),
+    (4, 4, 2064, 2064, 3, 100, 3, 1), (16, 16, 2064, 1408, 3, 128, 4, 2), (16, 16, 2048, 4112, 1, 100, 3, 3),
+    (8, 8, 5120, 1040, 2, 117, 3, 4), (8, 3, 272, 2064, 2, 1, 0, -1)])
+def test_beside(experts, top_k, hidden, inter, n_shared, T, gate_up, down):
+    announce(f"fp8 layer of {experts} experts, {hidden} x {inter}, {T} tokens: gate/up {gate_up}, down {down}, beside")
+    d = dataclasses.replace(D, hidden=hidden, inter=inter, experts=experts, top_k=top_k, n_shared=n_shared)
+    plan = lm.fp8_plan_layer(d.moe_config(num_layers=1), T)
+    assert (plan.beside, plan.gate_up.kernel, plan.down.kernel) == (1, gate_up, down)
+    m = wl.moe_layer(17, 0, d)
+    with lm.Context(d.moe_config(num_layers=1)) as ctx:
+        wl.upload_moe_layer(ctx, 0, m)
+        ctx.fp8_layer(0, only=True)
+        routed, shared = Ffn(ctx, m.gate, m.up, m.down), Ffn(ctx, [m.shared_gate], [m.shared_up], [m.shared_down])
+        got, want, _ = moe(ctx, 0, d, routed, shared, wl.tokens(7, T, hidden))
+        near(got, want, bool(plan.gate_up.fp32_sums))
 
 
 def test_every_launch_of_the_layers_ran():
